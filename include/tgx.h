@@ -790,6 +790,124 @@ int tgx_profile_count(void);
 int tgx_profile_entry(int index, char* name, int name_capacity, int64_t* launches,
                       double* total_ms);
 
+/* ------------------------------------------------------------------------ */
+/* Paged caches: attention, upkeep, page selection                           */
+/* ------------------------------------------------------------------------ */
+
+/* The relation of each sequence's newest tokens to the slots of a paged cache
+ * (Graph.paged).  Position j of sequence b lies in slot
+ * page_table[b][j / page_size] * page_size + j % page_size; a page id outside
+ * [0, num_pages) names no page: its positions hold nothing.  Table and lengths
+ * are read on the device at every launch, lengths clamped to
+ * [0, pages_per_seq * page_size]; no contents of theirs make a kernel access
+ * memory outside the operands.  The newest `queries` tokens of a sequence
+ * ask; token t of them sees the positions below length - (queries - 1 - t).
+ * table_heads > 1: a table for each head, page_table [n_seqs, table_heads,
+ * pages_per_seq] (Graph.select_pages), one length for all heads. */
+typedef struct {
+  const int32_t* page_table_dev;
+  int64_t seq_stride;        /* elements between two sequences' tables */
+  int64_t head_stride;       /* and two heads' */
+  const int32_t* lengths_dev;
+  int64_t n_seqs;
+  int32_t table_heads;
+  int32_t pages_per_seq;
+  int32_t page_size;
+  int64_t num_pages;
+  int32_t queries;
+} tgx_paged;
+
+/* Workspace bytes needed by tgx_paged_attn (0: no sequence can be split). */
+int tgx_paged_attn_workspace(const tgx_paged* p, int heads, int group, int D, int dtype,
+                             size_t* bytes);
+
+/* Dot-product attention over a paged relation, softmax in fp32:
+ *   out[r, h, g] = sum_j softmax_j(scale * q[r, h, g] . k[j, h]) v[j, h]
+ * with `group` query heads on each of `heads` key heads, D a multiple of 8 up
+ * to 512, q, k, v and out of one dtype.  A row that sees no key is 0.
+ *   q   row ((b * queries + t) * table_heads + table head)
+ *   out [rows, heads, group, D] contiguous
+ *   strides, host array of nine, in elements, multiples of 16 bytes: q's row,
+ *     head, group; k's slot, table head, head; v's slot, table head, head
+ * Other shapes: TGX_UNSUPPORTED. */
+int tgx_paged_attn(const tgx_paged* p, const void* q_dev, const void* k_dev, const void* v_dev,
+                   const int64_t* strides, float scale, void* out_dev, int heads, int group,
+                   int D, int dtype, void* workspace_dev, size_t workspace_bytes, void* stream);
+
+/* The newest tokens' keys and values into their slots (Graph.append): rows b *
+ * queries + t of key and value, `heads` rows of D values each; tokens at
+ * positions below zero do not exist.  Page sums, if given (fp32
+ * [num_pages, heads, D] contiguous), of every page a token was written to are
+ * formed again over the page's slots up to the newest token, in slot order.
+ * The pages that sequences append to must be their own.
+ *   strides, host array of eight, in elements: key cache's slot and head, key's
+ *     row and head, value cache's slot and head, value's row and head */
+int tgx_paged_append(const tgx_paged* p, void* key_cache_dev, const void* key_dev,
+                     void* value_cache_dev, const void* value_dev, const int64_t* strides,
+                     float* page_sums_dev, int heads, int D, int dtype, void* stream);
+
+/* Workspace bytes needed by tgx_select_pages. */
+int tgx_select_pages_workspace(const tgx_paged* p, int heads, int count, size_t* bytes);
+
+/* Pages a row attends to (Graph.select_pages): for each query row and key
+ * head, the newest page and the count - 1 others of largest score
+ *   sum_d (sum_g q[row, h, g, d]) * page_sums[page, h, d]   (fp64; NaN, and a
+ * page id that names no page, as -inf; equal scores to the lowest position),
+ * all pages where there are no more than count.
+ *   strides     host array of three: q's row, head, group
+ *   table_dev   [rows, heads, count] int32: page ids in order of position, then -1
+ *   lengths_dev [rows] int32: positions the chosen pages hold */
+int tgx_select_pages(const tgx_paged* p, const void* q_dev, const int64_t* strides,
+                     const float* page_sums_dev, int heads, int group, int D, int dtype,
+                     int count, int32_t* table_dev, int32_t* lengths_dev, void* workspace_dev,
+                     size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Norm and rotation of queries and keys                                     */
+/* ------------------------------------------------------------------------ */
+
+/* Operands of tg.nn.norm_rotary; index 0 the queries, 1 the keys (heads = 0
+ * where absent).  x is [n_tokens, heads, D] with the given element strides and
+ * unit last stride; w [D] or NULL (ones); positions [n_tokens, axes] contiguous;
+ * frequency i turns by the position of the axis whose section holds i.  D is a
+ * multiple of 4 up to 256, n_freqs even and at most D / 2. */
+typedef struct {
+  const void* x_dev[2];
+  int64_t token_stride[2];
+  int64_t head_stride[2];
+  int32_t heads[2];
+  const void* w_dev[2];
+  int32_t w_dtype;
+  const void* positions_dev;
+  int32_t positions_bits;    /* 32 or 64 */
+  int32_t axes;              /* 1 to 4 */
+  int32_t sections[4];       /* frequencies of each axis */
+  const float* freqs_dev;
+  int32_t n_freqs;
+  int32_t norm;              /* 0: rotation only */
+  int32_t interleaved;       /* pairs (2i, 2i + 1) instead of (i, i + n_freqs) */
+  float eps;
+  int64_t n_tokens;
+  int32_t D;
+  int32_t dtype;
+} tgx_norm_rotary;
+
+/* RMS norm over each row's D values (times w) and rotation of its pairs by
+ * position * frequency; outputs contiguous [n_tokens, heads, D]. */
+int tgx_norm_rotary_fwd(const tgx_norm_rotary* p, void* query_out_dev, void* key_out_dev,
+                        void* stream);
+
+/* Workspace bytes needed by tgx_norm_rotary_bwd when weight gradients are wanted. */
+int tgx_norm_rotary_bwd_workspace(const tgx_norm_rotary* p, size_t* bytes);
+
+/* Gradients of tgx_norm_rotary_fwd: output gradients contiguous, dquery and
+ * dkey contiguous [n_tokens, heads, D], weight gradients [D] in w_dtype (NULL:
+ * not wanted).  No atomics: the same inputs give the same bits. */
+int tgx_norm_rotary_bwd(const tgx_norm_rotary* p, const void* dquery_out_dev,
+                        const void* dkey_out_dev, void* dquery_dev, void* dkey_dev,
+                        void* dquery_weight_dev, void* dkey_weight_dev, void* workspace_dev,
+                        size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,209 @@
+"""tg.nn.norm_rotary on the HIP kernels, forward and backward, against the
+formula in float64: types, widths, partial and several-axis rotation, strides,
+far positions, captured passes."""
+
+import numpy as np
+import pytest
+import torch
+
+import tiga as tg
+
+import paged_reference as want
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda")
+TYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+F32 = 2.0 ** -24
+
+
+@pytest.fixture(autouse=True)
+def _strict():
+    tg.config.strict = True
+    yield
+    tg.config.strict = False
+
+
+f64 = lambda t: t.detach().double().cpu().numpy()
+
+
+def make(n, hq, hk, D, sections, dtype, seed=0, far=5000, wdtype=None, bits=64):
+    rng = np.random.default_rng(seed)
+    half = sum(sections)
+    freqs = torch.tensor(10000.0 ** (-np.arange(half) / max(half, 1)), device=DEV).float()
+    pos = torch.tensor(rng.integers(-far, far, size=(n, len(sections))), device=DEV,
+                       dtype=torch.int64 if bits == 64 else torch.int32)
+    qkv = torch.tensor(rng.standard_normal((n, hq + 2 * hk, D)), device=DEV).to(dtype)
+    q, k = (t.detach().requires_grad_(True) for t in (qkv[:, :hq], qkv[:, hq:hq + hk]))
+    w = [torch.tensor(1 + 0.2 * rng.standard_normal(D), device=DEV).to(wdtype or dtype)
+         .requires_grad_(True) for _ in range(2)]
+    dy = [torch.tensor(rng.standard_normal((n, h, D)), device=DEV).to(dtype) for h in (hq, hk)]
+    return q, k, w, pos, freqs, dy
+
+
+def check(n, hq, hk, D, sections, dtype, interleaved=False, norm=True, eps=1e-6, **kw):
+    print(f"rotary {dtype} n={n} heads={hq},{hk} D={D} {sections} inter={interleaved} "
+          f"norm={norm}", flush=True)
+    q, k, w, pos, freqs, dy = make(n, hq, hk, D, sections, dtype, **kw)
+    weights = dict(query_weight=w[0], key_weight=w[1]) if norm else {}
+    outs = tg.nn.norm_rotary(q, k, pos, freqs, norm=norm, eps=eps, sections=sections,
+                             interleaved=interleaved, **weights)
+    with torch.no_grad():
+        again = tg.nn.norm_rotary(q, k, pos, freqs, norm=norm, eps=eps, sections=sections,
+                                  interleaved=interleaved, **weights)
+    assert all(torch.equal(a, b) for a, b in zip(outs, again))
+    leaves = (q, k, *w) if norm else (q, k)
+    grads = torch.autograd.grad(outs, leaves, dy)
+    angle = want.angles(pos.cpu().numpy(), freqs.cpu().numpy(), sections)
+    half = torch.finfo(dtype).eps / 2
+    # Angles in 64 bits: one rounding of 2^-53 of the angle in the oracle's product,
+    # three in the kernel's (the product, 1 / 2 pi and the product with it).
+    turn = 4 * 2.0 ** -53 * (np.abs(angle).max() if angle.size else 0.0)
+    for i, (x, h) in enumerate(((q, hq), (k, hk))):
+        assert outs[i].dtype == dtype and grads[i].dtype == dtype
+        xw, xx, xd = f64(w[i]) if norm else None, f64(x), f64(dy[i])
+        exp = want.norm_rotary(xx, xw, angle, eps, norm, interleaved)
+        dx, dw = want.norm_rotary_grad(xx, xw, angle, eps, norm, interleaved, xd)
+        if exp.size == 0:
+            continue
+        # Half a step of the result, and of the some 16 fp32 operations on the way
+        # (products, a sine to 4 half steps, the mean of D squares in D / 16 + 4
+        # additions a lane) that each move a value of the row's largest size.
+        ops = 24 + D / 16
+        assert (np.abs(f64(outs[i]) - exp) <= half * np.abs(exp) + (ops * F32 + turn) *
+                np.abs(exp).max(-1, keepdims=True) * 2).all()
+        big = np.abs(dx).max(-1, keepdims=True)
+        r = 1 / np.sqrt((xx ** 2).mean(-1, keepdims=True) + eps) if norm else 1.0
+        # dx = r (h - n mean(h n)): both terms may be larger than their difference.
+        hn = np.abs(xd).max(-1, keepdims=True) * 2 * (np.abs(xw).max() if norm else 1) * r * \
+            (1 + (np.abs(xx) * r).max(-1, keepdims=True) ** 2 if norm else 1)
+        assert (np.abs(f64(grads[i]) - dx) <= half * np.abs(dx) + (ops * F32 + turn) *
+                (big + hn)).all()
+        if norm:
+            # n * heads terms, added in fp32 by lanes, waves and workgroups; the
+            # sum of the terms' sizes bounds what the roundings of all levels move.
+            g = want.rotate(xd, angle, interleaved, -1.0)
+            size = (np.abs(g) * np.abs(xx * r)).sum((0, 1))
+            depth = min(n * h, 4096) / 4 + n * h / 4096 + 64
+            got, whalf = f64(grads[2 + i]), torch.finfo(w[i].dtype).eps / 2
+            assert (np.abs(got - dw) <= whalf * np.abs(dw) + ((ops + depth) * F32 + turn) *
+                    2 * size).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("D,sections", [
+    (32, (16,)), (64, (32,)), (64, (16,)), (80, (40,)), (96, (16, 16, 16)), (128, (64,)),
+    (128, (16, 24, 24)), (192, (96,)), (256, (128,)), (256, (24, 40)), (128, (0,)),
+    (4, (2,)), (20, (4, 2)), (100, (50,)), (64, (10,)), (132, (20, 2, 10, 4))])
+def test_forward_and_gradients(dtype, interleaved, D, sections):
+    check(37, 5, 2, D, sections, TYPES[dtype], interleaved=interleaved)
+
+
+@pytest.mark.parametrize("n", [0, 1, 2, 3, 63, 4095, 4097])
+def test_token_counts(n):
+    check(n, 6, 2, 64, (32,), torch.bfloat16)
+    check(n, 3, 1, 20, (10,), torch.float32)
+
+
+@pytest.mark.parametrize("hq,hk", [(1, 1), (8, 0), (32, 8), (7, 13)])
+def test_head_counts(hq, hk):
+    check(65, hq, hk, 128, (64,), torch.bfloat16)
+    check(65, hq, hk, 128, (64,), torch.float16, norm=False, interleaved=True)
+
+
+def test_other_forms():
+    check(33, 3, 2, 64, (32,), torch.bfloat16, wdtype=torch.float32)
+    check(33, 3, 2, 64, (32,), torch.float32, wdtype=torch.bfloat16)
+    check(33, 3, 2, 64, (32,), torch.float16, bits=32)
+    check(33, 3, 2, 64, (8, 8, 8, 8), torch.float32, far=2 ** 40, eps=0.0)
+
+
+def test_rows_on_odd_addresses_and_query_alone():
+    q, k, w, pos, freqs, dy = make(9, 4, 2, 64, (32,), torch.bfloat16)
+    outs = tg.nn.norm_rotary(q, k, pos, freqs, query_weight=w[0], key_weight=w[1])
+    for shift in (1, 2):
+        odd = torch.zeros(9 * 4 * 80 + shift, device=DEV, dtype=torch.bfloat16)
+        view = torch.as_strided(odd, (9, 4, 64), (4 * 80, 80, 1), shift).copy_(q.detach())
+        got = tg.nn.norm_rotary(view, k, pos, freqs, query_weight=w[0], key_weight=w[1])
+        assert (got[0] - outs[0]).abs().max() <= outs[0].abs().max() * 2.0 ** -8
+    across = q.detach().transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(tg.nn.norm_rotary(across, None, pos[:, 0], freqs, query_weight=w[0]),
+                       outs[0])
+    wide = q.detach().transpose(1, 2).contiguous().transpose(1, 2)   # width not dense
+    assert torch.equal(tg.nn.norm_rotary(wide, None, pos, freqs, query_weight=w[0]), outs[0])
+    # Gradients where only some are wanted, or the output's is missing or expanded.
+    part = tg.nn.norm_rotary(q, k.detach(), pos, freqs, query_weight=w[0].detach(),
+                             key_weight=w[1])
+    full = tg.nn.norm_rotary(q, k, pos, freqs, query_weight=w[0], key_weight=w[1])
+    one = torch.ones((), device=DEV, dtype=torch.bfloat16).expand_as(part[0])
+    a = torch.autograd.grad(part[0], (q, w[1]), one, allow_unused=True)
+    b = torch.autograd.grad(full, (q, w[1]), (one.contiguous(), torch.zeros_like(part[1])))
+    assert torch.equal(a[0], b[0]) and (a[1] is None or not a[1].any())
+
+
+def test_what_no_kernel_covers():
+    q = torch.randn(3, 2, 6, device=DEV)
+    pos, freqs = torch.arange(3, device=DEV), torch.ones(3, device=DEV)
+    with pytest.raises(RuntimeError, match="no HIP kernel"):
+        tg.nn.norm_rotary(q, None, pos, freqs)
+    tg.config.strict = False
+    got = tg.nn.norm_rotary(q, None, pos, freqs)
+    exp = tg.nn.norm_rotary(q.cpu(), None, pos.cpu(), freqs.cpu())
+    assert (got.cpu() - exp).abs().max() <= 16 * F32 * exp.abs().max()
+
+
+def test_captured_forward_and_backward_replay_on_new_values():
+    q, k, w, pos, freqs, dy = make(50, 4, 2, 128, (64,), torch.bfloat16)
+    call = lambda: tg.nn.norm_rotary(q, k, pos, freqs, query_weight=w[0], key_weight=w[1])
+
+    def both():
+        outs = call()
+        return (*outs, *torch.autograd.grad(outs, (q, k, *w), dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        static = both()
+    for step in range(4):
+        with torch.no_grad():
+            for t in (q, k, *dy):
+                t.mul_(-1.25)
+            pos.add_(3)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(static, both()):
+            assert torch.equal(a, b)
+
+
+def test_training_attention_on_normed_and_rotated_fields():
+    """norm_rotary into varlen attention and back: the gradients of its inputs
+    from the attention's own, by the formula."""
+    class Attention(tg.MessagePassing):
+        reducer = tg.online_softmax()
+
+        def edge(self, src, dst, edge, scale):
+            return self.reducer((src.key * dst.query).sum(dim=-1) * scale, src.value)
+
+    lengths, H, D = [40, 1, 90], 2, 64
+    n = sum(lengths)
+    q, k, w, _, freqs, dy = make(n, H, H, D, (32,), torch.float16)
+    pos = torch.cat([torch.arange(l, device=DEV) for l in lengths])
+    v = torch.randn(n, H, D, device=DEV).half()
+    graph = tg.Graph.cat([tg.Graph.triangular(l, device=DEV) for l in lengths])
+    qr, kr = tg.nn.norm_rotary(q, k, pos, freqs, query_weight=w[0], key_weight=w[1])
+    kernel = Attention()
+    out = kernel(graph=graph, src={"key": kr, "value": v}, dst={"query": qr}, scale=D ** -0.5)
+    assert kernel.last_variant.pattern == "block-attention"
+    mid = torch.autograd.grad(out, (qr, kr), dy[0], retain_graph=True)
+    got = torch.autograd.grad(out, (q, k, *w), dy[0])
+    angle = want.angles(pos.cpu().numpy()[:, None], freqs.cpu().numpy(), (32,))
+    for i, x in enumerate((q, k)):
+        dx, dw = want.norm_rotary_grad(f64(x), f64(w[i]), angle, 1e-6, True, False, f64(mid[i]))
+        # (As in `check`, relative to the largest value.)
+        assert np.abs(f64(got[i]) - dx).max() <= (2.0 ** -11 + 200 * F32) * np.abs(dx).max()
+        assert np.abs(f64(got[2 + i]) - dw).max() <= (2.0 ** -11 + 200 * F32) * np.abs(dw).max()

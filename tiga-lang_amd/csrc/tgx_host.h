@@ -33,6 +33,10 @@ namespace tgx {
     }                                                                  \
   } while (0)
 
+// Workgroups of 256 threads that one launch dimension can count (the grid's
+// threads are a 32-bit number).
+constexpr int64_t kMaxBlocks256 = (int64_t{1} << 24) - 1;
+
 inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
 

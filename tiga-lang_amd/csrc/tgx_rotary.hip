@@ -1,0 +1,562 @@
+// RMS norm of every head's query or key and the rotation by its token's
+// positions, in one pass, with gradients (tg.nn.norm_rotary).
+//
+// For a row x of D values (one token, one head), with n_freqs = R / 2:
+//
+//   r = (mean_d x_d^2 + eps)^(-1/2),  n = r x,  u = w n      (norm; else u = x)
+//   theta_i = position[axis(i)] * frequency_i                 i < R / 2
+//   y_a = u_a cos theta_i - u_b sin theta_i
+//   y_b = u_b cos theta_i + u_a sin theta_i                   (a, b) the i-th pair
+//
+// pairs are (i, i + R / 2), or (2 i, 2 i + 1) when interleaved; values from R
+// on are not rotated.  With g the pairs of dy rotated back:
+//
+//   dw = sum over tokens and heads of g n,   h = w g,
+//   dx = r (h - n mean_d(h_d n_d))
+//
+// All of it in fp32 but the angle, which is reduced in fp64: at position 10^6
+// an fp32 angle is off by 0.03.
+//
+// Bound: x is read and y written once (backward: x and dy read, dx written)
+// against some 20 operations a value: memory.  A lane holds one chunk of each
+// half of the pairs (2 N values), LPR lanes a row, a wave 64 / LPR rows; the
+// sines of a token are formed once for all of its rows in the wave.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "tgx_device.h"
+#include "tgx_host.h"
+#include "tgx_profile.h"
+#include "tgx_vals.h"
+
+namespace tgx {
+namespace {
+
+struct RotaryArgs {
+  const void* x[2];         // queries, keys
+  int64_t xs_token[2], xs_head[2];
+  const void* dy[2];        // backward: contiguous [tokens, heads, D]
+  void* out[2];             // y, or dx: contiguous
+  const void* w[2];         // [D], null: ones
+  int heads[2];
+  const void* positions;    // [tokens, axes]
+  int wide_positions;       // int64, else int32
+  int axes;
+  int ends[4];              // frequencies before the end of each axis
+  const float* freqs;
+  int half;                 // R / 2
+  int64_t tokens;
+  int split;                // waves that share a token's rows
+  int D;
+  float eps;
+  int norm;
+  int w_dtype;
+  float* partial;           // backward: [workgroup, 2, D] sums of g n; null: not wanted
+};
+
+template <int DT, int N>
+struct Chunk;
+template <int DT>
+struct Chunk<DT, 8> {
+  using V = Vals<DT, 8>;
+  using T = typename V::T;
+  using Raw = typename V::Raw;
+  static __device__ __forceinline__ Raw load(const T* p) { return V::load(p); }
+  static __device__ __forceinline__ void unpack(const Raw& r, float (&f)[8]) { V::unpack(r, f); }
+  static __device__ __forceinline__ void store(T* p, const float (&f)[8]) { V::store(p, f); }
+};
+template <>
+struct Chunk<TGX_DTYPE_F32, 2> {
+  using T = float;
+  typedef float Raw __attribute__((ext_vector_type(2)));
+  static __device__ __forceinline__ Raw load(const T* p) {
+    return *reinterpret_cast<const Raw*>(p);
+  }
+  static __device__ __forceinline__ void unpack(Raw r, float (&f)[2]) {
+    f[0] = r[0];
+    f[1] = r[1];
+  }
+  static __device__ __forceinline__ void store(T* p, const float (&f)[2]) {
+    *reinterpret_cast<Raw*>(p) = Raw{f[0], f[1]};
+  }
+};
+template <>
+struct Chunk<TGX_DTYPE_BF16, 2> {
+  using T = uint16_t;
+  using Raw = uint32_t;
+  static __device__ __forceinline__ Raw load(const T* p) {
+    return *reinterpret_cast<const uint32_t*>(p);
+  }
+  static __device__ __forceinline__ void unpack(Raw r, float (&f)[2]) {
+    f[0] = bf16_lo(r);
+    f[1] = bf16_hi(r);
+  }
+  static __device__ __forceinline__ void store(T* p, const float (&f)[2]) {
+    *reinterpret_cast<uint32_t*>(p) = pack_bf16x2(f[0], f[1]);
+  }
+};
+template <>
+struct Chunk<TGX_DTYPE_F16, 2> {
+  using T = uint16_t;
+  using Raw = uint32_t;
+  static __device__ __forceinline__ Raw load(const T* p) {
+    return *reinterpret_cast<const uint32_t*>(p);
+  }
+  static __device__ __forceinline__ void unpack(Raw r, float (&f)[2]) { f16_pair(r, f[0], f[1]); }
+  static __device__ __forceinline__ void store(T* p, const float (&f)[2]) {
+    *reinterpret_cast<uint32_t*>(p) = pack_f16x2(f[0], f[1]);
+  }
+};
+
+__device__ __forceinline__ float scalar_value(const void* p, int dtype, int i) {
+  if (dtype == TGX_DTYPE_F32) return static_cast<const float*>(p)[i];
+  const uint16_t u = static_cast<const uint16_t*>(p)[i];
+  return dtype == TGX_DTYPE_BF16 ? bf16_lo(u) : static_cast<float>(__builtin_bit_cast(_Float16, u));
+}
+__device__ __forceinline__ void store_scalar(void* p, int dtype, int i, float v) {
+  if (dtype == TGX_DTYPE_F32) static_cast<float*>(p)[i] = v;
+  else if (dtype == TGX_DTYPE_BF16)
+    static_cast<uint16_t*>(p)[i] = static_cast<uint16_t>(f32_to_bf16_bits(v));
+  else static_cast<_Float16*>(p)[i] = static_cast<_Float16>(v);
+}
+
+// Where a lane's two chunks of a row are, and which pairs they make: pair j
+// of the chunks is frequency N * part + j.
+template <int N, bool INTER>
+struct Place {
+  int first, second;   // columns of the chunks
+  bool has;
+  __device__ __forceinline__ Place(const RotaryArgs& a, int part) {
+    has = 2 * N * part < a.D;
+    if (INTER || N * part >= a.half) {
+      // Adjacent pairs, or the columns that are not rotated.
+      first = 2 * N * part;
+      second = first + N;
+    } else {
+      first = N * part;
+      second = a.half + N * part;
+    }
+  }
+};
+
+// cos and sin of the token's angle for the lane's N pairs; pairs past the
+// rotated ones turn by nothing.
+template <int N>
+__device__ __forceinline__ void turns(const RotaryArgs& a, int64_t token, int part,
+                                      const float (&freq)[N], float (&c)[N], float (&s)[N]) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int i = N * part + j;
+    if (i >= a.half) {
+      c[j] = 1.f;
+      s[j] = 0.f;
+      continue;
+    }
+    const int axis = (i >= a.ends[0]) + (i >= a.ends[1]) + (i >= a.ends[2]);
+    const int64_t at = token * a.axes + axis;
+    const double pos = a.wide_positions
+                           ? static_cast<double>(static_cast<const int64_t*>(a.positions)[at])
+                           : static_cast<double>(static_cast<const int32_t*>(a.positions)[at]);
+    // The angle in half turns, without the whole turns; what its fp32 value
+    // leaves is put back to first order.
+    const double t = pos * static_cast<double>(freq[j]) * 0.15915494309189535;
+    const double u = 2.0 * (t - __builtin_rint(t));
+    const float uf = static_cast<float>(u);
+    const float rest = static_cast<float>((u - static_cast<double>(uf)) * 3.141592653589793);
+    float sn, cs;
+    sincospif(uf, &sn, &cs);
+    c[j] = fmaf(-sn, rest, cs);
+    s[j] = fmaf(cs, rest, sn);
+  }
+}
+
+// Turns pair j of the chunks (f, g) by (c, s): the halves of the pairs lie in
+// f and g, or next to each other.
+template <int N, bool INTER>
+__device__ __forceinline__ void rotate(float (&f)[N], float (&g)[N], const float (&c)[N],
+                                       const float (&s)[N], float sign) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    float* pa = INTER ? (j < N / 2 ? &f[2 * j] : &g[2 * j - N]) : &f[j];
+    float* pb = INTER ? pa + 1 : &g[j];
+    const float a = *pa, b = *pb, sj = sign * s[j];
+    *pa = a * c[j] - b * sj;
+    *pb = b * c[j] + a * sj;
+  }
+}
+
+template <int N>
+struct Weights {
+  float f[2][N], g[2][N];
+  template <bool INTER>
+  __device__ __forceinline__ void load(const RotaryArgs& a, const Place<N, INTER>& at) {
+#pragma unroll
+    for (int side = 0; side < 2; ++side)
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const bool have = a.norm && a.w[side] && at.has;
+        f[side][j] = have ? scalar_value(a.w[side], a.w_dtype, at.first + j) : 1.f;
+        g[side][j] = have ? scalar_value(a.w[side], a.w_dtype, at.second + j) : 1.f;
+      }
+  }
+};
+
+template <int DT, int N, int LPR, bool INTER>
+__global__ __launch_bounds__(256) void norm_rotary_fwd_kernel(RotaryArgs a) {
+  using C = Chunk<DT, N>;
+  using T = typename C::T;
+  const int lane = lane_id(), part = lane % LPR, sub = lane / LPR;
+  const Place<N, INTER> at(a, part);
+  Weights<N> w;
+  w.load(a, at);
+  float freq[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) freq[j] = N * part + j < a.half ? a.freqs[N * part + j] : 0.f;
+  const int rows = a.heads[0] + a.heads[1];
+  const int64_t items = a.tokens * a.split;
+  const float inv_d = 1.f / static_cast<float>(a.D);
+  for (int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); item < items;
+       item += static_cast<int64_t>(gridDim.x) * 4) {
+    const int64_t token = item / a.split;
+    float c[N], s[N];
+    turns<N>(a, token, part, freq, c, s);
+    for (int row = static_cast<int>(item % a.split) * (64 / LPR) + sub; row < rows;
+         row += a.split * (64 / LPR)) {
+      const int side = row >= a.heads[0];
+      const int head = row - (side ? a.heads[0] : 0);
+      const T* x = static_cast<const T*>(a.x[side]) + token * a.xs_token[side] +
+                   head * a.xs_head[side];
+      float f[N], g[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) f[j] = g[j] = 0.f;
+      if (at.has) {
+        C::unpack(C::load(x + at.first), f);
+        C::unpack(C::load(x + at.second), g);
+      }
+      if (a.norm) {
+        float ss = 0.f;
+#pragma unroll
+        for (int j = 0; j < N; ++j) ss += f[j] * f[j] + g[j] * g[j];
+        const float r = 1.f / sqrtf(group_sum<LPR>(ss) * inv_d + a.eps);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          f[j] *= r * (side ? w.f[1][j] : w.f[0][j]);
+          g[j] *= r * (side ? w.g[1][j] : w.g[0][j]);
+        }
+      }
+      rotate<N, INTER>(f, g, c, s, 1.f);
+      if (at.has) {
+        T* y = static_cast<T*>(a.out[side]) + (token * a.heads[side] + head) * a.D;
+        C::store(y + at.first, f);
+        C::store(y + at.second, g);
+      }
+    }
+  }
+}
+
+template <int DT, int N, int LPR, bool INTER>
+__global__ __launch_bounds__(256) void norm_rotary_bwd_kernel(RotaryArgs a) {
+  using C = Chunk<DT, N>;
+  using T = typename C::T;
+  const int lane = lane_id(), part = lane % LPR, sub = lane / LPR;
+  const Place<N, INTER> at(a, part);
+  Weights<N> w;
+  w.load(a, at);
+  float freq[N];
+  float wf[2][N], wg[2][N];   // sums of g n
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    freq[j] = N * part + j < a.half ? a.freqs[N * part + j] : 0.f;
+    wf[0][j] = wf[1][j] = wg[0][j] = wg[1][j] = 0.f;
+  }
+  const int64_t items = a.tokens * a.split;
+  const float inv_d = 1.f / static_cast<float>(a.D);
+  for (int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); item < items;
+       item += static_cast<int64_t>(gridDim.x) * 4) {
+    const int64_t token = item / a.split;
+    float c[N], s[N];
+    turns<N>(a, token, part, freq, c, s);
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+      for (int head = static_cast<int>(item % a.split) * (64 / LPR) + sub; head < a.heads[side];
+           head += a.split * (64 / LPR)) {
+        const T* x = static_cast<const T*>(a.x[side]) + token * a.xs_token[side] +
+                     head * a.xs_head[side];
+        const int64_t flat = (token * a.heads[side] + head) * a.D;
+        const T* dy = static_cast<const T*>(a.dy[side]) + flat;
+        float f[N], g[N], df[N], dg[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) f[j] = g[j] = df[j] = dg[j] = 0.f;
+        if (at.has) {
+          C::unpack(C::load(x + at.first), f);
+          C::unpack(C::load(x + at.second), g);
+          C::unpack(C::load(dy + at.first), df);
+          C::unpack(C::load(dy + at.second), dg);
+        }
+        rotate<N, INTER>(df, dg, c, s, -1.f);
+        if (a.norm) {
+          float ss = 0.f;
+#pragma unroll
+          for (int j = 0; j < N; ++j) ss += f[j] * f[j] + g[j] * g[j];
+          const float r = 1.f / sqrtf(group_sum<LPR>(ss) * inv_d + a.eps);
+          float hn = 0.f;
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            f[j] *= r;
+            g[j] *= r;
+            wf[side][j] += df[j] * f[j];
+            wg[side][j] += dg[j] * g[j];
+            df[j] *= w.f[side][j];
+            dg[j] *= w.g[side][j];
+            hn += df[j] * f[j] + dg[j] * g[j];
+          }
+          hn = group_sum<LPR>(hn) * inv_d;
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            df[j] = r * (df[j] - f[j] * hn);
+            dg[j] = r * (dg[j] - g[j] * hn);
+          }
+        }
+        if (at.has) {
+          T* dx = static_cast<T*>(a.out[side]) + flat;
+          C::store(dx + at.first, df);
+          C::store(dx + at.second, dg);
+        }
+      }
+    }
+  }
+  if (!a.partial) return;
+  // The rows of a wave, then the four waves, in a fixed order.
+  __shared__ float sums[4][2][2 * N * LPR];
+#pragma unroll
+  for (int side = 0; side < 2; ++side)
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+#pragma unroll
+      for (int mask = LPR; mask < 64; mask <<= 1) {
+        wf[side][j] += __shfl_xor(wf[side][j], mask, 64);
+        wg[side][j] += __shfl_xor(wg[side][j], mask, 64);
+      }
+      if (sub == 0 && at.has) {
+        sums[threadIdx.x >> 6][side][at.first + j] = wf[side][j];
+        sums[threadIdx.x >> 6][side][at.second + j] = wg[side][j];
+      }
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * a.D; i += 256) {
+    const int side = i / a.D, d = i % a.D;
+    a.partial[static_cast<int64_t>(blockIdx.x) * 2 * a.D + i] =
+        (sums[0][side][d] + sums[1][side][d]) + (sums[2][side][d] + sums[3][side][d]);
+  }
+}
+
+// dw[side][d] = sum over the workgroups of the backward, one wave per (side, d).
+__global__ __launch_bounds__(256) void norm_rotary_dw_kernel(const float* partial, int blocks,
+                                                             int D, int dtype, void* dwq,
+                                                             void* dwk) {
+  const int i = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (i >= 2 * D) return;
+  float s = 0.f;
+  for (int b = lane_id(); b < blocks; b += 64) s += partial[static_cast<int64_t>(b) * 2 * D + i];
+  s = group_sum<64>(s);
+  void* out = i < D ? dwq : dwk;
+  if (lane_id() == 0 && out) store_scalar(out, dtype, i % D, s);
+}
+
+bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+constexpr int64_t kBwdBlocks = 1024;
+
+// Waves that share a token's rows: with few tokens, so many that the rows of a
+// token do not queue behind each other.
+int rows_split(const tgx_norm_rotary& p, int rows_per_wave) {
+  const int passes = (std::max(p.heads[0], 1) + p.heads[1] + rows_per_wave - 1) / rows_per_wave;
+  if (p.n_tokens >= 4096) return 1;
+  return static_cast<int>(std::max<int64_t>(
+      1, std::min<int64_t>(passes, 4096 / std::max<int64_t>(p.n_tokens, 1))));
+}
+
+struct Form {
+  int n;     // values a chunk
+  int lpr;   // lanes a row
+};
+
+Form form_of(const tgx_norm_rotary& p, bool wide) {
+  // Chunks of 8 values where the pairs divide into them and every row starts
+  // on 16 bytes, of 2 elsewhere.
+  const bool eight = wide && p.D % 16 == 0 && (p.interleaved || p.n_freqs % 8 == 0);
+  if (!eight) return Form{2, 64};
+  const int lanes = p.D / 16;
+  return Form{8, lanes <= 2 ? 2 : lanes <= 4 ? 4 : lanes <= 8 ? 8 : 16};
+}
+
+int check(const tgx_norm_rotary* p) {
+  TGX_REQUIRE(p != nullptr, "null operands");
+  TGX_REQUIRE(dtype_bytes(p->dtype) != 0 && dtype_bytes(p->w_dtype) != 0, "unknown dtype");
+  TGX_REQUIRE(p->n_tokens >= 0 && p->heads[0] >= 0 && p->heads[1] >= 0, "negative sizes");
+  if (p->D < 4 || p->D > 256 || p->D % 4 || p->n_freqs % 2) {
+    set_error("head width %d with %d frequencies: norm_rotary takes widths that are multiples of "
+              "4 up to 256 and an even number of frequencies", p->D, p->n_freqs);
+    return TGX_UNSUPPORTED;
+  }
+  TGX_REQUIRE(p->n_freqs >= 0 && 2 * p->n_freqs <= p->D, "more frequencies than pairs");
+  TGX_REQUIRE(p->axes >= 1 && p->axes <= 4, "1 to 4 position axes");
+  int total = 0;
+  for (int i = 0; i < p->axes; ++i) {
+    TGX_REQUIRE(p->sections[i] >= 0, "negative section");
+    total += p->sections[i];
+  }
+  TGX_REQUIRE(total == p->n_freqs, "sections cover %d of %d frequencies", total, p->n_freqs);
+  TGX_REQUIRE(p->n_tokens == 0 || p->n_freqs == 0 || (p->positions_dev && p->freqs_dev),
+              "null positions or frequencies");
+  TGX_REQUIRE(p->positions_bits == 32 || p->positions_bits == 64, "positions are 32 or 64 bits");
+  for (int i = 0; i < 2; ++i)
+    TGX_REQUIRE(p->n_tokens == 0 || p->heads[i] == 0 || p->x_dev[i], "null input");
+  return TGX_OK;
+}
+
+// Fills the kernels' arguments; `wide`: all rows on 16 bytes (else on two values).
+int args_of(const tgx_norm_rotary& p, void* const out[2], const void* const dy[2], RotaryArgs* a,
+            bool* wide) {
+  const int size = dtype_bytes(p.dtype);
+  *wide = true;
+  for (int i = 0; i < 2; ++i) {
+    if (p.heads[i] == 0 || p.n_tokens == 0) continue;
+    TGX_REQUIRE(out[i] && (!dy || dy[i]), "null output or gradient");
+    const void* ptrs[3] = {p.x_dev[i], out[i], dy ? dy[i] : out[i]};
+    for (const void* q : ptrs) {
+      TGX_REQUIRE(aligned(q, 2 * size), "rows must start on two values");
+      *wide = *wide && aligned(q, 16);
+    }
+    TGX_REQUIRE(p.token_stride[i] % 2 == 0 && p.head_stride[i] % 2 == 0,
+                "rows must start on two values");
+    *wide = *wide && p.token_stride[i] * size % 16 == 0 && p.head_stride[i] * size % 16 == 0 &&
+            p.D * size % 16 == 0;
+    a->x[i] = p.x_dev[i];
+    a->xs_token[i] = p.token_stride[i];
+    a->xs_head[i] = p.head_stride[i];
+    a->out[i] = out[i];
+    a->dy[i] = dy ? dy[i] : nullptr;
+  }
+  int end = 0;
+  for (int i = 0; i < 4; ++i) {
+    end += i < p.axes ? p.sections[i] : 0;
+    // Axes past the last never start.
+    a->ends[i] = i + 1 < p.axes ? end : 1 << 30;
+  }
+  for (int i = 0; i < 2; ++i) {
+    a->w[i] = p.w_dev[i];
+    a->heads[i] = p.heads[i];
+  }
+  a->positions = p.positions_dev;
+  a->wide_positions = p.positions_bits == 64;
+  a->axes = p.axes;
+  a->freqs = p.freqs_dev;
+  a->half = p.n_freqs;
+  a->tokens = p.n_tokens;
+  a->D = p.D;
+  a->eps = p.eps;
+  a->norm = p.norm;
+  a->w_dtype = p.w_dtype;
+  return TGX_OK;
+}
+
+template <bool BWD, int DT, int N, int LPR>
+int launch(RotaryArgs a, bool inter, int64_t blocks, hipStream_t stream) {
+  const dim3 grid(static_cast<uint32_t>(blocks)), block(256);
+  if constexpr (BWD) {
+    TGX_PROFILE("norm_rotary_bwd", stream);
+    if (inter) norm_rotary_bwd_kernel<DT, N, LPR, true><<<grid, block, 0, stream>>>(a);
+    else norm_rotary_bwd_kernel<DT, N, LPR, false><<<grid, block, 0, stream>>>(a);
+  } else {
+    TGX_PROFILE("norm_rotary_fwd", stream);
+    if (inter) norm_rotary_fwd_kernel<DT, N, LPR, true><<<grid, block, 0, stream>>>(a);
+    else norm_rotary_fwd_kernel<DT, N, LPR, false><<<grid, block, 0, stream>>>(a);
+  }
+  TGX_LAUNCHED(BWD ? "norm_rotary_bwd" : "norm_rotary_fwd");
+  return TGX_OK;
+}
+
+template <bool BWD, int DT>
+int by_form(const RotaryArgs& a, Form f, bool inter, int64_t blocks, hipStream_t s) {
+  if (f.n == 2) return launch<BWD, DT, 2, 64>(a, inter, blocks, s);
+  switch (f.lpr) {
+    case 2: return launch<BWD, DT, 8, 2>(a, inter, blocks, s);
+    case 4: return launch<BWD, DT, 8, 4>(a, inter, blocks, s);
+    case 8: return launch<BWD, DT, 8, 8>(a, inter, blocks, s);
+    default: return launch<BWD, DT, 8, 16>(a, inter, blocks, s);
+  }
+}
+
+template <bool BWD>
+int run(const tgx_norm_rotary& p, RotaryArgs a, bool wide, int64_t max_blocks, hipStream_t s) {
+  const Form f = form_of(p, wide);
+  a.split = rows_split(p, 64 / f.lpr);
+  const int64_t blocks = std::min(max_blocks, ceil_div(p.n_tokens * a.split, 4));
+  switch (p.dtype) {
+    case TGX_DTYPE_BF16: return by_form<BWD, TGX_DTYPE_BF16>(a, f, p.interleaved, blocks, s);
+    case TGX_DTYPE_F16: return by_form<BWD, TGX_DTYPE_F16>(a, f, p.interleaved, blocks, s);
+    default: return by_form<BWD, TGX_DTYPE_F32>(a, f, p.interleaved, blocks, s);
+  }
+}
+
+}  // namespace
+}  // namespace tgx
+
+using namespace tgx;
+
+extern "C" int tgx_norm_rotary_fwd(const tgx_norm_rotary* p, void* query_out_dev,
+                                   void* key_out_dev, void* stream) {
+  if (int st = check(p)) return st;
+  if (p->n_tokens == 0 || p->heads[0] + p->heads[1] == 0) return TGX_OK;
+  void* const out[2] = {query_out_dev, key_out_dev};
+  RotaryArgs a{};
+  bool wide = true;
+  if (int st = args_of(*p, out, nullptr, &a, &wide)) return st;
+  return run<false>(*p, a, wide, int64_t{1} << 20, as_stream(stream));
+}
+
+extern "C" int tgx_norm_rotary_bwd_workspace(const tgx_norm_rotary* p, size_t* bytes) {
+  TGX_REQUIRE(bytes != nullptr, "null bytes");
+  if (int st = check(p)) return st;
+  *bytes = sizeof(float) * kBwdBlocks * 2 * p->D;
+  return TGX_OK;
+}
+
+extern "C" int tgx_norm_rotary_bwd(const tgx_norm_rotary* p, const void* dquery_out_dev,
+                                   const void* dkey_out_dev, void* dquery_dev, void* dkey_dev,
+                                   void* dquery_weight_dev, void* dkey_weight_dev,
+                                   void* workspace_dev, size_t workspace_bytes, void* stream) {
+  if (int st = check(p)) return st;
+  const bool weights = p->norm && (dquery_weight_dev || dkey_weight_dev);
+  const bool work = p->n_tokens > 0 && p->heads[0] + p->heads[1] > 0;
+  if (!work && !weights) return TGX_OK;
+  void* const out[2] = {dquery_dev, dkey_dev};
+  const void* const dy[2] = {dquery_out_dev, dkey_out_dev};
+  RotaryArgs a{};
+  bool wide = true;
+  if (int st = args_of(*p, out, dy, &a, &wide)) return st;
+  const int64_t max_blocks = kBwdBlocks;
+  const Form f = form_of(*p, wide);
+  const int64_t blocks =
+      work ? std::min(max_blocks, ceil_div(p->n_tokens * rows_split(*p, 64 / f.lpr), 4)) : 0;
+  if (weights) {
+    TGX_REQUIRE(workspace_dev && workspace_bytes >= sizeof(float) * blocks * 2 * p->D,
+                "workspace too small");
+    a.partial = static_cast<float*>(workspace_dev);
+  }
+  if (work)
+    if (int st = run<true>(*p, a, wide, max_blocks, as_stream(stream))) return st;
+  if (weights) {
+    {
+      TGX_PROFILE("norm_rotary_dw", as_stream(stream));
+      norm_rotary_dw_kernel<<<dim3(static_cast<uint32_t>(ceil_div(2 * p->D, 4))), dim3(256), 0,
+                              as_stream(stream)>>>(a.partial, static_cast<int>(blocks), p->D,
+                                                   p->w_dtype, dquery_weight_dev,
+                                                   dkey_weight_dev);
+    }
+    TGX_LAUNCHED("norm_rotary_dw");
+  }
+  return TGX_OK;
+}

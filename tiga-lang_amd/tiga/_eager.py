@@ -48,8 +48,13 @@ def reduce_online_softmax(reducer: OnlineSoftmaxReducer, item: OnlineSoftmaxItem
                          "[edges, *lanes, *payload]")
     if score.shape[0] != destination.numel() or value.shape[0] != score.shape[0]:
         raise ValueError("online_softmax score/value leading dimension must be edges")
-    if tuple(value.shape[1:score.ndim]) != tuple(score.shape[1:]):
-        raise ValueError("online_softmax value must begin with the score lane dimensions")
+    lane_dims = tuple(value.shape[1:score.ndim])
+    if lane_dims != tuple(score.shape[1:]):
+        # A value of width 1 in a lane dimension is shared by its lanes
+        # (query heads grouped on one key head).
+        if any(v not in (1, s) for v, s in zip(lane_dims, score.shape[1:])):
+            raise ValueError("online_softmax value must begin with the score lane dimensions")
+        value = value.expand(*score.shape, *value.shape[score.ndim:])
     if not score.is_floating_point() or not value.is_floating_point():
         raise TypeError("online_softmax score and value must be floating point")
     acc = _accumulation_dtype(reducer, score)

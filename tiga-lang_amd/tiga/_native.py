@@ -10,6 +10,7 @@ implementation when it is missing.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from pathlib import Path
@@ -51,6 +52,27 @@ class EdgeMlp(ctypes.Structure):
                 ("seg_stride", ctypes.c_int64 * 4), ("seg_dev", c_vp * 4),
                 ("out_width", ctypes.c_int32 * 3), ("act_param2", ctypes.c_float * 3),
                 ("norm", ctypes.c_int32 * 3), ("norm_eps", ctypes.c_float * 3)]
+
+
+class Paged(ctypes.Structure):
+    """Mirror of ``tgx_paged``."""
+
+    _fields_ = [("page_table_dev", c_vp), ("seq_stride", c_i64), ("head_stride", c_i64),
+                ("lengths_dev", c_vp), ("n_seqs", c_i64), ("table_heads", ctypes.c_int32),
+                ("pages_per_seq", ctypes.c_int32), ("page_size", ctypes.c_int32),
+                ("num_pages", c_i64), ("queries", ctypes.c_int32)]
+
+
+class NormRotary(ctypes.Structure):
+    """Mirror of ``tgx_norm_rotary``."""
+
+    _fields_ = [("x_dev", c_vp * 2), ("token_stride", c_i64 * 2), ("head_stride", c_i64 * 2),
+                ("heads", ctypes.c_int32 * 2), ("w_dev", c_vp * 2), ("w_dtype", ctypes.c_int32),
+                ("positions_dev", c_vp), ("positions_bits", ctypes.c_int32),
+                ("axes", ctypes.c_int32), ("sections", ctypes.c_int32 * 4),
+                ("freqs_dev", c_vp), ("n_freqs", ctypes.c_int32), ("norm", ctypes.c_int32),
+                ("interleaved", ctypes.c_int32), ("eps", c_f32), ("n_tokens", c_i64),
+                ("D", ctypes.c_int32), ("dtype", ctypes.c_int32)]
 
 
 # tgx_abi_version() of the library these signatures and structs mirror.
@@ -147,6 +169,18 @@ _SIGNATURES: dict[str, list] = {
                                        c_vp, c_vp],
     "tgx_segment_softmax_sum_fwd": [c_vp, c_vp, c_int, c_i64, c_vp, c_int, c_f32, c_vp, c_int,
                                     c_vp, c_vp, c_vp, c_vp],
+    "tgx_paged_attn_workspace": [P(Paged), c_int, c_int, c_int, c_int, P(c_size)],
+    "tgx_paged_attn": [P(Paged), c_vp, c_vp, c_vp, P(c_i64), c_f32, c_vp, c_int, c_int, c_int,
+                       c_int, c_vp, c_size, c_vp],
+    "tgx_paged_append": [P(Paged), c_vp, c_vp, c_vp, c_vp, P(c_i64), c_vp, c_int, c_int, c_int,
+                         c_vp],
+    "tgx_select_pages_workspace": [P(Paged), c_int, c_int, P(c_size)],
+    "tgx_select_pages": [P(Paged), c_vp, P(c_i64), c_vp, c_int, c_int, c_int, c_int, c_int, c_vp,
+                         c_vp, c_vp, c_size, c_vp],
+    "tgx_norm_rotary_fwd": [P(NormRotary), c_vp, c_vp, c_vp],
+    "tgx_norm_rotary_bwd_workspace": [P(NormRotary), P(c_size)],
+    "tgx_norm_rotary_bwd": [P(NormRotary), c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_size,
+                            c_vp],
     # CPU twins (include/tgx_cpu.h): host pointers, no stream.
     "tgx_cpu_set_threads": [c_int],
     "tgx_cpu_destination_index": [c_vp, c_int, c_i64, c_i64, c_vp, c_int],
@@ -268,6 +302,19 @@ def stream_of(tensor) -> int:
     if index is None:
         index = torch.cuda.current_device()
     return torch._C._cuda_getCurrentRawStream(index)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device(tensor):
+    """A context in which the tensor's device is the current one (a launch on
+    a stream of another device than the current one is refused)."""
+    import torch
+
+    if tensor.device.index == torch.cuda.current_device():
+        return _HERE
+    return torch.cuda.device(tensor.device)
 
 
 DTYPE_BF16, DTYPE_F16, DTYPE_F32 = 0, 1, 2

@@ -50,6 +50,39 @@ class GraphSchema:
                 str(self.index_dtype), self.sorted_by_dst)
 
 
+@dataclass
+class PagedState:
+    """The tables of a paged relation (``Graph.paged``): tensors whose contents
+    every use reads as they stand."""
+
+    page_table: torch.Tensor   # [sequences, pages] or [sequences, heads, pages] int32
+    lengths: torch.Tensor      # [sequences] int32
+    page_size: int
+    num_pages: int
+    queries: int
+
+    @property
+    def table_heads(self) -> int:
+        return self.page_table.shape[1] if self.page_table.ndim == 3 else 1
+
+    def native(self):
+        """The relation as the native entry points take it."""
+        t = self.page_table
+        return ctypes.byref(_native.Paged(
+            t.data_ptr() if t.numel() else None, t.stride(0), t.stride(1) if t.ndim == 3 else 0,
+            self.lengths.data_ptr() if self.lengths.numel() else None, t.shape[0],
+            self.table_heads, t.shape[-1], self.page_size, self.num_pages, self.queries))
+
+    def clamped_lengths(self) -> torch.Tensor:
+        """Cached tokens of each sequence that its page table can hold, int64."""
+        return self.lengths.long().clamp(min=0, max=self.page_table.shape[-1] * self.page_size)
+
+    def limits(self) -> torch.Tensor:
+        """Positions each query row sees, int64 [sequences, queries]."""
+        back = torch.arange(self.queries - 1, -1, -1, device=self.lengths.device)
+        return (self.clamped_lengths()[:, None] - back).clamp(min=0)
+
+
 class RowPlanHandle:
     """A ``tgx_row_plan`` plus the device tensors it points into."""
 
@@ -248,6 +281,7 @@ class Graph:
         self._causal = causal
         # Implicit dense relations: None (every pair) or "lower_inclusive".
         self._dense_boundary = None
+        self.paged_state: PagedState | None = None
         self._device = torch.device(device) if device is not None else None
         self._destination_index_cache = None
         self._degree_bounds_cache = None
@@ -411,6 +445,204 @@ class Graph:
         return graph
 
     @classmethod
+    def paged(cls, page_table: torch.Tensor, lengths: torch.Tensor, *, page_size: int,
+              num_pages: int, queries: int = 1,
+              validate: Literal["basic", "full"] = "basic") -> "Graph":
+        """Relation of each sequence's newest tokens to the slots of a paged cache.
+
+        The cache is ``num_pages * page_size`` source rows; position j of
+        sequence b lies in row ``page_table[b, j // page_size] * page_size +
+        j % page_size``.  lengths[b] counts the sequence's cached tokens, the
+        asking ones among them: its newest `queries` tokens are the destination
+        rows ``b * queries + t``, and token t relates to the positions
+        ``0 .. lengths[b] - queries + t`` (none where that is negative).
+
+        page_table [sequences, pages] and lengths [sequences] are int32.  Their
+        contents are read as they stand at every use, without copying them to
+        the host, so a program advances them in place and captures launches
+        into a HIP graph.  A page id outside ``[0, num_pages)`` names no page:
+        its positions relate to nothing.  Lengths are clamped to what a table
+        row can hold.  ``validate="full"`` refuses such contents now.
+
+        Dot-product attention over the relation, with query heads grouped on
+        key heads if the fields broadcast (query [rows, heads, group, D] on key
+        and value [slots, heads, 1, D]), runs on the paged kernels; any other
+        edge function, and attention that needs gradients, on `snapshot()`.
+
+        A page_table [sequences, heads, pages] is a table for each head
+        (`select_pages` returns such a relation): the rows are then
+        ``(b * queries + t) * heads + h``, the sources ``slot * heads + h``."""
+        for name, value in (("page_table", page_table), ("lengths", lengths)):
+            if not isinstance(value, torch.Tensor):
+                raise TypeError(f"{name} must be a torch.Tensor")
+            if value.dtype != torch.int32:
+                raise TypeError(f"{name} must have int32 dtype")
+        if page_table.ndim not in (2, 3):
+            raise ValueError("page_table must be [sequences, pages] or [sequences, heads, pages]")
+        if page_table.ndim == 3 and page_table.shape[1] == 0:
+            raise ValueError("page_table must have at least one head")
+        if lengths.ndim != 1 or lengths.shape[0] != page_table.shape[0]:
+            raise ValueError(f"lengths must be [{page_table.shape[0]}], got {tuple(lengths.shape)}")
+        if lengths.device != page_table.device:
+            raise ValueError("page_table and lengths must be on the same device")
+        if page_table.shape[-1] > 1 and page_table.stride(-1) != 1 or \
+                lengths.shape[0] > 1 and lengths.stride(0) != 1:
+            raise ValueError("the rows of page_table, and lengths, must be dense")
+        for name, value, least in (("page_size", page_size, 1), ("num_pages", num_pages, 0),
+                                   ("queries", queries, 1)):
+            if not isinstance(value, int) or isinstance(value, bool) or value < least:
+                raise ValueError(f"{name} must be an integer of at least {least}")
+        if max(num_pages * page_size, page_table.shape[-1] * page_size,
+               page_table.shape[0] * queries) >= 2**31:
+            raise ValueError("a paged relation has fewer than 2**31 slots, positions and rows")
+        state = PagedState(page_table, lengths, page_size, num_pages, queries)
+        if validate == "full":
+            state_lengths = lengths.long()
+            if bool(((state_lengths < 0) |
+                     (state_lengths > page_table.shape[-1] * page_size)).any()):
+                raise ValueError("lengths contains more tokens than its pages hold, or fewer than 0")
+            used = (state_lengths + page_size - 1) // page_size
+            ids = page_table if page_table.ndim == 3 else page_table[:, None]
+            named = torch.arange(page_table.shape[-1], device=ids.device) < used[:, None, None]
+            if bool((named & ((ids < 0) | (ids >= num_pages))).any()):
+                raise ValueError("page_table contains an out-of-range page")
+        elif validate != "basic":
+            raise ValueError("validate must be 'basic' or 'full'")
+        heads = state.table_heads
+        schema = GraphSchema(num_src=num_pages * page_size * heads,
+                             num_dst=page_table.shape[0] * queries * heads, origin="paged",
+                             realization="paged", index_dtype=torch.int64, lifecycle="live")
+        graph = cls(schema, device=page_table.device)
+        graph.paged_state = state
+        return graph
+
+    def snapshot(self) -> "Graph":
+        """A paged relation as its tables stand, as an explicit CSR (one host
+        synchronisation); any other relation is itself."""
+        if not self.is_paged:
+            return self
+        row_ptr, col_idx = self.resolve_csr()
+        return Graph.from_csr(row_ptr, col_idx, num_src=self._schema.num_src)
+
+    def _paged_only(self, method: str) -> PagedState:
+        if not self.is_paged:
+            raise TypeError(f"{method} needs a paged relation (Graph.paged), "
+                            f"not {self._schema.origin}")
+        if self.paged_state.page_table.ndim != 2:
+            raise ValueError(f"{method} needs one page table per sequence, not one per head")
+        return self.paged_state
+
+    def append(self, key_cache: torch.Tensor, key: torch.Tensor, value_cache: torch.Tensor,
+               value: torch.Tensor, *, page_sums: torch.Tensor | None = None) -> None:
+        """Write the newest tokens' keys and values into their slots of the
+        cache, in place.
+
+        key and value [rows, heads, D] hold this relation's destination rows
+        (row ``b * queries + t`` is position ``lengths[b] - queries + t``, rows of
+        negative positions are not written), key_cache and value_cache
+        [slots, heads, D] its sources; all of one type, strided as they come.
+        page_sums [num_pages, heads, D] fp32: the sum of the keys of every page
+        written to is formed again from the page's slots up to the newest token
+        (what `select_pages` ranks pages by).  No gradients.
+
+        Each sequence's written pages must be its own; two sequences writing
+        to one page leave either's rows there."""
+        from . import _paged
+
+        state = self._paged_only("append")
+        rows, slots = self._schema.num_dst, self._schema.num_src
+        tensors = {"key_cache": key_cache, "key": key, "value_cache": value_cache, "value": value}
+        for name, t in tensors.items():
+            if not isinstance(t, torch.Tensor):
+                raise TypeError(f"{name} must be a torch.Tensor")
+        for name, t in tensors.items():
+            want = slots if name.endswith("cache") else rows
+            if t.ndim != 3 or tuple(t.shape) != (want, *key.shape[1:]):
+                raise ValueError(f"{name} must have shape [{want}, heads, D] like the others, "
+                                 f"got {tuple(t.shape)}")
+            if t.dtype != key_cache.dtype or not t.is_floating_point():
+                raise TypeError("key_cache, key, value_cache and value must have one floating type")
+            if t.device != self.device:
+                raise ValueError(f"{name} is on {t.device}, but graph is on {self.device}")
+        for name in ("key_cache", "value_cache"):
+            t = tensors[name]
+            if t.shape[-1] > 1 and t.stride(-1) != 1:
+                raise ValueError(f"the rows of {name} must be dense")
+            if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+                raise ValueError(f"{name} must not be expanded: it is written to")
+        if page_sums is not None:
+            if not isinstance(page_sums, torch.Tensor) or page_sums.dtype != torch.float32:
+                raise TypeError("page_sums must be a float32 torch.Tensor")
+            if tuple(page_sums.shape) != (state.num_pages, *key.shape[1:]) or \
+                    not page_sums.is_contiguous():
+                raise ValueError(f"page_sums must be contiguous [{state.num_pages}, heads, D], got "
+                                 f"{tuple(page_sums.shape)}")
+            if page_sums.device != self.device:
+                raise ValueError(f"page_sums is on {page_sums.device}, but graph is on "
+                                 f"{self.device}")
+            tensors["page_sums"] = page_sums
+        if torch.is_grad_enabled() and any(t.requires_grad for t in tensors.values()):
+            raise NotImplementedError("append has no gradient: detach its operands or run it "
+                                      "under torch.no_grad()")
+        _paged.append(self, key_cache, key, value_cache, value, page_sums)
+
+    def select_pages(self, query: torch.Tensor, page_sums: torch.Tensor, count: int, *,
+                     out: "Graph | None" = None) -> "Graph":
+        """The paged relation of each query row and key head to `count` of its
+        pages: the newest, and those full pages whose keys' sum has the largest
+        product with the head's summed queries,
+
+            score = sum_d (sum_g query[row, h, g, d]) * page_sums[page, h, d],
+
+        formed in 64 bits; equal scores go to the earlier page, a NaN counts as
+        -inf, and a row of no more than `count` pages keeps them all.
+
+        query [rows, heads, group, D] or [rows, heads, D]; page_sums
+        [num_pages, heads, D] fp32, as `append` keeps them.  The result has a
+        table per head: attention over it takes query.view(rows * heads, group,
+        D) on caches viewed as [slots * heads, 1, D].  With `out`, a relation
+        returned for the same shapes before, its tables are rewritten in place
+        (a prepared or captured launch over it then sees them)."""
+        from . import _paged
+
+        state = self._paged_only("select_pages")
+        if not isinstance(query, torch.Tensor) or not isinstance(page_sums, torch.Tensor):
+            raise TypeError("query and page_sums must be torch.Tensor")
+        if query.ndim == 3:
+            query = query[:, :, None]
+        if query.ndim != 4 or query.shape[0] != self._schema.num_dst or \
+                not query.is_floating_point() or min(query.shape[1:]) < 1:
+            raise ValueError(f"query must be floating-point [{self._schema.num_dst}, heads, group, D]"
+                             f", got {query.dtype} {tuple(query.shape)}")
+        heads, D = query.shape[1], query.shape[3]
+        if page_sums.dtype != torch.float32 or not page_sums.is_contiguous() or \
+                tuple(page_sums.shape) != (state.num_pages, heads, D):
+            raise ValueError(f"page_sums must be contiguous float32 [{state.num_pages}, {heads}, {D}]"
+                             f", got {page_sums.dtype} {tuple(page_sums.shape)}")
+        for name, t in (("query", query), ("page_sums", page_sums)):
+            if t.device != self.device:
+                raise ValueError(f"{name} is on {t.device}, but graph is on {self.device}")
+        if not isinstance(count, int) or isinstance(count, bool) or count < 1:
+            raise ValueError("count must be a positive integer")
+        shape = (self._schema.num_dst, heads, count)
+        if out is None:
+            table = torch.empty(shape, dtype=torch.int32, device=self.device)
+            lengths = torch.empty(shape[0], dtype=torch.int32, device=self.device)
+            out = Graph.paged(table, lengths, page_size=state.page_size,
+                              num_pages=state.num_pages)
+        else:
+            got = getattr(out, "paged_state", None)
+            if got is None or tuple(got.page_table.shape) != shape or got is state or \
+                    (got.page_size, got.num_pages, got.queries) != (state.page_size,
+                                                                    state.num_pages, 1) or \
+                    out.device != self.device or not got.page_table.is_contiguous():
+                raise ValueError(f"out must be a relation that select_pages returned for {shape} "
+                                 "tables over the same cache")
+        _paged.select(self, query.detach(), page_sums.detach(), count,
+                      out.paged_state.page_table, out.paged_state.lengths)
+        return out
+
+    @classmethod
     def cat(cls, graphs) -> "Graph":
         blocks = list(graphs)
         if not blocks:
@@ -470,6 +702,20 @@ class Graph:
     def is_dense(self) -> bool:
         return self._schema.realization == "implicit_dense"
 
+    @property
+    def is_paged(self) -> bool:
+        return self.paged_state is not None
+
+    @property
+    def page_table(self) -> torch.Tensor | None:
+        """The page table of a paged relation, else None."""
+        return None if self.paged_state is None else self.paged_state.page_table
+
+    @property
+    def lengths(self) -> torch.Tensor | None:
+        """Cached tokens of each sequence of a paged relation, else None."""
+        return None if self.paged_state is None else self.paged_state.lengths
+
     def _square_blocks(self, causal: bool):
         """cu_seqlens (int64, on the graph's device) of an implicit relation
         made of square blocks with the given boundary, else None."""
@@ -494,9 +740,16 @@ class Graph:
             if self._causal:
                 return int((lengths * (lengths + 1) // 2).sum().item())
             return int((lengths * lengths).sum().item())
+        if self.is_paged:
+            return self.resolve_csr()[1].numel()
         return self._col_idx.numel()
 
     def resolve_csr(self) -> tuple[torch.Tensor, torch.Tensor]:
+        if self.is_paged:
+            # As the tables stand now: never kept.
+            from . import _paged
+
+            return _paged.csr(self.paged_state)
         if self._row_ptr is None and self.is_dense:
             # Only an edge function no tile covers gets here (eager path).
             dtype, dev = self._schema.index_dtype, self.device
@@ -574,6 +827,8 @@ class Graph:
         """(min, max, sum) of the destination-row degrees: closed forms for
         implicit relations, else one device reduction and one host transfer,
         cached for the graph (an immutable snapshot)."""
+        if self.is_paged:
+            return self.snapshot()._degree_stats()
         got = self._degree_bounds_cache
         if got is not None:
             return got
@@ -615,6 +870,8 @@ class Graph:
     def degree_histogram(self) -> tuple[int, ...]:
         """Exact row counts indexed by degree 0..max (reference graph.py:
         1258-1277); limited to a maximum degree of 4096, as there."""
+        if self.is_paged:
+            return self.snapshot().degree_histogram()
         _, maximum, _ = self._degree_stats()
         if maximum > 4096:
             raise ValueError("exact degree histogram is limited to degree_max <= 4096")
@@ -651,6 +908,8 @@ class Graph:
         |source id - destination id| over `samples` evenly spaced edge slots,
         over max(1, num_src, num_dst), clipped to [0, 1]; about 1/3 for random
         numbering, near 0 for index-local graphs.  Planning information only."""
+        if self.is_paged:
+            return self.snapshot().source_index_span_ratio(samples)
         key = ("span_ratio", samples)
         got = self._native_cache.get(key)
         if got is not None:
@@ -678,6 +937,11 @@ class Graph:
         the relation's kind and sizes, index dtype and device, the degree
         statistics, the gather locality and the dense boundary."""
         s = self._schema
+        if self.is_paged:
+            # The sizes only: what the tables hold may change between calls.
+            p = self.paged_state
+            return (s.origin, s.realization, s.num_src, s.num_dst, str(s.index_dtype),
+                    str(self.device), tuple(p.page_table.shape), p.page_size, p.queries)
         locality = (self.source_index_span_ratio()
                     if self._row_ptr is not None else "implicit")
         return (s.origin, s.realization, s.num_src, s.num_dst, str(s.index_dtype),
@@ -688,6 +952,8 @@ class Graph:
         (tgx_plan_reference_buckets: SelectKernelSchedule.cpp:136-163,
         PlanDegreeBuckets.cpp:32-143, PlanSplitRows.cpp:84-147), given the
         degree statistics and, up to degree 4096, the exact histogram."""
+        if self.is_paged:
+            return self.snapshot()._reference_plan_remarks(has_node_epilogue)
         key = ("reference_plan", bool(has_node_epilogue))
         got = self._native_cache.get(key)
         if got is None:
@@ -699,6 +965,8 @@ class Graph:
         """The reference planner's decision for this graph as a dict: plan name,
         padding utilization (per mille, -1 when not computed), bucket upper
         bounds, their mappings and row counts, row-split sizing."""
+        if self.is_paged:
+            return self.snapshot().reference_plan(has_node_epilogue)
         _, maximum, total = self._degree_stats()
         histogram = self.degree_histogram() if maximum <= 4096 else None
         return reference_plan(self._schema.num_dst, maximum, total, histogram,
@@ -908,5 +1176,5 @@ def _varlen_csr(cu_seqlens: torch.Tensor, causal: bool):
     return row_ptr, col_idx
 
 
-__all__ = ["Graph", "GraphSchema", "build_coo_csr", "build_row_plan", "build_transpose",
+__all__ = ["Graph", "GraphSchema", "PagedState", "build_coo_csr", "build_row_plan", "build_transpose",
            "build_varlen_csr", "describe_reference_plan", "reference_plan"]

@@ -328,7 +328,14 @@ class MessagePassing(Kernel):
                 "run exact softmax on a CSR relation")
         captured = self._captured(params)
         launch = None
-        if device.type == "cuda" and captured is not None:
+        if graph.is_paged:
+            if device.type == "cuda" and captured is not None:
+                launch = self._plan_paged(captured, graph, src, dst, params)
+            if launch is None:
+                # The relation as its tables stand, for everything the paged
+                # attention does not cover.
+                return self._dispatch(graph.snapshot(), src, dst, edge, params)
+        elif device.type == "cuda" and captured is not None:
             launch = self._plan_native(captured, graph, src, dst, edge, params)
         elif captured is not None:
             out = self._sparse_mm_sum(captured, graph, src, edge)
@@ -848,6 +855,70 @@ class MessagePassing(Kernel):
             "backward over the transposed CSR (dk, dv, each edge's ds kept) and the CSR "
             "(dq, dbias from the kept ds)")
         return _Launch(graph, tuple(operands), run, describe)
+
+    def _plan_paged(self, captured, graph, src, dst, params) -> _Launch | None:
+        """Dot-product attention over Graph.paged on the paged kernels: bf16,
+        fp16 or fp32 fields of one type, widths that are multiples of 8 up to
+        512, query heads grouped on key heads."""
+        from . import _paged
+
+        if not isinstance(self.reducer, OnlineSoftmaxReducer) or \
+                self.reducer.accumulation_dtype not in (None, torch.float32, "float32"):
+            return None
+        dot = cap.recognize_dot(captured)
+        if dot is None or dot.bias_field is not None:
+            return None
+        q, k, v = dst.get(dot.q_field), src.get(dot.k_field), src.get(dot.v_field)
+        if q is None or k is None or v is None:
+            return None
+        got = _paged.heads_of(q, k, v)
+        if got is None or not (q.dtype == k.dtype == v.dtype) or q.dtype not in _paged.DTYPES:
+            return None
+        heads, group = got
+        D = q.shape[-1]
+        if D % 8 or not 8 <= D <= 512 or not heads or not group:
+            return None
+        if not (_paged.rows_on_16_bytes(k) and _paged.rows_on_16_bytes(v)):
+            return None     # (a copy of the whole cache would be made each call)
+        _native.lib()
+        scale = dot.scale
+
+        def run(q, k, v):
+            if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
+                return self._paged_with_gradients(dot, graph, q, k, v, params)
+            return _paged.bind_attention(graph, q, k, v, scale, heads, group)()
+
+        def bind(q, k, v):
+            if any(t.data_ptr() % 16 for t in (q, k, v)) or not _paged.rows_on_16_bytes(q):
+                return None     # the launch reads a copy, which would not stay live
+            return _paged.bind_attention(graph, q, k, v, scale, heads, group)
+
+        kind = str(q.dtype).split(".")[-1]
+        describe = lambda: self._variant(
+            graph, "paged-attention", ("tgx_paged_attn",),
+            f"{kind} rows of the cache read once through the page tables, {group} query heads on "
+            f"each of {heads} key heads, fp32 online softmax; long sequences in pieces, joined "
+            "in order; gradients on the relation's snapshot")
+        operands = (("dst", dot.q_field), ("src", dot.k_field), ("src", dot.v_field))
+        return _Launch(graph, operands, run, describe, bind=bind)
+
+    def _paged_with_gradients(self, dot, graph, q, k, v, params):
+        """Paged attention whose fields need gradients: over the relation's
+        snapshot, shared key heads repeated for the heads on them (their
+        gradients add up again) where the CSR attention kernels take the
+        width, else on Torch operations in fp32."""
+        from . import _ops
+
+        snapshot = graph.snapshot()
+        D = q.shape[-1]
+        if D % 8 == 0 and D <= 512 and (D // 8) & (D // 8 - 1) == 0 and snapshot.num_edges:
+            each = lambda t: t.expand(t.shape[0], *q.shape[1:]).reshape(t.shape[0], -1, D)
+            out = _ops.DotAttnFunction.apply(q.reshape(q.shape[0], -1, D), each(k), each(v), None,
+                                             dot.scale, snapshot)
+            return out.reshape(q.shape)
+        fields = {dot.k_field: k.float(), dot.v_field: v.float()}
+        out = _eager.evaluate(self, snapshot, fields, {dot.q_field: q.float()}, {}, params)
+        return out.to(q.dtype)
 
     def _plan_block_attention(self, dot, graph, q, k, v) -> _Launch | None:
         """Dot-product attention over Graph.cu_seqlens / dense / triangular

@@ -397,4 +397,91 @@ def _extract_chain(module: nn.Module) -> tuple[ScoreLayer, ...]:
                  for l in layers)
 
 
-__all__ = ["ScoreLayer", "TracedModule", "trace"]
+def norm_rotary(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Tensor,
+                frequencies: torch.Tensor, *, query_weight: torch.Tensor | None = None,
+                key_weight: torch.Tensor | None = None, eps: float = 1e-6, norm: bool = True,
+                sections: tuple[int, ...] | None = None, interleaved: bool = False):
+    """RMS norm of every head's query and key, and the rotation by their
+    positions, in one pass with gradients: the fields dot-product attention
+    reads (``dst.query``, ``src.key``).
+
+    query [n, query heads, D] and key [n, key heads, D] (or None) may be strided
+    views, such as parts of one projection.  Each row x becomes
+    ``x / sqrt(mean(x^2) + eps) * weight`` (weights [D] or None for ones; none of
+    it with ``norm=False``), then its pairs (i, i + R/2) -- (2i, 2i + 1) when
+    ``interleaved`` -- turn by ``position * frequencies[i]``, R = 2 *
+    len(frequencies) <= D; values from R on only take the norm.
+
+    positions [n], or [n, axes] (time, height, width) with ``sections`` the
+    number of frequencies of each axis in order; integers, of either sign and
+    any size (angles are formed in 64 bits).  Arithmetic is in fp32, rounded
+    once.  Returns the new query, or (query, key).  Gradients: query, key and
+    weights; the same inputs give the same bits.
+
+    On the GPU bf16, fp16 and fp32, D a multiple of 4 up to 256, an even number
+    of frequencies, at most 4 axes and weights of one type run on the HIP
+    kernels; anything else, and host tensors, on Torch operations
+    (``tiga.config.strict`` refuses those on the GPU)."""
+    from . import _rotary
+    from .message_passing import config
+
+    for name, t in (("query", query), ("key", key)):
+        if t is None and name == "key":
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+        if t.ndim != 3 or not t.is_floating_point():
+            raise ValueError(f"{name} must be a floating-point [tokens, heads, width] tensor, got "
+                             f"{t.dtype} {tuple(t.shape)}")
+    if key is not None and (key.shape[0] != query.shape[0] or key.shape[2] != query.shape[2] or
+                            key.dtype != query.dtype):
+        raise ValueError(f"key {key.dtype} {tuple(key.shape)} must have the tokens, width and type "
+                         f"of query {query.dtype} {tuple(query.shape)}")
+    n, _, D = query.shape
+    if not isinstance(positions, torch.Tensor) or \
+            positions.dtype not in (torch.int32, torch.int64):
+        raise TypeError("positions must be an int32 or int64 torch.Tensor")
+    if not isinstance(frequencies, torch.Tensor) or frequencies.dtype != torch.float32:
+        raise TypeError("frequencies must be a float32 torch.Tensor")
+    if frequencies.ndim != 1 or 2 * frequencies.numel() > D:
+        raise ValueError(f"frequencies must be one-dimensional, at most {D // 2} for width {D}")
+    if frequencies.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError("norm_rotary has no gradient with respect to frequencies")
+    if positions.ndim == 1:
+        positions = positions[:, None]
+    if sections is None:
+        sections = (frequencies.numel(),)
+    sections = tuple(int(s) for s in sections)
+    if positions.ndim != 2 or positions.shape != (n, len(sections)):
+        raise ValueError(f"positions must be [{n}] or [{n}, {len(sections)}] for {len(sections)} "
+                         f"sections, got {tuple(positions.shape)}")
+    if any(s < 0 for s in sections) or sum(sections) != frequencies.numel():
+        raise ValueError(f"sections {sections} must add up to {frequencies.numel()} frequencies")
+    for name, w in (("query_weight", query_weight), ("key_weight", key_weight)):
+        if w is None:
+            continue
+        if not norm:
+            raise ValueError(f"{name} needs norm=True")
+        if not isinstance(w, torch.Tensor) or not w.is_floating_point() or \
+                tuple(w.shape) != (D,):
+            raise ValueError(f"{name} must be a floating-point [{D}] torch.Tensor")
+    if key is None and key_weight is not None:
+        raise ValueError("key_weight needs a key")
+    if norm and not eps >= 0.0:
+        raise ValueError("eps must not be negative")
+    given = [t for t in (key, positions, frequencies, query_weight, key_weight) if t is not None]
+    for t in given:
+        if t.device != query.device:
+            raise ValueError(f"operand on {t.device}, but query is on {query.device}")
+    form = _rotary.Form(float(eps), bool(norm), sections, bool(interleaved))
+    args = (form, query, key, query_weight, key_weight, positions.contiguous(),
+            frequencies.contiguous())
+    if _rotary.covered(form, query, key, (query_weight, key_weight)):
+        return _rotary.apply(*args)
+    if query.is_cuda and config.strict:
+        raise RuntimeError("norm_rotary: no HIP kernel covers these types and widths and "
+                           "tiga.config.strict is set")
+    return _rotary.reference(*args)
+
+
+__all__ = ["ScoreLayer", "TracedModule", "norm_rotary", "trace"]
