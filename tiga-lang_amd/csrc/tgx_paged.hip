@@ -239,6 +239,383 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedArgs a) {
   }
 }
 
+// ---------------------------------------------------------------------------
+// Matrix tiles (bf16, fp16; D = 32, 64, 128)
+//
+// A workgroup holds the queries of one (sequence, head) that share its keys,
+// 16 * QT of them, and each of its four waves runs through every fourth step
+// of KEYS keys by itself: there is no barrier before the end.  With lane l, g
+// = l / 16, lr = l % 16 (v_mfma_f32_16x16x32, as in the dense tiles): S^T = K
+// Q^T takes its K fragments straight from the cache, 16 bytes a lane and 64
+// contiguous bytes of each of 16 rows an instruction; the lane's results are
+// four keys of one query for each 16 keys, which is P^T as the B operand of
+// O^T = V^T P^T under the key order {4g .. 4g + 3, 16 + 4g ..}; V^T is read
+// down the columns of a V tile that the wave staged in its own LDS rows
+// (ds_read_b64_tr_b16).
+//
+// Memory is kept busy by order alone: a step's K loads are issued as soon as
+// the step before has multiplied its own, its V loads as soon as the step
+// before has staged its own, and the page ids one step ahead of that, so a wave
+// always has 16 KB (D = 128) or more on its way.  A weight is multiplied as the
+// sum of two 16-bit values (the matrix unit has time to spare: 48
+// instructions of 16 cycles a step against some 6000 cycles of memory), so
+// only the output's own rounding is left.
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+template <typename T>
+struct Frag;
+template <>
+struct Frag<__bf16> {
+  typedef bf16x8 v8;
+  typedef __bf16 v4 __attribute__((ext_vector_type(4)));
+  static constexpr uint32_t kExponent = 0x7F80u;
+};
+template <>
+struct Frag<_Float16> {
+  typedef f16x8 v8;
+  typedef _Float16 v4 __attribute__((ext_vector_type(4)));
+  static constexpr uint32_t kExponent = 0x7C00u;
+};
+__device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// Max and sum over the four lanes l, l ^ 16, l ^ 32, l ^ 48.
+__device__ __forceinline__ float group4_max(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16, 64));
+  return fmaxf(x, __shfl_xor(x, 32, 64));
+}
+__device__ __forceinline__ float group4_sum(float x) {
+  x += __shfl_xor(x, 16, 64);
+  return x + __shfl_xor(x, 32, 64);
+}
+
+// Row stride (elements) of a staged V tile: free of bank conflicts as in the
+// dense tiles.
+template <int D>
+constexpr int kRow = D == 128 ? 144 : D == 64 ? 80 : 48;
+
+// The running maximum only moves when a step's exceeds it by this (log2 units).
+constexpr float kRescaleLog2 = 8.f;
+
+// Workgroups per CU that the registers are held to, and keys a step: a step's K
+// and V fragments are D * KEYS / 64 registers.
+template <int D, int QT>
+constexpr int kTileBlocks = D == 128 && QT == 2 ? 1 : D == 128 || QT == 2 ? 2 : 3;
+template <int D, int QT>
+constexpr int kTileKeys = D == 128 || QT == 2 ? 32 : 64;
+
+template <int D, int QT, int KEYS>
+struct TileShape {
+  static constexpr size_t kStage = sizeof(uint16_t) * 4 * KEYS * kRow<D>;
+  static constexpr size_t kJoin = sizeof(float) * 4 * 16 * QT * (D + 4 + 2);
+  static constexpr size_t kBytes = kStage > kJoin ? kStage : kJoin;
+};
+
+template <typename T, int D, int QT, int KEYS>
+__global__ __launch_bounds__(256, (kTileBlocks<D, QT>)) void paged_tile_kernel(PagedArgs a) {
+  constexpr int KT = KEYS / 16, KC = D / 32, DT = D / 16, ROW = kRow<D>;
+  using v8 = typename Frag<T>::v8;
+  using v4 = typename Frag<T>::v4;
+  __shared__ __align__(16) char smem[TileShape<D, QT, KEYS>::kBytes];
+  const PagedRel& r = a.rel;
+  const int all_heads = r.heads * a.heads;
+  const int rows = r.queries * a.group;
+  const int row_groups = (rows + 16 * QT - 1) / (16 * QT);
+  const int64_t item = blockIdx.x;
+  const int row0 = static_cast<int>(item % row_groups) * (16 * QT);
+  const int head = static_cast<int>(item / row_groups % all_heads);
+  const int x = static_cast<int>(item / row_groups / all_heads);
+  const Piece p = find_piece(r, a.pieces, a.meta == nullptr, x);
+  if (p.seq < 0) return;
+  const int th = head / a.heads, kh = head % a.heads;
+  if (a.meta && p.index == 0 && row0 == 0 && head == 0 && threadIdx.x == 0)
+    a.meta[p.seq] = make_int2(x, p.count);
+
+  const int wave = uniform(threadIdx.x >> 6), lane = lane_id();
+  const int g = lane >> 4, lr = lane & 15;
+  // Positions each of the lane's queries sees, and the fewest and most of all.
+  int limit[QT];
+  v8 qf[QT][KC];
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    const int row = row0 + 16 * qt + lr;
+    const int t = min(row / a.group, r.queries - 1), gq = row % a.group;
+    limit[qt] = p.length - (r.queries - 1 - t);
+    const int64_t q_row = (static_cast<int64_t>(p.seq) * r.queries + t) * r.heads + th;
+    const T* q = static_cast<const T*>(a.q) + q_row * a.qs_row + kh * a.qs_head +
+                 gq * a.qs_group + 8 * g;
+#pragma unroll
+    for (int kc = 0; kc < KC; ++kc)
+      qf[qt][kc] = row < rows ? *reinterpret_cast<const v8*>(q + 32 * kc) : v8{};
+  }
+  const int t_low = row0 / a.group;
+  const int t_high = min((row0 + 16 * QT - 1) / a.group, r.queries - 1);
+  const int low = p.length - (r.queries - 1 - t_low);
+  const int high = min(p.length - (r.queries - 1 - t_high), p.tile1 * kTile);
+
+  const T* kb = static_cast<const T*>(a.k) + th * a.ks_table + kh * a.ks_head + 8 * g;
+  const T* vb = static_cast<const T*>(a.v) + th * a.vs_table + kh * a.vs_head + 8 * g;
+  const int32_t* table = r.table + p.seq * r.seq_stride + th * r.head_stride;
+  T* stage = reinterpret_cast<T*>(smem) + wave * KEYS * ROW;
+
+  // Steps of this wave: first + 4 i < last.  Lane l keeps the page id of key
+  // l (mod KEYS) of a step.
+  const int first = p.tile0 * (kTile / KEYS) + wave;
+  const int last = (high + KEYS - 1) / KEYS;
+  auto page_id = [&](int step) {
+    const int pos = min(step * KEYS + lane % KEYS, r.pages_per_seq * r.page_size - 1);
+    return table[static_cast<unsigned>(pos) / static_cast<unsigned>(r.page_size)];
+  };
+  auto slot_of = [&](int step, int id) {
+    const unsigned pos = step * KEYS + lane % KEYS;
+    const bool there = static_cast<int>(pos) < high &&
+                       static_cast<unsigned>(id) < static_cast<unsigned>(r.num_pages);
+    return there ? id * r.page_size + static_cast<int>(pos % static_cast<unsigned>(r.page_size))
+                 : -1;
+  };
+  // (A key that is not there loads slot 0, and is masked.)
+  auto load = [&](v8(&f)[KT][KC], const T* base, int64_t stride, int slot) {
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+      const int s = max(__shfl(slot, 16 * kt + lr, 64), 0);
+      const T* q = base + s * stride;
+#pragma unroll
+      for (int kc = 0; kc < KC; ++kc) f[kt][kc] = *reinterpret_cast<const v8*>(q + 32 * kc);
+    }
+  };
+
+  float m[QT], l[QT];
+  f32x4 o[DT][QT];
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    m[qt] = kNegInf;
+    l[qt] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[dt][qt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  if (first < last) {
+    v8 kf[KT][KC], vf[KT][KC];
+    int slot = slot_of(first, page_id(first));
+    load(kf, kb, a.ks_slot, slot);
+    load(vf, vb, a.vs_slot, slot);
+    int next_id = page_id(first + 4);
+    for (int step = first; step < last; step += 4) {
+      const int next = slot_of(step + 4, next_id);
+      next_id = page_id(step + 8);
+      const unsigned long long gone = __ballot(slot < 0);   // bit k: key k is not there
+      f32x4 c[KT][QT];
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) c[kt][qt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kc = 0; kc < KC; ++kc)
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) c[kt][qt] = mfma(kf[kt][kc], qf[qt][kc], c[kt][qt]);
+      load(kf, kb, a.ks_slot, next);
+
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) c[kt][qt] *= a.scale_log2;
+      const bool tail = step * KEYS + KEYS > low;   // some query sees only a part
+      if (gone || tail) {
+        const unsigned long long mine = gone >> (4 * g);
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int pos = step * KEYS + 16 * kt + 4 * g + i;
+            const bool hidden = mine >> (16 * kt + i) & 1;
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt)
+              if (hidden || pos >= limit[qt]) c[kt][qt][i] = kNegInf;
+          }
+      }
+      float top[QT];
+      bool grow = false;
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) {
+        top[qt] = kNegInf;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top[qt] = fmaxf(top[qt], c[kt][qt][i]);
+        top[qt] = group4_max(top[qt]);
+        grow |= top[qt] > m[qt] + kRescaleLog2;
+      }
+      if (__any(grow)) {
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) {
+          const float mn = fmaxf(m[qt], top[qt]);
+          const float alpha = m[qt] == kNegInf ? 0.f : exp2_hw(m[qt] - mn);
+          m[qt] = mn;
+          l[qt] *= alpha;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) o[dt][qt] *= alpha;
+        }
+      }
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) {
+        const float mo = m[qt] == kNegInf ? 0.f : m[qt];
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            c[kt][qt][i] = exp2_hw(c[kt][qt][i] - mo);
+            l[qt] += c[kt][qt][i];
+          }
+      }
+
+      // Stage V; a key that is not there counts as a row of zeros.
+      if (gone) {
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+          if (gone >> (16 * kt + lr) & 1) {
+#pragma unroll
+            for (int kc = 0; kc < KC; ++kc) vf[kt][kc] = v8{};
+          }
+      }
+      bool odd = false;   // a NaN or Inf where only some of the queries see it
+      if (tail && r.queries > 1) {
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int kc = 0; kc < KC; ++kc) {
+            const u32x4 w = __builtin_bit_cast(u32x4, vf[kt][kc]);
+            constexpr uint32_t e = Frag<T>::kExponent;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              odd |= (w[i] & e) == e || (w[i] >> 16 & e) == e;
+          }
+        odd = __any(odd);
+      }
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc)
+          *reinterpret_cast<v8*>(stage + (16 * kt + lr) * ROW + 32 * kc + 8 * g) = vf[kt][kc];
+      load(vf, vb, a.vs_slot, next);
+
+      if (!odd) {
+#pragma unroll
+        for (int k2 = 0; k2 < KT / 2; ++k2) {
+          v8 ph[QT], pl[QT];
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float w = c[2 * k2 + j / 4][qt][j % 4];
+              ph[qt][j] = static_cast<T>(w);
+              pl[qt][j] = static_cast<T>(w - static_cast<float>(ph[qt][j]));
+            }
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) {
+            const T* src = stage + (32 * k2 + 4 * g + (lr >> 2)) * ROW + 16 * dt + 4 * (lr & 3);
+            const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(src));
+            const i16x4 hi =
+                __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(src + 16 * ROW));
+            const u32x2 wl = __builtin_bit_cast(u32x2, lo), wh = __builtin_bit_cast(u32x2, hi);
+            const v8 vt = __builtin_bit_cast(v8, (u32x4{wl[0], wl[1], wh[0], wh[1]}));
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) {
+              o[dt][qt] = mfma(vt, ph[qt], o[dt][qt]);
+              o[dt][qt] = mfma(vt, pl[qt], o[dt][qt]);
+            }
+          }
+        }
+      } else {
+        // Key by key: what a query does not see is left out, not multiplied by 0.
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            for (int gk = 0; gk < 4; ++gk) {
+              const int key = 16 * kt + 4 * gk + i;
+#pragma unroll
+              for (int qt = 0; qt < QT; ++qt) {
+                const float w = __shfl(c[kt][qt][i], 16 * gk + lr, 64);
+                if (step * KEYS + key >= limit[qt]) continue;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                  const v4 vv = *reinterpret_cast<const v4*>(stage + key * ROW + 16 * dt + 4 * g);
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) o[dt][qt][e] += w * static_cast<float>(vv[e]);
+                }
+              }
+            }
+      }
+      slot = next;
+    }
+  }
+
+  // The four waves' states, joined in wave order.
+  float* jo = reinterpret_cast<float*>(smem);               // [wave][query][D + 4]
+  float* jm = jo + 4 * 16 * QT * (D + 4);                    // [wave][query][2]
+  __syncthreads();
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    const int at = wave * 16 * QT + 16 * qt + lr;
+    const float sum = group4_sum(l[qt]);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+      *reinterpret_cast<f32x4*>(jo + at * (D + 4) + 16 * dt + 4 * g) = o[dt][qt];
+    if (g == 0) {
+      jm[2 * at] = m[qt];
+      jm[2 * at + 1] = sum;
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 16 * QT * (D / 4); i += 256) {
+    const int qr = i / (D / 4), d = i % (D / 4) * 4, row = row0 + qr;
+    if (row >= rows) break;
+    float mw[4], mx = kNegInf;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      mw[w] = jm[2 * (w * 16 * QT + qr)];
+      mx = fmaxf(mx, mw[w]);
+    }
+    float sum = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const int at = w * 16 * QT + qr;
+      // (A wave without a maximum has no weight, or a NaN of its own.)
+      const float f = mw[w] == kNegInf ? 1.f : exp2_hw(mw[w] - mx);
+      sum += f * jm[2 * at + 1];
+      acc += f * *reinterpret_cast<const f32x4*>(jo + at * (D + 4) + d);
+    }
+    const int t = row / a.group, gq = row % a.group;
+    if (p.count == 1) {
+      const int64_t q_row = (static_cast<int64_t>(p.seq) * r.queries + t) * r.heads + th;
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      v4 w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = static_cast<T>(acc[e] * inv);
+      *reinterpret_cast<v4*>(static_cast<T*>(a.out) +
+                             ((q_row * a.heads + kh) * a.group + gq) * D + d) = w;
+    } else {
+      float* dst = a.partial +
+                   ((static_cast<int64_t>(x) * all_heads + head) * rows + row) * (D + 2);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dst[d + e] = acc[e];
+      if (d == 0) {
+        dst[D] = mx;
+        dst[D + 1] = sum;
+      }
+    }
+  }
+}
+
 // Joins the pieces of each (sequence, head, query) in a fixed order: a wave per query.
 template <int DT, int LPK>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
@@ -321,24 +698,42 @@ int check_attn(const tgx_paged* p, int heads, int group, int D, int dtype) {
   return TGX_OK;
 }
 
+// Whether the matrix tiles take the shape; the rows kernel takes every other.
+bool tiled(int D, int dtype) {
+  return dtype != TGX_DTYPE_F32 && (D == 32 || D == 64 || D == 128);
+}
+
+// Queries a workgroup of the tiles holds: one 16-query tile, or two that share
+// the keys' loads where there are more.
+int tile_queries(const tgx_paged& p, int group) {
+  return static_cast<int64_t>(p.queries) * group <= 16 ? 16 : 32;
+}
+
+int64_t workgroups_per_piece(const tgx_paged& p, int heads, int group, int D, int dtype) {
+  const int64_t queries = static_cast<int64_t>(p.queries) * group;
+  return static_cast<int64_t>(p.table_heads) * heads *
+         (tiled(D, dtype) ? ceil_div(queries, tile_queries(p, group)) : queries);
+}
+
 size_t meta_bytes(const tgx_paged& p) { return align_up(sizeof(int2) * p.n_seqs); }
 
 template <int DT, int LPK>
 int launch_rows(const PagedArgs& a, const Cut& cut, hipStream_t stream) {
   const int64_t queries = static_cast<int64_t>(a.rel.heads) * a.heads * a.rel.queries * a.group;
-  {
-    TGX_PROFILE("paged_rows", stream);
-    paged_rows_kernel<DT, LPK><<<dim3(static_cast<uint32_t>(cut.launched * queries)), dim3(256),
-                                 0, stream>>>(a);
-  }
+  TGX_PROFILE("paged_rows", stream);
+  paged_rows_kernel<DT, LPK><<<dim3(static_cast<uint32_t>(cut.launched * queries)), dim3(256), 0,
+                               stream>>>(a);
   TGX_LAUNCHED("paged_rows");
-  if (!cut.split) return TGX_OK;
-  {
-    TGX_PROFILE("paged_join", stream);
-    paged_join_kernel<DT, LPK>
-        <<<dim3(static_cast<uint32_t>(ceil_div(a.rel.n_seqs * queries, 4))), dim3(256), 0,
-           stream>>>(a);
-  }
+  return TGX_OK;
+}
+
+template <int DT, int LPK>
+int launch_join(const PagedArgs& a, hipStream_t stream) {
+  const int64_t queries = static_cast<int64_t>(a.rel.heads) * a.heads * a.rel.queries * a.group;
+  TGX_PROFILE("paged_join", stream);
+  paged_join_kernel<DT, LPK>
+      <<<dim3(static_cast<uint32_t>(ceil_div(a.rel.n_seqs * queries, 4))), dim3(256), 0,
+         stream>>>(a);
   TGX_LAUNCHED("paged_join");
   return TGX_OK;
 }
@@ -350,6 +745,41 @@ int dispatch_rows(const PagedArgs& a, const Cut& cut, hipStream_t stream) {
   if (a.D <= 128) return launch_rows<DT, 16>(a, cut, stream);
   if (a.D <= 256) return launch_rows<DT, 32>(a, cut, stream);
   return launch_rows<DT, 64>(a, cut, stream);
+}
+
+template <int DT>
+int dispatch_join(const PagedArgs& a, hipStream_t stream) {
+  if (a.D <= 32) return launch_join<DT, 4>(a, stream);
+  if (a.D <= 64) return launch_join<DT, 8>(a, stream);
+  if (a.D <= 128) return launch_join<DT, 16>(a, stream);
+  if (a.D <= 256) return launch_join<DT, 32>(a, stream);
+  return launch_join<DT, 64>(a, stream);
+}
+
+template <typename T, int D, int QT, int KEYS>
+int launch_tiles(const PagedArgs& a, const Cut& cut, hipStream_t stream) {
+  const int64_t rows = static_cast<int64_t>(a.rel.queries) * a.group;
+  const int64_t blocks = cut.launched * a.rel.heads * a.heads * ceil_div(rows, 16 * QT);
+  {
+    TGX_PROFILE("paged_tiles", stream);
+    paged_tile_kernel<T, D, QT, KEYS>
+        <<<dim3(static_cast<uint32_t>(blocks)), dim3(256), 0, stream>>>(a);
+  }
+  TGX_LAUNCHED("paged_tiles");
+  return TGX_OK;
+}
+
+template <typename T, int D>
+int launch_tiles(const PagedArgs& a, const Cut& cut, hipStream_t stream) {
+  return a.rel.queries * a.group <= 16 ? launch_tiles<T, D, 1, kTileKeys<D, 1>>(a, cut, stream)
+                                       : launch_tiles<T, D, 2, kTileKeys<D, 2>>(a, cut, stream);
+}
+
+template <typename T>
+int dispatch_tiles(const PagedArgs& a, const Cut& cut, hipStream_t stream) {
+  if (a.D == 32) return launch_tiles<T, 32>(a, cut, stream);
+  if (a.D == 64) return launch_tiles<T, 64>(a, cut, stream);
+  return launch_tiles<T, 128>(a, cut, stream);
 }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -364,7 +794,7 @@ extern "C" int tgx_paged_attn_workspace(const tgx_paged* p, int heads, int group
   TGX_REQUIRE(bytes != nullptr, "null bytes");
   if (int st = check_attn(p, heads, group, D, dtype)) return st;
   const int64_t groups = static_cast<int64_t>(p->table_heads) * heads;
-  const Cut cut = cut_of(*p, groups * group * p->queries);
+  const Cut cut = cut_of(*p, workgroups_per_piece(*p, heads, group, D, dtype));
   *bytes = !cut.split ? 0
                       : meta_bytes(*p) + sizeof(float) * cut.launched * groups * group *
                                              p->queries * (D + 2);
@@ -389,9 +819,11 @@ extern "C" int tgx_paged_attn(const tgx_paged* p, const void* q_dev, const void*
   if (int st = tgx_paged_attn_workspace(p, heads, group, D, dtype, &need)) return st;
   TGX_REQUIRE(workspace_bytes >= need && (need == 0 || workspace_dev),
               "workspace of %zu bytes, needs %zu", workspace_bytes, need);
-  const Cut cut = cut_of(*p, static_cast<int64_t>(p->table_heads) * heads * group * p->queries);
+  const Cut cut = cut_of(*p, workgroups_per_piece(*p, heads, group, D, dtype));
   PagedArgs a{};
   a.rel = paged_rel(*p);
+  // Without pages there is no slot to read, whatever the lengths say.
+  if (p->num_pages == 0) a.rel.pages_per_seq = 0;
   a.q = q_dev;
   a.k = k_dev;
   a.v = v_dev;
@@ -408,9 +840,18 @@ extern "C" int tgx_paged_attn(const tgx_paged* p, const void* q_dev, const void*
     a.meta = static_cast<int2*>(workspace_dev);
     a.partial = reinterpret_cast<float*>(static_cast<char*>(workspace_dev) + meta_bytes(*p));
   }
+  hipStream_t s = as_stream(stream);
+  const bool tiles = tiled(D, dtype);
+  int st;
   switch (dtype) {
-    case TGX_DTYPE_BF16: return dispatch_rows<TGX_DTYPE_BF16>(a, cut, as_stream(stream));
-    case TGX_DTYPE_F16: return dispatch_rows<TGX_DTYPE_F16>(a, cut, as_stream(stream));
-    default: return dispatch_rows<TGX_DTYPE_F32>(a, cut, as_stream(stream));
+    case TGX_DTYPE_BF16:
+      st = tiles ? dispatch_tiles<__bf16>(a, cut, s) : dispatch_rows<TGX_DTYPE_BF16>(a, cut, s);
+      return st || !cut.split ? st : dispatch_join<TGX_DTYPE_BF16>(a, s);
+    case TGX_DTYPE_F16:
+      st = tiles ? dispatch_tiles<_Float16>(a, cut, s) : dispatch_rows<TGX_DTYPE_F16>(a, cut, s);
+      return st || !cut.split ? st : dispatch_join<TGX_DTYPE_F16>(a, s);
+    default:
+      st = dispatch_rows<TGX_DTYPE_F32>(a, cut, s);
+      return st || !cut.split ? st : dispatch_join<TGX_DTYPE_F32>(a, s);
   }
 }
