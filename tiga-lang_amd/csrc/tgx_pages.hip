@@ -151,21 +151,95 @@ __device__ __forceinline__ uint64_t ordered(double s) {
   return u >> 63 ? ~u : u | (uint64_t{1} << 63);
 }
 
-// One thread per (row, head, full page): the whole dot product.
+// Whether the row's pages have to be ranked: fewer are wanted than there are.
+__device__ __forceinline__ bool ranked(int pages, int count) { return count > 1 && pages > count; }
+
+// Pages a workgroup of the scores covers: four waves, eight lanes a page, kUnroll
+// pages a lane group.
+constexpr int kUnroll = 4;
+constexpr int kScorePages = 4 * 8 * kUnroll;
+
+// Scores of kScorePages pages of one (row, head).  Eight lanes hold a page's
+// D sums, 4 NJ values each, in 16-byte loads that make whole 128-byte lines;
+// the lane's queries are summed over the group once, in fp64.  Bound: the
+// page sums are read once, 4 D bytes a page and head; kUnroll pages' loads
+// are issued before the first is used.
+template <int DT, int NJ>
+__global__ __launch_bounds__(256) void select_score_kernel(SelectArgs a) {
+  using C = Cell<DT, 1>;
+  const PagedRel& r = a.rel;
+  const int pair = blockIdx.x % (a.heads * r.n_seqs * r.queries);   // heads fastest
+  const int h = pair % a.heads, row = pair / a.heads;
+  const int limit = row_limit(r, row);
+  const int pages = (limit + r.page_size - 1) / r.page_size;
+  const int page0 = (blockIdx.x / (a.heads * r.n_seqs * r.queries)) * kScorePages;
+  if (!ranked(pages, a.count) || page0 >= pages - 1) return;
+  const int lane = lane_id(), part = lane & 7, wave = threadIdx.x >> 6;
+  const int32_t* ids = r.table + (row / r.queries) * r.seq_stride;
+  int id[kUnroll];
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const int page = page0 + (wave * kUnroll + u) * 8 + (lane >> 3);
+    id[u] = page < pages - 1 ? ids[page] : -1;
+  }
+  f32x4 s[kUnroll][NJ];
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const bool named = static_cast<unsigned>(id[u]) < static_cast<unsigned>(r.num_pages);
+    const float* p = a.sums + (static_cast<int64_t>(named ? id[u] : 0) * a.heads + h) * a.D;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const int d = 4 * (8 * j + part);
+      s[u][j] = d < a.D && named ? *reinterpret_cast<const f32x4*>(p + d)
+                                 : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+  const auto* q = static_cast<const typename C::T*>(a.q) + row * a.qs_row + h * a.qs_head;
+  double sum[NJ][4];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int d = 4 * (8 * j + part) + i;
+      sum[j][i] = 0.0;
+      for (int g = 0; d < a.D && g < a.group; ++g) {
+        float f[1] = {0.f};
+        C::add(C::load(q + g * a.qs_group + d), f);
+        sum[j][i] += f[0];
+      }
+    }
+  uint64_t* keys = a.keys + static_cast<int64_t>(pair) * r.pages_per_seq;
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    double score = 0.0;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) score += sum[j][i] * static_cast<double>(s[u][j][i]);
+#pragma unroll
+    for (int mask = 1; mask < 8; mask <<= 1) score += __shfl_xor(score, mask, 64);
+    if (static_cast<unsigned>(id[u]) >= static_cast<unsigned>(r.num_pages))
+      score = -__builtin_huge_val();
+    const int page = page0 + (wave * kUnroll + u) * 8 + (lane >> 3);
+    if (part == 0 && page < pages - 1) keys[page] = ordered(score);
+  }
+}
+
+// The same for widths the lanes do not hold: a thread per page.
 template <int DT>
-__global__ __launch_bounds__(256) void select_score_kernel(SelectArgs a, int64_t items) {
+__global__ __launch_bounds__(256) void select_score_any_kernel(SelectArgs a, int64_t items) {
+  using C = Cell<DT, 1>;
   const PagedRel& r = a.rel;
   for (int64_t item = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; item < items;
        item += static_cast<int64_t>(gridDim.x) * 256) {
     const int page = static_cast<int>(item % r.pages_per_seq);
     const int h = static_cast<int>(item / r.pages_per_seq % a.heads);
     const int row = static_cast<int>(item / r.pages_per_seq / a.heads);
-    const int limit = row_limit(r, row);
-    if (page >= (limit + r.page_size - 1) / r.page_size - 1) continue;
+    const int pages = (row_limit(r, row) + r.page_size - 1) / r.page_size;
+    if (!ranked(pages, a.count) || page >= pages - 1) continue;
     const int id = r.table[(row / r.queries) * r.seq_stride + page];
     double score = -__builtin_huge_val();
     if (static_cast<unsigned>(id) < static_cast<unsigned>(r.num_pages)) {
-      using C = Cell<DT, 1>;
       const auto* q = static_cast<const typename C::T*>(a.q) + row * a.qs_row + h * a.qs_head;
       const float* s = a.sums + (static_cast<int64_t>(id) * a.heads + h) * a.D;
       score = 0.0;
@@ -183,31 +257,28 @@ __global__ __launch_bounds__(256) void select_score_kernel(SelectArgs a, int64_t
   }
 }
 
-// Rank of this thread among the workgroup's threads with `flag` set, and their number.
-__device__ __forceinline__ int block_rank(bool flag, int* wave_counts, int& total) {
-  const unsigned long long set = __ballot(flag);
-  const int lane = lane_id(), wave = threadIdx.x >> 6;
-  __syncthreads();
-  if (lane == 0) wave_counts[wave] = __popcll(set);
-  __syncthreads();
-  int before = __popcll(set & ((1ull << lane) - 1));
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    if (w < wave) before += wave_counts[w];
-    total += wave_counts[w];
-  }
-  return before;
-}
+// One workgroup per (row, head) takes the `want` largest of n keys.  Byte by
+// byte from the top, a histogram of the keys that share the bytes before finds
+// the byte of the want-th largest; as soon as no more than THREADS keys share
+// it they are ranked against each other, and (last, last_page) is the key and
+// page of the want-th: a page is taken when its key is larger, or equal and the
+// page no later.  The first two bytes (sign, exponent, four bits) part most
+// scores; all eight are only gone through where more than THREADS are equal.
+// A thread's first kHeld keys stay in registers.  Bound: latency, of some four
+// barriers a pass.
+constexpr int kHeld = 8;
 
-// One workgroup per (row, head): the want-th largest key byte by byte from
-// the top, then the chosen pages in order of position.
-__global__ __launch_bounds__(256) void select_pages_kernel(SelectArgs a) {
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void select_pages_kernel(SelectArgs a) {
+  constexpr int WAVES = THREADS / 64;
   const PagedRel& r = a.rel;
   __shared__ int hist[256];
-  __shared__ int wave_counts[4];
-  __shared__ uint64_t sh_prefix;
-  __shared__ int sh_want;
+  __shared__ int counts[WAVES];
+  __shared__ int sh_byte, sh_left, sh_share, sh_n, sh_page;
+  __shared__ uint64_t sh_last;
+  __shared__ uint64_t cand[THREADS];
+  __shared__ int cand_page[THREADS];
+  const int tid = threadIdx.x, lane = lane_id(), wave = tid >> 6;
   const int h = blockIdx.x % a.heads;
   const int row = blockIdx.x / a.heads;
   const int limit = row_limit(r, row);
@@ -216,59 +287,152 @@ __global__ __launch_bounds__(256) void select_pages_kernel(SelectArgs a) {
   const int32_t* ids = r.table + (row / r.queries) * r.seq_stride;
   int32_t* out = a.table + static_cast<int64_t>(blockIdx.x) * a.count;
   const uint64_t* keys = a.keys + static_cast<int64_t>(blockIdx.x) * r.pages_per_seq;
-  for (int i = kept + threadIdx.x; i < a.count; i += 256) out[i] = -1;
-  if (threadIdx.x == 0 && h == 0)
+  for (int i = kept + tid; i < a.count; i += THREADS) out[i] = -1;
+  if (tid == 0 && h == 0)
     a.lengths[row] = kept ? (kept - 1) * r.page_size + limit - (pages - 1) * r.page_size : 0;
   if (kept == 0) return;
-  if (threadIdx.x == 0) out[kept - 1] = ids[pages - 1];
   const int n = pages - 1, want = kept - 1;
-  if (want == n) {
-    for (int i = threadIdx.x; i < n; i += 256) out[i] = ids[i];
+  if (!ranked(pages, a.count)) {
+    if (kept == pages)
+      for (int i = tid; i < pages; i += THREADS) out[i] = ids[i];
+    else if (tid == 0)
+      out[0] = ids[n];
     return;
   }
-  if (want == 0) return;
-  // Radix select: after each byte, `prefix` holds the want-th largest key's
-  // leading bytes and sh_want its rank among the keys that share them.
-  if (threadIdx.x == 0) {
-    sh_prefix = 0;
-    sh_want = want;
-  }
-  for (int shift = 56; shift >= 0; shift -= 8) {
-    hist[threadIdx.x] = 0;
+  if (tid == 0) out[want] = ids[n];
+  uint64_t held[kHeld];
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j) held[j] = j * THREADS + tid < n ? keys[j * THREADS + tid] : 0;
+  auto visit = [&](auto&& f) {
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j)
+      if (j * THREADS + tid < n) f(j * THREADS + tid, held[j]);
+    for (int i = kHeld * THREADS + tid; i < n; i += THREADS) f(i, keys[i]);
+  };
+
+  uint64_t prefix = 0, mask = 0;   // the bytes settled so far
+  int left = want;                 // rank of the want-th among the keys that share them
+  int share = n;
+  for (int shift = 56; share > THREADS && shift >= 0; shift -= 8) {
+    for (int i = tid; i < 256; i += THREADS) hist[i] = 0;
     __syncthreads();
-    const uint64_t prefix = sh_prefix;
-    for (int i = threadIdx.x; i < n; i += 256) {
-      const uint64_t key = keys[i];
-      if (shift == 56 || (key >> (shift + 8)) == (prefix >> (shift + 8)))
-        atomicAdd(&hist[(key >> shift) & 255], 1);
+    visit([&](int, uint64_t key) {
+      if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1);
+    });
+    __syncthreads();
+    if (wave == 0) {
+      // Keys in the bytes above the lane's four: lane 63 has the largest bytes.
+      int own[4], sum = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum += own[i] = hist[4 * lane + i];
+      int above = sum;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_down(above, d, 64);
+        if (lane + d < 64) above += o;
+      }
+      above -= sum;
+#pragma unroll
+      for (int i = 3; i >= 0; --i) {
+        if (above < left && left <= above + own[i]) {
+          sh_byte = 4 * lane + i;
+          sh_left = left - above;
+          sh_share = own[i];
+        }
+        above += own[i];
+      }
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-      int left = sh_want, byte = 255;
-      while (hist[byte] < left) left -= hist[byte--];
-      sh_want = left;
-      sh_prefix = prefix | (static_cast<uint64_t>(byte) << shift);
+    prefix |= static_cast<uint64_t>(sh_byte) << shift;
+    mask |= uint64_t{255} << shift;
+    left = sh_left;
+    share = sh_share;
+  }
+  uint64_t last = prefix;
+  int last_page = -1;    // -1: equal keys are counted off in order of position
+  if (share <= THREADS) {
+    if (tid == 0) sh_n = 0;
+    __syncthreads();
+    visit([&](int i, uint64_t key) {
+      if ((key & mask) == prefix) {
+        const int at = atomicAdd(&sh_n, 1);
+        cand[at] = key;
+        cand_page[at] = i;
+      }
+    });
+    __syncthreads();
+    if (tid < share) {
+      const uint64_t key = cand[tid];
+      const int page = cand_page[tid];
+      int rank = 0;
+      for (int i = 0; i < share; ++i)
+        rank += cand[i] > key || (cand[i] == key && cand_page[i] < page);
+      if (rank == left - 1) {
+        sh_last = key;
+        sh_page = page;
+      }
     }
     __syncthreads();
+    last = sh_last;
+    last_page = sh_page;
   }
-  const uint64_t last = sh_prefix;
-  const int equal = sh_want;   // of the pages with this score, the first so many
+  // The taken pages in order of position.
+  auto block_rank = [&](bool flag, int& total) {
+    const unsigned long long set = __ballot(flag);
+    __syncthreads();
+    if (lane == 0) counts[wave] = __popcll(set);
+    __syncthreads();
+    int before = __popcll(set & ((1ull << lane) - 1));
+    total = 0;
+    for (int w = 0; w < WAVES; ++w) {
+      if (w < wave) before += counts[w];
+      total += counts[w];
+    }
+    return before;
+  };
   int placed = 0, seen = 0;
-  for (int i0 = 0; i0 < n; i0 += 256) {
-    const int i = i0 + threadIdx.x;
-    const uint64_t key = i < n ? keys[i] : 0;
-    const bool tie = i < n && key == last;
-    int ties, taken;
-    const int tie_rank = block_rank(tie, wave_counts, ties);
-    const bool take = i < n && (key > last || (tie && seen + tie_rank < equal));
-    const int at = block_rank(take, wave_counts, taken);
+  auto place = [&](int i, uint64_t key) {
+    bool take = i < n && (key > last || (key == last && i <= last_page));
+    if (last_page < 0) {
+      int ties;
+      const bool tie = i < n && key == last;
+      const int tie_rank = block_rank(tie, ties);
+      take = i < n && (key > last || (tie && seen + tie_rank < left));
+      seen += ties;
+    }
+    int taken;
+    const int at = block_rank(take, taken);
     if (take) out[placed + at] = ids[i];
     placed += taken;
-    seen += ties;
-  }
+  };
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j)
+    if (j * THREADS < n) place(j * THREADS + tid, held[j]);
+  for (int i0 = kHeld * THREADS; i0 < n; i0 += THREADS)
+    place(i0 + tid, i0 + tid < n ? keys[i0 + tid] : 0);
 }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+template <int DT>
+int launch_scores(const SelectArgs& a, hipStream_t s) {
+  const int64_t pairs = static_cast<int64_t>(a.rel.n_seqs) * a.rel.queries * a.heads;
+  const int64_t chunks = ceil_div(std::max(a.rel.pages_per_seq, 1), kScorePages);
+  TGX_PROFILE("select_score", s);
+  if (a.D % 4 == 0 && a.D <= 256 && aligned16(a.sums) && pairs * chunks <= kMaxBlocks256) {
+    const dim3 grid(static_cast<uint32_t>(pairs * chunks));
+    if (a.D <= 32) select_score_kernel<DT, 1><<<grid, dim3(256), 0, s>>>(a);
+    else if (a.D <= 64) select_score_kernel<DT, 2><<<grid, dim3(256), 0, s>>>(a);
+    else if (a.D <= 128) select_score_kernel<DT, 4><<<grid, dim3(256), 0, s>>>(a);
+    else select_score_kernel<DT, 8><<<grid, dim3(256), 0, s>>>(a);
+  } else {
+    const int64_t items = pairs * a.rel.pages_per_seq;
+    const dim3 grid(static_cast<uint32_t>(std::min(ceil_div(items, 256), kMaxBlocks256)));
+    select_score_any_kernel<DT><<<grid, dim3(256), 0, s>>>(a, items);
+  }
+  TGX_LAUNCHED("select_score");
+  return TGX_OK;
+}
 
 template <int DT>
 int launch_append(const AppendArgs& a, bool vec, hipStream_t stream) {
@@ -287,7 +451,7 @@ int check_select(const tgx_paged* p, int heads, int group, int D, int count) {
   TGX_REQUIRE(p->table_heads == 1, "pages are selected from one table per sequence");
   TGX_REQUIRE(heads >= 1 && group >= 1 && D >= 1 && count >= 1,
               "heads, group, head width and count must be positive");
-  TGX_REQUIRE(p->n_seqs * p->queries * heads <= kMaxBlocks256,
+  TGX_REQUIRE(p->n_seqs * p->queries * heads <= kMaxBlocks256 / 4,
               "page selection: too many rows and heads for one launch");
   return TGX_OK;
 }
@@ -371,25 +535,20 @@ extern "C" int tgx_select_pages(const tgx_paged* p, const void* q_dev, const int
   a.lengths = lengths_dev;
   a.keys = static_cast<uint64_t*>(workspace_dev);
   hipStream_t s = as_stream(stream);
-  const int64_t pairs = p->n_seqs * p->queries * heads;
-  const int64_t items = pairs * p->pages_per_seq;
-  if (items > 0) {
-    const dim3 grid(static_cast<uint32_t>(std::min(ceil_div(items, 256), kMaxBlocks256)));
-    TGX_PROFILE("select_score", s);
+  if (p->pages_per_seq > count && count > 1) {
+    int st;
     switch (dtype) {
-      case TGX_DTYPE_BF16:
-        select_score_kernel<TGX_DTYPE_BF16><<<grid, dim3(256), 0, s>>>(a, items);
-        break;
-      case TGX_DTYPE_F16:
-        select_score_kernel<TGX_DTYPE_F16><<<grid, dim3(256), 0, s>>>(a, items);
-        break;
-      default: select_score_kernel<TGX_DTYPE_F32><<<grid, dim3(256), 0, s>>>(a, items);
+      case TGX_DTYPE_BF16: st = launch_scores<TGX_DTYPE_BF16>(a, s); break;
+      case TGX_DTYPE_F16: st = launch_scores<TGX_DTYPE_F16>(a, s); break;
+      default: st = launch_scores<TGX_DTYPE_F32>(a, s);
     }
+    if (st) return st;
   }
-  TGX_LAUNCHED("select_score");
   {
     TGX_PROFILE("select_pages", s);
-    select_pages_kernel<<<dim3(static_cast<uint32_t>(pairs)), dim3(256), 0, s>>>(a);
+    const dim3 grid(static_cast<uint32_t>(p->n_seqs * p->queries * heads));
+    if (p->pages_per_seq <= 1024) select_pages_kernel<256><<<grid, dim3(256), 0, s>>>(a);
+    else select_pages_kernel<1024><<<grid, dim3(1024), 0, s>>>(a);
   }
   TGX_LAUNCHED("select_pages");
   return TGX_OK;
