@@ -140,35 +140,56 @@ struct Place {
   }
 };
 
-// cos and sin of the token's angle for the lane's N pairs; pairs past the
-// rotated ones turn by nothing.
-template <int N>
-__device__ __forceinline__ void turns(const RotaryArgs& a, int64_t token, int part,
-                                      const float (&freq)[N], float (&c)[N], float (&s)[N]) {
+// cos and sin of the token's angles, [pair][2] in `cs` (LDS of the wave): a
+// lane forms every 64th pair's, and all lanes read those of their own pairs.
+// Pairs past the rotated ones turn by nothing.
+template <int PAIRS>
+__device__ __forceinline__ void form_turns(const RotaryArgs& a, int64_t token,
+                                           const float (&freq)[PAIRS / 64 + 1], float* cs) {
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const int i = N * part + j;
-    if (i >= a.half) {
-      c[j] = 1.f;
-      s[j] = 0.f;
-      continue;
+  for (int k = 0; 64 * k < PAIRS; ++k) {
+    const int i = 64 * k + lane_id();
+    if (PAIRS % 64 && i >= PAIRS) break;
+    float sn = 0.f, c = 1.f;
+    if (i < a.half) {
+      const int axis = (i >= a.ends[0]) + (i >= a.ends[1]) + (i >= a.ends[2]);
+      const int64_t at = token * a.axes + axis;
+      const double pos = a.wide_positions
+                             ? static_cast<double>(static_cast<const int64_t*>(a.positions)[at])
+                             : static_cast<double>(static_cast<const int32_t*>(a.positions)[at]);
+      // The angle in half turns, without the whole turns; what its fp32 value
+      // leaves is put back to first order.
+      const double t = pos * static_cast<double>(freq[k]) * 0.15915494309189535;
+      const double u = 2.0 * (t - __builtin_rint(t));
+      const float uf = static_cast<float>(u);
+      const float rest = static_cast<float>((u - static_cast<double>(uf)) * 3.141592653589793);
+      float s0, c0;
+      sincospif(uf, &s0, &c0);
+      c = fmaf(-s0, rest, c0);
+      sn = fmaf(c0, rest, s0);
     }
-    const int axis = (i >= a.ends[0]) + (i >= a.ends[1]) + (i >= a.ends[2]);
-    const int64_t at = token * a.axes + axis;
-    const double pos = a.wide_positions
-                           ? static_cast<double>(static_cast<const int64_t*>(a.positions)[at])
-                           : static_cast<double>(static_cast<const int32_t*>(a.positions)[at]);
-    // The angle in half turns, without the whole turns; what its fp32 value
-    // leaves is put back to first order.
-    const double t = pos * static_cast<double>(freq[j]) * 0.15915494309189535;
-    const double u = 2.0 * (t - __builtin_rint(t));
-    const float uf = static_cast<float>(u);
-    const float rest = static_cast<float>((u - static_cast<double>(uf)) * 3.141592653589793);
-    float sn, cs;
-    sincospif(uf, &sn, &cs);
-    c[j] = fmaf(-sn, rest, cs);
-    s[j] = fmaf(cs, rest, sn);
+    cs[2 * i] = c;
+    cs[2 * i + 1] = sn;
   }
+}
+
+// The turns of pairs N * part .. N * part + N - 1.
+template <int N>
+__device__ __forceinline__ void read_turns(const float* cs, int part, float (&c)[N],
+                                           float (&s)[N]) {
+#pragma unroll
+  for (int j = 0; j < N; j += 2) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(cs + 2 * (N * part + j));
+    c[j] = v[0], s[j] = v[1], c[j + 1] = v[2], s[j + 1] = v[3];
+  }
+}
+
+// 1 / sqrt(v): the hardware's value and one Newton step.
+__device__ __forceinline__ float inverse_root(float v) {
+  const float r = __builtin_amdgcn_rsqf(v);
+  // (v = 0 or Inf: r is Inf or 0, and stays.)
+  const float e = fmaf(-v * r, r, 1.f);
+  return v > 0.f && v < __builtin_huge_valf() ? fmaf(0.5f * r, e, r) : r;
 }
 
 // Turns pair j of the chunks (f, g) by (c, s): the halves of the pairs lie in
@@ -202,126 +223,181 @@ struct Weights {
   }
 };
 
+// Passes of 64 / LPR rows whose loads are issued together.
+constexpr int kPasses = 4;
+
 template <int DT, int N, int LPR, bool INTER>
 __global__ __launch_bounds__(256) void norm_rotary_fwd_kernel(RotaryArgs a) {
   using C = Chunk<DT, N>;
   using T = typename C::T;
+  constexpr int RPP = 64 / LPR, PAIRS = N * LPR;
+  __shared__ __align__(16) float turns[4][2 * PAIRS];
+  float* cs = turns[threadIdx.x >> 6];
   const int lane = lane_id(), part = lane % LPR, sub = lane / LPR;
   const Place<N, INTER> at(a, part);
   Weights<N> w;
   w.load(a, at);
-  float freq[N];
+  float freq[PAIRS / 64 + 1];
 #pragma unroll
-  for (int j = 0; j < N; ++j) freq[j] = N * part + j < a.half ? a.freqs[N * part + j] : 0.f;
+  for (int k = 0; 64 * k < PAIRS; ++k) freq[k] = 64 * k + lane < a.half ? a.freqs[64 * k + lane] : 0.f;
   const int rows = a.heads[0] + a.heads[1];
   const int64_t items = a.tokens * a.split;
   const float inv_d = 1.f / static_cast<float>(a.D);
   for (int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); item < items;
        item += static_cast<int64_t>(gridDim.x) * 4) {
     const int64_t token = item / a.split;
+    const int step = a.split * RPP;
     float c[N], s[N];
-    turns<N>(a, token, part, freq, c, s);
-    for (int row = static_cast<int>(item % a.split) * (64 / LPR) + sub; row < rows;
-         row += a.split * (64 / LPR)) {
-      const int side = row >= a.heads[0];
-      const int head = row - (side ? a.heads[0] : 0);
-      const T* x = static_cast<const T*>(a.x[side]) + token * a.xs_token[side] +
-                   head * a.xs_head[side];
-      float f[N], g[N];
+    bool formed = false;
+    for (int row0 = static_cast<int>(item % a.split) * RPP + sub; row0 - sub < rows;
+         row0 += kPasses * step) {
+      typename C::Raw first[kPasses], second[kPasses];
 #pragma unroll
-      for (int j = 0; j < N; ++j) f[j] = g[j] = 0.f;
-      if (at.has) {
-        C::unpack(C::load(x + at.first), f);
-        C::unpack(C::load(x + at.second), g);
-      }
-      if (a.norm) {
-        float ss = 0.f;
-#pragma unroll
-        for (int j = 0; j < N; ++j) ss += f[j] * f[j] + g[j] * g[j];
-        const float r = 1.f / sqrtf(group_sum<LPR>(ss) * inv_d + a.eps);
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-          f[j] *= r * (side ? w.f[1][j] : w.f[0][j]);
-          g[j] *= r * (side ? w.g[1][j] : w.g[0][j]);
+      for (int p = 0; p < kPasses; ++p) {
+        const int row = row0 + p * step;
+        const int side = row >= a.heads[0];
+        if (row < rows && at.has) {
+          const T* x = static_cast<const T*>(a.x[side]) + token * a.xs_token[side] +
+                       (row - (side ? a.heads[0] : 0)) * a.xs_head[side];
+          first[p] = C::load(x + at.first);
+          second[p] = C::load(x + at.second);
+        } else {
+          first[p] = typename C::Raw{};
+          second[p] = typename C::Raw{};
         }
       }
-      rotate<N, INTER>(f, g, c, s, 1.f);
-      if (at.has) {
-        T* y = static_cast<T*>(a.out[side]) + (token * a.heads[side] + head) * a.D;
-        C::store(y + at.first, f);
-        C::store(y + at.second, g);
+      if (!formed) {
+        form_turns<PAIRS>(a, token, freq, cs);
+        __builtin_amdgcn_wave_barrier();
+        read_turns<N>(cs, part, c, s);
+        formed = true;
+      }
+#pragma unroll
+      for (int p = 0; p < kPasses; ++p) {
+        const int row = row0 + p * step;
+        if (row - sub >= rows) break;
+        const int side = row >= a.heads[0];
+        float f[N], g[N];
+        C::unpack(first[p], f);
+        C::unpack(second[p], g);
+        if (a.norm) {
+          float ss = 0.f;
+#pragma unroll
+          for (int j = 0; j < N; ++j) ss += f[j] * f[j] + g[j] * g[j];
+          const float r = inverse_root(group_sum<LPR>(ss) * inv_d + a.eps);
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            f[j] *= r * (side ? w.f[1][j] : w.f[0][j]);
+            g[j] *= r * (side ? w.g[1][j] : w.g[0][j]);
+          }
+        }
+        rotate<N, INTER>(f, g, c, s, 1.f);
+        if (row < rows && at.has) {
+          T* y = static_cast<T*>(a.out[side]) +
+                 (token * a.heads[side] + row - (side ? a.heads[0] : 0)) * a.D;
+          C::store(y + at.first, f);
+          C::store(y + at.second, g);
+        }
       }
     }
   }
 }
 
+constexpr int kBwdPasses = 2;
+
 template <int DT, int N, int LPR, bool INTER>
 __global__ __launch_bounds__(256) void norm_rotary_bwd_kernel(RotaryArgs a) {
   using C = Chunk<DT, N>;
   using T = typename C::T;
+  constexpr int RPP = 64 / LPR, PAIRS = N * LPR;
+  __shared__ __align__(16) float turns[4][2 * PAIRS];
+  float* cs = turns[threadIdx.x >> 6];
   const int lane = lane_id(), part = lane % LPR, sub = lane / LPR;
   const Place<N, INTER> at(a, part);
   Weights<N> w;
   w.load(a, at);
-  float freq[N];
+  float freq[PAIRS / 64 + 1];
+#pragma unroll
+  for (int k = 0; 64 * k < PAIRS; ++k) freq[k] = 64 * k + lane < a.half ? a.freqs[64 * k + lane] : 0.f;
   float wf[2][N], wg[2][N];   // sums of g n
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    freq[j] = N * part + j < a.half ? a.freqs[N * part + j] : 0.f;
-    wf[0][j] = wf[1][j] = wg[0][j] = wg[1][j] = 0.f;
-  }
+  for (int j = 0; j < N; ++j) wf[0][j] = wf[1][j] = wg[0][j] = wg[1][j] = 0.f;
   const int64_t items = a.tokens * a.split;
   const float inv_d = 1.f / static_cast<float>(a.D);
   for (int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); item < items;
        item += static_cast<int64_t>(gridDim.x) * 4) {
     const int64_t token = item / a.split;
+    const int step = a.split * RPP;
     float c[N], s[N];
-    turns<N>(a, token, part, freq, c, s);
+    bool formed = false;
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
-      for (int head = static_cast<int>(item % a.split) * (64 / LPR) + sub; head < a.heads[side];
-           head += a.split * (64 / LPR)) {
-        const T* x = static_cast<const T*>(a.x[side]) + token * a.xs_token[side] +
-                     head * a.xs_head[side];
-        const int64_t flat = (token * a.heads[side] + head) * a.D;
-        const T* dy = static_cast<const T*>(a.dy[side]) + flat;
-        float f[N], g[N], df[N], dg[N];
+      const int heads = a.heads[side];
+      for (int head0 = static_cast<int>(item % a.split) * RPP + sub; head0 - sub < heads;
+           head0 += kBwdPasses * step) {
+        typename C::Raw x1[kBwdPasses], x2[kBwdPasses], d1[kBwdPasses], d2[kBwdPasses];
 #pragma unroll
-        for (int j = 0; j < N; ++j) f[j] = g[j] = df[j] = dg[j] = 0.f;
-        if (at.has) {
-          C::unpack(C::load(x + at.first), f);
-          C::unpack(C::load(x + at.second), g);
-          C::unpack(C::load(dy + at.first), df);
-          C::unpack(C::load(dy + at.second), dg);
-        }
-        rotate<N, INTER>(df, dg, c, s, -1.f);
-        if (a.norm) {
-          float ss = 0.f;
-#pragma unroll
-          for (int j = 0; j < N; ++j) ss += f[j] * f[j] + g[j] * g[j];
-          const float r = 1.f / sqrtf(group_sum<LPR>(ss) * inv_d + a.eps);
-          float hn = 0.f;
-#pragma unroll
-          for (int j = 0; j < N; ++j) {
-            f[j] *= r;
-            g[j] *= r;
-            wf[side][j] += df[j] * f[j];
-            wg[side][j] += dg[j] * g[j];
-            df[j] *= w.f[side][j];
-            dg[j] *= w.g[side][j];
-            hn += df[j] * f[j] + dg[j] * g[j];
-          }
-          hn = group_sum<LPR>(hn) * inv_d;
-#pragma unroll
-          for (int j = 0; j < N; ++j) {
-            df[j] = r * (df[j] - f[j] * hn);
-            dg[j] = r * (dg[j] - g[j] * hn);
+        for (int p = 0; p < kBwdPasses; ++p) {
+          const int head = head0 + p * step;
+          if (head < heads && at.has) {
+            const T* x = static_cast<const T*>(a.x[side]) + token * a.xs_token[side] +
+                         head * a.xs_head[side];
+            const T* dy = static_cast<const T*>(a.dy[side]) + (token * heads + head) * a.D;
+            x1[p] = C::load(x + at.first);
+            x2[p] = C::load(x + at.second);
+            d1[p] = C::load(dy + at.first);
+            d2[p] = C::load(dy + at.second);
+          } else {
+            x1[p] = x2[p] = d1[p] = d2[p] = typename C::Raw{};
           }
         }
-        if (at.has) {
-          T* dx = static_cast<T*>(a.out[side]) + flat;
-          C::store(dx + at.first, df);
-          C::store(dx + at.second, dg);
+        if (!formed) {
+          form_turns<PAIRS>(a, token, freq, cs);
+          __builtin_amdgcn_wave_barrier();
+          read_turns<N>(cs, part, c, s);
+          formed = true;
+        }
+#pragma unroll
+        for (int p = 0; p < kBwdPasses; ++p) {
+          const int head = head0 + p * step;
+          if (head - sub >= heads) break;
+          float f[N], g[N], df[N], dg[N];
+          C::unpack(x1[p], f);
+          C::unpack(x2[p], g);
+          C::unpack(d1[p], df);
+          C::unpack(d2[p], dg);
+          rotate<N, INTER>(df, dg, c, s, -1.f);
+          if (a.norm) {
+            float ss = 0.f;
+#pragma unroll
+            for (int j = 0; j < N; ++j) ss += f[j] * f[j] + g[j] * g[j];
+            const float r = inverse_root(group_sum<LPR>(ss) * inv_d + a.eps);
+            float hn = 0.f;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+              f[j] *= r;
+              g[j] *= r;
+              // (A row that is not there is zero, and with eps = 0 its r is Inf.)
+              if (head < heads) {
+                wf[side][j] += df[j] * f[j];
+                wg[side][j] += dg[j] * g[j];
+              }
+              df[j] *= w.f[side][j];
+              dg[j] *= w.g[side][j];
+              hn += df[j] * f[j] + dg[j] * g[j];
+            }
+            hn = group_sum<LPR>(hn) * inv_d;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+              df[j] = r * (df[j] - f[j] * hn);
+              dg[j] = r * (dg[j] - g[j] * hn);
+            }
+          }
+          if (head < heads && at.has) {
+            T* dx = static_cast<T*>(a.out[side]) + (token * heads + head) * a.D;
+            C::store(dx + at.first, df);
+            C::store(dx + at.second, dg);
+          }
         }
       }
     }
@@ -366,6 +442,9 @@ __global__ __launch_bounds__(256) void norm_rotary_dw_kernel(const float* partia
 
 bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
+// Workgroups at most: enough to fill the GPU, few enough that the weights and
+// frequencies a wave loads first serve many tokens.
+constexpr int64_t kFwdBlocks = 2048;
 constexpr int64_t kBwdBlocks = 1024;
 
 // Waves that share a token's rows: with few tokens, so many that the rows of a
@@ -514,7 +593,7 @@ extern "C" int tgx_norm_rotary_fwd(const tgx_norm_rotary* p, void* query_out_dev
   RotaryArgs a{};
   bool wide = true;
   if (int st = args_of(*p, out, nullptr, &a, &wide)) return st;
-  return run<false>(*p, a, wide, int64_t{1} << 20, as_stream(stream));
+  return run<false>(*p, a, wide, kFwdBlocks, as_stream(stream));
 }
 
 extern "C" int tgx_norm_rotary_bwd_workspace(const tgx_norm_rotary* p, size_t* bytes) {
