@@ -78,12 +78,14 @@ def bind_attention(graph, q, k, v, scale: float, heads: int, group: int):
     def launch(keep=(q, k, v)):
         out = torch.empty(shape, dtype=dtype, device=device)
         work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-        if out.numel():
-            with _native.on_device(out):
-                _native.call("tgx_paged_attn", state.native(), *tensors, strides, scale,
-                             out.data_ptr(), heads, group, D, code, _native.ptr(work), need,
-                             _native.stream_of(out))
+        with _native.on_device(out):
+            _native.call("tgx_paged_attn", state.native(), *tensors, strides, scale,
+                         out.data_ptr(), heads, group, D, code,
+                         work.data_ptr() if need else None, need, _native.stream_of(out))
         return out
+
+    if not q.numel():
+        return lambda: torch.empty(shape, dtype=dtype, device=device)
 
     return launch
 
@@ -96,20 +98,20 @@ def append(graph, key_cache, key, value_cache, value, page_sums) -> None:
     if not key_cache.is_cuda or key_cache.dtype not in DTYPES:
         _append_torch(state, key_cache, key, value_cache, value, page_sums)
         return
-    dense = lambda t: t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
-    key, value = dense(key), dense(value)
-    heads, D = key.shape[1:]
-    strides = (ctypes.c_int64 * 8)(*(s for t in (key_cache, key, value_cache, value)
-                                     for s in t.stride()[:2]))
-    if key.numel() == 0 or key_cache.numel() == 0:
+    rows, heads, D = key.shape
+    if D > 1:
+        key = key if key.stride(2) == 1 else key.contiguous()
+        value = value if value.stride(2) == 1 else value.contiguous()
+    if rows * heads * D == 0 or key_cache.shape[0] == 0:
         return
+    strides = (ctypes.c_int64 * 8)(*key_cache.stride()[:2], *key.stride()[:2],
+                                   *value_cache.stride()[:2], *value.stride()[:2])
     with _native.on_device(key_cache):
         _native.call("tgx_paged_append", state.native(), key_cache.data_ptr(), key.data_ptr(),
                      value_cache.data_ptr(), value.data_ptr(), strides, _native.ptr(page_sums),
                      heads, D, DTYPES[key.dtype], _native.stream_of(key_cache))
-    for t in (key_cache, value_cache, page_sums):
-        if t is not None:
-            torch.autograd.graph.increment_version(t)
+    torch.autograd.graph.increment_version(
+        (key_cache, value_cache) if page_sums is None else (key_cache, value_cache, page_sums))
 
 
 def _append_torch(state, key_cache, key, value_cache, value, page_sums) -> None:
@@ -145,6 +147,7 @@ def select(graph, query, page_sums, count: int, table, lengths) -> None:
     """Write the chosen pages of every (row, key head) to `table`
     [rows, heads, count] and the positions they hold to `lengths` [rows]."""
     state = graph.paged_state
+    query, page_sums = query.detach(), page_sums.detach()
     if not query.is_cuda or query.dtype not in DTYPES:
         _select_torch(state, query, page_sums, count, table, lengths)
         return
@@ -154,17 +157,19 @@ def select(graph, query, page_sums, count: int, table, lengths) -> None:
     if rows == 0:
         return
     relation = state.native()
-    bytes_ = ctypes.c_size_t()
-    _native.call("tgx_select_pages_workspace", relation, heads, count, ctypes.byref(bytes_))
-    work = torch.empty(bytes_.value, dtype=torch.uint8, device=query.device)
+    need = state.checked.get(("select-workspace", heads, count))
+    if need is None:
+        bytes_ = ctypes.c_size_t()
+        _native.call("tgx_select_pages_workspace", relation, heads, count, ctypes.byref(bytes_))
+        need = state.checked["select-workspace", heads, count] = bytes_.value
+    work = torch.empty(need, dtype=torch.uint8, device=query.device)
     strides = (ctypes.c_int64 * 3)(*query.stride()[:3])
     with _native.on_device(query):
         _native.call("tgx_select_pages", relation, query.data_ptr(), strides,
                      page_sums.data_ptr() if page_sums.numel() else None, heads, group, D,
                      DTYPES[query.dtype], count, table.data_ptr(), lengths.data_ptr(),
-                     work.data_ptr(), bytes_.value, _native.stream_of(query))
-    for t in (table, lengths):
-        torch.autograd.graph.increment_version(t)
+                     work.data_ptr(), need, _native.stream_of(query))
+    torch.autograd.graph.increment_version((table, lengths))
 
 
 def _select_torch(state, query, page_sums, count, table, lengths) -> None:

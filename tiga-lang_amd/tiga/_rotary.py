@@ -35,44 +35,64 @@ def covered(form: Form, query, key, weights) -> bool:
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """`t` with dense rows that start on two values."""
-    pair = 2 * t.element_size()
-    if t.numel() and (t.stride(-1) != 1 or t.stride(0) % 2 or t.stride(1) % 2):
+    s = t.stride()
+    if (s[2] != 1 or s[0] % 2 or s[1] % 2) and t.numel():
         t = t.contiguous()
-    return t if t.data_ptr() % pair == 0 else t.clone(memory_format=torch.contiguous_format)
+    return t if t.data_ptr() % (2 * t.element_size()) == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+_TEMPLATES: dict[tuple, _native.NormRotary] = {}
 
 
 def _operands(form: Form, query, key, query_weight, key_weight, positions, frequencies):
     """The native operands, and the tensors they point into."""
-    sides = [None if t is None else _rows(t) for t in (query, key)]
-    weights = [None if w is None else w.contiguous() for w in (query_weight, key_weight)]
-    p = _native.NormRotary()
-    for i, (x, w) in enumerate(zip(sides, weights)):
-        if x is not None:
-            p.x_dev[i] = x.data_ptr()
-            p.token_stride[i], p.head_stride[i] = x.stride(0), x.stride(1)
-            p.heads[i] = x.shape[1]
-        p.w_dev[i] = _native.ptr(w)
-    p.w_dtype = next((_DTYPES[w.dtype] for w in weights if w is not None), 2)
+    query, key = _rows(query), None if key is None else _rows(key)
+    spec = (form, query.dtype, query.shape, query.stride(),
+            None if key is None else (key.shape, key.stride()),
+            None if query_weight is None else query_weight.dtype,
+            None if key_weight is None else key_weight.dtype, positions.dtype)
+    template = _TEMPLATES.get(spec)
+    if template is None:
+        template = _native.NormRotary()
+        for i, x in enumerate((query, key)):
+            if x is not None:
+                template.token_stride[i], template.head_stride[i] = x.stride()[:2]
+                template.heads[i] = x.shape[1]
+        template.w_dtype = next((_DTYPES[w.dtype] for w in (query_weight, key_weight)
+                                 if w is not None), 2)
+        template.positions_bits = _native.idx_bits(positions)
+        template.axes = len(form.sections)
+        for i, n in enumerate(form.sections):
+            template.sections[i] = n
+        template.n_freqs = frequencies.numel()
+        template.norm, template.interleaved = int(form.norm), int(form.interleaved)
+        template.eps = form.eps
+        template.n_tokens, template.D = query.shape[0], query.shape[-1]
+        template.dtype = _DTYPES[query.dtype]
+        if len(_TEMPLATES) >= 1024:
+            _TEMPLATES.clear()
+        _TEMPLATES[spec] = template
+    p = _native.NormRotary.from_buffer_copy(template)
+    p.x_dev[0] = query.data_ptr()
+    if key is not None:
+        p.x_dev[1] = key.data_ptr()
+    weights = [query_weight, key_weight]
+    for i in (0, 1):
+        if weights[i] is not None:
+            weights[i] = weights[i].contiguous()
+            p.w_dev[i] = weights[i].data_ptr()
     p.positions_dev, p.freqs_dev = positions.data_ptr(), frequencies.data_ptr()
-    p.positions_bits = _native.idx_bits(positions)
-    p.axes = len(form.sections)
-    for i, n in enumerate(form.sections):
-        p.sections[i] = n
-    p.n_freqs = frequencies.numel()
-    p.norm, p.interleaved, p.eps = int(form.norm), int(form.interleaved), form.eps
-    p.n_tokens, p.D = query.shape[0], query.shape[-1]
-    p.dtype = _DTYPES[query.dtype]
-    return p, (*sides, *weights, positions, frequencies)
+    return p, (query, key, *weights, positions, frequencies)
 
 
 def forward(form: Form, query, key, query_weight, key_weight, positions, frequencies):
     p, keep = _operands(form, query, key, query_weight, key_weight, positions, frequencies)
-    outs = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)
-            for t in (query, key)]
+    out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    key_out = None if key is None else torch.empty(key.shape, dtype=key.dtype, device=key.device)
     with _native.on_device(query):
-        _native.call("tgx_norm_rotary_fwd", ctypes.byref(p), _native.ptr(outs[0]),
-                     _native.ptr(outs[1]), _native.stream_of(query))
-    return outs
+        _native.call("tgx_norm_rotary_fwd", ctypes.byref(p), out.data_ptr(),
+                     None if key is None else key_out.data_ptr(), _native.stream_of(query))
+    return out, key_out
 
 
 class NormRotaryFunction(torch.autograd.Function):
@@ -84,7 +104,7 @@ class NormRotaryFunction(torch.autograd.Function):
         ctx.save_for_backward(query, key, query_weight, key_weight, positions, frequencies)
         ctx.set_materialize_grads(True)
         outs = forward(form, query, key, query_weight, key_weight, positions, frequencies)
-        return outs[0] if key is None else tuple(outs)
+        return outs[0] if key is None else outs
 
     @staticmethod
     @once_differentiable
@@ -115,12 +135,12 @@ class NormRotaryFunction(torch.autograd.Function):
 
 
 def apply(form: Form, query, key, query_weight, key_weight, positions, frequencies):
-    tensors = [t for t in (query, key, query_weight, key_weight) if t is not None]
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+    if torch.is_grad_enabled() and any(
+            [t is not None and t.requires_grad for t in (query, key, query_weight, key_weight)]):
         return NormRotaryFunction.apply(query, key, query_weight, key_weight, positions,
                                         frequencies, form)
     outs = forward(form, query, key, query_weight, key_weight, positions, frequencies)
-    return outs[0] if key is None else tuple(outs)
+    return outs[0] if key is None else outs
 
 
 def reference(form: Form, query, key, query_weight, key_weight, positions, frequencies):
@@ -130,6 +150,7 @@ def reference(form: Form, query, key, query_weight, key_weight, positions, frequ
     axis = torch.repeat_interleave(
         torch.arange(len(form.sections), device=query.device),
         torch.tensor(form.sections, device=query.device), output_size=half)
+    positions = positions[:, None] if positions.ndim == 1 else positions
     angle = (positions.double()[:, axis] * frequencies.double())[:, None]
 
     def one(x, weight):

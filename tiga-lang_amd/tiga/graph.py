@@ -61,6 +61,11 @@ class PagedState:
     num_pages: int
     queries: int
 
+    def __post_init__(self):
+        self._native = None
+        # Operand shapes and layouts that append and select_pages have checked.
+        self.checked: dict[tuple, object] = {}
+
     @property
     def table_heads(self) -> int:
         return self.page_table.shape[1] if self.page_table.ndim == 3 else 1
@@ -68,10 +73,14 @@ class PagedState:
     def native(self):
         """The relation as the native entry points take it."""
         t = self.page_table
-        return ctypes.byref(_native.Paged(
-            t.data_ptr() if t.numel() else None, t.stride(0), t.stride(1) if t.ndim == 3 else 0,
-            self.lengths.data_ptr() if self.lengths.numel() else None, t.shape[0],
-            self.table_heads, t.shape[-1], self.page_size, self.num_pages, self.queries))
+        if self._native is None:
+            self._native = _native.Paged(
+                None, t.stride(0), t.stride(1) if t.ndim == 3 else 0, None, t.shape[0],
+                self.table_heads, t.shape[-1], self.page_size, self.num_pages, self.queries)
+            self._native_ref = ctypes.byref(self._native)
+        self._native.page_table_dev = t.data_ptr() or None
+        self._native.lengths_dev = self.lengths.data_ptr() or None
+        return self._native_ref
 
     def clamped_lengths(self) -> torch.Tensor:
         """Cached tokens of each sequence that its page table can hold, int64."""
@@ -81,6 +90,13 @@ class PagedState:
         """Positions each query row sees, int64 [sequences, queries]."""
         back = torch.arange(self.queries - 1, -1, -1, device=self.lengths.device)
         return (self.clamped_lengths()[:, None] - back).clamp(min=0)
+
+
+def _paged():
+    """The launches over paged relations (a module that imports this one's users)."""
+    from . import _paged as module
+
+    return module
 
 
 class RowPlanHandle:
@@ -547,8 +563,22 @@ class Graph:
 
         Each sequence's written pages must be its own; two sequences writing
         to one page leave either's rows there."""
-        from . import _paged
+        state = self.paged_state
+        tensors = (key_cache, key, value_cache, value, page_sums)
+        try:
+            spec = tuple([None if x is None else (x.dtype, x.shape, x.stride(), x.device)
+                          for x in tensors])
+        except AttributeError:
+            spec = None
+        if state is None or spec is None or ("append", spec) not in state.checked:
+            self._check_append(*tensors)
+            state.checked["append", spec] = True
+        if torch.is_grad_enabled() and any([x is not None and x.requires_grad for x in tensors]):
+            raise NotImplementedError("append has no gradient: detach its operands or run it "
+                                      "under torch.no_grad()")
+        _paged().append(self, key_cache, key, value_cache, value, page_sums)
 
+    def _check_append(self, key_cache, key, value_cache, value, page_sums) -> None:
         state = self._paged_only("append")
         rows, slots = self._schema.num_dst, self._schema.num_src
         tensors = {"key_cache": key_cache, "key": key, "value_cache": value_cache, "value": value}
@@ -580,11 +610,6 @@ class Graph:
             if page_sums.device != self.device:
                 raise ValueError(f"page_sums is on {page_sums.device}, but graph is on "
                                  f"{self.device}")
-            tensors["page_sums"] = page_sums
-        if torch.is_grad_enabled() and any(t.requires_grad for t in tensors.values()):
-            raise NotImplementedError("append has no gradient: detach its operands or run it "
-                                      "under torch.no_grad()")
-        _paged.append(self, key_cache, key, value_cache, value, page_sums)
 
     def select_pages(self, query: torch.Tensor, page_sums: torch.Tensor, count: int, *,
                      out: "Graph | None" = None) -> "Graph":
@@ -603,18 +628,44 @@ class Graph:
         D) on caches viewed as [slots * heads, 1, D].  With `out`, a relation
         returned for the same shapes before, its tables are rewritten in place
         (a prepared or captured launch over it then sees them)."""
-        from . import _paged
+        state = self.paged_state
+        try:
+            spec = ("select", query.dtype, query.shape, query.device, page_sums.dtype,
+                    page_sums.shape, page_sums.stride(), page_sums.device, count, type(count))
+        except AttributeError:
+            spec = None
+        if state is None or spec is None or spec not in state.checked:
+            self._check_select(query, page_sums, count)
+            state.checked[spec] = True
+        if query.ndim == 3:
+            query = query[:, :, None]
+        shape = (query.shape[0], query.shape[1], count)
+        if out is None:
+            table = torch.empty(shape, dtype=torch.int32, device=self.device)
+            lengths = torch.empty(shape[0], dtype=torch.int32, device=self.device)
+            out = Graph.paged(table, lengths, page_size=state.page_size,
+                              num_pages=state.num_pages)
+        else:
+            got = getattr(out, "paged_state", None)
+            if got is None or got.page_table.shape != shape or got is state or \
+                    got.page_size != state.page_size or got.num_pages != state.num_pages or \
+                    got.queries != 1 or out.device != self.device or \
+                    not got.page_table.is_contiguous():
+                raise ValueError(f"out must be a relation that select_pages returned for {shape} "
+                                 "tables over the same cache")
+        _paged().select(self, query, page_sums, count, out.paged_state.page_table,
+                        out.paged_state.lengths)
+        return out
 
+    def _check_select(self, query, page_sums, count) -> None:
         state = self._paged_only("select_pages")
         if not isinstance(query, torch.Tensor) or not isinstance(page_sums, torch.Tensor):
             raise TypeError("query and page_sums must be torch.Tensor")
-        if query.ndim == 3:
-            query = query[:, :, None]
-        if query.ndim != 4 or query.shape[0] != self._schema.num_dst or \
+        if query.ndim not in (3, 4) or query.shape[0] != self._schema.num_dst or \
                 not query.is_floating_point() or min(query.shape[1:]) < 1:
             raise ValueError(f"query must be floating-point [{self._schema.num_dst}, heads, group, D]"
                              f", got {query.dtype} {tuple(query.shape)}")
-        heads, D = query.shape[1], query.shape[3]
+        heads, D = query.shape[1], query.shape[-1]
         if page_sums.dtype != torch.float32 or not page_sums.is_contiguous() or \
                 tuple(page_sums.shape) != (state.num_pages, heads, D):
             raise ValueError(f"page_sums must be contiguous float32 [{state.num_pages}, {heads}, {D}]"
@@ -624,23 +675,6 @@ class Graph:
                 raise ValueError(f"{name} is on {t.device}, but graph is on {self.device}")
         if not isinstance(count, int) or isinstance(count, bool) or count < 1:
             raise ValueError("count must be a positive integer")
-        shape = (self._schema.num_dst, heads, count)
-        if out is None:
-            table = torch.empty(shape, dtype=torch.int32, device=self.device)
-            lengths = torch.empty(shape[0], dtype=torch.int32, device=self.device)
-            out = Graph.paged(table, lengths, page_size=state.page_size,
-                              num_pages=state.num_pages)
-        else:
-            got = getattr(out, "paged_state", None)
-            if got is None or tuple(got.page_table.shape) != shape or got is state or \
-                    (got.page_size, got.num_pages, got.queries) != (state.page_size,
-                                                                    state.num_pages, 1) or \
-                    out.device != self.device or not got.page_table.is_contiguous():
-                raise ValueError(f"out must be a relation that select_pages returned for {shape} "
-                                 "tables over the same cache")
-        _paged.select(self, query.detach(), page_sums.detach(), count,
-                      out.paged_state.page_table, out.paged_state.lengths)
-        return out
 
     @classmethod
     def cat(cls, graphs) -> "Graph":
@@ -747,9 +781,7 @@ class Graph:
     def resolve_csr(self) -> tuple[torch.Tensor, torch.Tensor]:
         if self.is_paged:
             # As the tables stand now: never kept.
-            from . import _paged
-
-            return _paged.csr(self.paged_state)
+            return _paged().csr(self.paged_state)
         if self._row_ptr is None and self.is_dense:
             # Only an edge function no tile covers gets here (eager path).
             dtype, dev = self._schema.index_dtype, self.device

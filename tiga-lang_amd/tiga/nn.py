@@ -37,6 +37,8 @@ from dataclasses import dataclass
 import torch
 from torch import nn
 
+from . import _rotary
+
 # Score chains by module object: tracing a module with torch.fx costs
 # milliseconds, and edge() usually wraps the same module on every call.
 _CHAINS: "weakref.WeakKeyDictionary[nn.Module, object]" = weakref.WeakKeyDictionary()
@@ -422,9 +424,42 @@ def norm_rotary(query: torch.Tensor, key: torch.Tensor | None, positions: torch.
     of frequencies, at most 4 axes and weights of one type run on the HIP
     kernels; anything else, and host tensors, on Torch operations
     (``tiga.config.strict`` refuses those on the GPU)."""
-    from . import _rotary
+    tensors = (query, key, positions, frequencies, query_weight, key_weight)
+    try:
+        spec = (tuple([None if t is None else (t.dtype, t.shape, t.device) for t in tensors]),
+                eps, norm, sections, interleaved)
+        form = _ROTARY_FORMS.get(spec)
+    except (AttributeError, TypeError):
+        form = spec = None
+    if form is None:
+        form = _check_norm_rotary(*tensors, eps, norm, sections, interleaved)
+        if spec is not None:
+            if len(_ROTARY_FORMS) >= 1024:
+                _ROTARY_FORMS.clear()
+            _ROTARY_FORMS[spec] = form
+    form, run = form
+    if frequencies.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError("norm_rotary has no gradient with respect to frequencies")
+    if query.is_cuda and run is _rotary.reference and _config().strict:
+        raise RuntimeError("norm_rotary: no HIP kernel covers these types and widths and "
+                           "tiga.config.strict is set")
+    return run(form, query, key, query_weight, key_weight, positions.contiguous(),
+               frequencies.contiguous())
+
+
+# What norm_rotary found for operands of these types and shapes: its form and
+# whether the kernels take them.
+_ROTARY_FORMS: dict[tuple, tuple] = {}
+
+
+def _config():
     from .message_passing import config
 
+    return config
+
+
+def _check_norm_rotary(query, key, positions, frequencies, query_weight, key_weight, eps, norm,
+                       sections, interleaved):
     for name, t in (("query", query), ("key", key)):
         if t is None and name == "key":
             continue
@@ -445,14 +480,9 @@ def norm_rotary(query: torch.Tensor, key: torch.Tensor | None, positions: torch.
         raise TypeError("frequencies must be a float32 torch.Tensor")
     if frequencies.ndim != 1 or 2 * frequencies.numel() > D:
         raise ValueError(f"frequencies must be one-dimensional, at most {D // 2} for width {D}")
-    if frequencies.requires_grad and torch.is_grad_enabled():
-        raise NotImplementedError("norm_rotary has no gradient with respect to frequencies")
-    if positions.ndim == 1:
-        positions = positions[:, None]
-    if sections is None:
-        sections = (frequencies.numel(),)
-    sections = tuple(int(s) for s in sections)
-    if positions.ndim != 2 or positions.shape != (n, len(sections)):
+    sections = (frequencies.numel(),) if sections is None else tuple(int(s) for s in sections)
+    shape = tuple(positions.shape) if positions.ndim != 1 else (positions.shape[0], 1)
+    if shape != (n, len(sections)):
         raise ValueError(f"positions must be [{n}] or [{n}, {len(sections)}] for {len(sections)} "
                          f"sections, got {tuple(positions.shape)}")
     if any(s < 0 for s in sections) or sum(sections) != frequencies.numel():
@@ -469,19 +499,12 @@ def norm_rotary(query: torch.Tensor, key: torch.Tensor | None, positions: torch.
         raise ValueError("key_weight needs a key")
     if norm and not eps >= 0.0:
         raise ValueError("eps must not be negative")
-    given = [t for t in (key, positions, frequencies, query_weight, key_weight) if t is not None]
-    for t in given:
-        if t.device != query.device:
+    for t in (key, positions, frequencies, query_weight, key_weight):
+        if t is not None and t.device != query.device:
             raise ValueError(f"operand on {t.device}, but query is on {query.device}")
     form = _rotary.Form(float(eps), bool(norm), sections, bool(interleaved))
-    args = (form, query, key, query_weight, key_weight, positions.contiguous(),
-            frequencies.contiguous())
-    if _rotary.covered(form, query, key, (query_weight, key_weight)):
-        return _rotary.apply(*args)
-    if query.is_cuda and config.strict:
-        raise RuntimeError("norm_rotary: no HIP kernel covers these types and widths and "
-                           "tiga.config.strict is set")
-    return _rotary.reference(*args)
+    covered = _rotary.covered(form, query, key, (query_weight, key_weight))
+    return form, _rotary.apply if covered else _rotary.reference
 
 
 __all__ = ["ScoreLayer", "TracedModule", "norm_rotary", "trace"]
