@@ -838,7 +838,7 @@ int tgx_paged_attn(const tgx_paged* p, const void* q_dev, const void* k_dev, con
  * queries + t of key and value, `heads` rows of D values each; tokens at
  * positions below zero do not exist.  Page sums, if given (fp32
  * [num_pages, heads, D] contiguous), of every page a token was written to are
- * formed again over the page's slots up to the newest token, in slot order.
+ * formed again over the page's slots up to the newest token, in one fixed order.
  * The pages that sequences append to must be their own.
  *   strides, host array of eight, in elements: key cache's slot and head, key's
  *     row and head, value cache's slot and head, value's row and head */

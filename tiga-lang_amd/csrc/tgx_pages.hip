@@ -5,7 +5,7 @@
 // (those below zero do not exist), are rows b * queries + t of the new keys
 // and values; each goes to its slot.  With page sums, every touched page's
 // sum is formed again from the page's first row to its newest token, in fp32
-// and in slot order: a sum depends on what the page holds now and on nothing
+// and in one order: a sum depends on what the page holds now and on nothing
 // before it, so a program that takes tokens back and writes others keeps
 // right sums.
 //
@@ -77,16 +77,29 @@ struct Cell<DT, 1> {
   }
 };
 
-// One workgroup per (sequence, touched page); a thread per N values of a row.
+// One workgroup per (sequence, touched page, kCells cells of N values of a
+// row): kSlices threads share a cell, thread s taking the page's slots s, s +
+// kSlices, ..., kBatch of them in flight at once; their sums are added in the
+// order of s, so a page's sum is in one fixed order however its rows came in.
+// Bound: memory for prompts (rows read and written once), latency for a
+// single token.
+constexpr int kCells = 32, kSlices = 8, kBatch = 4;
+
 template <int DT, int N>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   using C = Cell<DT, N>;
   using T = typename C::T;
+  using Raw = typename C::Raw;
+  __shared__ float part[kSlices][kCells][N + 1];
   const PagedRel& r = a.rel;
-  const int b = blockIdx.x / a.touched;
+  const int per_head = a.D / N, cells = a.heads * per_head;
+  const int blocks = (cells + kCells - 1) / kCells;
+  const int cell = blockIdx.x % blocks * kCells + threadIdx.x % kCells;
+  const int slice = threadIdx.x / kCells;
+  const int b = blockIdx.x / blocks / a.touched;
   const int length = paged_length(r, b);
   const int fresh = min(length, r.queries);        // new tokens that exist
-  const int page = (length - fresh) / r.page_size + blockIdx.x % a.touched;
+  const int page = (length - fresh) / r.page_size + blockIdx.x / blocks % a.touched;
   const int base = page * r.page_size;             // position of the page's first slot
   if (fresh == 0 || base >= length) return;
   const int id = r.table[b * r.seq_stride + page];
@@ -94,32 +107,51 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   const int held = min(length - base, r.page_size);
   const int old = max(length - fresh - base, 0);   // slots filled before this call
   const int64_t slot0 = static_cast<int64_t>(id) * r.page_size;
-  // New row of the page's slot `old`.
-  const int64_t row0 = static_cast<int64_t>(b) * r.queries + (base + old) - (length - r.queries);
-  const int per_head = a.D / N;
-  for (int i = threadIdx.x; i < a.heads * per_head; i += 256) {
-    const int h = i / per_head, d = i % per_head * N;
+  // Where the new row of the page's slot 0 would be.
+  const int64_t row0 = static_cast<int64_t>(b) * r.queries + base - (length - r.queries);
+  float s[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) s[j] = 0.f;
+  const int h = cell / per_head, d = cell % per_head * N;
+  if (cell < cells) {
     T* kc = static_cast<T*>(a.kc) + slot0 * a.kc_slot + h * a.kc_head + d;
     T* vc = static_cast<T*>(a.vc) + slot0 * a.vc_slot + h * a.vc_head + d;
     const T* k = static_cast<const T*>(a.k) + row0 * a.k_row + h * a.k_head + d;
     const T* v = static_cast<const T*>(a.v) + row0 * a.v_row + h * a.v_head + d;
-    float s[N];
+    // Without sums the older slots are not read.
+    const int first = a.sums ? slice : slice + (max(old - slice, 0) + kSlices - 1) / kSlices * kSlices;
+    for (int o0 = first; o0 < held; o0 += kSlices * kBatch) {
+      Raw kr[kBatch], vr[kBatch];
 #pragma unroll
-    for (int j = 0; j < N; ++j) s[j] = 0.f;
-    if (a.sums)
-      for (int o = 0; o < old; ++o) C::add(C::load(kc + o * a.kc_slot), s);
-    for (int o = old; o < held; ++o) {
-      const typename C::Raw kr = C::load(k + (o - old) * a.k_row);
-      C::store(kc + o * a.kc_slot, kr);
-      C::store(vc + o * a.vc_slot, C::load(v + (o - old) * a.v_row));
-      if (a.sums) C::add(kr, s);
-    }
-    if (a.sums) {
-      float* dst = a.sums + (static_cast<int64_t>(id) * a.heads + h) * a.D + d;
+      for (int u = 0; u < kBatch; ++u) {
+        const int o = o0 + u * kSlices;
+        if (o >= held) continue;
+        kr[u] = C::load(o < old ? kc + o * a.kc_slot : k + o * a.k_row);
+        if (o >= old) vr[u] = C::load(v + o * a.v_row);
+      }
 #pragma unroll
-      for (int j = 0; j < N; ++j) dst[j] = s[j];
+      for (int u = 0; u < kBatch; ++u) {
+        const int o = o0 + u * kSlices;
+        if (o >= held) continue;
+        if (o >= old) {
+          C::store(kc + o * a.kc_slot, kr[u]);
+          C::store(vc + o * a.vc_slot, vr[u]);
+        }
+        if (a.sums) C::add(kr[u], s);
+      }
     }
   }
+  if (!a.sums) return;
+#pragma unroll
+  for (int j = 0; j < N; ++j) part[slice][threadIdx.x % kCells][j] = s[j];
+  __syncthreads();
+  const int c = threadIdx.x / N, j = threadIdx.x % N;   // one value a thread
+  const int out = blockIdx.x % blocks * kCells + c;
+  if (c >= kCells || out >= cells) return;
+  float sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < kSlices; ++w) sum += part[w][c][j];
+  a.sums[(static_cast<int64_t>(id) * a.heads + out / per_head) * a.D + out % per_head * N + j] = sum;
 }
 
 // ---------------------------------------------------------------------------
@@ -195,19 +227,23 @@ __global__ __launch_bounds__(256) void select_score_kernel(SelectArgs a) {
     }
   }
   const auto* q = static_cast<const typename C::T*>(a.q) + row * a.qs_row + h * a.qs_head;
+  __shared__ __align__(16) double summed[32 * NJ];
+  if (threadIdx.x < 32 * NJ) {
+    const int d = threadIdx.x;
+    double total = 0.0;
+    for (int g = 0; d < a.D && g < a.group; ++g) {
+      float f[1] = {0.f};
+      C::add(C::load(q + g * a.qs_group + d), f);
+      total += f[0];
+    }
+    summed[d] = total;
+  }
+  __syncthreads();
   double sum[NJ][4];
 #pragma unroll
   for (int j = 0; j < NJ; ++j)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int d = 4 * (8 * j + part) + i;
-      sum[j][i] = 0.0;
-      for (int g = 0; d < a.D && g < a.group; ++g) {
-        float f[1] = {0.f};
-        C::add(C::load(q + g * a.qs_group + d), f);
-        sum[j][i] += f[0];
-      }
-    }
+    for (int i = 0; i < 4; ++i) sum[j][i] = summed[4 * (8 * j + part) + i];
   uint64_t* keys = a.keys + static_cast<int64_t>(pair) * r.pages_per_seq;
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
@@ -260,10 +296,10 @@ __global__ __launch_bounds__(256) void select_score_any_kernel(SelectArgs a, int
 // One workgroup per (row, head) takes the `want` largest of n keys.  Byte by
 // byte from the top, a histogram of the keys that share the bytes before finds
 // the byte of the want-th largest; as soon as no more than THREADS keys share
-// it they are ranked against each other, and (last, last_page) is the key and
+// it a wave ranks them against each other, and (last, last_page) is the key and
 // page of the want-th: a page is taken when its key is larger, or equal and the
 // page no later.  The first two bytes (sign, exponent, four bits) part most
-// scores; all eight are only gone through where more than THREADS are equal.
+// scores; all eight are only gone through where more than 64 are equal.
 // A thread's first kHeld keys stay in registers.  Bound: latency, of some four
 // barriers a pass.
 constexpr int kHeld = 8;
@@ -276,8 +312,8 @@ __global__ __launch_bounds__(THREADS) void select_pages_kernel(SelectArgs a) {
   __shared__ int counts[WAVES];
   __shared__ int sh_byte, sh_left, sh_share, sh_n, sh_page;
   __shared__ uint64_t sh_last;
-  __shared__ uint64_t cand[THREADS];
-  __shared__ int cand_page[THREADS];
+  __shared__ uint64_t cand[64];
+  __shared__ int cand_page[64];
   const int tid = threadIdx.x, lane = lane_id(), wave = tid >> 6;
   const int h = blockIdx.x % a.heads;
   const int row = blockIdx.x / a.heads;
@@ -313,7 +349,7 @@ __global__ __launch_bounds__(THREADS) void select_pages_kernel(SelectArgs a) {
   uint64_t prefix = 0, mask = 0;   // the bytes settled so far
   int left = want;                 // rank of the want-th among the keys that share them
   int share = n;
-  for (int shift = 56; share > THREADS && shift >= 0; shift -= 8) {
+  for (int shift = 56; share > 64 && shift >= 0; shift -= 8) {
     for (int i = tid; i < 256; i += THREADS) hist[i] = 0;
     __syncthreads();
     visit([&](int, uint64_t key) {
@@ -350,7 +386,7 @@ __global__ __launch_bounds__(THREADS) void select_pages_kernel(SelectArgs a) {
   }
   uint64_t last = prefix;
   int last_page = -1;    // -1: equal keys are counted off in order of position
-  if (share <= THREADS) {
+  if (share <= 64) {
     if (tid == 0) sh_n = 0;
     __syncthreads();
     visit([&](int i, uint64_t key) {
@@ -361,13 +397,18 @@ __global__ __launch_bounds__(THREADS) void select_pages_kernel(SelectArgs a) {
       }
     });
     __syncthreads();
-    if (tid < share) {
-      const uint64_t key = cand[tid];
-      const int page = cand_page[tid];
+    if (wave == 0) {
+      const uint64_t key = lane < share ? cand[lane] : 0;
+      const int page = lane < share ? cand_page[lane] : 0;
+      const int key_hi = static_cast<int>(key >> 32), key_lo = static_cast<int>(key);
       int rank = 0;
-      for (int i = 0; i < share; ++i)
-        rank += cand[i] > key || (cand[i] == key && cand_page[i] < page);
-      if (rank == left - 1) {
+      for (int i = 0; i < share; ++i) {
+        const uint64_t other =
+            static_cast<uint64_t>(static_cast<uint32_t>(read_lane(key_hi, i))) << 32 |
+            static_cast<uint32_t>(read_lane(key_lo, i));
+        rank += other > key || (other == key && read_lane(page, i) < page);
+      }
+      if (lane < share && rank == left - 1) {
         sh_last = key;
         sh_page = page;
       }
@@ -436,7 +477,10 @@ int launch_scores(const SelectArgs& a, hipStream_t s) {
 
 template <int DT>
 int launch_append(const AppendArgs& a, bool vec, hipStream_t stream) {
-  const dim3 grid(static_cast<uint32_t>(static_cast<int64_t>(a.rel.n_seqs) * a.touched));
+  const int64_t blocks = static_cast<int64_t>(a.rel.n_seqs) * a.touched *
+                         ceil_div(static_cast<int64_t>(a.heads) * (vec ? a.D / 8 : a.D), kCells);
+  TGX_REQUIRE(blocks <= kMaxBlocks256, "append: too many pages and heads for one launch");
+  const dim3 grid(static_cast<uint32_t>(blocks));
   {
     TGX_PROFILE("paged_append", stream);
     if (vec) append_kernel<DT, 8><<<grid, dim3(256), 0, stream>>>(a);
