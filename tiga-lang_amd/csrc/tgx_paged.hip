@@ -84,6 +84,18 @@ __device__ __forceinline__ Piece find_piece(const PagedRel& r, int pieces, bool 
     return p;
   }
   const int lane = lane_id();
+  if (r.n_seqs == 1) {
+    p.length = paged_length(r, 0);
+    const int n = (p.length + kTile - 1) / kTile;
+    const int c = max(kMinTiles, (n + pieces - 1) / pieces);
+    p.count = max(1, (n + c - 1) / c);
+    if (x >= p.count) return p;
+    p.seq = 0;
+    p.index = x;
+    p.tile0 = static_cast<int>(static_cast<int64_t>(x) * n / p.count);
+    p.tile1 = static_cast<int>(static_cast<int64_t>(x + 1) * n / p.count);
+    return p;
+  }
   const int per = (r.n_seqs + 63) / 64;
   const int b0 = lane * per, b1 = min(r.n_seqs, b0 + per);
   int tiles = 0;
@@ -91,8 +103,11 @@ __device__ __forceinline__ Piece find_piece(const PagedRel& r, int pieces, bool 
   const int total = wave_sum(tiles);
   const int c = max(kMinTiles, (total + pieces - 1) / pieces);
   int mine = 0;
-  for (int b = b0; b < b1; ++b)
-    mine += max(1, ((paged_length(r, b) + kTile - 1) / kTile + c - 1) / c);
+  if (per == 1)
+    mine = b0 < b1 ? max(1, (tiles + c - 1) / c) : 0;
+  else
+    for (int b = b0; b < b1; ++b)
+      mine += max(1, ((paged_length(r, b) + kTile - 1) / kTile + c - 1) / c);
   int end = mine;   // inclusive prefix over the lanes
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
@@ -616,7 +631,9 @@ __global__ __launch_bounds__(256, (kTileBlocks<D, QT>)) void paged_tile_kernel(P
   }
 }
 
-// Joins the pieces of each (sequence, head, query) in a fixed order: a wave per query.
+// Joins the pieces of each (sequence, head, query), a workgroup per query: each
+// of its 256 / LPK lane groups takes every 256 / LPK-th piece, the next one's
+// loads in flight; groups and waves are then merged in a fixed order.
 template <int DT, int LPK>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
   using V = Vals<DT, 8>;
@@ -624,29 +641,58 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
   const PagedRel& r = a.rel;
   const int all_heads = r.heads * a.heads;
   const int rows = r.queries * a.group;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (item >= static_cast<int64_t>(r.n_seqs) * all_heads * rows) return;
+  const int64_t item = blockIdx.x;
   const int row = static_cast<int>(item % rows);
   const int head = static_cast<int>(item / rows % all_heads);
   const int b = static_cast<int>(item / rows / all_heads);
   const int2 m = a.meta[b];
   if (m.y <= 1) return;
-  const int lane = lane_id(), part = lane % LPK, sub = lane / LPK;
+  const int wave = threadIdx.x >> 6, lane = lane_id(), part = lane % LPK, sub = lane / LPK;
   const bool has = 8 * part < a.D;
   State8 s;
   s.init();
-  for (int j = sub; j < m.y; j += 64 / LPK) {
-    const float* src = a.partial +
-                       ((static_cast<int64_t>(m.x + j) * all_heads + head) * rows + row) *
-                           (a.D + 2);
-    float o[8];
+  const int64_t stride = static_cast<int64_t>(all_heads) * rows * (a.D + 2);
+  const float* src = a.partial + (static_cast<int64_t>(m.x) * all_heads + head) * rows * (a.D + 2) +
+                     static_cast<int64_t>(row) * (a.D + 2);
+  float o[8], om = kNegInf, ol = 0.f;
+  auto load = [&](int j) {
+    const bool there = j < m.y;
+    const float* p = src + (there ? j : 0) * stride;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = has ? src[8 * part + i] : 0.f;
-    s.merge(src[a.D], src[a.D + 1], o);
+    for (int i = 0; i < 8; ++i) o[i] = has ? p[8 * part + i] : 0.f;
+    om = there ? p[a.D] : kNegInf;
+    ol = p[a.D + 1];
+  };
+  const int first = wave * (64 / LPK) + sub;
+  load(first);
+  for (int j = first; j < m.y; j += 256 / LPK) {
+    float c[8], cm = om, cl = ol;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = o[i];
+    load(j + 256 / LPK);
+    s.merge(cm, cl, c);
   }
 #pragma unroll
   for (int mask = LPK; mask < 64; mask <<= 1) s.merge_xor(mask);
-  if (sub != 0 || !has) return;
+  __shared__ float ml[4][2];
+  __shared__ float acc[4][8 * LPK];
+  if (sub == 0) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[wave][8 * part + i] = s.acc[i];
+    if (part == 0) {
+      ml[wave][0] = s.m;
+      ml[wave][1] = s.l;
+    }
+  }
+  __syncthreads();
+  if (wave != 0 || sub != 0 || !has) return;
+#pragma unroll
+  for (int w = 1; w < 4; ++w) {
+    float c[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = acc[w][8 * part + i];
+    s.merge(ml[w][0], ml[w][1], c);
+  }
   const int th = head / a.heads, kh = head % a.heads;
   const int t = row / a.group, g = row % a.group;
   const int64_t q_row = (static_cast<int64_t>(b) * r.queries + t) * r.heads + th;
@@ -732,8 +778,7 @@ int launch_join(const PagedArgs& a, hipStream_t stream) {
   const int64_t queries = static_cast<int64_t>(a.rel.heads) * a.heads * a.rel.queries * a.group;
   TGX_PROFILE("paged_join", stream);
   paged_join_kernel<DT, LPK>
-      <<<dim3(static_cast<uint32_t>(ceil_div(a.rel.n_seqs * queries, 4))), dim3(256), 0,
-         stream>>>(a);
+      <<<dim3(static_cast<uint32_t>(a.rel.n_seqs * queries)), dim3(256), 0, stream>>>(a);
   TGX_LAUNCHED("paged_join");
   return TGX_OK;
 }
