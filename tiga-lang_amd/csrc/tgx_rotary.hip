@@ -427,17 +427,31 @@ __global__ __launch_bounds__(256) void norm_rotary_bwd_kernel(RotaryArgs a) {
   }
 }
 
-// dw[side][d] = sum over the workgroups of the backward, one wave per (side, d).
-__global__ __launch_bounds__(256) void norm_rotary_dw_kernel(const float* partial, int blocks,
-                                                             int D, int dtype, void* dwq,
-                                                             void* dwk) {
-  const int i = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (i >= 2 * D) return;
+// dw[side][d] = sum over the workgroups of the backward: 16 columns a
+// workgroup, 64 threads on each, whole 64-byte lines a load.
+__global__ __launch_bounds__(1024) void norm_rotary_dw_kernel(const float* partial, int blocks,
+                                                              int D, int dtype, void* dwq,
+                                                              void* dwk) {
+  __shared__ float sums[64][17];
+  const int col = threadIdx.x % 16, part = threadIdx.x / 16;
+  const int i = blockIdx.x * 16 + col;
   float s = 0.f;
-  for (int b = lane_id(); b < blocks; b += 64) s += partial[static_cast<int64_t>(b) * 2 * D + i];
-  s = group_sum<64>(s);
-  void* out = i < D ? dwq : dwk;
-  if (lane_id() == 0 && out) store_scalar(out, dtype, i % D, s);
+  if (i < 2 * D) {
+#pragma unroll 8
+    for (int b = part; b < blocks; b += 64) s += partial[static_cast<int64_t>(b) * 2 * D + i];
+  }
+  sums[part][col] = s;
+  __syncthreads();
+  if (threadIdx.x >= 64 * 16 / 4) return;
+  // Wave w adds the columns 4 w .. 4 w + 3.
+  const int wave = threadIdx.x >> 6, lane = lane_id();
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int c = 4 * wave + k, at = blockIdx.x * 16 + c;
+    const float total = group_sum<64>(sums[lane][c]);
+    void* out = at < D ? dwq : dwk;
+    if (lane == 0 && at < 2 * D && out) store_scalar(out, dtype, at % D, total);
+  }
 }
 
 bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
@@ -630,7 +644,7 @@ extern "C" int tgx_norm_rotary_bwd(const tgx_norm_rotary* p, const void* dquery_
   if (weights) {
     {
       TGX_PROFILE("norm_rotary_dw", as_stream(stream));
-      norm_rotary_dw_kernel<<<dim3(static_cast<uint32_t>(ceil_div(2 * p->D, 4))), dim3(256), 0,
+      norm_rotary_dw_kernel<<<dim3(static_cast<uint32_t>(ceil_div(2 * p->D, 16))), dim3(1024), 0,
                               as_stream(stream)>>>(a.partial, static_cast<int>(blocks), p->D,
                                                    p->w_dtype, dquery_weight_dev,
                                                    dkey_weight_dev);
