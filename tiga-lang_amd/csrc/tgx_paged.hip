@@ -15,9 +15,9 @@
 // Work split.  Lengths are only known on the device, so the launch is sized
 // from the host's bounds and every workgroup finds its piece itself: the keys
 // of all sequences, in tiles of 64, are cut into pieces of at most `c` tiles,
-// c the smallest number (at least kMinTiles) for which W pieces cover them
-// all; sequence b gets k_b = max(1, ceil(tiles_b / c)) pieces of equal size,
-// at most W + n_seqs together.  A sequence of one piece writes its output; of
+// c at least kMinTiles and just large enough for W pieces to cover them all;
+// sequence b gets k_b = max(1, ceil(tiles_b / c)) pieces of equal size, W
+// together where there are fewer than W / 2 sequences, W + n_seqs at most.  A sequence of one piece writes its output; of
 // several, each piece writes its running maximum, sum and unnormalized
 // output, which a second launch joins in piece order.
 #include <hip/hip_runtime.h>
@@ -72,6 +72,13 @@ __device__ __forceinline__ int wave_sum(int v) {
   return v;
 }
 
+// Cuts n tiles into p.count pieces whose sizes differ by one at most.
+__device__ __forceinline__ void cut_tiles(Piece& p, int n) {
+  const int each = n / p.count, more = n % p.count;
+  p.tile0 = p.index * each + min(p.index, more);
+  p.tile1 = p.tile0 + each + (p.index < more);
+}
+
 // Piece `x` of the launch; every wave finds it by itself.  Lane l looks
 // after the sequences [l, l + 1) * ceil(n / 64).
 __device__ __forceinline__ Piece find_piece(const PagedRel& r, int pieces, bool whole, int x) {
@@ -92,8 +99,7 @@ __device__ __forceinline__ Piece find_piece(const PagedRel& r, int pieces, bool 
     if (x >= p.count) return p;
     p.seq = 0;
     p.index = x;
-    p.tile0 = static_cast<int>(static_cast<int64_t>(x) * n / p.count);
-    p.tile1 = static_cast<int>(static_cast<int64_t>(x + 1) * n / p.count);
+    cut_tiles(p, n);
     return p;
   }
   const int per = (r.n_seqs + 63) / 64;
@@ -101,7 +107,9 @@ __device__ __forceinline__ Piece find_piece(const PagedRel& r, int pieces, bool 
   int tiles = 0;
   for (int b = b0; b < b1; ++b) tiles += (paged_length(r, b) + kTile - 1) / kTile;
   const int total = wave_sum(tiles);
-  const int c = max(kMinTiles, (total + pieces - 1) / pieces);
+  // Rounding up adds a piece a sequence at most, which are taken off first.
+  const int room = max(pieces - r.n_seqs, (pieces + 1) / 2);
+  const int c = max(kMinTiles, (total + room - 1) / room);
   int mine = 0;
   if (per == 1)
     mine = b0 < b1 ? max(1, (tiles + c - 1) / c) : 0;
@@ -129,9 +137,7 @@ __device__ __forceinline__ Piece find_piece(const PagedRel& r, int pieces, bool 
   p.length = read_lane(len, owner);
   p.count = read_lane(k, owner);
   p.index = x - read_lane(at, owner);
-  n = read_lane(n, owner);
-  p.tile0 = static_cast<int>(static_cast<int64_t>(p.index) * n / p.count);
-  p.tile1 = static_cast<int>(static_cast<int64_t>(p.index + 1) * n / p.count);
+  cut_tiles(p, read_lane(n, owner));
   return p;
 }
 
@@ -172,10 +178,10 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedArgs a) {
   const PagedRel& r = a.rel;
   const int all_heads = r.heads * a.heads;
   const int rows = r.queries * a.group;   // queries of one (sequence, head)
-  const int64_t item = blockIdx.x;
-  const int row = static_cast<int>(item % rows);
-  const int head = static_cast<int>(item / rows % all_heads);
-  const int x = static_cast<int>(item / rows / all_heads);
+  const unsigned item = blockIdx.x / static_cast<unsigned>(rows);
+  const int row = static_cast<int>(blockIdx.x % static_cast<unsigned>(rows));
+  const int head = static_cast<int>(item % static_cast<unsigned>(all_heads));
+  const int x = static_cast<int>(item / static_cast<unsigned>(all_heads));
   const Piece p = find_piece(r, a.pieces, a.meta == nullptr, x);
   if (p.seq < 0) return;
   const int th = head / a.heads, kh = head % a.heads;
@@ -319,34 +325,40 @@ constexpr int kRow = D == 128 ? 144 : D == 64 ? 80 : 48;
 // The running maximum only moves when a step's exceeds it by this (log2 units).
 constexpr float kRescaleLog2 = 8.f;
 
-// Workgroups per CU that the registers are held to, and keys a step: a step's K
-// and V fragments are D * KEYS / 64 registers.
+// Keys a step.  A step's K and V fragments are D / 2 registers; 64 keys a step
+// leave room for fewer workgroups (24 sequences of up to 3000 tokens, 16 heads
+// of 64: 47 us, 38 us with 32).
+constexpr int KEYS = 32;
+// Workgroups per CU that the registers are held to.  At D = 128 three would
+// need the fragments of K and V to share registers: measured equal.
 template <int D, int QT>
-constexpr int kTileBlocks = D == 128 && QT == 2 ? 1 : D == 128 || QT == 2 ? 2 : 3;
-template <int D, int QT>
-constexpr int kTileKeys = D == 128 || QT == 2 ? 32 : 64;
+constexpr int kTileBlocks = D == 128 && QT == 2 ? 1 : D == 128 || QT == 2 ? 2 : 4;
 
-template <int D, int QT, int KEYS>
+template <int D, int QT>
 struct TileShape {
   static constexpr size_t kStage = sizeof(uint16_t) * 4 * KEYS * kRow<D>;
   static constexpr size_t kJoin = sizeof(float) * 4 * 16 * QT * (D + 4 + 2);
-  static constexpr size_t kBytes = kStage > kJoin ? kStage : kJoin;
+  static constexpr size_t kWeights = sizeof(float) * 4 * KEYS * 16 * QT;
+  static constexpr size_t kBytes = kStage + kWeights > kJoin ? kStage + kWeights : kJoin;
 };
 
-template <typename T, int D, int QT, int KEYS>
+template <typename T, int D, int QT>
 __global__ __launch_bounds__(256, (kTileBlocks<D, QT>)) void paged_tile_kernel(PagedArgs a) {
   constexpr int KT = KEYS / 16, KC = D / 32, DT = D / 16, ROW = kRow<D>;
   using v8 = typename Frag<T>::v8;
   using v4 = typename Frag<T>::v4;
-  __shared__ __align__(16) char smem[TileShape<D, QT, KEYS>::kBytes];
+  __shared__ __align__(16) char smem[TileShape<D, QT>::kBytes];
   const PagedRel& r = a.rel;
   const int all_heads = r.heads * a.heads;
   const int rows = r.queries * a.group;
   const int row_groups = (rows + 16 * QT - 1) / (16 * QT);
-  const int64_t item = blockIdx.x;
-  const int row0 = static_cast<int>(item % row_groups) * (16 * QT);
-  const int head = static_cast<int>(item / row_groups % all_heads);
-  const int x = static_cast<int>(item / row_groups / all_heads);
+  // Workgroups go to the 8 XCDs in turn: the groups of queries that read the same
+  // keys are 8 apart, on one L2.
+  const unsigned of8 = blockIdx.x / 8u, groups = static_cast<unsigned>(row_groups);
+  const unsigned item = of8 / groups * 8u + blockIdx.x % 8u;
+  const int row0 = static_cast<int>(of8 % groups) * (16 * QT);
+  const int head = static_cast<int>(item % static_cast<unsigned>(all_heads));
+  const int x = static_cast<int>(item / static_cast<unsigned>(all_heads));
   const Piece p = find_piece(r, a.pieces, a.meta == nullptr, x);
   if (p.seq < 0) return;
   const int th = head / a.heads, kh = head % a.heads;
@@ -378,7 +390,10 @@ __global__ __launch_bounds__(256, (kTileBlocks<D, QT>)) void paged_tile_kernel(P
   const T* kb = static_cast<const T*>(a.k) + th * a.ks_table + kh * a.ks_head + 8 * g;
   const T* vb = static_cast<const T*>(a.v) + th * a.vs_table + kh * a.vs_head + 8 * g;
   const int32_t* table = r.table + p.seq * r.seq_stride + th * r.head_stride;
+  // The wave's staged V, and its weights where they are taken key by key.
   T* stage = reinterpret_cast<T*>(smem) + wave * KEYS * ROW;
+  float* weights = reinterpret_cast<float*>(smem + TileShape<D, QT>::kStage) +
+                   wave * KEYS * 16 * QT;
 
   // Steps of this wave: first + 4 i < last.  Lane l keeps the page id of key
   // l (mod KEYS) of a step.
@@ -553,21 +568,23 @@ __global__ __launch_bounds__(256, (kTileBlocks<D, QT>)) void paged_tile_kernel(P
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            for (int gk = 0; gk < 4; ++gk) {
-              const int key = 16 * kt + 4 * gk + i;
+          for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
-              for (int qt = 0; qt < QT; ++qt) {
-                const float w = __shfl(c[kt][qt][i], 16 * gk + lr, 64);
-                if (step * KEYS + key >= limit[qt]) continue;
+            for (int i = 0; i < 4; ++i)
+              weights[(16 * kt + 4 * g + i) * (16 * QT) + 16 * qt + lr] = c[kt][qt][i];
+#pragma unroll 1
+        for (int key = 0; key < KEYS; ++key)
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) {
-                  const v4 vv = *reinterpret_cast<const v4*>(stage + key * ROW + 16 * dt + 4 * g);
+          for (int qt = 0; qt < QT; ++qt) {
+            if (step * KEYS + key >= limit[qt]) continue;
+            const float w = weights[key * (16 * QT) + 16 * qt + lr];
 #pragma unroll
-                  for (int e = 0; e < 4; ++e) o[dt][qt][e] += w * static_cast<float>(vv[e]);
-                }
-              }
+            for (int dt = 0; dt < DT; ++dt) {
+              const v4 vv = *reinterpret_cast<const v4*>(stage + key * ROW + 16 * dt + 4 * g);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[dt][qt][e] += w * static_cast<float>(vv[e]);
             }
+          }
       }
       slot = next;
     }
@@ -641,10 +658,10 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
   const PagedRel& r = a.rel;
   const int all_heads = r.heads * a.heads;
   const int rows = r.queries * a.group;
-  const int64_t item = blockIdx.x;
-  const int row = static_cast<int>(item % rows);
-  const int head = static_cast<int>(item / rows % all_heads);
-  const int b = static_cast<int>(item / rows / all_heads);
+  const unsigned item = blockIdx.x / static_cast<unsigned>(rows);
+  const int row = static_cast<int>(blockIdx.x % static_cast<unsigned>(rows));
+  const int head = static_cast<int>(item % static_cast<unsigned>(all_heads));
+  const int b = static_cast<int>(item / static_cast<unsigned>(all_heads));
   const int2 m = a.meta[b];
   if (m.y <= 1) return;
   const int wave = threadIdx.x >> 6, lane = lane_id(), part = lane % LPK, sub = lane / LPK;
@@ -710,13 +727,15 @@ struct Cut {
   bool split;
 };
 
-// Workgroups wanted in all: what the GPU holds at once, several times over, so
-// that pieces of uneven length even out.
+// Workgroups wanted in all: what the GPU holds at once (two a CU at D = 128, four
+// below), twice over at D = 128.  Four of 100k to 131k tokens: 346 us with
+// two rounds that fit, 368-420 us with rounds that end half full; more and
+// smaller pieces pay for their first loads, fewer end unevenly.
 int64_t wanted_workgroups() {
   int dev = 0, cus = 256;
   if (hipGetDevice(&dev) == hipSuccess)
     (void)hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
-  return static_cast<int64_t>(cus) * 8;
+  return static_cast<int64_t>(cus) * 4;
 }
 
 Cut cut_of(const tgx_paged& p, int64_t groups) {
@@ -725,23 +744,6 @@ Cut cut_of(const tgx_paged& p, int64_t groups) {
   const int64_t wanted = std::max<int64_t>(1, wanted_workgroups() / groups);
   const int64_t most = p.n_seqs * ceil_div(tiles, kMinTiles);
   return Cut{wanted, std::min(wanted + p.n_seqs, most), true};
-}
-
-int check_attn(const tgx_paged* p, int heads, int group, int D, int dtype) {
-  if (int st = check_paged(p)) return st;
-  TGX_REQUIRE(heads >= 1 && group >= 1, "heads and group must be positive");
-  TGX_REQUIRE(dtype_bytes(dtype) != 0, "unknown dtype %d", dtype);
-  if (D < 8 || D > 512 || D % 8) {
-    set_error("head width %d: the paged attention takes multiples of 8 up to 512", D);
-    return TGX_UNSUPPORTED;
-  }
-  const int64_t queries = static_cast<int64_t>(p->table_heads) * heads * group * p->queries;
-  const int64_t tiles = ceil_div(static_cast<int64_t>(p->pages_per_seq) * p->page_size, kTile);
-  TGX_REQUIRE(queries < (int64_t{1} << 28) &&
-                  p->n_seqs * std::max<int64_t>(tiles, 1) < (int64_t{1} << 31) &&
-                  (p->n_seqs + wanted_workgroups()) * queries <= kMaxBlocks256,
-              "paged attention: too many sequences, heads and queries for one launch");
-  return TGX_OK;
 }
 
 // Whether the matrix tiles take the shape; the rows kernel takes every other.
@@ -759,6 +761,28 @@ int64_t workgroups_per_piece(const tgx_paged& p, int heads, int group, int D, in
   const int64_t queries = static_cast<int64_t>(p.queries) * group;
   return static_cast<int64_t>(p.table_heads) * heads *
          (tiled(D, dtype) ? ceil_div(queries, tile_queries(p, group)) : queries);
+}
+
+int check_attn(const tgx_paged* p, int heads, int group, int D, int dtype) {
+  if (int st = check_paged(p)) return st;
+  TGX_REQUIRE(heads >= 1 && group >= 1, "heads and group must be positive");
+  TGX_REQUIRE(dtype_bytes(dtype) != 0, "unknown dtype %d", dtype);
+  if (D < 8 || D > 512 || D % 8) {
+    set_error("head width %d: the paged attention takes multiples of 8 up to 512", D);
+    return TGX_UNSUPPORTED;
+  }
+  const int64_t tiles = ceil_div(static_cast<int64_t>(p->pages_per_seq) * p->page_size, kTile);
+  const int64_t rows = static_cast<int64_t>(group) * p->queries;
+  TGX_REQUIRE(rows < (int64_t{1} << 28) && static_cast<int64_t>(p->table_heads) * heads < 1 << 28 &&
+                  p->n_seqs * std::max<int64_t>(tiles, 1) < (int64_t{1} << 31),
+              "paged attention: sizes past 32 bits");
+  const int64_t each = workgroups_per_piece(*p, heads, group, D, dtype);
+  const int64_t pairs = static_cast<int64_t>(p->table_heads) * heads;
+  TGX_REQUIRE(each <= kMaxBlocks256 && pairs * rows <= kMaxBlocks256 &&
+                  cut_of(*p, each).launched <= kMaxBlocks256 / each - 8 &&
+                  p->n_seqs <= kMaxBlocks256 / (pairs * rows),
+              "paged attention: too many sequences, heads and queries for one launch");
+  return TGX_OK;
 }
 
 size_t meta_bytes(const tgx_paged& p) { return align_up(sizeof(int2) * p.n_seqs); }
@@ -801,13 +825,14 @@ int dispatch_join(const PagedArgs& a, hipStream_t stream) {
   return launch_join<DT, 64>(a, stream);
 }
 
-template <typename T, int D, int QT, int KEYS>
+template <typename T, int D, int QT>
 int launch_tiles(const PagedArgs& a, const Cut& cut, hipStream_t stream) {
   const int64_t rows = static_cast<int64_t>(a.rel.queries) * a.group;
-  const int64_t blocks = cut.launched * a.rel.heads * a.heads * ceil_div(rows, 16 * QT);
+  const int64_t blocks =
+      ceil_div(cut.launched * a.rel.heads * a.heads, 8) * 8 * ceil_div(rows, 16 * QT);
   {
     TGX_PROFILE("paged_tiles", stream);
-    paged_tile_kernel<T, D, QT, KEYS>
+    paged_tile_kernel<T, D, QT>
         <<<dim3(static_cast<uint32_t>(blocks)), dim3(256), 0, stream>>>(a);
   }
   TGX_LAUNCHED("paged_tiles");
@@ -816,8 +841,8 @@ int launch_tiles(const PagedArgs& a, const Cut& cut, hipStream_t stream) {
 
 template <typename T, int D>
 int launch_tiles(const PagedArgs& a, const Cut& cut, hipStream_t stream) {
-  return a.rel.queries * a.group <= 16 ? launch_tiles<T, D, 1, kTileKeys<D, 1>>(a, cut, stream)
-                                       : launch_tiles<T, D, 2, kTileKeys<D, 2>>(a, cut, stream);
+  return a.rel.queries * a.group <= 16 ? launch_tiles<T, D, 1>(a, cut, stream)
+                                       : launch_tiles<T, D, 2>(a, cut, stream);
 }
 
 template <typename T>

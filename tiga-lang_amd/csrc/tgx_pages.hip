@@ -309,7 +309,7 @@ __global__ __launch_bounds__(THREADS) void select_pages_kernel(SelectArgs a) {
   constexpr int WAVES = THREADS / 64;
   const PagedRel& r = a.rel;
   __shared__ int hist[256];
-  __shared__ int counts[WAVES];
+  __shared__ int places[kHeld * WAVES];
   __shared__ int sh_byte, sh_left, sh_share, sh_n, sh_page;
   __shared__ uint64_t sh_last;
   __shared__ uint64_t cand[64];
@@ -353,7 +353,22 @@ __global__ __launch_bounds__(THREADS) void select_pages_kernel(SelectArgs a) {
     for (int i = tid; i < 256; i += THREADS) hist[i] = 0;
     __syncthreads();
     visit([&](int, uint64_t key) {
-      if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1);
+      if ((key & mask) != prefix) return;
+      const int byte = static_cast<int>(key >> shift) & 255;
+      if (shift < 56) {
+        atomicAdd(&hist[byte], 1);
+        return;
+      }
+      // Sign and exponent: few values, each added once a wave.
+      bool mine = true;
+      while (mine) {
+        const int one = uniform(byte);
+        const unsigned long long same = __ballot(byte == one);
+        if (byte == one) {
+          mine = false;
+          if (lane == __builtin_ctzll(same)) atomicAdd(&hist[one], __popcll(same));
+        }
+      }
     });
     __syncthreads();
     if (wave == 0) {
@@ -417,40 +432,77 @@ __global__ __launch_bounds__(THREADS) void select_pages_kernel(SelectArgs a) {
     last = sh_last;
     last_page = sh_page;
   }
-  // The taken pages in order of position.
-  auto block_rank = [&](bool flag, int& total) {
-    const unsigned long long set = __ballot(flag);
+  // The taken pages in order of position: the ballots of kHeld * THREADS keys, one
+  // scan of their counts, then every taken page's place.
+  auto scan = [&](const unsigned long long (&set)[kHeld]) {
     __syncthreads();
-    if (lane == 0) counts[wave] = __popcll(set);
-    __syncthreads();
-    int before = __popcll(set & ((1ull << lane) - 1));
-    total = 0;
-    for (int w = 0; w < WAVES; ++w) {
-      if (w < wave) before += counts[w];
-      total += counts[w];
+    if (lane == 0) {
+#pragma unroll
+      for (int j = 0; j < kHeld; ++j) places[j * WAVES + wave] = __popcll(set[j]);
     }
-    return before;
+    __syncthreads();
+    if (wave == 0) {
+      constexpr int EACH = (kHeld * WAVES + 63) / 64;
+      int own[EACH], sum = 0;
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {
+        const int at = EACH * lane + i;
+        own[i] = at < kHeld * WAVES ? places[at] : 0;
+        sum += own[i];
+      }
+      int before = sum;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(before, d, 64);
+        if (lane >= d) before += o;
+      }
+      if (lane == 63) sh_n = before;
+      before -= sum;
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {
+        const int at = EACH * lane + i;
+        if (at < kHeld * WAVES) places[at] = before;
+        before += own[i];
+      }
+    }
+    __syncthreads();
+  };
+  auto place = [&](unsigned long long set, int j) {
+    return places[j * WAVES + wave] + __popcll(set & ((1ull << lane) - 1));
   };
   int placed = 0, seen = 0;
-  auto place = [&](int i, uint64_t key) {
-    bool take = i < n && (key > last || (key == last && i <= last_page));
-    if (last_page < 0) {
-      int ties;
-      const bool tie = i < n && key == last;
-      const int tie_rank = block_rank(tie, ties);
-      take = i < n && (key > last || (tie && seen + tie_rank < left));
-      seen += ties;
-    }
-    int taken;
-    const int at = block_rank(take, taken);
-    if (take) out[placed + at] = ids[i];
-    placed += taken;
-  };
+  for (int i0 = 0; i0 < n; i0 += kHeld * THREADS) {
+    unsigned long long set[kHeld];
+    if (i0 > 0) {
 #pragma unroll
-  for (int j = 0; j < kHeld; ++j)
-    if (j * THREADS < n) place(j * THREADS + tid, held[j]);
-  for (int i0 = kHeld * THREADS; i0 < n; i0 += THREADS)
-    place(i0 + tid, i0 + tid < n ? keys[i0 + tid] : 0);
+      for (int j = 0; j < kHeld; ++j) {
+        const int i = i0 + j * THREADS + tid;
+        held[j] = i < n ? keys[i] : 0;
+      }
+    }
+    unsigned counted = 0;   // bit j: the key is among the equal ones that are taken
+    if (last_page < 0) {
+#pragma unroll
+      for (int j = 0; j < kHeld; ++j)
+        set[j] = __ballot(i0 + j * THREADS + tid < n && held[j] == last);
+      scan(set);
+#pragma unroll
+      for (int j = 0; j < kHeld; ++j)
+        if (seen + place(set[j], j) < left) counted |= 1u << j;
+      seen += sh_n;
+    }
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+      const int i = i0 + j * THREADS + tid;
+      const bool equal = last_page < 0 ? (counted >> j & 1) != 0 : i <= last_page;
+      set[j] = __ballot(i < n && (held[j] > last || (held[j] == last && equal)));
+    }
+    scan(set);
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j)
+      if (set[j] >> lane & 1) out[placed + place(set[j], j)] = ids[i0 + j * THREADS + tid];
+    placed += sh_n;
+  }
 }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
