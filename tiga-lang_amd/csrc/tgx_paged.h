@@ -37,7 +37,8 @@ inline int check_paged(const tgx_paged* p) {
                   p->page_size >= 1 && p->num_pages >= 0 && p->queries >= 1,
               "paged relation with negative or zero sizes");
   TGX_REQUIRE(p->n_seqs < (int64_t{1} << 31) && p->num_pages < (int64_t{1} << 31) &&
-                  static_cast<int64_t>(p->pages_per_seq) * p->page_size < (int64_t{1} << 31) &&
+                  static_cast<int64_t>(p->pages_per_seq) * p->page_size <
+                      (int64_t{1} << 31) - 4096 &&   // (kernels look a few tiles ahead)
                   p->num_pages * p->page_size < (int64_t{1} << 31) &&
                   p->n_seqs * p->queries < (int64_t{1} << 31),
               "paged relation: sequences, rows, positions and slots must be fewer than 2^31");

@@ -263,24 +263,20 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedArgs a) {
 // ---------------------------------------------------------------------------
 // Matrix tiles (bf16, fp16; D = 32, 64, 128)
 //
-// A workgroup holds the queries of one (sequence, head) that share its keys,
-// 16 * QT of them, and each of its four waves runs through every fourth step
-// of KEYS keys by itself: there is no barrier before the end.  With lane l, g
-// = l / 16, lr = l % 16 (v_mfma_f32_16x16x32, as in the dense tiles): S^T = K
-// Q^T takes its K fragments straight from the cache, 16 bytes a lane and 64
-// contiguous bytes of each of 16 rows an instruction; the lane's results are
-// four keys of one query for each 16 keys, which is P^T as the B operand of
-// O^T = V^T P^T under the key order {4g .. 4g + 3, 16 + 4g ..}; V^T is read
-// down the columns of a V tile that the wave staged in its own LDS rows
-// (ds_read_b64_tr_b16).
+// With lane l, g = l / 16, lr = l % 16 (v_mfma_f32_16x16x32, as in the dense
+// tiles): S^T = K Q^T of 16 queries takes K fragments of 16 bytes a lane, 64
+// contiguous bytes of each of 16 rows; the lane's results are four keys of
+// one query for each 16 keys, which is P^T as the B operand of O^T = V^T P^T
+// under the key order {4g .. 4g + 3, 16 + 4g ..}; V^T is read down the columns
+// of a V tile staged in LDS (ds_read_b64_tr_b16).  A weight is multiplied as
+// the sum of two 16-bit values (the matrix unit has time to spare: at D = 128,
+// 24 instructions of 16 cycles for the 16 KB of 32 keys, which take some 700
+// cycles of a CU's share of memory), so only the output's rounding is left.
 //
-// Memory is kept busy by order alone: a step's K loads are issued as soon as
-// the step before has multiplied its own, its V loads as soon as the step
-// before has staged its own, and the page ids one step ahead of that, so a wave
-// always has 16 KB (D = 128) or more on its way.  A weight is multiplied as the
-// sum of two 16-bit values (the matrix unit has time to spare: 48
-// instructions of 16 cycles a step against some 6000 cycles of memory), so
-// only the output's own rounding is left.
+// Two kernels.  Up to 16 queries of one (sequence, head): paged_tile_kernel,
+// whose four waves run through every fourth step of KEYS keys by themselves
+// with no barrier before the end.  More: paged_block_kernel, whose waves take
+// 16 queries each of tiles of 64 keys that all four stage together.
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -300,6 +296,10 @@ struct Frag<_Float16> {
   typedef _Float16 v4 __attribute__((ext_vector_type(4)));
   static constexpr uint32_t kExponent = 0x7C00u;
 };
+template <typename T>
+using vec8 = typename Frag<T>::v8;
+template <typename T>
+using vec4 = typename Frag<T>::v4;
 __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
@@ -317,7 +317,7 @@ __device__ __forceinline__ float group4_sum(float x) {
   return x + __shfl_xor(x, 32, 64);
 }
 
-// Row stride (elements) of a staged V tile: free of bank conflicts as in the
+// Row stride (elements) of a staged tile: free of bank conflicts as in the
 // dense tiles.
 template <int D>
 constexpr int kRow = D == 128 ? 144 : D == 64 ? 80 : 48;
@@ -325,75 +325,235 @@ constexpr int kRow = D == 128 ? 144 : D == 64 ? 80 : 48;
 // The running maximum only moves when a step's exceeds it by this (log2 units).
 constexpr float kRescaleLog2 = 8.f;
 
-// Keys a step.  A step's K and V fragments are D / 2 registers; 64 keys a step
-// leave room for fewer workgroups (24 sequences of up to 3000 tokens, 16 heads
-// of 64: 47 us, 38 us with 32).
-constexpr int KEYS = 32;
-// Workgroups per CU that the registers are held to.  At D = 128 three would
-// need the fragments of K and V to share registers: measured equal.
-template <int D, int QT>
-constexpr int kTileBlocks = D == 128 && QT == 2 ? 1 : D == 128 || QT == 2 ? 2 : 4;
-
-template <int D, int QT>
-struct TileShape {
-  static constexpr size_t kStage = sizeof(uint16_t) * 4 * KEYS * kRow<D>;
-  static constexpr size_t kJoin = sizeof(float) * 4 * 16 * QT * (D + 4 + 2);
-  static constexpr size_t kWeights = sizeof(float) * 4 * KEYS * 16 * QT;
-  static constexpr size_t kBytes = kStage + kWeights > kJoin ? kStage + kWeights : kJoin;
+// The lane's part of 16 queries: row `row` of the (sequence, head), its
+// fragments, and the positions it sees (rows past the last see as the last).
+template <typename T, int D>
+struct Query {
+  vec8<T> f[D / 32];
+  int limit;
+  __device__ __forceinline__ Query(const PagedArgs& a, const Piece& p, int th, int kh, int row,
+                                   int rows, int g) {
+    const int t = min(row / a.group, a.rel.queries - 1), gq = row % a.group;
+    limit = p.length - (a.rel.queries - 1 - t);
+    const int64_t q_row = (static_cast<int64_t>(p.seq) * a.rel.queries + t) * a.rel.heads + th;
+    const T* q = static_cast<const T*>(a.q) + q_row * a.qs_row + kh * a.qs_head +
+                 gq * a.qs_group + 8 * g;
+#pragma unroll
+    for (int kc = 0; kc < D / 32; ++kc)
+      f[kc] = row < rows ? *reinterpret_cast<const vec8<T>*>(q + 32 * kc) : vec8<T>{};
+  }
 };
 
-template <typename T, int D, int QT>
-__global__ __launch_bounds__(256, (kTileBlocks<D, QT>)) void paged_tile_kernel(PagedArgs a) {
-  constexpr int KT = KEYS / 16, KC = D / 32, DT = D / 16, ROW = kRow<D>;
-  using v8 = typename Frag<T>::v8;
-  using v4 = typename Frag<T>::v4;
-  __shared__ __align__(16) char smem[TileShape<D, QT>::kBytes];
+// Scores of 16 KT keys from position `pos` become weights 2^(s - m) under the
+// running maximum m; l and o follow it.  `gone`: bit k set, key k is not
+// there; `masked`: some key may be hidden from the lane's query.
+template <int KT, int DT>
+__device__ __forceinline__ void weigh(f32x4 (&c)[KT], float scale, bool masked,
+                                      unsigned long long gone, int pos, int limit, int g,
+                                      float& m, float& l, f32x4 (&o)[DT]) {
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt) c[kt] *= scale;
+  if (masked) {
+    gone >>= 4 * g;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if ((gone >> (16 * kt + i) & 1) || pos + 16 * kt + 4 * g + i >= limit) c[kt][i] = kNegInf;
+  }
+  float top = kNegInf;
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = fmaxf(top, c[kt][i]);
+  top = group4_max(top);
+  if (__any(top > m + kRescaleLog2)) {
+    const float mn = fmaxf(m, top);
+    const float alpha = m == kNegInf ? 0.f : exp2_hw(m - mn);
+    m = mn;
+    l *= alpha;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
+  }
+  const float mo = m == kNegInf ? 0.f : m;
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      c[kt][i] = exp2_hw(c[kt][i] - mo);
+      l += c[kt][i];
+    }
+}
+
+// o += V^T P^T over the 16 KT staged rows at `v`.
+template <typename T, int D, int KT>
+__device__ __forceinline__ void add_values(const T* v, const f32x4 (&c)[KT], int g, int lr,
+                                           f32x4 (&o)[D / 16]) {
+  constexpr int ROW = kRow<D>;
+#pragma unroll
+  for (int k2 = 0; k2 < KT / 2; ++k2) {
+    vec8<T> ph, pl;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float w = c[2 * k2 + j / 4][j % 4];
+      ph[j] = static_cast<T>(w);
+      pl[j] = static_cast<T>(w - static_cast<float>(ph[j]));
+    }
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) {
+      const T* src = v + (32 * k2 + 4 * g + (lr >> 2)) * ROW + 16 * dt + 4 * (lr & 3);
+      const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(src));
+      const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(src + 16 * ROW));
+      const u32x2 wl = __builtin_bit_cast(u32x2, lo), wh = __builtin_bit_cast(u32x2, hi);
+      const vec8<T> vt = __builtin_bit_cast(vec8<T>, (u32x4{wl[0], wl[1], wh[0], wh[1]}));
+      o[dt] = mfma(vt, ph, o[dt]);
+      o[dt] = mfma(vt, pl, o[dt]);
+    }
+  }
+}
+
+// The same key by key (`weights`: the wave's [16 KT][16] floats of LDS), for
+// steps that hold a NaN or Inf in a value some of the queries do not see:
+// what a query does not see is left out, not multiplied by 0.
+template <typename T, int D, int KT>
+__device__ __forceinline__ void add_seen_values(const T* v, const f32x4 (&c)[KT], int g, int lr,
+                                                int pos, int limit, float* weights,
+                                                f32x4 (&o)[D / 16]) {
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) weights[(16 * kt + 4 * g + i) * 16 + lr] = c[kt][i];
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+  for (int key = 0; key < 16 * KT; ++key) {
+    if (pos + key >= limit) continue;
+    const float w = weights[key * 16 + lr];
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) {
+      const vec4<T> vv = *reinterpret_cast<const vec4<T>*>(v + key * kRow<D> + 16 * dt + 4 * g);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[dt][e] += w * static_cast<float>(vv[e]);
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ bool any_odd(const vec8<T>& v) {
+  const u32x4 w = __builtin_bit_cast(u32x4, v);
+  constexpr uint32_t e = Frag<T>::kExponent;
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) odd |= (w[i] & e) == e || (w[i] >> 16 & e) == e;
+  return odd;
+}
+
+// The states of the WAVES waves that share 16 queries, joined in wave order and
+// written: the output, or the piece's partial.  `smem` holds [group][wave][16][D
+// + 4] outputs, then maxima and sums; row0 is the first group's first row.
+template <typename T, int D, int WAVES>
+__device__ __forceinline__ void join_waves(const PagedArgs& a, const Piece& p, int x, int head,
+                                           int th, int kh, int row0, int rows, char* smem, float m,
+                                           float l, const f32x4 (&o)[D / 16]) {
+  constexpr int GROUPS = 4 / WAVES;
+  float* jo = reinterpret_cast<float*>(smem);
+  float* jm = jo + 4 * 16 * (D + 4);
+  const int wave = threadIdx.x >> 6, lane = lane_id(), g = lane >> 4, lr = lane & 15;
+  __syncthreads();
+  const float sum_l = group4_sum(l);
+#pragma unroll
+  for (int dt = 0; dt < D / 16; ++dt)
+    *reinterpret_cast<f32x4*>(jo + (wave * 16 + lr) * (D + 4) + 16 * dt + 4 * g) = o[dt];
+  if (g == 0) {
+    jm[2 * (wave * 16 + lr)] = m;
+    jm[2 * (wave * 16 + lr) + 1] = sum_l;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < GROUPS * 16 * (D / 4); i += 256) {
+    const int qr = i / (D / 4), d = i % (D / 4) * 4, row = row0 + qr;
+    if (row >= rows) break;
+    const int at0 = qr / 16 * WAVES * 16 + qr % 16;
+    float mw[WAVES], mx = kNegInf;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      mw[w] = jm[2 * (at0 + 16 * w)];
+      mx = fmaxf(mx, mw[w]);
+    }
+    float sum = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      // (A wave without a maximum has no weight, or a NaN of its own.)
+      const float f = mw[w] == kNegInf ? 1.f : exp2_hw(mw[w] - mx);
+      sum += f * jm[2 * (at0 + 16 * w) + 1];
+      acc += f * *reinterpret_cast<const f32x4*>(jo + (at0 + 16 * w) * (D + 4) + d);
+    }
+    if (p.count == 1) {
+      const int t = row / a.group, gq = row % a.group;
+      const int64_t q_row = (static_cast<int64_t>(p.seq) * a.rel.queries + t) * a.rel.heads + th;
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      vec4<T> w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = static_cast<T>(acc[e] * inv);
+      *reinterpret_cast<vec4<T>*>(static_cast<T*>(a.out) +
+                                  ((q_row * a.heads + kh) * a.group + gq) * D + d) = w;
+    } else {
+      float* dst = a.partial +
+                   ((static_cast<int64_t>(x) * a.rel.heads * a.heads + head) * rows + row) *
+                       (D + 2);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dst[d + e] = acc[e];
+      if (d == 0) {
+        dst[D] = mx;
+        dst[D + 1] = sum;
+      }
+    }
+  }
+}
+template <int D>
+constexpr size_t kJoinBytes = sizeof(float) * 4 * 16 * (D + 4 + 2);
+
+// Up to 16 queries.  Memory is kept busy by order alone: a step's K loads are
+// issued as soon as the step before has multiplied its own, its V loads as
+// soon as the step before has staged its own, and the page ids one step ahead
+// of that, so a wave always has 8 KB (D = 128) or more on its way.  Measured:
+// four sequences of 100k to 131k, 8 x 4 heads of 128, 347 us (5.6 TB/s, of 6.3
+// that plain reads reach); 64 of 100 to 4000 tokens 120 us (4.6 TB/s, the
+// first loads and the join among them).
+//
+// Keys a step: 64 leave room for fewer workgroups (24 sequences of up to 3000
+// tokens, 16 heads of 64: 47 us, 38 us with 32).  Workgroups a CU: at D = 128
+// three would need K's and V's fragments to share registers, and measured
+// equal.
+constexpr int KEYS = 32;
+template <typename T, int D>
+__global__ __launch_bounds__(256, (D == 128 ? 2 : 4)) void paged_tile_kernel(PagedArgs a) {
+  constexpr int KT = KEYS / 16, KC = D / 32, ROW = kRow<D>;
+  constexpr size_t kStage = sizeof(T) * 4 * KEYS * ROW;
+  constexpr size_t kBytes = kStage + sizeof(float) * 4 * KEYS * 16;
+  __shared__ __align__(16) char smem[kBytes > kJoinBytes<D> ? kBytes : kJoinBytes<D>];
   const PagedRel& r = a.rel;
-  const int all_heads = r.heads * a.heads;
+  const unsigned all_heads = r.heads * a.heads;
   const int rows = r.queries * a.group;
-  const int row_groups = (rows + 16 * QT - 1) / (16 * QT);
-  // Workgroups go to the 8 XCDs in turn: the groups of queries that read the same
-  // keys are 8 apart, on one L2.
-  const unsigned of8 = blockIdx.x / 8u, groups = static_cast<unsigned>(row_groups);
-  const unsigned item = of8 / groups * 8u + blockIdx.x % 8u;
-  const int row0 = static_cast<int>(of8 % groups) * (16 * QT);
-  const int head = static_cast<int>(item % static_cast<unsigned>(all_heads));
-  const int x = static_cast<int>(item / static_cast<unsigned>(all_heads));
+  const int head = static_cast<int>(blockIdx.x % all_heads);
+  const int x = static_cast<int>(blockIdx.x / all_heads);
   const Piece p = find_piece(r, a.pieces, a.meta == nullptr, x);
   if (p.seq < 0) return;
   const int th = head / a.heads, kh = head % a.heads;
-  if (a.meta && p.index == 0 && row0 == 0 && head == 0 && threadIdx.x == 0)
+  if (a.meta && p.index == 0 && head == 0 && threadIdx.x == 0)
     a.meta[p.seq] = make_int2(x, p.count);
 
   const int wave = uniform(threadIdx.x >> 6), lane = lane_id();
   const int g = lane >> 4, lr = lane & 15;
-  // Positions each of the lane's queries sees, and the fewest and most of all.
-  int limit[QT];
-  v8 qf[QT][KC];
-#pragma unroll
-  for (int qt = 0; qt < QT; ++qt) {
-    const int row = row0 + 16 * qt + lr;
-    const int t = min(row / a.group, r.queries - 1), gq = row % a.group;
-    limit[qt] = p.length - (r.queries - 1 - t);
-    const int64_t q_row = (static_cast<int64_t>(p.seq) * r.queries + t) * r.heads + th;
-    const T* q = static_cast<const T*>(a.q) + q_row * a.qs_row + kh * a.qs_head +
-                 gq * a.qs_group + 8 * g;
-#pragma unroll
-    for (int kc = 0; kc < KC; ++kc)
-      qf[qt][kc] = row < rows ? *reinterpret_cast<const v8*>(q + 32 * kc) : v8{};
-  }
-  const int t_low = row0 / a.group;
-  const int t_high = min((row0 + 16 * QT - 1) / a.group, r.queries - 1);
-  const int low = p.length - (r.queries - 1 - t_low);
-  const int high = min(p.length - (r.queries - 1 - t_high), p.tile1 * kTile);
-
+  const Query<T, D> q(a, p, th, kh, lr, rows, g);
+  // The fewest and most positions any of the queries sees.
+  const int low = p.length - (r.queries - 1);
+  const int high = min(p.length, p.tile1 * kTile);
   const T* kb = static_cast<const T*>(a.k) + th * a.ks_table + kh * a.ks_head + 8 * g;
   const T* vb = static_cast<const T*>(a.v) + th * a.vs_table + kh * a.vs_head + 8 * g;
   const int32_t* table = r.table + p.seq * r.seq_stride + th * r.head_stride;
   // The wave's staged V, and its weights where they are taken key by key.
   T* stage = reinterpret_cast<T*>(smem) + wave * KEYS * ROW;
-  float* weights = reinterpret_cast<float*>(smem + TileShape<D, QT>::kStage) +
-                   wave * KEYS * 16 * QT;
+  float* weights = reinterpret_cast<float*>(smem + kStage) + wave * KEYS * 16;
 
   // Steps of this wave: first + 4 i < last.  Lane l keeps the page id of key
   // l (mod KEYS) of a step.
@@ -411,27 +571,22 @@ __global__ __launch_bounds__(256, (kTileBlocks<D, QT>)) void paged_tile_kernel(P
                  : -1;
   };
   // (A key that is not there loads slot 0, and is masked.)
-  auto load = [&](v8(&f)[KT][KC], const T* base, int64_t stride, int slot) {
+  auto load = [&](vec8<T>(&f)[KT][KC], const T* base, int64_t stride, int slot) {
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
       const int s = max(__shfl(slot, 16 * kt + lr, 64), 0);
-      const T* q = base + s * stride;
+      const T* row = base + s * stride;
 #pragma unroll
-      for (int kc = 0; kc < KC; ++kc) f[kt][kc] = *reinterpret_cast<const v8*>(q + 32 * kc);
+      for (int kc = 0; kc < KC; ++kc) f[kt][kc] = *reinterpret_cast<const vec8<T>*>(row + 32 * kc);
     }
   };
 
-  float m[QT], l[QT];
-  f32x4 o[DT][QT];
+  float m = kNegInf, l = 0.f;
+  f32x4 o[D / 16];
 #pragma unroll
-  for (int qt = 0; qt < QT; ++qt) {
-    m[qt] = kNegInf;
-    l[qt] = 0.f;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) o[dt][qt] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+  for (int dt = 0; dt < D / 16; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   if (first < last) {
-    v8 kf[KT][KC], vf[KT][KC];
+    vec8<T> kf[KT][KC], vf[KT][KC];
     int slot = slot_of(first, page_id(first));
     load(kf, kb, a.ks_slot, slot);
     load(vf, vb, a.vs_slot, slot);
@@ -440,71 +595,17 @@ __global__ __launch_bounds__(256, (kTileBlocks<D, QT>)) void paged_tile_kernel(P
       const int next = slot_of(step + 4, next_id);
       next_id = page_id(step + 8);
       const unsigned long long gone = __ballot(slot < 0);   // bit k: key k is not there
-      f32x4 c[KT][QT];
+      f32x4 c[KT];
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt) c[kt][qt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int kt = 0; kt < KT; ++kt) c[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int kc = 0; kc < KC; ++kc)
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-          for (int qt = 0; qt < QT; ++qt) c[kt][qt] = mfma(kf[kt][kc], qf[qt][kc], c[kt][qt]);
+        for (int kt = 0; kt < KT; ++kt) c[kt] = mfma(kf[kt][kc], q.f[kc], c[kt]);
       load(kf, kb, a.ks_slot, next);
 
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt) c[kt][qt] *= a.scale_log2;
       const bool tail = step * KEYS + KEYS > low;   // some query sees only a part
-      if (gone || tail) {
-        const unsigned long long mine = gone >> (4 * g);
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int pos = step * KEYS + 16 * kt + 4 * g + i;
-            const bool hidden = mine >> (16 * kt + i) & 1;
-#pragma unroll
-            for (int qt = 0; qt < QT; ++qt)
-              if (hidden || pos >= limit[qt]) c[kt][qt][i] = kNegInf;
-          }
-      }
-      float top[QT];
-      bool grow = false;
-#pragma unroll
-      for (int qt = 0; qt < QT; ++qt) {
-        top[qt] = kNegInf;
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) top[qt] = fmaxf(top[qt], c[kt][qt][i]);
-        top[qt] = group4_max(top[qt]);
-        grow |= top[qt] > m[qt] + kRescaleLog2;
-      }
-      if (__any(grow)) {
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt) {
-          const float mn = fmaxf(m[qt], top[qt]);
-          const float alpha = m[qt] == kNegInf ? 0.f : exp2_hw(m[qt] - mn);
-          m[qt] = mn;
-          l[qt] *= alpha;
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) o[dt][qt] *= alpha;
-        }
-      }
-#pragma unroll
-      for (int qt = 0; qt < QT; ++qt) {
-        const float mo = m[qt] == kNegInf ? 0.f : m[qt];
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            c[kt][qt][i] = exp2_hw(c[kt][qt][i] - mo);
-            l[qt] += c[kt][qt][i];
-          }
-      }
+      weigh(c, a.scale_log2, gone || tail, gone, step * KEYS, q.limit, g, m, l, o);
 
       // Stage V; a key that is not there counts as a row of zeros.
       if (gone) {
@@ -512,140 +613,154 @@ __global__ __launch_bounds__(256, (kTileBlocks<D, QT>)) void paged_tile_kernel(P
         for (int kt = 0; kt < KT; ++kt)
           if (gone >> (16 * kt + lr) & 1) {
 #pragma unroll
-            for (int kc = 0; kc < KC; ++kc) vf[kt][kc] = v8{};
+            for (int kc = 0; kc < KC; ++kc) vf[kt][kc] = vec8<T>{};
           }
       }
-      bool odd = false;   // a NaN or Inf where only some of the queries see it
+      bool odd = false;
       if (tail && r.queries > 1) {
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-          for (int kc = 0; kc < KC; ++kc) {
-            const u32x4 w = __builtin_bit_cast(u32x4, vf[kt][kc]);
-            constexpr uint32_t e = Frag<T>::kExponent;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              odd |= (w[i] & e) == e || (w[i] >> 16 & e) == e;
-          }
+          for (int kc = 0; kc < KC; ++kc) odd |= any_odd<T>(vf[kt][kc]);
         odd = __any(odd);
       }
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
         for (int kc = 0; kc < KC; ++kc)
-          *reinterpret_cast<v8*>(stage + (16 * kt + lr) * ROW + 32 * kc + 8 * g) = vf[kt][kc];
+          *reinterpret_cast<vec8<T>*>(stage + (16 * kt + lr) * ROW + 32 * kc + 8 * g) = vf[kt][kc];
       load(vf, vb, a.vs_slot, next);
-
-      if (!odd) {
-#pragma unroll
-        for (int k2 = 0; k2 < KT / 2; ++k2) {
-          v8 ph[QT], pl[QT];
-#pragma unroll
-          for (int qt = 0; qt < QT; ++qt)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float w = c[2 * k2 + j / 4][qt][j % 4];
-              ph[qt][j] = static_cast<T>(w);
-              pl[qt][j] = static_cast<T>(w - static_cast<float>(ph[qt][j]));
-            }
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) {
-            const T* src = stage + (32 * k2 + 4 * g + (lr >> 2)) * ROW + 16 * dt + 4 * (lr & 3);
-            const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(src));
-            const i16x4 hi =
-                __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(src + 16 * ROW));
-            const u32x2 wl = __builtin_bit_cast(u32x2, lo), wh = __builtin_bit_cast(u32x2, hi);
-            const v8 vt = __builtin_bit_cast(v8, (u32x4{wl[0], wl[1], wh[0], wh[1]}));
-#pragma unroll
-            for (int qt = 0; qt < QT; ++qt) {
-              o[dt][qt] = mfma(vt, ph[qt], o[dt][qt]);
-              o[dt][qt] = mfma(vt, pl[qt], o[dt][qt]);
-            }
-          }
-        }
-      } else {
-        // Key by key: what a query does not see is left out, not multiplied by 0.
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-          for (int qt = 0; qt < QT; ++qt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              weights[(16 * kt + 4 * g + i) * (16 * QT) + 16 * qt + lr] = c[kt][qt][i];
-#pragma unroll 1
-        for (int key = 0; key < KEYS; ++key)
-#pragma unroll
-          for (int qt = 0; qt < QT; ++qt) {
-            if (step * KEYS + key >= limit[qt]) continue;
-            const float w = weights[key * (16 * QT) + 16 * qt + lr];
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-              const v4 vv = *reinterpret_cast<const v4*>(stage + key * ROW + 16 * dt + 4 * g);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o[dt][qt][e] += w * static_cast<float>(vv[e]);
-            }
-          }
-      }
+      __builtin_amdgcn_wave_barrier();
+      if (!odd)
+        add_values<T, D, KT>(stage, c, g, lr, o);
+      else
+        add_seen_values<T, D, KT>(stage, c, g, lr, step * KEYS, q.limit, weights, o);
       slot = next;
     }
   }
+  join_waves<T, D, 4>(a, p, x, head, th, kh, 0, rows, smem, m, l, o);
+}
 
-  // The four waves' states, joined in wave order.
-  float* jo = reinterpret_cast<float*>(smem);               // [wave][query][D + 4]
-  float* jm = jo + 4 * 16 * QT * (D + 4);                    // [wave][query][2]
-  __syncthreads();
+// More than 16 queries.  The four waves stage 64 keys together, the next tile's
+// loads in flight in registers while this one is multiplied; KW waves share
+// 16 queries and take 64 / KW keys of a tile each, so a workgroup holds 64 / KW
+// queries: 32 with KW = 2, 64 with KW = 1.  Workgroups of the same keys are 8
+// apart, on one XCD's L2.
+template <typename T, int D, int KW>
+__global__ __launch_bounds__(256, (D == 128 ? 2 : 3)) void paged_block_kernel(PagedArgs a) {
+  constexpr int KT = 4 / KW, KC = D / 32, ROW = kRow<D>, QUERIES = 64 / KW;
+  constexpr int CPR = D / 8, N = 64 * CPR / 256;   // 16-byte chunks a row, and of a thread
+  constexpr size_t kTileBytes = sizeof(T) * 64 * ROW;
+  constexpr size_t kBytes = 2 * kTileBytes + sizeof(float) * 4 * 16 * KT * 16;
+  __shared__ __align__(16) char smem[kBytes > kJoinBytes<D> ? kBytes : kJoinBytes<D>];
+  __shared__ int sh_odd[2];
+  const PagedRel& r = a.rel;
+  const unsigned all_heads = r.heads * a.heads;
+  const int rows = r.queries * a.group;
+  const unsigned groups = (rows + QUERIES - 1) / QUERIES;
+  const unsigned of8 = blockIdx.x / 8u, item = of8 / groups * 8u + blockIdx.x % 8u;
+  const int row0 = static_cast<int>(of8 % groups) * QUERIES;
+  const int head = static_cast<int>(item % all_heads);
+  const int x = static_cast<int>(item / all_heads);
+  const Piece p = find_piece(r, a.pieces, a.meta == nullptr, x);
+  if (p.seq < 0) return;
+  const int th = head / a.heads, kh = head % a.heads;
+  if (a.meta && p.index == 0 && head == 0 && row0 == 0 && threadIdx.x == 0)
+    a.meta[p.seq] = make_int2(x, p.count);
+
+  const int wave = uniform(threadIdx.x >> 6), lane = lane_id();
+  const int g = lane >> 4, lr = lane & 15;
+  const int wrow = row0 + wave / KW * 16;      // the wave's first query
+  const int key0 = wave % KW * 16 * KT;        // and first key of a tile
+  const Query<T, D> q(a, p, th, kh, wrow + lr, rows, g);
+  // Fewest positions any of the wave's queries sees, most of the workgroup's and the wave's.
+  auto sees = [&](int row) {
+    return p.length - (r.queries - 1 - min(row, rows - 1) / a.group);
+  };
+  const int low = sees(wrow), wave_high = sees(wrow + 15);
+  const int group_low = sees(row0), high = min(sees(row0 + QUERIES - 1), p.tile1 * kTile);
+  const T* kb = static_cast<const T*>(a.k) + th * a.ks_table + kh * a.ks_head;
+  const T* vb = static_cast<const T*>(a.v) + th * a.vs_table + kh * a.vs_head;
+  const int32_t* table = r.table + p.seq * r.seq_stride + th * r.head_stride;
+  T* ks = reinterpret_cast<T*>(smem);
+  T* vs = reinterpret_cast<T*>(smem + kTileBytes);
+  float* weights = reinterpret_cast<float*>(smem + 2 * kTileBytes) + wave * 16 * KT * 16;
+
+  auto page_id = [&](int tile) {
+    const int pos = min(tile * kTile + lane, r.pages_per_seq * r.page_size - 1);
+    return table[static_cast<unsigned>(pos) / static_cast<unsigned>(r.page_size)];
+  };
+  auto slot_of = [&](int tile, int id) {
+    const unsigned pos = tile * kTile + lane;
+    const bool there = static_cast<int>(pos) < high &&
+                       static_cast<unsigned>(id) < static_cast<unsigned>(r.num_pages);
+    return there ? id * r.page_size + static_cast<int>(pos % static_cast<unsigned>(r.page_size))
+                 : -1;
+  };
+  // Chunk threadIdx.x + 256 i of a tile is row / CPR, column % CPR.
+  vec8<T> kr[N], vr[N];
+  auto load = [&](int slot) {
 #pragma unroll
-  for (int qt = 0; qt < QT; ++qt) {
-    const int at = wave * 16 * QT + 16 * qt + lr;
-    const float sum = group4_sum(l[qt]);
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-      *reinterpret_cast<f32x4*>(jo + at * (D + 4) + 16 * dt + 4 * g) = o[dt][qt];
-    if (g == 0) {
-      jm[2 * at] = m[qt];
-      jm[2 * at + 1] = sum;
+    for (int i = 0; i < N; ++i) {
+      const int at = threadIdx.x + 256 * i;
+      const int s = __shfl(slot, at / CPR, 64);
+      kr[i] = *reinterpret_cast<const vec8<T>*>(kb + max(s, 0) * a.ks_slot + at % CPR * 8);
+      vr[i] = *reinterpret_cast<const vec8<T>*>(vb + max(s, 0) * a.vs_slot + at % CPR * 8);
+      if (s < 0) vr[i] = vec8<T>{};   // a key that is not there
     }
+  };
+
+  float m = kNegInf, l = 0.f;
+  f32x4 o[D / 16];
+#pragma unroll
+  for (int dt = 0; dt < D / 16; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int last = (high + kTile - 1) / kTile;
+  if (threadIdx.x < 2) sh_odd[threadIdx.x] = 0;
+  int slot = -1, next_id = 0;
+  if (p.tile0 < last) {
+    slot = slot_of(p.tile0, page_id(p.tile0));
+    load(slot);
+    next_id = page_id(p.tile0 + 1);
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < 16 * QT * (D / 4); i += 256) {
-    const int qr = i / (D / 4), d = i % (D / 4) * 4, row = row0 + qr;
-    if (row >= rows) break;
-    float mw[4], mx = kNegInf;
+  for (int tile = p.tile0; tile < last; ++tile) {
+    const bool check = r.queries > 1 && tile * kTile + kTile > group_low;
+    __syncthreads();   // the tile before has been read
+    bool odd = false;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      mw[w] = jm[2 * (w * 16 * QT + qr)];
-      mx = fmaxf(mx, mw[w]);
+    for (int i = 0; i < N; ++i) {
+      const int at = threadIdx.x + 256 * i;
+      if (check) odd |= any_odd<T>(vr[i]);
+      *reinterpret_cast<vec8<T>*>(ks + at / CPR * ROW + at % CPR * 8) = kr[i];
+      *reinterpret_cast<vec8<T>*>(vs + at / CPR * ROW + at % CPR * 8) = vr[i];
     }
-    float sum = 0.f;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const int at = w * 16 * QT + qr;
-      // (A wave without a maximum has no weight, or a NaN of its own.)
-      const float f = mw[w] == kNegInf ? 1.f : exp2_hw(mw[w] - mx);
-      sum += f * jm[2 * at + 1];
-      acc += f * *reinterpret_cast<const f32x4*>(jo + at * (D + 4) + d);
+    if (odd) sh_odd[tile & 1] = 1;
+    if (threadIdx.x == 0) sh_odd[(tile + 1) & 1] = 0;
+    __syncthreads();
+    const unsigned long long gone = __ballot(slot < 0);
+    if (tile + 1 < last) {
+      slot = slot_of(tile + 1, next_id);
+      next_id = page_id(tile + 2);
+      load(slot);
     }
-    const int t = row / a.group, gq = row % a.group;
-    if (p.count == 1) {
-      const int64_t q_row = (static_cast<int64_t>(p.seq) * r.queries + t) * r.heads + th;
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      v4 w;
+    const int pos = tile * kTile + key0;
+    if (wrow >= rows || pos >= wave_high) continue;
+    f32x4 c[KT];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = static_cast<T>(acc[e] * inv);
-      *reinterpret_cast<v4*>(static_cast<T*>(a.out) +
-                             ((q_row * a.heads + kh) * a.group + gq) * D + d) = w;
-    } else {
-      float* dst = a.partial +
-                   ((static_cast<int64_t>(x) * all_heads + head) * rows + row) * (D + 2);
+    for (int kt = 0; kt < KT; ++kt) c[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) dst[d + e] = acc[e];
-      if (d == 0) {
-        dst[D] = mx;
-        dst[D + 1] = sum;
-      }
-    }
+    for (int kc = 0; kc < KC; ++kc)
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+        c[kt] = mfma(*reinterpret_cast<const vec8<T>*>(ks + (key0 + 16 * kt + lr) * ROW + 32 * kc +
+                                                       8 * g),
+                     q.f[kc], c[kt]);
+    weigh(c, a.scale_log2, gone || pos + 16 * KT > low, gone >> key0, pos, q.limit, g, m, l, o);
+    if (!check || !sh_odd[tile & 1])
+      add_values<T, D, KT>(vs + key0 * ROW, c, g, lr, o);
+    else
+      add_seen_values<T, D, KT>(vs + key0 * ROW, c, g, lr, pos, q.limit, weights, o);
   }
+  join_waves<T, D, KW>(a, p, x, head, th, kh, row0, rows, smem, m, l, o);
 }
 
 // Joins the pieces of each (sequence, head, query), a workgroup per query: each
@@ -751,10 +866,10 @@ bool tiled(int D, int dtype) {
   return dtype != TGX_DTYPE_F32 && (D == 32 || D == 64 || D == 128);
 }
 
-// Queries a workgroup of the tiles holds: one 16-query tile, or two that share
-// the keys' loads where there are more.
+// Queries a workgroup of the tiles holds.
 int tile_queries(const tgx_paged& p, int group) {
-  return static_cast<int64_t>(p.queries) * group <= 16 ? 16 : 32;
+  const int64_t queries = static_cast<int64_t>(p.queries) * group;
+  return queries <= 16 ? 16 : queries <= 32 ? 32 : 64;
 }
 
 int64_t workgroups_per_piece(const tgx_paged& p, int heads, int group, int D, int dtype) {
@@ -825,24 +940,21 @@ int dispatch_join(const PagedArgs& a, hipStream_t stream) {
   return launch_join<DT, 64>(a, stream);
 }
 
-template <typename T, int D, int QT>
+template <typename T, int D>
 int launch_tiles(const PagedArgs& a, const Cut& cut, hipStream_t stream) {
   const int64_t rows = static_cast<int64_t>(a.rel.queries) * a.group;
-  const int64_t blocks =
-      ceil_div(cut.launched * a.rel.heads * a.heads, 8) * 8 * ceil_div(rows, 16 * QT);
-  {
-    TGX_PROFILE("paged_tiles", stream);
-    paged_tile_kernel<T, D, QT>
-        <<<dim3(static_cast<uint32_t>(blocks)), dim3(256), 0, stream>>>(a);
+  const int64_t pieces = cut.launched * a.rel.heads * a.heads;
+  TGX_PROFILE("paged_tiles", stream);
+  if (rows <= 16) {
+    paged_tile_kernel<T, D><<<dim3(static_cast<uint32_t>(pieces)), dim3(256), 0, stream>>>(a);
+  } else {
+    const int held = rows <= 32 ? 32 : 64;
+    const dim3 grid(static_cast<uint32_t>(ceil_div(pieces, 8) * 8 * ceil_div(rows, held)));
+    if (held == 32) paged_block_kernel<T, D, 2><<<grid, dim3(256), 0, stream>>>(a);
+    else paged_block_kernel<T, D, 1><<<grid, dim3(256), 0, stream>>>(a);
   }
   TGX_LAUNCHED("paged_tiles");
   return TGX_OK;
-}
-
-template <typename T, int D>
-int launch_tiles(const PagedArgs& a, const Cut& cut, hipStream_t stream) {
-  return a.rel.queries * a.group <= 16 ? launch_tiles<T, D, 1>(a, cut, stream)
-                                       : launch_tiles<T, D, 2>(a, cut, stream);
 }
 
 template <typename T>
