@@ -269,9 +269,10 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedArgs a) {
 // one query for each 16 keys, which is P^T as the B operand of O^T = V^T P^T
 // under the key order {4g .. 4g + 3, 16 + 4g ..}; V^T is read down the columns
 // of a V tile staged in LDS (ds_read_b64_tr_b16).  A weight is multiplied as
-// the sum of two 16-bit values (the matrix unit has time to spare: at D = 128,
-// 24 instructions of 16 cycles for the 16 KB of 32 keys, which take some 700
-// cycles of a CU's share of memory), so only the output's rounding is left.
+// the sum of two 16-bit values where the matrix unit has time to spare (up to
+// 64 queries: at D = 128, 24 instructions of 16 cycles for the 16 KB of 32
+// keys, which take some 700 cycles of a CU's share of memory), so that only
+// the output's rounding is left.
 //
 // Two kernels.  Up to 16 queries of one (sequence, head): paged_tile_kernel,
 // whose four waves run through every fourth step of KEYS keys by themselves
@@ -331,6 +332,7 @@ template <typename T, int D>
 struct Query {
   vec8<T> f[D / 32];
   int limit;
+  Query() = default;
   __device__ __forceinline__ Query(const PagedArgs& a, const Piece& p, int th, int kh, int row,
                                    int rows, int g) {
     const int t = min(row / a.group, a.rel.queries - 1), gq = row % a.group;
@@ -385,20 +387,25 @@ __device__ __forceinline__ void weigh(f32x4 (&c)[KT], float scale, bool masked,
     }
 }
 
-// o += V^T P^T over the 16 KT staged rows at `v`.
-template <typename T, int D, int KT>
-__device__ __forceinline__ void add_values(const T* v, const f32x4 (&c)[KT], int g, int lr,
-                                           f32x4 (&o)[D / 16]) {
+// o += V^T P^T over the 16 KT staged rows at `v`, for QT tiles of 16 queries.  Two
+// tiles a wave (more than 64 queries of a key head) are bound by the matrix
+// unit: their weights are multiplied in 16 bits, half a step off each, as the
+// dense tiles multiply theirs.
+template <typename T, int D, int KT, int QT>
+__device__ __forceinline__ void add_values(const T* v, const f32x4 (&c)[QT][KT], int g, int lr,
+                                           f32x4 (&o)[QT][D / 16]) {
   constexpr int ROW = kRow<D>;
 #pragma unroll
   for (int k2 = 0; k2 < KT / 2; ++k2) {
-    vec8<T> ph, pl;
+    vec8<T> ph[QT], pl[QT];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float w = c[2 * k2 + j / 4][j % 4];
-      ph[j] = static_cast<T>(w);
-      pl[j] = static_cast<T>(w - static_cast<float>(ph[j]));
-    }
+    for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float w = c[qt][2 * k2 + j / 4][j % 4];
+        ph[qt][j] = static_cast<T>(w);
+        if constexpr (QT == 1) pl[qt][j] = static_cast<T>(w - static_cast<float>(ph[qt][j]));
+      }
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) {
       const T* src = v + (32 * k2 + 4 * g + (lr >> 2)) * ROW + 16 * dt + 4 * (lr & 3);
@@ -406,8 +413,11 @@ __device__ __forceinline__ void add_values(const T* v, const f32x4 (&c)[KT], int
       const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(src + 16 * ROW));
       const u32x2 wl = __builtin_bit_cast(u32x2, lo), wh = __builtin_bit_cast(u32x2, hi);
       const vec8<T> vt = __builtin_bit_cast(vec8<T>, (u32x4{wl[0], wl[1], wh[0], wh[1]}));
-      o[dt] = mfma(vt, ph, o[dt]);
-      o[dt] = mfma(vt, pl, o[dt]);
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) {
+        o[qt][dt] = mfma(vt, ph[qt], o[qt][dt]);
+        if constexpr (QT == 1) o[qt][dt] = mfma(vt, pl[qt], o[qt][dt]);
+      }
     }
   }
 }
@@ -452,8 +462,9 @@ __device__ __forceinline__ bool any_odd(const vec8<T>& v) {
 // + 4] outputs, then maxima and sums; row0 is the first group's first row.
 template <typename T, int D, int WAVES>
 __device__ __forceinline__ void join_waves(const PagedArgs& a, const Piece& p, int x, int head,
-                                           int th, int kh, int row0, int rows, char* smem, float m,
-                                           float l, const f32x4 (&o)[D / 16]) {
+                                           int th, int kh, int row0, int apart, int rows,
+                                           char* smem, float m, float l,
+                                           const f32x4 (&o)[D / 16]) {
   constexpr int GROUPS = 4 / WAVES;
   float* jo = reinterpret_cast<float*>(smem);
   float* jm = jo + 4 * 16 * (D + 4);
@@ -469,8 +480,8 @@ __device__ __forceinline__ void join_waves(const PagedArgs& a, const Piece& p, i
   }
   __syncthreads();
   for (int i = threadIdx.x; i < GROUPS * 16 * (D / 4); i += 256) {
-    const int qr = i / (D / 4), d = i % (D / 4) * 4, row = row0 + qr;
-    if (row >= rows) break;
+    const int qr = i / (D / 4), d = i % (D / 4) * 4, row = row0 + qr / 16 * apart + qr % 16;
+    if (row >= rows) continue;
     const int at0 = qr / 16 * WAVES * 16 + qr % 16;
     float mw[WAVES], mx = kNegInf;
 #pragma unroll
@@ -582,9 +593,9 @@ __global__ __launch_bounds__(256, (D == 128 ? 2 : 4)) void paged_tile_kernel(Pag
   };
 
   float m = kNegInf, l = 0.f;
-  f32x4 o[D / 16];
+  f32x4 o[1][D / 16];
 #pragma unroll
-  for (int dt = 0; dt < D / 16; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int dt = 0; dt < D / 16; ++dt) o[0][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   if (first < last) {
     vec8<T> kf[KT][KC], vf[KT][KC];
     int slot = slot_of(first, page_id(first));
@@ -595,17 +606,17 @@ __global__ __launch_bounds__(256, (D == 128 ? 2 : 4)) void paged_tile_kernel(Pag
       const int next = slot_of(step + 4, next_id);
       next_id = page_id(step + 8);
       const unsigned long long gone = __ballot(slot < 0);   // bit k: key k is not there
-      f32x4 c[KT];
+      f32x4 c[1][KT];
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt) c[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int kt = 0; kt < KT; ++kt) c[0][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int kc = 0; kc < KC; ++kc)
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) c[kt] = mfma(kf[kt][kc], q.f[kc], c[kt]);
+        for (int kt = 0; kt < KT; ++kt) c[0][kt] = mfma(kf[kt][kc], q.f[kc], c[0][kt]);
       load(kf, kb, a.ks_slot, next);
 
       const bool tail = step * KEYS + KEYS > low;   // some query sees only a part
-      weigh(c, a.scale_log2, gone || tail, gone, step * KEYS, q.limit, g, m, l, o);
+      weigh(c[0], a.scale_log2, gone || tail, gone, step * KEYS, q.limit, g, m, l, o[0]);
 
       // Stage V; a key that is not there counts as a row of zeros.
       if (gone) {
@@ -632,23 +643,25 @@ __global__ __launch_bounds__(256, (D == 128 ? 2 : 4)) void paged_tile_kernel(Pag
       load(vf, vb, a.vs_slot, next);
       __builtin_amdgcn_wave_barrier();
       if (!odd)
-        add_values<T, D, KT>(stage, c, g, lr, o);
+        add_values<T, D, KT, 1>(stage, c, g, lr, o);
       else
-        add_seen_values<T, D, KT>(stage, c, g, lr, step * KEYS, q.limit, weights, o);
+        add_seen_values<T, D, KT>(stage, c[0], g, lr, step * KEYS, q.limit, weights, o[0]);
       slot = next;
     }
   }
-  join_waves<T, D, 4>(a, p, x, head, th, kh, 0, rows, smem, m, l, o);
+  join_waves<T, D, 4>(a, p, x, head, th, kh, 0, 16, rows, smem, m, l, o[0]);
 }
 
 // More than 16 queries.  The four waves stage 64 keys together, the next tile's
-// loads in flight in registers while this one is multiplied; KW waves share
-// 16 queries and take 64 / KW keys of a tile each, so a workgroup holds 64 / KW
-// queries: 32 with KW = 2, 64 with KW = 1.  Workgroups of the same keys are 8
-// apart, on one XCD's L2.
-template <typename T, int D, int KW>
-__global__ __launch_bounds__(256, (D == 128 ? 2 : 3)) void paged_block_kernel(PagedArgs a) {
-  constexpr int KT = 4 / KW, KC = D / 32, ROW = kRow<D>, QUERIES = 64 / KW;
+// loads in flight in registers while this one is multiplied.  KW waves share
+// 16 QT queries and take 64 / KW keys of a tile each, so a workgroup holds 64 QT
+// / KW queries: 32 (KW = 2), 64, or 128 (QT = 2), the smallest that holds all
+// of them (one read of the keys), 128 where none does.  Workgroups of the same
+// keys are 8 apart, on one XCD's L2.
+template <typename T, int D, int KW, int QT>
+__global__ __launch_bounds__(256, (D == 128 || QT == 2 ? 2 : 3)) void paged_block_kernel(
+    PagedArgs a) {
+  constexpr int KT = 4 / KW, KC = D / 32, ROW = kRow<D>, QUERIES = 64 * QT / KW;
   constexpr int CPR = D / 8, N = 64 * CPR / 256;   // 16-byte chunks a row, and of a thread
   constexpr size_t kTileBytes = sizeof(T) * 64 * ROW;
   constexpr size_t kBytes = 2 * kTileBytes + sizeof(float) * 4 * 16 * KT * 16;
@@ -670,14 +683,17 @@ __global__ __launch_bounds__(256, (D == 128 ? 2 : 3)) void paged_block_kernel(Pa
 
   const int wave = uniform(threadIdx.x >> 6), lane = lane_id();
   const int g = lane >> 4, lr = lane & 15;
-  const int wrow = row0 + wave / KW * 16;      // the wave's first query
+  const int wrow = row0 + wave / KW * 16 * QT;  // the wave's first query
   const int key0 = wave % KW * 16 * KT;        // and first key of a tile
-  const Query<T, D> q(a, p, th, kh, wrow + lr, rows, g);
+  Query<T, D> q[QT];
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt)
+    q[qt] = Query<T, D>(a, p, th, kh, wrow + 16 * qt + lr, rows, g);
   // Fewest positions any of the wave's queries sees, most of the workgroup's and the wave's.
   auto sees = [&](int row) {
     return p.length - (r.queries - 1 - min(row, rows - 1) / a.group);
   };
-  const int low = sees(wrow), wave_high = sees(wrow + 15);
+  const int low = sees(wrow), wave_high = sees(wrow + 16 * QT - 1);
   const int group_low = sees(row0), high = min(sees(row0 + QUERIES - 1), p.tile1 * kTile);
   const T* kb = static_cast<const T*>(a.k) + th * a.ks_table + kh * a.ks_head;
   const T* vb = static_cast<const T*>(a.v) + th * a.vs_table + kh * a.vs_head;
@@ -710,10 +726,15 @@ __global__ __launch_bounds__(256, (D == 128 ? 2 : 3)) void paged_block_kernel(Pa
     }
   };
 
-  float m = kNegInf, l = 0.f;
-  f32x4 o[D / 16];
+  float m[QT], l[QT];
+  f32x4 o[QT][D / 16];
 #pragma unroll
-  for (int dt = 0; dt < D / 16; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int qt = 0; qt < QT; ++qt) {
+    m[qt] = kNegInf;
+    l[qt] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) o[qt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
   const int last = (high + kTile - 1) / kTile;
   if (threadIdx.x < 2) sh_odd[threadIdx.x] = 0;
   int slot = -1, next_id = 0;
@@ -744,23 +765,36 @@ __global__ __launch_bounds__(256, (D == 128 ? 2 : 3)) void paged_block_kernel(Pa
     }
     const int pos = tile * kTile + key0;
     if (wrow >= rows || pos >= wave_high) continue;
-    f32x4 c[KT];
+    f32x4 c[QT][KT];
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt) c[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) c[qt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int kc = 0; kc < KC; ++kc)
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt)
-        c[kt] = mfma(*reinterpret_cast<const vec8<T>*>(ks + (key0 + 16 * kt + lr) * ROW + 32 * kc +
-                                                       8 * g),
-                     q.f[kc], c[kt]);
-    weigh(c, a.scale_log2, gone || pos + 16 * KT > low, gone >> key0, pos, q.limit, g, m, l, o);
-    if (!check || !sh_odd[tile & 1])
-      add_values<T, D, KT>(vs + key0 * ROW, c, g, lr, o);
-    else
-      add_seen_values<T, D, KT>(vs + key0 * ROW, c, g, lr, pos, q.limit, weights, o);
+      for (int kt = 0; kt < KT; ++kt) {
+        const vec8<T> kf = *reinterpret_cast<const vec8<T>*>(
+            ks + (key0 + 16 * kt + lr) * ROW + 32 * kc + 8 * g);
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) c[qt][kt] = mfma(kf, q[qt].f[kc], c[qt][kt]);
+      }
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt)
+      weigh(c[qt], a.scale_log2, gone || pos + 16 * KT > low, gone >> key0, pos, q[qt].limit, g,
+            m[qt], l[qt], o[qt]);
+    if (!check || !sh_odd[tile & 1]) {
+      add_values<T, D, KT, QT>(vs + key0 * ROW, c, g, lr, o);
+    } else {
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt)
+        add_seen_values<T, D, KT>(vs + key0 * ROW, c[qt], g, lr, pos, q[qt].limit, weights, o[qt]);
+    }
   }
-  join_waves<T, D, KW>(a, p, x, head, th, kh, row0, rows, smem, m, l, o);
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt)
+    join_waves<T, D, KW>(a, p, x, head, th, kh, row0 + 16 * qt, 16 * QT, rows, smem, m[qt], l[qt],
+                         o[qt]);
 }
 
 // Joins the pieces of each (sequence, head, query), a workgroup per query: each
@@ -835,47 +869,56 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
            s.acc);
 }
 
-// How a launch is cut: W pieces wanted for each head's query group, pieces
-// launched at most, and whether any sequence can have several.
+// Whether the matrix tiles take the shape; the rows kernel takes every other.
+bool tiled(int D, int dtype) {
+  return dtype != TGX_DTYPE_F32 && (D == 32 || D == 64 || D == 128);
+}
+
+// Queries a workgroup holds.
+int held_queries(const tgx_paged& p, int group, int D, int dtype) {
+  if (!tiled(D, dtype)) return 1;
+  const int64_t queries = static_cast<int64_t>(p.queries) * group;
+  return queries <= 16 ? 16 : queries <= 32 ? 32 : queries <= 64 ? 64 : 128;
+}
+
+// Workgroups that read the same keys or another head's: those of one piece.
+int64_t workgroups_per_piece(const tgx_paged& p, int heads, int group, int D, int dtype) {
+  return static_cast<int64_t>(p.table_heads) * heads *
+         ceil_div(static_cast<int64_t>(p.queries) * group, held_queries(p, group, D, dtype));
+}
+
+// How a launch is cut: W pieces wanted, pieces launched at most, and whether
+// any sequence can have several.
 struct Cut {
   int64_t wanted, launched;
   bool split;
 };
 
 // Workgroups wanted in all: what the GPU holds at once (two a CU at D = 128, four
-// below), twice over at D = 128.  Four of 100k to 131k tokens: 346 us with
-// two rounds that fit, 368-420 us with rounds that end half full; more and
-// smaller pieces pay for their first loads, fewer end unevenly.
-int64_t wanted_workgroups() {
+// below), twice over at D = 128.  Four sequences of 100k to 131k tokens: 346 us
+// with two rounds that fit, 368-420 us with rounds that end half full; more
+// and smaller pieces pay for their first loads, fewer end unevenly.  A
+// workgroup of more than 64 queries writes and joins as much as it reads of a
+// few tiles of keys: half as many (512 new tokens of four sequences: 322 us,
+// 242 us).
+//
+// Nothing is split where it cannot be (a table of kMinTiles), where one
+// piece has as many workgroups as are wanted, and where short tables (up
+// to kWholeTiles) of many sequences give every CU a workgroup: the join's
+// launch costs more than the unevenness (32 sequences of 8 heads over 24
+// pages of 64: attention 44 us, 36 us).
+constexpr int kWholeTiles = 32;
+
+Cut cut_of(const tgx_paged& p, int heads, int group, int D, int dtype) {
   int dev = 0, cus = 256;
   if (hipGetDevice(&dev) == hipSuccess)
     (void)hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
-  return static_cast<int64_t>(cus) * 4;
-}
-
-Cut cut_of(const tgx_paged& p, int64_t groups) {
+  const int64_t each = workgroups_per_piece(p, heads, group, D, dtype);
   const int64_t tiles = ceil_div(static_cast<int64_t>(p.pages_per_seq) * p.page_size, kTile);
-  if (tiles <= kMinTiles) return Cut{1, p.n_seqs, false};
-  const int64_t wanted = std::max<int64_t>(1, wanted_workgroups() / groups);
-  const int64_t most = p.n_seqs * ceil_div(tiles, kMinTiles);
-  return Cut{wanted, std::min(wanted + p.n_seqs, most), true};
-}
-
-// Whether the matrix tiles take the shape; the rows kernel takes every other.
-bool tiled(int D, int dtype) {
-  return dtype != TGX_DTYPE_F32 && (D == 32 || D == 64 || D == 128);
-}
-
-// Queries a workgroup of the tiles holds.
-int tile_queries(const tgx_paged& p, int group) {
-  const int64_t queries = static_cast<int64_t>(p.queries) * group;
-  return queries <= 16 ? 16 : queries <= 32 ? 32 : 64;
-}
-
-int64_t workgroups_per_piece(const tgx_paged& p, int heads, int group, int D, int dtype) {
-  const int64_t queries = static_cast<int64_t>(p.queries) * group;
-  return static_cast<int64_t>(p.table_heads) * heads *
-         (tiled(D, dtype) ? ceil_div(queries, tile_queries(p, group)) : queries);
+  const int64_t wanted = cus * (held_queries(p, group, D, dtype) > 64 ? 2 : 4) / each;
+  if (tiles <= kMinTiles || wanted <= 1 || (tiles <= kWholeTiles && p.n_seqs * each >= cus))
+    return Cut{1, p.n_seqs, false};
+  return Cut{wanted, std::min(wanted + p.n_seqs, p.n_seqs * ceil_div(tiles, kMinTiles)), true};
 }
 
 int check_attn(const tgx_paged* p, int heads, int group, int D, int dtype) {
@@ -894,7 +937,7 @@ int check_attn(const tgx_paged* p, int heads, int group, int D, int dtype) {
   const int64_t each = workgroups_per_piece(*p, heads, group, D, dtype);
   const int64_t pairs = static_cast<int64_t>(p->table_heads) * heads;
   TGX_REQUIRE(each <= kMaxBlocks256 && pairs * rows <= kMaxBlocks256 &&
-                  cut_of(*p, each).launched <= kMaxBlocks256 / each - 8 &&
+                  cut_of(*p, heads, group, D, dtype).launched <= kMaxBlocks256 / each - 8 &&
                   p->n_seqs <= kMaxBlocks256 / (pairs * rows),
               "paged attention: too many sequences, heads and queries for one launch");
   return TGX_OK;
@@ -941,27 +984,27 @@ int dispatch_join(const PagedArgs& a, hipStream_t stream) {
 }
 
 template <typename T, int D>
-int launch_tiles(const PagedArgs& a, const Cut& cut, hipStream_t stream) {
+int launch_tiles(const PagedArgs& a, const Cut& cut, int held, hipStream_t stream) {
   const int64_t rows = static_cast<int64_t>(a.rel.queries) * a.group;
   const int64_t pieces = cut.launched * a.rel.heads * a.heads;
   TGX_PROFILE("paged_tiles", stream);
-  if (rows <= 16) {
+  if (held == 16) {
     paged_tile_kernel<T, D><<<dim3(static_cast<uint32_t>(pieces)), dim3(256), 0, stream>>>(a);
   } else {
-    const int held = rows <= 32 ? 32 : 64;
     const dim3 grid(static_cast<uint32_t>(ceil_div(pieces, 8) * 8 * ceil_div(rows, held)));
-    if (held == 32) paged_block_kernel<T, D, 2><<<grid, dim3(256), 0, stream>>>(a);
-    else paged_block_kernel<T, D, 1><<<grid, dim3(256), 0, stream>>>(a);
+    if (held == 32) paged_block_kernel<T, D, 2, 1><<<grid, dim3(256), 0, stream>>>(a);
+    else if (held == 64) paged_block_kernel<T, D, 1, 1><<<grid, dim3(256), 0, stream>>>(a);
+    else paged_block_kernel<T, D, 1, 2><<<grid, dim3(256), 0, stream>>>(a);
   }
   TGX_LAUNCHED("paged_tiles");
   return TGX_OK;
 }
 
 template <typename T>
-int dispatch_tiles(const PagedArgs& a, const Cut& cut, hipStream_t stream) {
-  if (a.D == 32) return launch_tiles<T, 32>(a, cut, stream);
-  if (a.D == 64) return launch_tiles<T, 64>(a, cut, stream);
-  return launch_tiles<T, 128>(a, cut, stream);
+int dispatch_tiles(const PagedArgs& a, const Cut& cut, int held, hipStream_t stream) {
+  if (a.D == 32) return launch_tiles<T, 32>(a, cut, held, stream);
+  if (a.D == 64) return launch_tiles<T, 64>(a, cut, held, stream);
+  return launch_tiles<T, 128>(a, cut, held, stream);
 }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -976,7 +1019,7 @@ extern "C" int tgx_paged_attn_workspace(const tgx_paged* p, int heads, int group
   TGX_REQUIRE(bytes != nullptr, "null bytes");
   if (int st = check_attn(p, heads, group, D, dtype)) return st;
   const int64_t groups = static_cast<int64_t>(p->table_heads) * heads;
-  const Cut cut = cut_of(*p, workgroups_per_piece(*p, heads, group, D, dtype));
+  const Cut cut = cut_of(*p, heads, group, D, dtype);
   *bytes = !cut.split ? 0
                       : meta_bytes(*p) + sizeof(float) * cut.launched * groups * group *
                                              p->queries * (D + 2);
@@ -1001,7 +1044,7 @@ extern "C" int tgx_paged_attn(const tgx_paged* p, const void* q_dev, const void*
   if (int st = tgx_paged_attn_workspace(p, heads, group, D, dtype, &need)) return st;
   TGX_REQUIRE(workspace_bytes >= need && (need == 0 || workspace_dev),
               "workspace of %zu bytes, needs %zu", workspace_bytes, need);
-  const Cut cut = cut_of(*p, workgroups_per_piece(*p, heads, group, D, dtype));
+  const Cut cut = cut_of(*p, heads, group, D, dtype);
   PagedArgs a{};
   a.rel = paged_rel(*p);
   // Without pages there is no slot to read, whatever the lengths say.
@@ -1024,13 +1067,14 @@ extern "C" int tgx_paged_attn(const tgx_paged* p, const void* q_dev, const void*
   }
   hipStream_t s = as_stream(stream);
   const bool tiles = tiled(D, dtype);
+  const int held = held_queries(*p, group, D, dtype);
   int st;
   switch (dtype) {
     case TGX_DTYPE_BF16:
-      st = tiles ? dispatch_tiles<__bf16>(a, cut, s) : dispatch_rows<TGX_DTYPE_BF16>(a, cut, s);
+      st = tiles ? dispatch_tiles<__bf16>(a, cut, held, s) : dispatch_rows<TGX_DTYPE_BF16>(a, cut, s);
       return st || !cut.split ? st : dispatch_join<TGX_DTYPE_BF16>(a, s);
     case TGX_DTYPE_F16:
-      st = tiles ? dispatch_tiles<_Float16>(a, cut, s) : dispatch_rows<TGX_DTYPE_F16>(a, cut, s);
+      st = tiles ? dispatch_tiles<_Float16>(a, cut, held, s) : dispatch_rows<TGX_DTYPE_F16>(a, cut, s);
       return st || !cut.split ? st : dispatch_join<TGX_DTYPE_F16>(a, s);
     default:
       st = dispatch_rows<TGX_DTYPE_F32>(a, cut, s);
