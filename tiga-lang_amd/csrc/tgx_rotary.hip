@@ -33,6 +33,8 @@
 namespace tgx {
 namespace {
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
 struct RotaryArgs {
   const void* x[2];         // queries, keys
   int64_t xs_token[2], xs_head[2];
@@ -64,7 +66,24 @@ struct Chunk<DT, 8> {
   using Raw = typename V::Raw;
   static __device__ __forceinline__ Raw load(const T* p) { return V::load(p); }
   static __device__ __forceinline__ void unpack(const Raw& r, float (&f)[8]) { V::unpack(r, f); }
-  static __device__ __forceinline__ void store(T* p, const float (&f)[8]) { V::store(p, f); }
+  // FAR: past the caches, for outputs that they would not hold anyway.
+  template <bool FAR>
+  static __device__ __forceinline__ void store(T* p, const float (&f)[8]) {
+    if constexpr (!FAR) {
+      V::store(p, f);
+    } else if constexpr (DT == TGX_DTYPE_F32) {
+      f32x4* q = reinterpret_cast<f32x4*>(p);
+      __builtin_nontemporal_store(f32x4{f[0], f[1], f[2], f[3]}, q);
+      __builtin_nontemporal_store(f32x4{f[4], f[5], f[6], f[7]}, q + 1);
+    } else {
+      u32x4 w;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        w[k] = DT == TGX_DTYPE_BF16 ? pack_bf16x2(f[2 * k], f[2 * k + 1])
+                                    : pack_f16x2(f[2 * k], f[2 * k + 1]);
+      __builtin_nontemporal_store(w, reinterpret_cast<u32x4*>(p));
+    }
+  }
 };
 template <>
 struct Chunk<TGX_DTYPE_F32, 2> {
@@ -77,6 +96,7 @@ struct Chunk<TGX_DTYPE_F32, 2> {
     f[0] = r[0];
     f[1] = r[1];
   }
+  template <bool>
   static __device__ __forceinline__ void store(T* p, const float (&f)[2]) {
     *reinterpret_cast<Raw*>(p) = Raw{f[0], f[1]};
   }
@@ -92,6 +112,7 @@ struct Chunk<TGX_DTYPE_BF16, 2> {
     f[0] = bf16_lo(r);
     f[1] = bf16_hi(r);
   }
+  template <bool>
   static __device__ __forceinline__ void store(T* p, const float (&f)[2]) {
     *reinterpret_cast<uint32_t*>(p) = pack_bf16x2(f[0], f[1]);
   }
@@ -104,6 +125,7 @@ struct Chunk<TGX_DTYPE_F16, 2> {
     return *reinterpret_cast<const uint32_t*>(p);
   }
   static __device__ __forceinline__ void unpack(Raw r, float (&f)[2]) { f16_pair(r, f[0], f[1]); }
+  template <bool>
   static __device__ __forceinline__ void store(T* p, const float (&f)[2]) {
     *reinterpret_cast<uint32_t*>(p) = pack_f16x2(f[0], f[1]);
   }
@@ -121,22 +143,30 @@ __device__ __forceinline__ void store_scalar(void* p, int dtype, int i, float v)
   else static_cast<_Float16*>(p)[i] = static_cast<_Float16>(v);
 }
 
-// Where a lane's two chunks of a row are, and which pairs they make: pair j
-// of the chunks is frequency N * part + j.
+// Where a lane's two chunks of a row are, so that the lanes of a row take one
+// run of columns with each: the two halves of the rotated columns and of the
+// rest, or (adjacent pairs) of the row.  The lane's pair j is frequency `low` +
+// j, from j = N / 2 on `high` + j; pairs of columns that are not rotated
+// have frequencies from n_freqs on.
 template <int N, bool INTER>
 struct Place {
   int first, second;   // columns of the chunks
+  int low, high;
   bool has;
   __device__ __forceinline__ Place(const RotaryArgs& a, int part) {
     has = 2 * N * part < a.D;
-    if (INTER || N * part >= a.half) {
-      // Adjacent pairs, or the columns that are not rotated.
-      first = 2 * N * part;
-      second = first + N;
-    } else {
+    if constexpr (INTER) {
       first = N * part;
-      second = a.half + N * part;
+      second = a.D / 2 + N * part;
+      low = N / 2 * part;
+      high = a.D / 4 + N / 2 * part - N / 2;
+    } else {
+      const int c = N * part;
+      first = c < a.half ? c : c + a.half;
+      second = c < a.half ? c + a.half : c + a.D / 2;
+      low = high = c;
     }
+    if (!has) low = high = 0;
   }
 };
 
@@ -173,14 +203,15 @@ __device__ __forceinline__ void form_turns(const RotaryArgs& a, int64_t token,
   }
 }
 
-// The turns of pairs N * part .. N * part + N - 1.
-template <int N>
-__device__ __forceinline__ void read_turns(const float* cs, int part, float (&c)[N],
-                                           float (&s)[N]) {
+// The turns of the lane's pairs.
+template <int N, bool INTER>
+__device__ __forceinline__ void read_turns(const float* cs, const Place<N, INTER>& at,
+                                           float (&c)[N], float (&s)[N]) {
 #pragma unroll
-  for (int j = 0; j < N; j += 2) {
-    const f32x4 v = *reinterpret_cast<const f32x4*>(cs + 2 * (N * part + j));
-    c[j] = v[0], s[j] = v[1], c[j + 1] = v[2], s[j + 1] = v[3];
+  for (int j = 0; j < N; ++j) {
+    const f32x2 v = *reinterpret_cast<const f32x2*>(cs + 2 * ((j < N / 2 ? at.low : at.high) + j));
+    c[j] = v[0];
+    s[j] = v[1];
   }
 }
 
@@ -224,9 +255,9 @@ struct Weights {
 };
 
 // Passes of 64 / LPR rows whose loads are issued together.
-constexpr int kPasses = 4;
+constexpr int kPasses = 2;
 
-template <int DT, int N, int LPR, bool INTER>
+template <int DT, int N, int LPR, bool INTER, bool FAR>
 __global__ __launch_bounds__(256) void norm_rotary_fwd_kernel(RotaryArgs a) {
   using C = Chunk<DT, N>;
   using T = typename C::T;
@@ -269,7 +300,7 @@ __global__ __launch_bounds__(256) void norm_rotary_fwd_kernel(RotaryArgs a) {
       if (!formed) {
         form_turns<PAIRS>(a, token, freq, cs);
         __builtin_amdgcn_wave_barrier();
-        read_turns<N>(cs, part, c, s);
+        read_turns<N, INTER>(cs, at, c, s);
         formed = true;
       }
 #pragma unroll
@@ -295,17 +326,17 @@ __global__ __launch_bounds__(256) void norm_rotary_fwd_kernel(RotaryArgs a) {
         if (row < rows && at.has) {
           T* y = static_cast<T*>(a.out[side]) +
                  (token * a.heads[side] + row - (side ? a.heads[0] : 0)) * a.D;
-          C::store(y + at.first, f);
-          C::store(y + at.second, g);
+          C::template store<FAR>(y + at.first, f);
+          C::template store<FAR>(y + at.second, g);
         }
       }
     }
   }
 }
 
-constexpr int kBwdPasses = 2;
+constexpr int kBwdPasses = 1;
 
-template <int DT, int N, int LPR, bool INTER>
+template <int DT, int N, int LPR, bool INTER, bool FAR>
 __global__ __launch_bounds__(256) void norm_rotary_bwd_kernel(RotaryArgs a) {
   using C = Chunk<DT, N>;
   using T = typename C::T;
@@ -354,7 +385,7 @@ __global__ __launch_bounds__(256) void norm_rotary_bwd_kernel(RotaryArgs a) {
         if (!formed) {
           form_turns<PAIRS>(a, token, freq, cs);
           __builtin_amdgcn_wave_barrier();
-          read_turns<N>(cs, part, c, s);
+          read_turns<N, INTER>(cs, at, c, s);
           formed = true;
         }
 #pragma unroll
@@ -395,8 +426,8 @@ __global__ __launch_bounds__(256) void norm_rotary_bwd_kernel(RotaryArgs a) {
           }
           if (head < heads && at.has) {
             T* dx = static_cast<T*>(a.out[side]) + (token * heads + head) * a.D;
-            C::store(dx + at.first, df);
-            C::store(dx + at.second, dg);
+            C::template store<FAR>(dx + at.first, df);
+            C::template store<FAR>(dx + at.second, dg);
           }
         }
       }
@@ -456,10 +487,15 @@ __global__ __launch_bounds__(1024) void norm_rotary_dw_kernel(const float* parti
 
 bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
+// Outputs of more bytes than this are stored past the caches (a fraction of
+// the last level, so that what reads a smaller one next finds it there): 16384
+// tokens of 32 + 8 heads of 128, bf16, forward and backward 187 -> 160 us.
+constexpr int64_t kCached = int64_t{64} << 20;
+
 // Workgroups at most: enough to fill the GPU, few enough that the weights and
 // frequencies a wave loads first serve many tokens.
-constexpr int64_t kFwdBlocks = 2048;
-constexpr int64_t kBwdBlocks = 1024;
+constexpr int64_t kFwdBlocks = 1024;
+constexpr int64_t kBwdBlocks = 512;
 
 // Waves that share a token's rows: with few tokens, so many that the rows of a
 // token do not queue behind each other.
@@ -555,30 +591,36 @@ int args_of(const tgx_norm_rotary& p, void* const out[2], const void* const dy[2
   return TGX_OK;
 }
 
-template <bool BWD, int DT, int N, int LPR>
-int launch(RotaryArgs a, bool inter, int64_t blocks, hipStream_t stream) {
+template <bool BWD, int DT, int N, int LPR, bool FAR>
+int launch(const RotaryArgs& a, bool inter, int64_t blocks, hipStream_t stream) {
   const dim3 grid(static_cast<uint32_t>(blocks)), block(256);
   if constexpr (BWD) {
     TGX_PROFILE("norm_rotary_bwd", stream);
-    if (inter) norm_rotary_bwd_kernel<DT, N, LPR, true><<<grid, block, 0, stream>>>(a);
-    else norm_rotary_bwd_kernel<DT, N, LPR, false><<<grid, block, 0, stream>>>(a);
+    if (inter) norm_rotary_bwd_kernel<DT, N, LPR, true, FAR><<<grid, block, 0, stream>>>(a);
+    else norm_rotary_bwd_kernel<DT, N, LPR, false, FAR><<<grid, block, 0, stream>>>(a);
   } else {
     TGX_PROFILE("norm_rotary_fwd", stream);
-    if (inter) norm_rotary_fwd_kernel<DT, N, LPR, true><<<grid, block, 0, stream>>>(a);
-    else norm_rotary_fwd_kernel<DT, N, LPR, false><<<grid, block, 0, stream>>>(a);
+    if (inter) norm_rotary_fwd_kernel<DT, N, LPR, true, FAR><<<grid, block, 0, stream>>>(a);
+    else norm_rotary_fwd_kernel<DT, N, LPR, false, FAR><<<grid, block, 0, stream>>>(a);
   }
   TGX_LAUNCHED(BWD ? "norm_rotary_bwd" : "norm_rotary_fwd");
   return TGX_OK;
 }
 
+template <bool BWD, int DT, int LPR>
+int launch_wide(const RotaryArgs& a, bool far, bool inter, int64_t blocks, hipStream_t s) {
+  return far ? launch<BWD, DT, 8, LPR, true>(a, inter, blocks, s)
+             : launch<BWD, DT, 8, LPR, false>(a, inter, blocks, s);
+}
+
 template <bool BWD, int DT>
-int by_form(const RotaryArgs& a, Form f, bool inter, int64_t blocks, hipStream_t s) {
-  if (f.n == 2) return launch<BWD, DT, 2, 64>(a, inter, blocks, s);
+int by_form(const RotaryArgs& a, Form f, bool far, bool inter, int64_t blocks, hipStream_t s) {
+  if (f.n == 2) return launch<BWD, DT, 2, 64, false>(a, inter, blocks, s);
   switch (f.lpr) {
-    case 2: return launch<BWD, DT, 8, 2>(a, inter, blocks, s);
-    case 4: return launch<BWD, DT, 8, 4>(a, inter, blocks, s);
-    case 8: return launch<BWD, DT, 8, 8>(a, inter, blocks, s);
-    default: return launch<BWD, DT, 8, 16>(a, inter, blocks, s);
+    case 2: return launch_wide<BWD, DT, 2>(a, far, inter, blocks, s);
+    case 4: return launch_wide<BWD, DT, 4>(a, far, inter, blocks, s);
+    case 8: return launch_wide<BWD, DT, 8>(a, far, inter, blocks, s);
+    default: return launch_wide<BWD, DT, 16>(a, far, inter, blocks, s);
   }
 }
 
@@ -586,11 +628,16 @@ template <bool BWD>
 int run(const tgx_norm_rotary& p, RotaryArgs a, bool wide, int64_t max_blocks, hipStream_t s) {
   const Form f = form_of(p, wide);
   a.split = rows_split(p, 64 / f.lpr);
+  const int size = dtype_bytes(p.dtype);
+  // (Lines that a store instruction fills only in part belong in the caches.)
+  const int runs[2] = {p.interleaved ? p.D / 2 : p.n_freqs, p.interleaved ? 0 : p.D / 2 - p.n_freqs};
+  const bool far = p.n_tokens * (p.heads[0] + p.heads[1]) * p.D * size > kCached &&
+                   runs[0] * size % 128 == 0 && runs[1] * size % 128 == 0;
   const int64_t blocks = std::min(max_blocks, ceil_div(p.n_tokens * a.split, 4));
   switch (p.dtype) {
-    case TGX_DTYPE_BF16: return by_form<BWD, TGX_DTYPE_BF16>(a, f, p.interleaved, blocks, s);
-    case TGX_DTYPE_F16: return by_form<BWD, TGX_DTYPE_F16>(a, f, p.interleaved, blocks, s);
-    default: return by_form<BWD, TGX_DTYPE_F32>(a, f, p.interleaved, blocks, s);
+    case TGX_DTYPE_BF16: return by_form<BWD, TGX_DTYPE_BF16>(a, f, far, p.interleaved, blocks, s);
+    case TGX_DTYPE_F16: return by_form<BWD, TGX_DTYPE_F16>(a, f, far, p.interleaved, blocks, s);
+    default: return by_form<BWD, TGX_DTYPE_F32>(a, f, far, p.interleaved, blocks, s);
   }
 }
 
