@@ -152,6 +152,16 @@ def test_many_sequences():
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_launches_that_are_not_split(dtype):
+    """Short tables of many sequences, and as many workgroups of one piece as the
+    GPU holds."""
+    rng = np.random.default_rng(15)
+    check([int(n) for n in rng.integers(0, 1000, size=150)], 16, 2, 2, 64, TYPES[dtype])
+    if dtype != "f32":
+        check([400, 20], 16, 8, 16, 128, TYPES[dtype], queries=300)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_pages_that_are_not_there(dtype):
     check([40, 64, 300, 1000], 16, 2, 3, 64, TYPES[dtype], queries=2, missing=12)
 
@@ -200,6 +210,34 @@ def test_newer_tokens_never_reach_older_rows(dtype):
     lim = bound(TYPES[dtype], *clean, exp, 0.125, 131)
     assert (np.abs(got - exp)[:, :3] <= lim[:, :3]).all()
     assert not np.isfinite(got[:, 3]).any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("queries,group", [(1, 4), (6, 4), (12, 4), (30, 4)])
+def test_values_that_are_infinite_where_they_are_seen(dtype, queries, group):
+    """Inf, -Inf and NaN of a seen value come out as the formula has them."""
+    rng = np.random.default_rng(14)
+    table, lengths, pages = relation(rng, [100, 300], 16)
+    g = tg.Graph.paged(torch.tensor(table, device=DEV), torch.tensor(lengths, device=DEV),
+                       page_size=16, num_pages=pages, queries=queries)
+    mk = lambda *s: torch.tensor(rng.standard_normal(s), device=DEV).to(TYPES[dtype])
+    q, k, v = mk(2 * queries, 2, group, 64), mk(pages * 16, 2, 64), mk(pages * 16, 2, 64)
+    for pos, d, x in ((3, 5, np.inf), (50, 9, -np.inf), (60, 11, np.nan), (40, 13, np.inf),
+                      (41, 13, -np.inf)):
+        for b in range(2):
+            v[int(table[b, pos // 16]) * 16 + pos % 16, :, d] = x
+    out = Attention()(graph=g, src={"key": k[:, :, None], "value": v[:, :, None]},
+                      dst={"query": q}, scale=0.125)
+    with np.errstate(invalid="ignore"):
+        exp = want.attention(table, lengths, 16, pages, queries, f64(q), f64(k), f64(v), 0.125)
+    got = f64(out)
+    assert np.array_equal(np.isnan(got), np.isnan(exp))
+    assert np.array_equal(np.isposinf(got), np.isposinf(exp))
+    assert np.array_equal(np.isneginf(got), np.isneginf(exp))
+    fin = np.isfinite(exp)
+    lim = bound(TYPES[dtype], f64(q), f64(k), np.nan_to_num(f64(v), posinf=0, neginf=0), exp,
+                0.125, 300)
+    assert (np.abs(got - exp)[fin] <= lim[fin]).all()
 
 
 @pytest.mark.parametrize("scale", [0.0, -0.25, 30.0])
@@ -362,6 +400,70 @@ def test_other_edge_functions_run_on_the_snapshot():
             exp = f64(x)[at].sum(0)
             assert np.abs(f64(out[b]) - exp).max() <= 80 * 2 ** -24 * 70 * float(x.abs().max())
         live -= torch.tensor([0, 5, 7], dtype=torch.int32, device=DEV)
+
+
+def test_a_cache_whose_offsets_pass_32_bits():
+    """The last pages of a cache of 9 GB, attended to, appended to and selected."""
+    heads, D, size = 8, 256, 16
+    pages = 72000          # 72000 * 16 * 8 * 256 * 2 bytes = 4.7 GB each
+    k = torch.empty(pages * size, heads, D, device=DEV, dtype=torch.float16)
+    v = torch.empty_like(k)
+    rng = np.random.default_rng(12)
+    for width in (256, 64):     # (64: the first columns, on the matrix tiles)
+        ids = np.arange(pages - 12, pages)[rng.permutation(12)].reshape(2, 6)
+        table = torch.tensor(ids, dtype=torch.int32, device=DEV)
+        lengths = torch.tensor([90, 33], dtype=torch.int32, device=DEV)
+        g = tg.Graph.paged(table, lengths, page_size=size, num_pages=pages)
+        mk = lambda *s: torch.tensor(rng.standard_normal(s), device=DEV).half()
+        kc, vc = k[..., :width], v[..., :width]
+        lo = (pages - 12) * size
+        kc[lo:], vc[lo:] = mk(12 * size, heads, width), mk(12 * size, heads, width)
+        new_k, new_v = mk(2, heads, width), mk(2, heads, width)
+        sums = torch.zeros(pages, heads, width, device=DEV)
+        small = [f64(kc[lo:]), f64(new_k), f64(vc[lo:]), f64(new_v), f64(sums[-12:])]
+        exp = want.append(ids - (pages - 12), [90, 33], size, 12, 1, *small)
+        g.append(kc, new_k, vc, new_v, page_sums=sums)
+        assert np.array_equal(f64(kc[lo:]), exp[0]) and np.array_equal(f64(vc[lo:]), exp[1])
+        assert np.abs(f64(sums[-12:]) - exp[2]).max() <= 16 * 2 ** -24 * 16 * 6
+        q = mk(2, heads, 2, width)
+        out = Attention()(graph=g, src={"key": kc[:, :, None], "value": vc[:, :, None]},
+                          dst={"query": q}, scale=width ** -0.5)
+        ref = want.attention(ids - (pages - 12), [90, 33], size, 12, 1, f64(q), exp[0], exp[1],
+                             width ** -0.5)
+        lim = bound(torch.float16, f64(q), exp[0], exp[1], ref, width ** -0.5, 90)
+        assert (np.abs(f64(out) - ref) <= lim).all()
+        chosen = g.select_pages(q, sums, 3)
+        pick, held = want.select(ids, [90, 33], size, pages, 1, f64(q),
+                                 _Offset(f64(sums[-12:]), pages - 12), 3)
+        assert np.array_equal(chosen.page_table.cpu().numpy(), pick)
+        assert np.array_equal(chosen.lengths.cpu().numpy(), held)
+
+
+class _Offset:
+    """An array whose first row has index `start`."""
+
+    def __init__(self, rows, start):
+        self.rows, self.start = rows, start
+
+    def __getitem__(self, at):
+        return self.rows[at[0] - self.start, at[1]]
+
+
+def test_under_inference_mode():
+    with torch.inference_mode():
+        table = torch.tensor([[1, 0]], dtype=torch.int32, device=DEV)
+        g = tg.Graph.paged(table, torch.tensor([17], dtype=torch.int32, device=DEV), page_size=16,
+                           num_pages=2)
+        kc = torch.zeros(32, 1, 64, device=DEV, dtype=torch.bfloat16)
+        new = torch.ones(1, 1, 64, device=DEV, dtype=torch.bfloat16)
+        sums = torch.zeros(2, 1, 64, device=DEV)
+        q, k = tg.nn.norm_rotary(new, new, torch.tensor([16], device=DEV),
+                                 torch.ones(32, device=DEV), query_weight=new[0, 0])
+        g.append(kc, k, kc.clone(), new, page_sums=sums)
+        chosen = g.select_pages(q, sums, 1)
+        assert chosen.page_table.tolist() == [[[0]]] and chosen.lengths.tolist() == [1]
+        out = Attention()(graph=chosen, src={"key": kc, "value": kc}, dst={"query": q}, scale=1.0)
+        assert torch.equal(out, kc[:1])
 
 
 def test_empty_relations():

@@ -423,8 +423,9 @@ __device__ __forceinline__ void add_values(const T* v, const f32x4 (&c)[QT][KT],
 }
 
 // The same key by key (`weights`: the wave's [16 KT][16] floats of LDS), for
-// steps that hold a NaN or Inf in a value some of the queries do not see:
-// what a query does not see is left out, not multiplied by 0.
+// steps that hold a NaN or Inf among their values: what a query does not see is
+// left out, not multiplied by 0, and an Inf is weighed once, not by the two
+// parts of its weight (Inf - Inf).
 template <typename T, int D, int KT>
 __device__ __forceinline__ void add_seen_values(const T* v, const f32x4 (&c)[KT], int g, int lr,
                                                 int pos, int limit, float* weights,
@@ -447,15 +448,22 @@ __device__ __forceinline__ void add_seen_values(const T* v, const f32x4 (&c)[KT]
   }
 }
 
+// Largest magnitudes (as bits) of the even and odd elements seen: an element
+// is a NaN or Inf when its exponent is all ones.
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 template <typename T>
-__device__ __forceinline__ bool any_odd(const vec8<T>& v) {
-  const u32x4 w = __builtin_bit_cast(u32x4, v);
-  constexpr uint32_t e = Frag<T>::kExponent;
-  bool odd = false;
+struct Largest {
+  u16x2 top = {0, 0};
+  __device__ __forceinline__ void see(const vec8<T>& v) {
+    const u32x4 w = __builtin_bit_cast(u32x4, v);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) odd |= (w[i] & e) == e || (w[i] >> 16 & e) == e;
-  return odd;
-}
+    for (int i = 0; i < 4; ++i)
+      top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[i] & 0x7FFF7FFFu));
+  }
+  __device__ __forceinline__ bool odd() const {
+    return top[0] >= Frag<T>::kExponent || top[1] >= Frag<T>::kExponent;
+  }
+};
 
 // The states of the WAVES waves that share 16 queries, joined in wave order and
 // written: the output, or the piece's partial.  `smem` holds [group][wave][16][D
@@ -532,12 +540,12 @@ constexpr size_t kJoinBytes = sizeof(float) * 4 * 16 * (D + 4 + 2);
 // first loads and the join among them).
 //
 // Keys a step: 64 leave room for fewer workgroups (24 sequences of up to 3000
-// tokens, 16 heads of 64: 47 us, 38 us with 32).  Workgroups a CU: at D = 128
+// tokens, 16 heads of 64: 47 us, 37 us with 32).  Workgroups a CU: at D = 128
 // three would need K's and V's fragments to share registers, and measured
-// equal.
+// equal; at D = 64 four spill (42 us).
 constexpr int KEYS = 32;
 template <typename T, int D>
-__global__ __launch_bounds__(256, (D == 128 ? 2 : 4)) void paged_tile_kernel(PagedArgs a) {
+__global__ __launch_bounds__(256, (D == 128 ? 2 : D == 64 ? 3 : 4)) void paged_tile_kernel(PagedArgs a) {
   constexpr int KT = KEYS / 16, KC = D / 32, ROW = kRow<D>;
   constexpr size_t kStage = sizeof(T) * 4 * KEYS * ROW;
   constexpr size_t kBytes = kStage + sizeof(float) * 4 * KEYS * 16;
@@ -627,14 +635,12 @@ __global__ __launch_bounds__(256, (D == 128 ? 2 : 4)) void paged_tile_kernel(Pag
             for (int kc = 0; kc < KC; ++kc) vf[kt][kc] = vec8<T>{};
           }
       }
-      bool odd = false;
-      if (tail && r.queries > 1) {
+      Largest<T> largest;
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
+      for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-          for (int kc = 0; kc < KC; ++kc) odd |= any_odd<T>(vf[kt][kc]);
-        odd = __any(odd);
-      }
+        for (int kc = 0; kc < KC; ++kc) largest.see(vf[kt][kc]);
+      const bool odd = __any(largest.odd());
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -689,7 +695,7 @@ __global__ __launch_bounds__(256, (D == 128 || QT == 2 ? 2 : 3)) void paged_bloc
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt)
     q[qt] = Query<T, D>(a, p, th, kh, wrow + 16 * qt + lr, rows, g);
-  // Fewest positions any of the wave's queries sees, most of the workgroup's and the wave's.
+  // The fewest and most positions any of the wave's queries sees, and of the workgroup's.
   auto sees = [&](int row) {
     return p.length - (r.queries - 1 - min(row, rows - 1) / a.group);
   };
@@ -744,17 +750,18 @@ __global__ __launch_bounds__(256, (D == 128 || QT == 2 ? 2 : 3)) void paged_bloc
     next_id = page_id(p.tile0 + 1);
   }
   for (int tile = p.tile0; tile < last; ++tile) {
-    const bool check = r.queries > 1 && tile * kTile + kTile > group_low;
+    // (Weights in one part need the look for NaN and Inf only where some are hidden.)
+    const bool look = QT == 1 || (r.queries > 1 && tile * kTile + kTile > group_low);
     __syncthreads();   // the tile before has been read
-    bool odd = false;
+    Largest<T> largest;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int at = threadIdx.x + 256 * i;
-      if (check) odd |= any_odd<T>(vr[i]);
+      if (look) largest.see(vr[i]);
       *reinterpret_cast<vec8<T>*>(ks + at / CPR * ROW + at % CPR * 8) = kr[i];
       *reinterpret_cast<vec8<T>*>(vs + at / CPR * ROW + at % CPR * 8) = vr[i];
     }
-    if (odd) sh_odd[tile & 1] = 1;
+    if (largest.odd()) sh_odd[tile & 1] = 1;
     if (threadIdx.x == 0) sh_odd[(tile + 1) & 1] = 0;
     __syncthreads();
     const unsigned long long gone = __ballot(slot < 0);
@@ -783,7 +790,7 @@ __global__ __launch_bounds__(256, (D == 128 || QT == 2 ? 2 : 3)) void paged_bloc
     for (int qt = 0; qt < QT; ++qt)
       weigh(c[qt], a.scale_log2, gone || pos + 16 * KT > low, gone >> key0, pos, q[qt].limit, g,
             m[qt], l[qt], o[qt]);
-    if (!check || !sh_odd[tile & 1]) {
+    if (!look || !sh_odd[tile & 1]) {
       add_values<T, D, KT, QT>(vs + key0 * ROW, c, g, lr, o);
     } else {
 #pragma unroll

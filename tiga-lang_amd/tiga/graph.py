@@ -509,7 +509,7 @@ class Graph:
             if not isinstance(value, int) or isinstance(value, bool) or value < least:
                 raise ValueError(f"{name} must be an integer of at least {least}")
         if max(num_pages * page_size, page_table.shape[-1] * page_size + 4096,
-               page_table.shape[0] * queries) >= 2**31:
+               page_table.shape[0] * queries, page_size, queries) >= 2**31:
             raise ValueError("a paged relation has fewer than 2**31 slots, positions and rows")
         state = PagedState(page_table, lengths, page_size, num_pages, queries)
         if validate == "full":
@@ -561,8 +561,9 @@ class Graph:
         written to is formed again from the page's slots up to the newest token
         (what `select_pages` ranks pages by).  No gradients.
 
-        Each sequence's written pages must be its own; two sequences writing
-        to one page leave either's rows there."""
+        Each sequence's written pages must be its own and named once in its
+        table (two writers of a slot leave either's row there), and key and
+        value must not lie in the caches they are written to."""
         state = self.paged_state
         tensors = (key_cache, key, value_cache, value, page_sums)
         try:
