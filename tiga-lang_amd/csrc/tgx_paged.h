@@ -48,6 +48,31 @@ inline int check_paged(const tgx_paged* p) {
   return TGX_OK;
 }
 
+// Inclusive prefix sum over the wave's lanes: shifts inside rows of 16 lanes,
+// then the rows' last lanes broadcast to the rows after them (no LDS).
+__device__ __forceinline__ int wave_prefix(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);   // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);   // row_shr:2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);   // row_shr:4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);   // row_shr:8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // row_bcast:15
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);   // row_bcast:31
+  return v;
+}
+
+// Largest value of the wave's lanes.
+__device__ __forceinline__ uint32_t wave_largest(uint32_t u) {
+  int v = static_cast<int>(u);
+  auto step = [&](int o) { v = static_cast<int>(max(static_cast<uint32_t>(v), static_cast<uint32_t>(o))); };
+  step(__builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false));
+  step(__builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false));
+  step(__builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false));
+  step(__builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false));
+  step(__builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false));
+  step(__builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false));
+  return static_cast<uint32_t>(read_lane(v, 63));
+}
+
 // Cached tokens of sequence b: what its page table can hold at most.
 __device__ __forceinline__ int paged_length(const PagedRel& r, int b) {
   return min(max(r.lengths[b], 0), r.pages_per_seq * r.page_size);

@@ -66,12 +66,6 @@ struct Piece {
   int tile0, tile1;
 };
 
-__device__ __forceinline__ int wave_sum(int v) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
-  return v;
-}
-
 // Cuts n tiles into p.count pieces whose sizes differ by one at most.
 __device__ __forceinline__ void cut_tiles(Piece& p, int n) {
   const int each = n / p.count, more = n % p.count;
@@ -106,7 +100,7 @@ __device__ __forceinline__ Piece find_piece(const PagedRel& r, int pieces, bool 
   const int b0 = lane * per, b1 = min(r.n_seqs, b0 + per);
   int tiles = 0;
   for (int b = b0; b < b1; ++b) tiles += (paged_length(r, b) + kTile - 1) / kTile;
-  const int total = wave_sum(tiles);
+  const int total = read_lane(wave_prefix(tiles), 63);
   // Rounding up adds a piece a sequence at most, which are taken off first.
   const int room = max(pieces - r.n_seqs, (pieces + 1) / 2);
   const int c = max(kMinTiles, (total + room - 1) / room);
@@ -116,12 +110,7 @@ __device__ __forceinline__ Piece find_piece(const PagedRel& r, int pieces, bool 
   else
     for (int b = b0; b < b1; ++b)
       mine += max(1, ((paged_length(r, b) + kTile - 1) / kTile + c - 1) / c);
-  int end = mine;   // inclusive prefix over the lanes
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int o = __shfl_up(end, d, 64);
-    if (lane >= d) end += o;
-  }
+  const int end = wave_prefix(mine);
   const unsigned long long hit = __ballot(x < end && x >= end - mine);
   if (!hit) return p;
   const int owner = __builtin_ctzll(hit);

@@ -293,15 +293,15 @@ __global__ __launch_bounds__(256) void select_score_any_kernel(SelectArgs a, int
   }
 }
 
-// One workgroup per (row, head) takes the `want` largest of n keys.  Byte by
-// byte from the top, a histogram of the keys that share the bytes before finds
-// the byte of the want-th largest; as soon as no more than THREADS keys share
-// it a wave ranks them against each other, and (last, last_page) is the key and
-// page of the want-th: a page is taken when its key is larger, or equal and the
-// page no later.  The first two bytes (sign, exponent, four bits) part most
-// scores; all eight are only gone through where more than 64 are equal.
-// A thread's first kHeld keys stay in registers.  Bound: latency, of some four
-// barriers a pass.
+// One workgroup per (row, head) takes the `want` largest of n keys.  A histogram
+// of the keys' 16 leading bits (sign, exponent, four bits of the fraction),
+// counted down from the largest key's, finds those of the want-th largest: among
+// a few hundred or thousand scores, some twenty share them.  Where more than 64
+// do, or the want-th lies further down, a histogram of each byte goes on (from
+// the top).  The 64 or fewer that are left are ranked by a wave against each
+// other, and (last, last_page) is the key and page of the want-th: a page is
+// taken when its key is larger, or equal and the page no later.  A thread's
+// first kHeld keys stay in registers.  Bound: latency, of some ten barriers.
 constexpr int kHeld = 8;
 
 template <int THREADS>
@@ -310,7 +310,7 @@ __global__ __launch_bounds__(THREADS) void select_pages_kernel(SelectArgs a) {
   const PagedRel& r = a.rel;
   __shared__ int hist[256];
   __shared__ int places[kHeld * WAVES];
-  __shared__ int sh_byte, sh_left, sh_share, sh_n, sh_page;
+  __shared__ int sh_bin, sh_left, sh_share, sh_n, sh_page;
   __shared__ uint64_t sh_last;
   __shared__ uint64_t cand[64];
   __shared__ int cand_page[64];
@@ -346,55 +346,67 @@ __global__ __launch_bounds__(THREADS) void select_pages_kernel(SelectArgs a) {
     for (int i = kHeld * THREADS + tid; i < n; i += THREADS) f(i, keys[i]);
   };
 
-  uint64_t prefix = 0, mask = 0;   // the bytes settled so far
+  uint64_t prefix = 0, mask = 0;   // the leading bits settled so far
   int left = want;                 // rank of the want-th among the keys that share them
   int share = n;
-  for (int shift = 56; share > 64 && shift >= 0; shift -= 8) {
+  // Wave 0: the bin of hist (bins in descending order of key) that holds the
+  // left-th largest; sh_share = 0 where the bins count too few.
+  auto find = [&]() {
+    if (wave != 0) return;
+    int own[4], sum = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum += own[i] = hist[4 * lane + i];
+    const int end = wave_prefix(sum);
+    int above = end - sum;
+    if (lane == 63 && end < left) sh_share = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (above < left && left <= above + own[i]) {
+        sh_bin = 4 * lane + i;
+        sh_left = left - above;
+        sh_share = own[i];
+      }
+      above += own[i];
+    }
+  };
+  int shift = 56;
+  if (share > 64) {
+    // The largest key's 16 leading bits (sign, exponent, four bits), and the 255
+    // values below.
+    uint32_t top = 0;
+    visit([&](int, uint64_t key) { top = max(top, static_cast<uint32_t>(key >> 48)); });
+    top = wave_largest(top);
+    if (lane == 0) places[wave] = static_cast<int>(top);
+    for (int i = tid; i < 256; i += THREADS) hist[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) top = max(top, static_cast<uint32_t>(places[w]));
+    visit([&](int, uint64_t key) {
+      const uint32_t bin = top - static_cast<uint32_t>(key >> 48);
+      if (bin < 256) atomicAdd(&hist[bin], 1);
+    });
+    __syncthreads();
+    find();
+    __syncthreads();
+    if (sh_share > 0) {
+      prefix = static_cast<uint64_t>(top - sh_bin) << 48;
+      mask = uint64_t{0xFFFF} << 48;
+      left = sh_left;
+      share = sh_share;
+      shift = 40;
+    }
+  }
+  for (; share > 64 && shift >= 0; shift -= 8) {
+    __syncthreads();
     for (int i = tid; i < 256; i += THREADS) hist[i] = 0;
     __syncthreads();
     visit([&](int, uint64_t key) {
-      if ((key & mask) != prefix) return;
-      const int byte = static_cast<int>(key >> shift) & 255;
-      if (shift < 56) {
-        atomicAdd(&hist[byte], 1);
-        return;
-      }
-      // Sign and exponent: few values, each added once a wave.
-      bool mine = true;
-      while (mine) {
-        const int one = uniform(byte);
-        const unsigned long long same = __ballot(byte == one);
-        if (byte == one) {
-          mine = false;
-          if (lane == __builtin_ctzll(same)) atomicAdd(&hist[one], __popcll(same));
-        }
-      }
+      if ((key & mask) == prefix) atomicAdd(&hist[255 - (static_cast<int>(key >> shift) & 255)], 1);
     });
     __syncthreads();
-    if (wave == 0) {
-      // Keys in the bytes above the lane's four: lane 63 has the largest bytes.
-      int own[4], sum = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sum += own[i] = hist[4 * lane + i];
-      int above = sum;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_down(above, d, 64);
-        if (lane + d < 64) above += o;
-      }
-      above -= sum;
-#pragma unroll
-      for (int i = 3; i >= 0; --i) {
-        if (above < left && left <= above + own[i]) {
-          sh_byte = 4 * lane + i;
-          sh_left = left - above;
-          sh_share = own[i];
-        }
-        above += own[i];
-      }
-    }
+    find();
     __syncthreads();
-    prefix |= static_cast<uint64_t>(sh_byte) << shift;
+    prefix |= static_cast<uint64_t>(255 - sh_bin) << shift;
     mask |= uint64_t{255} << shift;
     left = sh_left;
     share = sh_share;
@@ -450,12 +462,7 @@ __global__ __launch_bounds__(THREADS) void select_pages_kernel(SelectArgs a) {
         own[i] = at < kHeld * WAVES ? places[at] : 0;
         sum += own[i];
       }
-      int before = sum;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(before, d, 64);
-        if (lane >= d) before += o;
-      }
+      int before = wave_prefix(sum);
       if (lane == 63) sh_n = before;
       before -= sum;
 #pragma unroll
