@@ -256,6 +256,26 @@ def test_scales(scale):
         assert (np.abs(f64(out) - exp) <= lim).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_table_per_head(dtype):
+    """Rows of (sequence, token, head), sources of (slot, head), and key heads
+    inside a table head."""
+    rng = np.random.default_rng(16)
+    B, T, P, size, pages, queries, heads, group, D = 3, 4, 6, 16, 30, 2, 2, 3, 64
+    table = rng.integers(-1, pages, size=(B, T, P)).astype(np.int32)
+    lengths = np.array([90, 1, 33], dtype=np.int32)
+    g = tg.Graph.paged(torch.tensor(table, device=DEV), torch.tensor(lengths, device=DEV),
+                       page_size=size, num_pages=pages, queries=queries)
+    mk = lambda *s: torch.tensor(rng.standard_normal(s), device=DEV).to(TYPES[dtype])
+    q = mk(B * queries * T, heads, group, D)
+    k, v = mk(pages * size * T, heads, 1, D), mk(pages * size * T, heads, 1, D)
+    out = Attention()(graph=g, src={"key": k, "value": v}, dst={"query": q}, scale=0.125)
+    by = lambda t: f64(t).reshape(pages * size, T, heads, D)
+    exp = want.attention(table, lengths, size, pages, queries, f64(q), by(k), by(v), 0.125)
+    lim = bound(TYPES[dtype], f64(q), f64(k), f64(v), exp, 0.125, 90)
+    assert (np.abs(f64(out) - exp) <= lim).all()
+
+
 def test_field_shapes_without_a_group_dimension():
     rng = np.random.default_rng(3)
     table, lengths, pages = relation(rng, [33, 100], 16)

@@ -163,6 +163,8 @@ def test_paged_refusals():
             mk(TABLE, LENGTHS, **{**ok, **bad})
     with pytest.raises(ValueError, match="2\\*\\*31"):
         mk(TABLE, LENGTHS, page_size=SIZE, num_pages=2 ** 30)
+    with pytest.raises(ValueError, match="2\\*\\*30"):
+        mk(TABLE[:, :0], LENGTHS, page_size=2 ** 30, num_pages=1)
     with pytest.raises(ValueError, match="validate must be"):
         mk(TABLE, LENGTHS, validate="some", **ok)
     with pytest.raises(ValueError, match="more tokens"):

@@ -36,6 +36,7 @@ inline int check_paged(const tgx_paged* p) {
   TGX_REQUIRE(p->n_seqs >= 0 && p->table_heads >= 1 && p->pages_per_seq >= 0 &&
                   p->page_size >= 1 && p->num_pages >= 0 && p->queries >= 1,
               "paged relation with negative or zero sizes");
+  TGX_REQUIRE(p->page_size < (1 << 30), "pages of fewer than 2^30 slots");
   TGX_REQUIRE(p->n_seqs < (int64_t{1} << 31) && p->num_pages < (int64_t{1} << 31) &&
                   static_cast<int64_t>(p->pages_per_seq) * p->page_size <
                       (int64_t{1} << 31) - 4096 &&   // (kernels look a few tiles ahead)

@@ -17,9 +17,10 @@
 // of all sequences, in tiles of 64, are cut into pieces of at most `c` tiles,
 // c at least kMinTiles and just large enough for W pieces to cover them all;
 // sequence b gets k_b = max(1, ceil(tiles_b / c)) pieces of equal size, W
-// together where there are fewer than W / 2 sequences, W + n_seqs at most.  A sequence of one piece writes its output; of
-// several, each piece writes its running maximum, sum and unnormalized
-// output, which a second launch joins in piece order.
+// together where there are fewer than W / 2 sequences, W + n_seqs at most.  A
+// sequence of one piece writes its output; of several, each piece writes its
+// running maximum, sum and unnormalized output, which a second launch joins in
+// piece order.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -526,7 +527,7 @@ constexpr size_t kJoinBytes = sizeof(float) * 4 * 16 * (D + 4 + 2);
 // of that, so a wave always has 8 KB (D = 128) or more on its way.  Measured:
 // four sequences of 100k to 131k, 8 x 4 heads of 128, 347 us (5.6 TB/s, of 6.3
 // that plain reads reach); 64 of 100 to 4000 tokens 120 us (4.6 TB/s, the
-// first loads and the join among them).
+// join among them).
 //
 // Keys a step: 64 leave room for fewer workgroups (24 sequences of up to 3000
 // tokens, 16 heads of 64: 47 us, 37 us with 32).  Workgroups a CU: at D = 128
@@ -534,7 +535,8 @@ constexpr size_t kJoinBytes = sizeof(float) * 4 * 16 * (D + 4 + 2);
 // equal; at D = 64 four spill (42 us).
 constexpr int KEYS = 32;
 template <typename T, int D>
-__global__ __launch_bounds__(256, (D == 128 ? 2 : D == 64 ? 3 : 4)) void paged_tile_kernel(PagedArgs a) {
+__global__ __launch_bounds__(256, (D == 128 ? 2 : D == 64 ? 3 : 4)) void paged_tile_kernel(
+    PagedArgs a) {
   constexpr int KT = KEYS / 16, KC = D / 32, ROW = kRow<D>;
   constexpr size_t kStage = sizeof(T) * 4 * KEYS * ROW;
   constexpr size_t kBytes = kStage + sizeof(float) * 4 * KEYS * 16;
@@ -1067,10 +1069,12 @@ extern "C" int tgx_paged_attn(const tgx_paged* p, const void* q_dev, const void*
   int st;
   switch (dtype) {
     case TGX_DTYPE_BF16:
-      st = tiles ? dispatch_tiles<__bf16>(a, cut, held, s) : dispatch_rows<TGX_DTYPE_BF16>(a, cut, s);
+      st = tiles ? dispatch_tiles<__bf16>(a, cut, held, s)
+                 : dispatch_rows<TGX_DTYPE_BF16>(a, cut, s);
       return st || !cut.split ? st : dispatch_join<TGX_DTYPE_BF16>(a, s);
     case TGX_DTYPE_F16:
-      st = tiles ? dispatch_tiles<_Float16>(a, cut, held, s) : dispatch_rows<TGX_DTYPE_F16>(a, cut, s);
+      st = tiles ? dispatch_tiles<_Float16>(a, cut, held, s)
+                 : dispatch_rows<TGX_DTYPE_F16>(a, cut, s);
       return st || !cut.split ? st : dispatch_join<TGX_DTYPE_F16>(a, s);
     default:
       st = dispatch_rows<TGX_DTYPE_F32>(a, cut, s);

@@ -100,8 +100,9 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   const int length = paged_length(r, b);
   const int fresh = min(length, r.queries);        // new tokens that exist
   const int page = (length - fresh) / r.page_size + blockIdx.x / blocks % a.touched;
+  if (fresh == 0 || page >= r.pages_per_seq) return;
   const int base = page * r.page_size;             // position of the page's first slot
-  if (fresh == 0 || base >= length) return;
+  if (base >= length) return;
   const int id = r.table[b * r.seq_stride + page];
   if (static_cast<unsigned>(id) >= static_cast<unsigned>(r.num_pages)) return;
   const int held = min(length - base, r.page_size);

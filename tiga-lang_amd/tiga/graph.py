@@ -508,8 +508,10 @@ class Graph:
                                    ("queries", queries, 1)):
             if not isinstance(value, int) or isinstance(value, bool) or value < least:
                 raise ValueError(f"{name} must be an integer of at least {least}")
+        if page_size >= 2**30:
+            raise ValueError("page_size must be below 2**30")
         if max(num_pages * page_size, page_table.shape[-1] * page_size + 4096,
-               page_table.shape[0] * queries, page_size, queries) >= 2**31:
+               page_table.shape[0] * queries, queries) >= 2**31:
             raise ValueError("a paged relation has fewer than 2**31 slots, positions and rows")
         state = PagedState(page_table, lengths, page_size, num_pages, queries)
         if validate == "full":
