@@ -304,17 +304,27 @@ def stream_of(tensor) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
-_HERE = contextlib.nullcontext()
-
-
 def on_device(tensor):
-    """A context in which the tensor's device is the current one (a launch on
-    a stream of another device than the current one is refused)."""
+    """A context in which the tensor's device is the current one."""
     import torch
 
     if tensor.device.index == torch.cuda.current_device():
-        return _HERE
+        return contextlib.nullcontext()
     return torch.cuda.device(tensor.device)
+
+
+def launch(tensor, name: str, *args) -> None:
+    """Call entry point `name` with Torch's current stream on the tensor's
+    device as its last argument, that device being the current one (a launch
+    on a stream of another device is refused)."""
+    import torch
+
+    index = tensor.device.index
+    if index == torch._C._cuda_getDevice():
+        call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+        return
+    with torch.cuda.device(index):
+        call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
 DTYPE_BF16, DTYPE_F16, DTYPE_F32 = 0, 1, 2

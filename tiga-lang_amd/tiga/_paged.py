@@ -78,10 +78,9 @@ def bind_attention(graph, q, k, v, scale: float, heads: int, group: int):
     def launch(keep=(q, k, v)):
         out = torch.empty(shape, dtype=dtype, device=device)
         work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-        with _native.on_device(out):
-            _native.call("tgx_paged_attn", state.native(), *tensors, strides, scale,
-                         out.data_ptr(), heads, group, D, code,
-                         work.data_ptr() if need else None, need, _native.stream_of(out))
+        _native.launch(out, "tgx_paged_attn", state.native(), *tensors, strides, scale,
+                       out.data_ptr(), heads, group, D, code,
+                       work.data_ptr() if need else None, need)
         return out
 
     if not q.numel():
@@ -106,10 +105,9 @@ def append(graph, key_cache, key, value_cache, value, page_sums) -> None:
         return
     strides = (ctypes.c_int64 * 8)(*key_cache.stride()[:2], *key.stride()[:2],
                                    *value_cache.stride()[:2], *value.stride()[:2])
-    with _native.on_device(key_cache):
-        _native.call("tgx_paged_append", state.native(), key_cache.data_ptr(), key.data_ptr(),
-                     value_cache.data_ptr(), value.data_ptr(), strides, _native.ptr(page_sums),
-                     heads, D, DTYPES[key.dtype], _native.stream_of(key_cache))
+    _native.launch(key_cache, "tgx_paged_append", state.native(), key_cache.data_ptr(),
+                   key.data_ptr(), value_cache.data_ptr(), value.data_ptr(), strides,
+                   _native.ptr(page_sums), heads, D, DTYPES[key.dtype])
     torch.autograd.graph.increment_version(
         (key_cache, value_cache) if page_sums is None else (key_cache, value_cache, page_sums))
 
@@ -164,11 +162,10 @@ def select(graph, query, page_sums, count: int, table, lengths) -> None:
         need = state.checked["select-workspace", heads, count] = bytes_.value
     work = torch.empty(need, dtype=torch.uint8, device=query.device)
     strides = (ctypes.c_int64 * 3)(*query.stride()[:3])
-    with _native.on_device(query):
-        _native.call("tgx_select_pages", relation, query.data_ptr(), strides,
-                     page_sums.data_ptr() if page_sums.numel() else None, heads, group, D,
-                     DTYPES[query.dtype], count, table.data_ptr(), lengths.data_ptr(),
-                     work.data_ptr(), need, _native.stream_of(query))
+    _native.launch(query, "tgx_select_pages", relation, query.data_ptr(), strides,
+                   page_sums.data_ptr() if page_sums.numel() else None, heads, group, D,
+                   DTYPES[query.dtype], count, table.data_ptr(), lengths.data_ptr(),
+                   work.data_ptr(), need)
     torch.autograd.graph.increment_version((table, lengths))
 
 

@@ -33,65 +33,81 @@ def covered(form: Form, query, key, weights) -> bool:
             (key is None or key.dtype == dtype) and given <= set(_DTYPES) and len(given) <= 1)
 
 
+def _rows_ok(t: torch.Tensor) -> bool:
+    """Rows are dense and start on two values, counted from the tensor's start."""
+    s = t.stride()
+    return t.numel() == 0 or (s[2] == 1 and s[0] % 2 == 0 and s[1] % 2 == 0)
+
+
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """`t` with dense rows that start on two values."""
-    s = t.stride()
-    if (s[2] != 1 or s[0] % 2 or s[1] % 2) and t.numel():
+    if not _rows_ok(t):
         t = t.contiguous()
-    return t if t.data_ptr() % (2 * t.element_size()) == 0 else t.clone(memory_format=torch.contiguous_format)
+    return t if t.data_ptr() % (2 * t.element_size()) == 0 else \
+        t.clone(memory_format=torch.contiguous_format)
 
 
-_TEMPLATES: dict[tuple, _native.NormRotary] = {}
+def _struct(form: Form, query, key, query_weight, key_weight, positions,
+            frequencies) -> _native.NormRotary:
+    """The native operands but for their pointers."""
+    p = _native.NormRotary()
+    for i, x in enumerate((query, key)):
+        if x is not None:
+            p.token_stride[i], p.head_stride[i] = x.stride()[:2]
+            p.heads[i] = x.shape[1]
+    p.w_dtype = next((_DTYPES[w.dtype] for w in (query_weight, key_weight) if w is not None), 2)
+    p.positions_bits = _native.idx_bits(positions)
+    p.axes = len(form.sections)
+    for i, n in enumerate(form.sections):
+        p.sections[i] = n
+    p.n_freqs = frequencies.numel()
+    p.norm, p.interleaved, p.eps = int(form.norm), int(form.interleaved), form.eps
+    p.n_tokens, p.D = query.shape[0], query.shape[-1]
+    p.dtype = _DTYPES[query.dtype]
+    return p
 
 
-def _operands(form: Form, query, key, query_weight, key_weight, positions, frequencies):
+class Plan:
+    """What norm_rotary found for operands of some types, shapes and strides:
+    the form, whether the kernels take them, and the native operands of
+    rows that need no copy."""
+
+    def __init__(self, form: Form, query, key, query_weight, key_weight, positions, frequencies):
+        self.form = form
+        self.covered = covered(form, query, key, (query_weight, key_weight))
+        self.template, self.mask = None, 0
+        if self.covered and _rows_ok(query) and (key is None or _rows_ok(key)):
+            self.template = _struct(form, query, key, query_weight, key_weight, positions,
+                                    frequencies)
+            self.mask = 2 * query.element_size() - 1
+
+
+def _operands(plan: Plan, query, key, query_weight, key_weight, positions, frequencies):
     """The native operands, and the tensors they point into."""
-    query, key = _rows(query), None if key is None else _rows(key)
-    spec = (form, query.dtype, query.shape, query.stride(),
-            None if key is None else (key.shape, key.stride()),
-            None if query_weight is None else query_weight.dtype,
-            None if key_weight is None else key_weight.dtype, positions.dtype)
-    template = _TEMPLATES.get(spec)
-    if template is None:
-        template = _native.NormRotary()
-        for i, x in enumerate((query, key)):
-            if x is not None:
-                template.token_stride[i], template.head_stride[i] = x.stride()[:2]
-                template.heads[i] = x.shape[1]
-        template.w_dtype = next((_DTYPES[w.dtype] for w in (query_weight, key_weight)
-                                 if w is not None), 2)
-        template.positions_bits = _native.idx_bits(positions)
-        template.axes = len(form.sections)
-        for i, n in enumerate(form.sections):
-            template.sections[i] = n
-        template.n_freqs = frequencies.numel()
-        template.norm, template.interleaved = int(form.norm), int(form.interleaved)
-        template.eps = form.eps
-        template.n_tokens, template.D = query.shape[0], query.shape[-1]
-        template.dtype = _DTYPES[query.dtype]
-        if len(_TEMPLATES) >= 1024:
-            _TEMPLATES.clear()
-        _TEMPLATES[spec] = template
-    p = _native.NormRotary.from_buffer_copy(template)
-    p.x_dev[0] = query.data_ptr()
-    if key is not None:
-        p.x_dev[1] = key.data_ptr()
-    weights = [query_weight, key_weight]
-    for i in (0, 1):
-        if weights[i] is not None:
-            weights[i] = weights[i].contiguous()
-            p.w_dev[i] = weights[i].data_ptr()
+    q_at, k_at = query.data_ptr(), 0 if key is None else key.data_ptr()
+    if plan.template is None or (q_at | k_at) & plan.mask:
+        query, key = _rows(query), None if key is None else _rows(key)
+        q_at, k_at = query.data_ptr(), 0 if key is None else key.data_ptr()
+        p = _struct(plan.form, query, key, query_weight, key_weight, positions, frequencies)
+    else:
+        p = _native.NormRotary.from_buffer_copy(plan.template)
+    p.x_dev[0], p.x_dev[1] = q_at, k_at or None
+    if query_weight is not None:
+        query_weight = query_weight.contiguous()
+        p.w_dev[0] = query_weight.data_ptr()
+    if key_weight is not None:
+        key_weight = key_weight.contiguous()
+        p.w_dev[1] = key_weight.data_ptr()
     p.positions_dev, p.freqs_dev = positions.data_ptr(), frequencies.data_ptr()
-    return p, (query, key, *weights, positions, frequencies)
+    return p, (query, key, query_weight, key_weight, positions, frequencies)
 
 
-def forward(form: Form, query, key, query_weight, key_weight, positions, frequencies):
-    p, keep = _operands(form, query, key, query_weight, key_weight, positions, frequencies)
+def forward(plan: Plan, query, key, query_weight, key_weight, positions, frequencies):
+    p, keep = _operands(plan, query, key, query_weight, key_weight, positions, frequencies)
     out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
     key_out = None if key is None else torch.empty(key.shape, dtype=key.dtype, device=key.device)
-    with _native.on_device(query):
-        _native.call("tgx_norm_rotary_fwd", ctypes.byref(p), out.data_ptr(),
-                     None if key is None else key_out.data_ptr(), _native.stream_of(query))
+    _native.launch(query, "tgx_norm_rotary_fwd", ctypes.byref(p), out.data_ptr(),
+                   None if key is None else key_out.data_ptr())
     return out, key_out
 
 
@@ -99,47 +115,48 @@ class NormRotaryFunction(torch.autograd.Function):
     """(query, key) normed and rotated; gradients of query, key and weights."""
 
     @staticmethod
-    def forward(ctx, query, key, query_weight, key_weight, positions, frequencies, form):
-        ctx.form = form
+    def forward(ctx, query, key, query_weight, key_weight, positions, frequencies, plan):
+        ctx.plan = plan
         ctx.save_for_backward(query, key, query_weight, key_weight, positions, frequencies)
         ctx.set_materialize_grads(True)
-        outs = forward(form, query, key, query_weight, key_weight, positions, frequencies)
+        outs = forward(plan, query, key, query_weight, key_weight, positions, frequencies)
         return outs[0] if key is None else outs
 
     @staticmethod
     @once_differentiable
     def backward(ctx, *douts):
         query, key, query_weight, key_weight, positions, frequencies = ctx.saved_tensors
-        p, keep = _operands(ctx.form, query, key, query_weight, key_weight, positions,
+        p, keep = _operands(ctx.plan, query, key, query_weight, key_weight, positions,
                             frequencies)
         pair = 2 * query.element_size()
-        dense = []
-        for t, d in zip((query, key), douts):
-            d = d.to(t.dtype).contiguous()
-            dense.append(d if d.data_ptr() % pair == 0 else d.clone())
-        grads = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)
-                 for t in (query, key)]
-        dw = [torch.empty_like(w, memory_format=torch.contiguous_format)
+        given, grads = [None, None], [None, None]   # of the outputs; of query and key
+        for i, (t, d) in enumerate(zip((query, key), douts)):
+            d = (d if d.dtype == t.dtype else d.to(t.dtype)).contiguous()
+            given[i] = d if d.data_ptr() % pair == 0 else d.clone()
+            grads[i] = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        dw = [torch.empty(w.shape, dtype=w.dtype, device=w.device)
               if w is not None and need else None
               for w, need in zip((query_weight, key_weight), ctx.needs_input_grad[2:4])]
         work, size = None, ctypes.c_size_t(0)
-        if any(w is not None for w in dw):
+        if dw[0] is not None or dw[1] is not None:
             _native.call("tgx_norm_rotary_bwd_workspace", ctypes.byref(p), ctypes.byref(size))
             work = torch.empty(size.value, dtype=torch.uint8, device=query.device)
-        dense += [None] * (2 - len(dense))
-        with _native.on_device(query):
-            _native.call("tgx_norm_rotary_bwd", ctypes.byref(p),
-                         *(_native.ptr(t) for t in (*dense, *grads, *dw, work)), size.value,
-                         _native.stream_of(query))
+        _native.launch(query, "tgx_norm_rotary_bwd", ctypes.byref(p),
+                       *[None if t is None else t.data_ptr() for t in (*given, *grads, *dw, work)],
+                       size.value)
         return (*grads, *dw, None, None, None)
 
 
-def apply(form: Form, query, key, query_weight, key_weight, positions, frequencies):
-    if torch.is_grad_enabled() and any(
-            [t is not None and t.requires_grad for t in (query, key, query_weight, key_weight)]):
+def apply(plan: Plan, query, key, query_weight, key_weight, positions, frequencies):
+    if not plan.covered:
+        return reference(plan.form, query, key, query_weight, key_weight, positions, frequencies)
+    if torch.is_grad_enabled() and (
+            query.requires_grad or (key is not None and key.requires_grad) or
+            (query_weight is not None and query_weight.requires_grad) or
+            (key_weight is not None and key_weight.requires_grad)):
         return NormRotaryFunction.apply(query, key, query_weight, key_weight, positions,
-                                        frequencies, form)
-    outs = forward(form, query, key, query_weight, key_weight, positions, frequencies)
+                                        frequencies, plan)
+    outs = forward(plan, query, key, query_weight, key_weight, positions, frequencies)
     return outs[0] if key is None else outs
 
 

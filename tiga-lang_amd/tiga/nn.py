@@ -426,30 +426,28 @@ def norm_rotary(query: torch.Tensor, key: torch.Tensor | None, positions: torch.
     (``tiga.config.strict`` refuses those on the GPU)."""
     tensors = (query, key, positions, frequencies, query_weight, key_weight)
     try:
-        spec = (tuple([None if t is None else (t.dtype, t.shape, t.device) for t in tensors]),
-                eps, norm, sections, interleaved)
-        form = _ROTARY_FORMS.get(spec)
+        spec = (*[None if t is None else (t.dtype, t.shape, t.stride(), t.device)
+                  for t in tensors], eps, norm, sections, interleaved)
+        plan = _ROTARY_PLANS.get(spec)
     except (AttributeError, TypeError):
-        form = spec = None
-    if form is None:
-        form = _check_norm_rotary(*tensors, eps, norm, sections, interleaved)
+        plan = spec = None
+    if plan is None:
+        plan = _plan_norm_rotary(*tensors, eps, norm, sections, interleaved)
         if spec is not None:
-            if len(_ROTARY_FORMS) >= 1024:
-                _ROTARY_FORMS.clear()
-            _ROTARY_FORMS[spec] = form
-    form, run = form
+            if len(_ROTARY_PLANS) >= 1024:
+                _ROTARY_PLANS.clear()
+            _ROTARY_PLANS[spec] = plan
     if frequencies.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("norm_rotary has no gradient with respect to frequencies")
-    if query.is_cuda and run is _rotary.reference and _config().strict:
+    if not plan.covered and query.is_cuda and _config().strict:
         raise RuntimeError("norm_rotary: no HIP kernel covers these types and widths and "
                            "tiga.config.strict is set")
-    return run(form, query, key, query_weight, key_weight, positions.contiguous(),
-               frequencies.contiguous())
+    return _rotary.apply(plan, query, key, query_weight, key_weight, positions.contiguous(),
+                         frequencies.contiguous())
 
 
-# What norm_rotary found for operands of these types and shapes: its form and
-# whether the kernels take them.
-_ROTARY_FORMS: dict[tuple, tuple] = {}
+# norm_rotary's plans by the types, shapes and strides of its operands.
+_ROTARY_PLANS: dict[tuple, _rotary.Plan] = {}
 
 
 def _config():
@@ -458,8 +456,8 @@ def _config():
     return config
 
 
-def _check_norm_rotary(query, key, positions, frequencies, query_weight, key_weight, eps, norm,
-                       sections, interleaved):
+def _plan_norm_rotary(query, key, positions, frequencies, query_weight, key_weight, eps, norm,
+                      sections, interleaved) -> _rotary.Plan:
     for name, t in (("query", query), ("key", key)):
         if t is None and name == "key":
             continue
@@ -503,8 +501,7 @@ def _check_norm_rotary(query, key, positions, frequencies, query_weight, key_wei
         if t is not None and t.device != query.device:
             raise ValueError(f"operand on {t.device}, but query is on {query.device}")
     form = _rotary.Form(float(eps), bool(norm), sections, bool(interleaved))
-    covered = _rotary.covered(form, query, key, (query_weight, key_weight))
-    return form, _rotary.apply if covered else _rotary.reference
+    return _rotary.Plan(form, query, key, query_weight, key_weight, positions, frequencies)
 
 
 __all__ = ["ScoreLayer", "TracedModule", "norm_rotary", "trace"]
