@@ -10,7 +10,6 @@ implementation when it is missing.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 from pathlib import Path
@@ -302,15 +301,6 @@ def stream_of(tensor) -> int:
     if index is None:
         index = torch.cuda.current_device()
     return torch._C._cuda_getCurrentRawStream(index)
-
-
-def on_device(tensor):
-    """A context in which the tensor's device is the current one."""
-    import torch
-
-    if tensor.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(tensor.device)
 
 
 def launch(tensor, name: str, *args) -> None:

@@ -22,9 +22,13 @@ DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 def rows_on_16_bytes(t: torch.Tensor) -> bool:
     """Every row of `t` (its last dimension, dense) starts a multiple of 16
     bytes from the tensor's start."""
-    vec = 16 // t.element_size()
-    return (t.shape[-1] <= 1 or t.stride(-1) == 1) and all(
-        n <= 1 or s % vec == 0 for n, s in zip(t.shape[:-1], t.stride()[:-1]))
+    vec, shape, strides = 16 // t.element_size(), t.shape, t.stride()
+    if shape[-1] > 1 and strides[-1] != 1:
+        return False
+    for n, s in zip(shape[:-1], strides):
+        if n > 1 and s % vec:
+            return False
+    return True
 
 
 def _on_16_bytes(t: torch.Tensor) -> torch.Tensor:
@@ -66,12 +70,14 @@ def bind_attention(graph, q, k, v, scale: float, heads: int, group: int):
         k.stride(0) * tables, k.stride(0) if tables > 1 else 0, by_head(k),
         v.stride(0) * tables, v.stride(0) if tables > 1 else 0, by_head(v))
     code = DTYPES[q.dtype]
-    relation = state.native()
-    bytes_ = ctypes.c_size_t()
-    with _native.on_device(q):
-        _native.call("tgx_paged_attn_workspace", relation, heads, group, D, code,
-                     ctypes.byref(bytes_))
-    need, shape, dtype, device = bytes_.value, q.shape, q.dtype, q.device
+    need = state.checked.get(("attention-workspace", heads, group, D, code))
+    if need is None:
+        bytes_ = ctypes.c_size_t()
+        with torch.cuda.device(q.device):
+            _native.call("tgx_paged_attn_workspace", state.native(), heads, group, D, code,
+                         ctypes.byref(bytes_))
+        need = state.checked["attention-workspace", heads, group, D, code] = bytes_.value
+    shape, dtype, device = q.shape, q.dtype, q.device
     tensors = (q.data_ptr(), k.data_ptr() if k.numel() else None,
                v.data_ptr() if v.numel() else None)
 
