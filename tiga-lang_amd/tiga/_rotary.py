@@ -76,6 +76,7 @@ class Plan:
         self.form = form
         self.covered = covered(form, query, key, (query_weight, key_weight))
         self.template, self.mask = None, 0
+        self.work_bytes = None      # of the backward pass, asked at its first use
         if self.covered and _rows_ok(query) and (key is None or _rows_ok(key)):
             self.template = _struct(form, query, key, query_weight, key_weight, positions,
                                     frequencies)
@@ -137,13 +138,18 @@ class NormRotaryFunction(torch.autograd.Function):
         dw = [torch.empty(w.shape, dtype=w.dtype, device=w.device)
               if w is not None and need else None
               for w, need in zip((query_weight, key_weight), ctx.needs_input_grad[2:4])]
-        work, size = None, ctypes.c_size_t(0)
+        work, size = None, 0
         if dw[0] is not None or dw[1] is not None:
-            _native.call("tgx_norm_rotary_bwd_workspace", ctypes.byref(p), ctypes.byref(size))
-            work = torch.empty(size.value, dtype=torch.uint8, device=query.device)
+            size = ctx.plan.work_bytes
+            if size is None:
+                asked = ctypes.c_size_t()
+                _native.call("tgx_norm_rotary_bwd_workspace", ctypes.byref(p),
+                             ctypes.byref(asked))
+                size = ctx.plan.work_bytes = asked.value
+            work = torch.empty(size, dtype=torch.uint8, device=query.device)
         _native.launch(query, "tgx_norm_rotary_bwd", ctypes.byref(p),
                        *[None if t is None else t.data_ptr() for t in (*given, *grads, *dw, work)],
-                       size.value)
+                       size)
         return (*grads, *dw, None, None, None)
 
 
