@@ -141,6 +141,35 @@ def test_rows_on_odd_addresses_and_query_alone():
     assert torch.equal(a[0], b[0]) and (a[1] is None or not a[1].any())
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_one_layout_on_even_and_odd_addresses(dtype):
+    """Rows of one shape and strides, forward and back, wherever they start."""
+    dtype = TYPES[dtype]
+    q, k, w, pos, freqs, dy = make(9, 4, 2, 64, (32,), dtype)
+    results = []
+    for shift in (0, 1, 0, 3):
+        leaves = []
+        for x in (q, k):
+            room = torch.zeros(x.numel() + shift, device=DEV, dtype=dtype)[shift:]
+            leaves.append(room.view(x.shape).copy_(x.detach()).requires_grad_(True))
+        outs = tg.nn.norm_rotary(*leaves, pos, freqs, query_weight=w[0], key_weight=w[1])
+        results.append((*outs, *torch.autograd.grad(outs, (*leaves, *w), dy)))
+    for other in results[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(results[0], other))
+
+
+def test_calls_of_one_shape_keep_their_own_forms():
+    q, k, w, pos, freqs, dy = make(7, 2, 2, 32, (16,), torch.float32)
+    for forms in (dict(eps=1e-6), dict(eps=0.5), dict(interleaved=True), dict(norm=False),
+                  dict(sections=(16,)), dict(eps=1e-6)):
+        weights = dict(query_weight=w[0], key_weight=w[1]) if forms.get("norm", True) else {}
+        got = tg.nn.norm_rotary(q, k, pos, freqs, **forms, **weights)
+        same = tg.nn.norm_rotary(q.cpu(), k.cpu(), pos.cpu(), freqs.cpu(), **forms,
+                                 **{name: x.cpu() for name, x in weights.items()})
+        for a, b in zip(got, same):
+            assert (a.cpu() - b).abs().max() <= 64 * F32 * b.abs().max()
+
+
 def test_what_no_kernel_covers():
     q = torch.randn(3, 2, 6, device=DEV)
     pos, freqs = torch.arange(3, device=DEV), torch.ones(3, device=DEV)
