@@ -236,3 +236,61 @@ def test_training_attention_on_normed_and_rotated_fields():
         # (As in `check`, relative to the largest value.)
         assert np.abs(f64(got[i]) - dx).max() <= (2.0 ** -11 + 200 * F32) * np.abs(dx).max()
         assert np.abs(f64(got[2 + i]) - dw).max() <= (2.0 ** -11 + 200 * F32) * np.abs(dw).max()
+
+
+def same_kind(got, exp):
+    """NaN, Inf and -Inf in the same places."""
+    return all(np.array_equal(kind(got), kind(exp))
+               for kind in (np.isnan, np.isposinf, np.isneginf))
+
+
+@pytest.mark.parametrize("norm", [True, False])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("D,half,dtype", [
+    (8, 2, "f32"), (64, 16, "bf16"), (64, 10, "f16"), (128, 32, "f32"), (20, 6, "bf16"),
+    (64, 0, "bf16"), (64, 2, "f32"), (256, 64, "f16")])
+def test_infinite_values_in_columns_that_are_not_rotated(D, half, dtype, interleaved, norm):
+    """They come out as the formula has them, and reach no other column but
+    through the norm; the same of output gradients on the way back."""
+    n, h = 2 * (D - 2 * half) + 1, 3
+    q, _, w, pos, freqs, dy = make(n, h, 0, D, (half,), TYPES[dtype])
+    weights = dict(query_weight=w[0]) if norm else {}
+    call = lambda x: tg.nn.norm_rotary(x, None, pos, freqs, norm=norm, interleaved=interleaved,
+                                       **weights)
+
+    def spoiled(x):
+        """Token 2 i has an Inf, 2 i + 1 a -Inf in column 2 half + i of its first
+        head, and every third token a NaN there in its second."""
+        x = x.detach().clone()
+        for t in range(n - 1):
+            x[t, 0, 2 * half + t // 2] = float("-inf") if t % 2 else float("inf")
+            if t % 3 == 0:
+                x[t, 1, 2 * half + t // 2] = float("nan")
+        return x
+
+    angle = want.angles(pos.cpu().numpy(), freqs.cpu().numpy(), (half,))
+    xw, step = f64(w[0]) if norm else None, torch.finfo(TYPES[dtype]).eps / 2
+    # (As in `check`; a row's finite values are those of a clean row, or zero.)
+    ops, turn = 24 + D / 16, 4 * 2.0 ** -53 * np.abs(angle).max(initial=0.0)
+    with np.errstate(invalid="ignore"):
+        x = spoiled(q)
+        exp = want.norm_rotary(f64(x), xw, angle, 1e-6, norm, interleaved)
+        got = f64(call(x))
+        assert same_kind(got, exp)
+        fin = np.isfinite(exp)
+        top = np.where(fin, np.abs(exp), 0.0)
+        lim = step * top + (ops * F32 + turn) * 2 * top.max(-1, keepdims=True)
+        assert (np.abs(got - exp)[fin] <= lim[fin]).all()
+
+        d = spoiled(dy[0])
+        leaves = (q, w[0]) if norm else (q,)
+        grads = torch.autograd.grad(call(q), leaves, d)
+        dx, dw = want.norm_rotary_grad(f64(q), xw, angle, 1e-6, norm, interleaved, f64(d))
+        assert same_kind(f64(grads[0]), dx)
+        if norm:
+            assert same_kind(f64(grads[1]), dw)
+        else:
+            fin = np.isfinite(dx)
+            top = np.where(fin, np.abs(dx), 0.0)
+            lim = step * top + (ops * F32 + turn) * 2 * top.max(-1, keepdims=True)
+            assert (np.abs(f64(grads[0]) - dx)[fin] <= lim[fin]).all()

@@ -224,17 +224,22 @@ __device__ __forceinline__ float inverse_root(float v) {
 }
 
 // Turns pair j of the chunks (f, g) by (c, s): the halves of the pairs lie in
-// f and g, or next to each other.
+// f and g, or next to each other.  Pairs that are not rotated stay as they are
+// (turning them by nothing would multiply one's Inf by the other's sine of 0).
 template <int N, bool INTER>
-__device__ __forceinline__ void rotate(float (&f)[N], float (&g)[N], const float (&c)[N],
+__device__ __forceinline__ void rotate(const RotaryArgs& a, const Place<N, INTER>& at,
+                                       float (&f)[N], float (&g)[N], const float (&c)[N],
                                        const float (&s)[N], float sign) {
+  // (Apart, a lane's pairs are all rotated or none: half is a multiple of N.)
+  if (!INTER && at.low >= a.half) return;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     float* pa = INTER ? (j < N / 2 ? &f[2 * j] : &g[2 * j - N]) : &f[j];
     float* pb = INTER ? pa + 1 : &g[j];
-    const float a = *pa, b = *pb, sj = sign * s[j];
-    *pa = a * c[j] - b * sj;
-    *pb = b * c[j] + a * sj;
+    const float x = *pa, y = *pb, sj = sign * s[j];
+    const bool turns = !INTER || (j < N / 2 ? at.low : at.high) + j < a.half;
+    *pa = turns ? x * c[j] - y * sj : x;
+    *pb = turns ? y * c[j] + x * sj : y;
   }
 }
 
@@ -322,7 +327,7 @@ __global__ __launch_bounds__(256) void norm_rotary_fwd_kernel(RotaryArgs a) {
             g[j] *= r * (side ? w.g[1][j] : w.g[0][j]);
           }
         }
-        rotate<N, INTER>(f, g, c, s, 1.f);
+        rotate<N, INTER>(a, at, f, g, c, s, 1.f);
         if (row < rows && at.has) {
           T* y = static_cast<T*>(a.out[side]) +
                  (token * a.heads[side] + row - (side ? a.heads[0] : 0)) * a.D;
@@ -397,7 +402,7 @@ __global__ __launch_bounds__(256) void norm_rotary_bwd_kernel(RotaryArgs a) {
           C::unpack(x2[p], g);
           C::unpack(d1[p], df);
           C::unpack(d2[p], dg);
-          rotate<N, INTER>(df, dg, c, s, -1.f);
+          rotate<N, INTER>(a, at, df, dg, c, s, -1.f);
           if (a.norm) {
             float ss = 0.f;
 #pragma unroll
