@@ -294,3 +294,40 @@ def test_infinite_values_in_columns_that_are_not_rotated(D, half, dtype, interle
             top = np.where(fin, np.abs(dx), 0.0)
             lim = step * top + (ops * F32 + turn) * 2 * top.max(-1, keepdims=True)
             assert (np.abs(f64(grads[0]) - dx)[fin] <= lim[fin]).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("D", [64, 20])
+@pytest.mark.parametrize("exponent", [-60, -63, -64, -66, -68])
+def test_rows_whose_mean_square_is_below_the_normal_numbers(exponent, D, dtype):
+    """eps = 0 and values whose squares are subnormal: the root is finite, and
+    the row's norm is that of the same row at an ordinary size."""
+    rng = np.random.default_rng(20)
+    # Multiples of 2^exponent up to 15: their squares, multiples of 2^-136 at
+    # least, and the sum of 64 of them are exact in 32 bits.
+    whole = rng.integers(1, 16, size=(5, 3, D)) * rng.choice([-1, 1], size=(5, 3, D))
+    q = torch.tensor(whole * 2.0 ** exponent, device=DEV).to(TYPES[dtype]).requires_grad_(True)
+    assert np.array_equal(f64(q), whole * 2.0 ** exponent)
+    pos = torch.arange(5, device=DEV)
+    freqs = torch.tensor(100.0 ** (-np.arange(D // 2) / (D // 2)), device=DEV).float()
+    w = torch.tensor(1 + 0.2 * rng.standard_normal(D), device=DEV).to(TYPES[dtype])
+    out = tg.nn.norm_rotary(q, None, pos, freqs, query_weight=w, eps=0.0)
+    angle = want.angles(pos.cpu().numpy()[:, None], freqs.cpu().numpy(), (D // 2,))
+    exp = want.norm_rotary(whole.astype(np.float64), f64(w), angle, 0.0, True, False)
+    step = torch.finfo(TYPES[dtype]).eps / 2
+    # The mean's product with 1 / D rounds in units of 2^-149; half of one against
+    # a mean of 2^-136 or more.  The rest as in `check`.
+    mean = (whole.astype(np.float64) ** 2).mean() * 4.0 ** exponent
+    mean_off = 2.0 ** -150 / min(mean, 4.0 ** exponent)
+    off = (24 + D / 16) * F32 + mean_off
+    assert (np.abs(f64(out) - exp) <= step * np.abs(exp) +
+            2 * off * np.abs(exp).max(-1, keepdims=True)).all()
+    # dx = r (h - n mean(h n)), with r = 2^-exponent times the ordinary row's.
+    d = torch.tensor(rng.standard_normal((5, 3, D)), device=DEV).to(TYPES[dtype])
+    (dx,) = torch.autograd.grad(out, (q,), d)
+    edx, _ = want.norm_rotary_grad(whole.astype(np.float64), f64(w), angle, 0.0, True, False,
+                                   f64(d))
+    got = f64(dx) * 2.0 ** exponent
+    size = np.abs(f64(d)).max() * 2 * np.abs(f64(w)).max() * \
+        (1 + 15.0 ** 2) / np.sqrt((whole.astype(np.float64) ** 2).mean(-1)).min()
+    assert (np.abs(got - edx) <= step * np.abs(edx) + 2 * off * size).all()

@@ -215,12 +215,17 @@ __device__ __forceinline__ void read_turns(const float* cs, const Place<N, INTER
   }
 }
 
-// 1 / sqrt(v): the hardware's value and one Newton step.
+// 1 / sqrt(v): the hardware's value and one Newton step.  The hardware takes
+// subnormal numbers for 0 (eps = 0 and rows of values below 2^-63), so those
+// are multiplied by an even power of two first.
 __device__ __forceinline__ float inverse_root(float v) {
-  const float r = __builtin_amdgcn_rsqf(v);
-  // (v = 0 or Inf: r is Inf or 0, and stays.)
-  const float e = fmaf(-v * r, r, 1.f);
-  return v > 0.f && v < __builtin_huge_valf() ? fmaf(0.5f * r, e, r) : r;
+  const bool small = v < 0x1p-126f;
+  const float u = small ? v * 0x1p64f : v;
+  const float r = __builtin_amdgcn_rsqf(u);
+  // (u = 0 or Inf: r is Inf or 0, and stays.)
+  const float e = fmaf(-u * r, r, 1.f);
+  const float root = u > 0.f && u < __builtin_huge_valf() ? fmaf(0.5f * r, e, r) : r;
+  return small ? root * 0x1p32f : root;
 }
 
 // Turns pair j of the chunks (f, g) by (c, s): the halves of the pairs lie in
