@@ -704,3 +704,58 @@ def test_c_entries_refuse_what_does_not_fit():
     p.queries = 0
     with pytest.raises(RuntimeError, match="negative or zero"):
         _native.call("tgx_paged_attn", *args())
+
+
+def test_gradients_tell_what_ran():
+    """Under `strict` a width without CSR kernels is refused when gradients are
+    wanted; the record names the CSR kernels, or Torch, where they ran."""
+    rng = np.random.default_rng(24)
+    table, lengths, pages = relation(rng, [20, 70], 16)
+    g = tg.Graph.paged(torch.tensor(table, device=DEV), torch.tensor(lengths, device=DEV),
+                       page_size=16, num_pages=pages)
+    for D in (64, 24):
+        q = torch.randn(2, 2, 3, D, device=DEV).half()
+        k, v = torch.randn(2, pages * 16, 2, 1, D, device=DEV).half()
+        kernel = Attention()
+        call = lambda q: kernel(graph=g, src={"key": k, "value": v}, dst={"query": q}, scale=0.2)
+        plain = call(q)
+        assert kernel.last_variant.entry_points == ("tgx_paged_attn",)
+        leaf = q.clone().requires_grad_(True)
+        if D == 24:
+            with pytest.raises(RuntimeError, match="strict"):
+                call(leaf)
+            tg.config.strict = False
+            out = call(leaf)
+            assert kernel.last_variant.backend == "torch-eager"
+            assert not kernel.last_variant.entry_points
+            with pytest.raises(NotImplementedError, match="prepared"):
+                kernel.prepare(graph=g, src={"key": k, "value": v}, dst={"query": leaf}, scale=0.2)
+            tg.config.strict = True
+        else:
+            out = call(leaf)
+            assert kernel.last_variant.entry_points == ("tgx_dot_attn_fwd", "tgx_dot_attn_bwd")
+            run = kernel.prepare(graph=g, src={"key": k, "value": v}, dst={"query": leaf},
+                                 scale=0.2)
+            assert run.variant.pattern == "dot-product"
+            assert torch.equal(run(), out) and run().requires_grad
+        assert out.requires_grad
+        # (A step of 16 bits between two ways of rounding the same sums.)
+        assert (out - plain).abs().max() <= 2.0 ** -9 * plain.abs().max()
+        with torch.no_grad():
+            assert torch.equal(call(leaf), plain)
+        assert kernel.last_variant.entry_points == ("tgx_paged_attn",)
+        assert torch.equal(call(q), plain)
+
+
+def test_gradients_where_nobody_sees_a_key():
+    """Zeros, without an error under `strict`: how many keys there are is data."""
+    lengths = torch.zeros(2, dtype=torch.int32, device=DEV)
+    g = tg.Graph.paged(torch.zeros(2, 3, dtype=torch.int32, device=DEV), lengths, page_size=16,
+                       num_pages=1)
+    leaves = [torch.randn(n, 2, m, 64, device=DEV).half().requires_grad_(True)
+              for n, m in ((2, 3), (16, 1), (16, 1))]
+    out = Attention()(graph=g, src={"key": leaves[1], "value": leaves[2]},
+                      dst={"query": leaves[0]}, scale=0.2)
+    assert out.shape == leaves[0].shape and not out.any()
+    for grad in torch.autograd.grad(out.sum(), leaves):
+        assert not grad.any()

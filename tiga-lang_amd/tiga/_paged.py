@@ -53,6 +53,16 @@ def heads_of(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor):
     return (1, q.shape[1]) if k.shape[1] == 1 else None
 
 
+def wants_derivative(*tensors) -> bool:
+    """Whether a result of these tensors has to carry gradients."""
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+
+
+def csr_takes(D: int) -> bool:
+    """Whether the CSR attention kernels take heads of this width."""
+    return D % 8 == 0 and 8 <= D <= 512 and (D // 8) & (D // 8 - 1) == 0
+
+
 def bind_attention(graph, q, k, v, scale: float, heads: int, group: int):
     """The attention launch with its native arguments bound: a zero-argument
     callable that returns a new output."""

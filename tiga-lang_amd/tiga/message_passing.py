@@ -204,6 +204,8 @@ class _Launch:
     # Optional: operands -> a zero-argument launch with its native arguments
     # bound (prepare()'s no-grad form), or None where that does not apply.
     bind: Callable | None = None
+    # Optional: whether these operands still take what `describe` tells.
+    holds: Callable | None = None
 
     @property
     def guardable(self) -> bool:
@@ -250,6 +252,8 @@ class _Guarded:
         if self._names(src, dst, edge) != self.names or \
                 _param_signature(params) != self.param_sig or \
                 not self.environment.holds(kernel):
+            return _MISS
+        if launch.holds is not None and not launch.holds(*operands):
             return _MISS
         return launch.runner(*operands)
 
@@ -350,15 +354,8 @@ class MessagePassing(Kernel):
                     "block_prune_threshold requires the dense attention tile (dot-product "
                     "score, bf16/fp16, head_dim 32, 64 or 128, on the GPU); refusing to silently "
                     "execute exact softmax or materialize the Cartesian relation")
-            if config.strict:
-                raise RuntimeError(
-                    f"{type(self).__qualname__}: no HIP kernel covers this edge function / "
-                    "dtype / shape and tiga.config.strict is set")
-            self._record_variant(CompiledVariant(
-                key=(type(self).__qualname__, "eager", graph.planning_key()),
-                backend="torch-eager", provider="torch", pattern="generic",
-                lowering="gather -> edge() -> scatter reduce (Torch ops)",
-                remarks=("edge function not covered by a HIP kernel",)))
+            self._refuse_eager_if_strict()
+            self._record_variant(self._eager_variant(graph))
             return _eager.evaluate(self, graph, src, dst, edge, params)
         operands = launch.gather(src, dst, edge, params)
         result = launch.runner(*operands)
@@ -372,6 +369,19 @@ class MessagePassing(Kernel):
             guarded.names = _Guarded._names(src, dst, edge)
             self._guarded = guarded
         return result
+
+    def _refuse_eager_if_strict(self) -> None:
+        if config.strict:
+            raise RuntimeError(
+                f"{type(self).__qualname__}: no HIP kernel covers this edge function / "
+                "dtype / shape and tiga.config.strict is set")
+
+    def _eager_variant(self, graph) -> CompiledVariant:
+        return CompiledVariant(
+            key=(type(self).__qualname__, "eager", graph.planning_key()),
+            backend="torch-eager", provider="torch", pattern="generic",
+            lowering="gather -> edge() -> scatter reduce (Torch ops)",
+            remarks=("edge function not covered by a HIP kernel",))
 
     def _sparse_mm_sum(self, captured, graph, src, edge) -> torch.Tensor | None:
         """tg.sum() of edge.w * src.x on host tensors as the reference runs it
@@ -434,7 +444,7 @@ class MessagePassing(Kernel):
         edge = {} if edge is None else edge
         self(graph=graph, src=src, dst=dst, edge=edge, **params)
         launch = self._launch
-        if launch is None or launch.graph is not graph:
+        if launch is None or launch.graph is not graph or launch.variant.backend != "hip":
             raise NotImplementedError(
                 "prepared MessagePassing needs an edge function, dtype and shape that a HIP "
                 f"kernel covers; this call ran {self.last_variant.backend} "
@@ -884,7 +894,7 @@ class MessagePassing(Kernel):
         scale = dot.scale
 
         def run(q, k, v):
-            if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
+            if _paged.wants_derivative(q, k, v):
                 return self._paged_with_gradients(dot, graph, q, k, v, params)
             return _paged.bind_attention(graph, q, k, v, scale, heads, group)()
 
@@ -894,28 +904,43 @@ class MessagePassing(Kernel):
             return _paged.bind_attention(graph, q, k, v, scale, heads, group)
 
         kind = str(q.dtype).split(".")[-1]
-        describe = lambda: self._variant(
-            graph, "paged-attention", ("tgx_paged_attn",),
-            f"{kind} rows of the cache read once through the page tables, {group} query heads on "
-            f"each of {heads} key heads, fp32 online softmax; long sequences in pieces, joined "
-            "in order; gradients on the relation's snapshot")
+        derivative = _paged.wants_derivative(q, k, v)
+
+        def describe():
+            if not derivative:
+                return self._variant(
+                    graph, "paged-attention", ("tgx_paged_attn",),
+                    f"{kind} rows of the cache read once through the page tables, {group} query "
+                    f"heads on each of {heads} key heads, fp32 online softmax; long sequences in "
+                    "pieces, joined in order; gradients on the relation's snapshot")
+            if not _paged.csr_takes(D):
+                return self._eager_variant(graph)
+            return self._variant(
+                graph, "dot-product", ("tgx_dot_attn_fwd", "tgx_dot_attn_bwd"),
+                f"{kind} attention with gradients on the paged relation's snapshot: its CSR "
+                f"gathered in fp32 online softmax, {group} query heads on each of {heads} key "
+                "heads, which are repeated and their gradients added")
+
         operands = (("dst", dot.q_field), ("src", dot.k_field), ("src", dot.v_field))
-        return _Launch(graph, operands, run, describe, bind=bind)
+        return _Launch(graph, operands, run, describe, bind=bind,
+                       holds=lambda *t: _paged.wants_derivative(*t) == derivative)
 
     def _paged_with_gradients(self, dot, graph, q, k, v, params):
         """Paged attention whose fields need gradients: over the relation's
         snapshot, shared key heads repeated for the heads on them (their
         gradients add up again) where the CSR attention kernels take the
         width, else on Torch operations in fp32."""
-        from . import _ops
+        from . import _ops, _paged
 
         snapshot = graph.snapshot()
         D = q.shape[-1]
-        if D % 8 == 0 and D <= 512 and (D // 8) & (D // 8 - 1) == 0 and snapshot.num_edges:
+        if _paged.csr_takes(D) and snapshot.num_edges:
             each = lambda t: t.expand(t.shape[0], *q.shape[1:]).reshape(t.shape[0], -1, D)
             out = _ops.DotAttnFunction.apply(q.reshape(q.shape[0], -1, D), each(k), each(v), None,
                                              dot.scale, snapshot)
             return out.reshape(q.shape)
+        if not _paged.csr_takes(D):
+            self._refuse_eager_if_strict()
         fields = {dot.k_field: k.float(), dot.v_field: v.float()}
         out = _eager.evaluate(self, snapshot, fields, {dot.q_field: q.float()}, {}, params)
         return out.to(q.dtype)
