@@ -759,3 +759,58 @@ def test_gradients_where_nobody_sees_a_key():
     assert out.shape == leaves[0].shape and not out.any()
     for grad in torch.autograd.grad(out.sum(), leaves):
         assert not grad.any()
+
+
+def dual(t):
+    return torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+
+
+@pytest.mark.parametrize("D", [64, 24])
+def test_forward_mode_never_loses_a_tangent(D):
+    """Refused like the other attention kernels where a kernel would run; carried
+    by Torch operations where they do, which `strict` refuses."""
+    unpack = torch.autograd.forward_ad.unpack_dual
+    rng = np.random.default_rng(23)
+    table, lengths, pages = relation(rng, [0, 20, 70], 16)
+    g = tg.Graph.paged(torch.tensor(table, device=DEV), torch.tensor(lengths, device=DEV),
+                       page_size=16, num_pages=pages, queries=2)
+    mk = lambda *s: torch.tensor(rng.standard_normal(s), device=DEV).float()
+    args = [mk(6, 2, 3, D), mk(pages * 16, 2, 1, D), mk(pages * 16, 2, 1, D)]
+    kernel = Attention()
+    call = lambda q, k, v: kernel(graph=g, src={"key": k, "value": v}, dst={"query": q},
+                                  scale=0.2)
+    call(*args)     # (a warm launch is no way around)
+    for i in range(3):
+        with torch.autograd.forward_ad.dual_level():
+            duals = [dual(t) if j == i else t for j, t in enumerate(args)]
+            with pytest.raises(NotImplementedError if D == 64 else RuntimeError):
+                call(*duals)
+            if D == 24:
+                tg.config.strict = False
+                got = unpack(call(*duals)).tangent
+                assert got is not None and kernel.last_variant.backend == "torch-eager"
+        if D == 24:
+            up, down = ([t + h if j == i else t for j, t in enumerate(x.double().cpu()
+                         for x in args)] for h in (1e-5, -1e-5))
+            host = tg.Graph.paged(torch.tensor(table), torch.tensor(lengths), page_size=16,
+                                  num_pages=pages, queries=2)
+            f = lambda q, k, v: Attention()(graph=host, src={"key": k, "value": v},
+                                            dst={"query": q}, scale=0.2)
+            exp = (f(*up) - f(*down)) / 2e-5
+            # (As in the gradients' test: 1e-5 of the largest value in 32 bits.)
+            assert (got.double().cpu() - exp).abs().max() <= 1e-5 * max(1.0, exp.abs().max())
+            tg.config.strict = True
+
+
+def test_append_refuses_forward_mode():
+    """The caches would lose the tangent."""
+    g = tg.Graph.paged(torch.arange(4, dtype=torch.int32, device=DEV)[None],
+                       torch.tensor([9], dtype=torch.int32, device=DEV), page_size=16, num_pages=4)
+    args = [torch.zeros(n, 2, 8, device=DEV) for n in (64, 1, 64, 1)]
+    sums = torch.zeros(4, 2, 8, device=DEV)
+    for i in range(4):
+        with torch.autograd.forward_ad.dual_level():
+            duals = [dual(t) if j == i else t for j, t in enumerate(args)]
+            with pytest.raises(NotImplementedError, match="detach"):
+                g.append(*duals, page_sums=sums)
+    g.append(*args, page_sums=sums)

@@ -331,3 +331,20 @@ def test_rows_whose_mean_square_is_below_the_normal_numbers(exponent, D, dtype):
     size = np.abs(f64(d)).max() * 2 * np.abs(f64(w)).max() * \
         (1 + 15.0 ** 2) / np.sqrt((whole.astype(np.float64) ** 2).mean(-1)).min()
     assert (np.abs(got - edx) <= step * np.abs(edx) + 2 * off * size).all()
+
+
+def test_forward_mode_is_refused_on_the_kernels():
+    """A launch would drop the tangent without a word."""
+    q, k, w, pos, freqs, _ = make(3, 2, 2, 32, (16,), torch.float32)
+    args = [t.detach() for t in (q, k, *w, freqs)]
+    call = lambda q, k, wq, wk, f: tg.nn.norm_rotary(q, k, pos, f, query_weight=wq, key_weight=wk)
+    for i in range(5):
+        with torch.autograd.forward_ad.dual_level():
+            dual = [torch.autograd.forward_ad.make_dual(t, torch.ones_like(t)) if j == i else t
+                    for j, t in enumerate(args)]
+            with pytest.raises(NotImplementedError, match="forward"):
+                call(*dual)
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward"):
+                call(*dual)
+            call(*args)     # (a level alone changes nothing)
+    call(*args)

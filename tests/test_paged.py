@@ -227,3 +227,21 @@ def test_select_pages_refusals():
         g.select_pages(q, sums, 2, out=g)
     with pytest.raises(ValueError, match="not one per head"):
         chosen.select_pages(q, sums, 2)
+
+
+def test_forward_mode_over_host_tensors():
+    """Attention and norm_rotary of host tensors carry tangents."""
+    make_dual, unpack = torch.autograd.forward_ad.make_dual, torch.autograd.forward_ad.unpack_dual
+    rng = np.random.default_rng(31)
+    g = graph()
+    mk = lambda *s: torch.tensor(rng.standard_normal(s))
+    q, k, v, dq = mk(4, 2, 8), mk(PAGES * SIZE, 2, 8), mk(PAGES * SIZE, 2, 8), mk(4, 2, 8)
+    attend = lambda q: Attention()(graph=g, src={"key": k, "value": v}, dst={"query": q},
+                                   scale=0.5)
+    rotate = lambda q: tg.nn.norm_rotary(q, None, torch.arange(4), torch.ones(4))
+    for f in (attend, rotate):
+        with torch.autograd.forward_ad.dual_level():
+            got = unpack(f(make_dual(q, dq))).tangent
+        assert got is not None
+        # Central differences in 64 bits: h^2 times third derivatives of order 10.
+        assert ((f(q + 1e-5 * dq) - f(q - 1e-5 * dq)) / 2e-5 - got).abs().max() <= 1e-8

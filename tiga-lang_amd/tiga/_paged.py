@@ -14,6 +14,7 @@ import ctypes
 import torch
 
 from . import _native
+from ._dual import carries_tangent
 
 # Element types of the paged kernels (TGX_DTYPE_*).
 DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -54,8 +55,9 @@ def heads_of(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor):
 
 
 def wants_derivative(*tensors) -> bool:
-    """Whether a result of these tensors has to carry gradients."""
-    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+    """Whether a result of these tensors has to carry gradients or a tangent."""
+    return carries_tangent(*tensors) or (
+        torch.is_grad_enabled() and any(t.requires_grad for t in tensors))
 
 
 def csr_takes(D: int) -> bool:
@@ -92,6 +94,8 @@ def bind_attention(graph, q, k, v, scale: float, heads: int, group: int):
                v.data_ptr() if v.numel() else None)
 
     def launch(keep=(q, k, v)):
+        if carries_tangent(*keep):
+            raise NotImplementedError("paged attention has no forward-mode derivative")
         out = torch.empty(shape, dtype=dtype, device=device)
         work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
         _native.launch(out, "tgx_paged_attn", state.native(), *tensors, strides, scale,
@@ -113,6 +117,8 @@ def append(graph, key_cache, key, value_cache, value, page_sums) -> None:
     if not key_cache.is_cuda or key_cache.dtype not in DTYPES:
         _append_torch(state, key_cache, key, value_cache, value, page_sums)
         return
+    if carries_tangent(key_cache, key, value_cache, value, page_sums):
+        raise NotImplementedError("append has no forward-mode derivative: detach its operands")
     rows, heads, D = key.shape
     if D > 1:
         key = key if key.stride(2) == 1 else key.contiguous()

@@ -10,6 +10,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native
+from ._dual import carries_tangent
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
@@ -156,6 +157,8 @@ class NormRotaryFunction(torch.autograd.Function):
 def apply(plan: Plan, query, key, query_weight, key_weight, positions, frequencies):
     if not plan.covered:
         return reference(plan.form, query, key, query_weight, key_weight, positions, frequencies)
+    if carries_tangent(query, key, query_weight, key_weight, frequencies):
+        raise NotImplementedError("norm_rotary has no forward-mode derivative on the HIP kernels")
     if torch.is_grad_enabled() and (
             query.requires_grad or (key is not None and key.requires_grad) or
             (query_weight is not None and query_weight.requires_grad) or
