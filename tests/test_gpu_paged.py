@@ -814,3 +814,24 @@ def test_append_refuses_forward_mode():
             with pytest.raises(NotImplementedError, match="detach"):
                 g.append(*duals, page_sums=sums)
     g.append(*args, page_sums=sums)
+
+
+def test_strict_refuses_torch_operations_on_the_gpu():
+    g = tg.Graph.paged(torch.arange(4, dtype=torch.int32, device=DEV)[None],
+                       torch.tensor([40], dtype=torch.int32, device=DEV), page_size=16,
+                       num_pages=4)
+    mk = lambda n: torch.randn(n, 2, 8, device=DEV, dtype=torch.float64)
+    kc, k, vc, v, sums = mk(64), mk(1), mk(64), mk(1), torch.randn(4, 2, 8, device=DEV)
+    before = kc.clone()
+    with pytest.raises(RuntimeError, match="strict"):
+        g.append(kc, k, vc, v)
+    assert torch.equal(kc, before)
+    with pytest.raises(RuntimeError, match="strict"):
+        g.select_pages(k, sums, 2)
+    tg.config.strict = False
+    g.append(kc, k, vc, v)
+    assert torch.equal(kc[39], k[0]) and torch.equal(vc[39], v[0])
+    chosen = g.select_pages(k, sums, 2)
+    exp, held = want.select(np.arange(4)[None], [40], 16, 4, 1, f64(k)[:, :, None], f64(sums), 2)
+    assert np.array_equal(chosen.page_table.cpu().numpy(), exp)
+    assert np.array_equal(chosen.lengths.cpu().numpy(), held)

@@ -112,9 +112,23 @@ def bind_attention(graph, q, k, v, scale: float, heads: int, group: int):
 # ---------------------------------------------------------------------------
 # append
 
+def _on_torch_operations(name: str, t: torch.Tensor) -> bool:
+    """Whether operands of t's device and type run on Torch operations, which
+    strict mode refuses on the GPU."""
+    if not t.is_cuda:
+        return True
+    if t.dtype in DTYPES:
+        return False
+    from .message_passing import config
+
+    if config.strict:
+        raise RuntimeError(f"{name}: no HIP kernel covers {t.dtype} and tiga.config.strict is set")
+    return True
+
+
 def append(graph, key_cache, key, value_cache, value, page_sums) -> None:
     state = graph.paged_state
-    if not key_cache.is_cuda or key_cache.dtype not in DTYPES:
+    if _on_torch_operations("append", key_cache):
         _append_torch(state, key_cache, key, value_cache, value, page_sums)
         return
     if carries_tangent(key_cache, key, value_cache, value, page_sums):
@@ -168,7 +182,7 @@ def select(graph, query, page_sums, count: int, table, lengths) -> None:
     [rows, heads, count] and the positions they hold to `lengths` [rows]."""
     state = graph.paged_state
     query, page_sums = query.detach(), page_sums.detach()
-    if not query.is_cuda or query.dtype not in DTYPES:
+    if _on_torch_operations("select_pages", query):
         _select_torch(state, query, page_sums, count, table, lengths)
         return
     if query.shape[-1] > 1 and query.stride(-1) != 1:
