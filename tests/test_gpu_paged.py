@@ -835,3 +835,50 @@ def test_strict_refuses_torch_operations_on_the_gpu():
     exp, held = want.select(np.arange(4)[None], [40], 16, 4, 1, f64(k)[:, :, None], f64(sums), 2)
     assert np.array_equal(chosen.page_table.cpu().numpy(), exp)
     assert np.array_equal(chosen.lengths.cpu().numpy(), held)
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("queries", [1, 5, 12, 30])
+@pytest.mark.parametrize("gap", [17.0, 18.0, 20.0])
+def test_small_weights_of_many_keys_add_up(gap, queries, D):
+    """One key far above the rest whose value is 0: the output is the rest's
+    weights, each of them below half a step of fp16 relative to the largest."""
+    n = 200
+    g = tg.Graph.paged(torch.arange(13, dtype=torch.int32, device=DEV)[None],
+                       torch.tensor([n], dtype=torch.int32, device=DEV), page_size=16,
+                       num_pages=13, queries=queries)
+    for dtype in (torch.float16, torch.bfloat16):
+        q = torch.zeros(queries, 1, 4, D, device=DEV, dtype=dtype)
+        k, v = torch.zeros(2, 208, 1, 1, D, device=DEV, dtype=dtype)
+        q[..., 0] = 1.0
+        k[0, ..., 0] = gap
+        v[1:] = 32768.0
+        out = f64(Attention()(graph=g, src={"key": k, "value": v}, dst={"query": q}, scale=1.0))
+        seen = (n - np.arange(queries - 1, -1, -1))[:, None, None, None] - 1
+        exp = 32768.0 * seen * np.exp(-gap) / (1 + seen * np.exp(-gap))
+        # Half a step of the output and as much for the weights: e^-20 = 2^-28.9 in parts
+        # that are off by 2^-39 at most, 2^-10.1 of it; a step where it is smallest.
+        step = 2.0 ** (-10 if dtype == torch.float16 else -8)
+        assert (np.abs(out - exp) <= 1.5 * step * exp).all(), (out / exp).min()
+
+
+def test_small_weights_of_a_long_sequence_add_up():
+    """131072 keys, one of them far above the rest, for sequences enough that
+    each is one piece."""
+    n, B = 131072, 600
+    table = torch.arange(n // 64, dtype=torch.int32, device=DEV).expand(B, -1)
+    g = tg.Graph.paged(table, torch.full((B,), n, dtype=torch.int32, device=DEV), page_size=64,
+                       num_pages=n // 64)
+    q = torch.zeros(B, 1, 1, 32, device=DEV, dtype=torch.float16)
+    k, v = torch.zeros(2, n, 1, 1, 32, device=DEV, dtype=torch.float16)
+    q[..., 0] = 1.0
+    v.fill_(1.0)
+    for gap in (17.40625, 18.0):
+        for first in (1.0, 0.0, -1.0):
+            k[0, ..., 0], v[0] = gap, first
+            out = f64(Attention()(graph=g, src={"key": k, "value": v}, dst={"query": q},
+                                  scale=1.0))
+            rest = (n - 1) * np.exp(-gap)
+            exp = (first + rest) / (1 + rest)
+            # A step of the output, and of each weight 2^-11.
+            assert np.abs(out - exp).max() <= 2.0 ** -10 * abs(exp) + 2.0 ** -11 * rest

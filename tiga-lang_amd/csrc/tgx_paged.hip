@@ -280,12 +280,14 @@ struct Frag<__bf16> {
   typedef bf16x8 v8;
   typedef __bf16 v4 __attribute__((ext_vector_type(4)));
   static constexpr uint32_t kExponent = 0x7F80u;
+  static constexpr float kRescaleLog2 = 8.f, kLiftLog2 = 0.f;
 };
 template <>
 struct Frag<_Float16> {
   typedef f16x8 v8;
   typedef _Float16 v4 __attribute__((ext_vector_type(4)));
   static constexpr uint32_t kExponent = 0x7C00u;
+  static constexpr float kRescaleLog2 = 1.f, kLiftLog2 = 14.f;
 };
 template <typename T>
 using vec8 = typename Frag<T>::v8;
@@ -313,8 +315,13 @@ __device__ __forceinline__ float group4_sum(float x) {
 template <int D>
 constexpr int kRow = D == 128 ? 144 : D == 64 ? 80 : 48;
 
-// The running maximum only moves when a step's exceeds it by this (log2 units).
-constexpr float kRescaleLog2 = 8.f;
+// The running maximum m only moves when a step's exceeds it by kRescaleLog2
+// (log2 units), and a weight is 2^(s - m + kLiftLog2): a factor that the sum of
+// the weights carries too.  fp16 has no numbers below 2^-24, so there the
+// weights fill the range up to 2^15: their two parts are off by 2^-39 of the
+// largest at most, a weight of e^-20 by 2^-10 of itself.  (Unlifted, those
+// below 2^-25 = e^-17.3 are lost from the output and kept in the sum.)  It
+// costs nothing: 24 sequences of up to 3000 tokens x 4, 16 heads of 64, 35.5 us.
 
 // The lane's part of 16 queries: row `row` of the (sequence, head), its
 // fragments, and the positions it sees (rows past the last see as the last).
@@ -336,10 +343,10 @@ struct Query {
   }
 };
 
-// Scores of 16 KT keys from position `pos` become weights 2^(s - m) under the
-// running maximum m; l and o follow it.  `gone`: bit k set, key k is not
+// Scores of 16 KT keys from position `pos` become weights 2^(s - m + lift) under
+// the running maximum m; l and o follow it.  `gone`: bit k set, key k is not
 // there; `masked`: some key may be hidden from the lane's query.
-template <int KT, int DT>
+template <typename T, int KT, int DT>
 __device__ __forceinline__ void weigh(f32x4 (&c)[KT], float scale, bool masked,
                                       unsigned long long gone, int pos, int limit, int g,
                                       float& m, float& l, f32x4 (&o)[DT]) {
@@ -359,7 +366,8 @@ __device__ __forceinline__ void weigh(f32x4 (&c)[KT], float scale, bool masked,
 #pragma unroll
     for (int i = 0; i < 4; ++i) top = fmaxf(top, c[kt][i]);
   top = group4_max(top);
-  if (__any(top > m + kRescaleLog2)) {
+  // (The difference, not the sum: m + 1 may round away from where m is large.)
+  if (__any(top - m > Frag<T>::kRescaleLog2)) {
     const float mn = fmaxf(m, top);
     const float alpha = m == kNegInf ? 0.f : exp2_hw(m - mn);
     m = mn;
@@ -367,7 +375,7 @@ __device__ __forceinline__ void weigh(f32x4 (&c)[KT], float scale, bool masked,
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
   }
-  const float mo = m == kNegInf ? 0.f : m;
+  const float mo = (m == kNegInf ? 0.f : m) - Frag<T>::kLiftLog2;
 #pragma unroll
   for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -615,7 +623,7 @@ __global__ __launch_bounds__(256, (D == 128 ? 2 : D == 64 ? 3 : 4)) void paged_t
       load(kf, kb, a.ks_slot, next);
 
       const bool tail = step * KEYS + KEYS > low;   // some query sees only a part
-      weigh(c[0], a.scale_log2, gone || tail, gone, step * KEYS, q.limit, g, m, l, o[0]);
+      weigh<T>(c[0], a.scale_log2, gone || tail, gone, step * KEYS, q.limit, g, m, l, o[0]);
 
       // Stage V; a key that is not there counts as a row of zeros.
       if (gone) {
@@ -779,7 +787,7 @@ __global__ __launch_bounds__(256, (D == 128 || QT == 2 ? 2 : 3)) void paged_bloc
       }
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt)
-      weigh(c[qt], a.scale_log2, gone || pos + 16 * KT > low, gone >> key0, pos, q[qt].limit, g,
+      weigh<T>(c[qt], a.scale_log2, gone || pos + 16 * KT > low, gone >> key0, pos, q[qt].limit, g,
             m[qt], l[qt], o[qt]);
     if (!look || !sh_odd[tile & 1]) {
       add_values<T, D, KT, QT>(vs + key0 * ROW, c, g, lr, o);
