@@ -118,3 +118,47 @@ def norm_rotary_grad(x, w, angle, eps, norm, interleaved, dy):
     n = x * r
     h = g if w is None else g * w
     return r * (h - n * (h * n).mean(-1, keepdims=True)), (g * n).sum((0, 1))
+
+
+def attention_bound(table, lengths, size, num_pages, queries, q, k, v, scale, dtype, tiles):
+    """What rounding may do to each value of `attention` (shapes as there, one
+    table a sequence), by the row's own weights p:
+
+        step |out| + sum_j p_j |v_j| (parts + adds) + 2 sum_j p_j ds_j (|v_j| + |out|)
+
+    step: half a step of the output's type; parts: a weight as two 16-bit values
+    (`tiles`: the matrix kernels; fp16's may be off by 2^-39 of the largest as
+    well), or in fp32; adds: two fp32 roundings for each addition one after the other
+    (a key at a time on a quarter of the row at least, 32 keys at a time in a
+    tile), and 64 for waves, pieces and exponentials; ds_j: the fp32 score's D
+    products and its scaling."""
+    f32 = 2.0 ** -24
+    step = {"f32": 2.0 ** -24, "bf16": 2.0 ** -8, "f16": 2.0 ** -11}[dtype]
+    parts = 2 * step ** 2 if tiles else f32
+    table = np.asarray(table)
+    heads, group, D = q.shape[1:]
+    lim = np.zeros(q.shape)
+    for b in range(table.shape[0]):
+        for t in range(queries):
+            row = b * queries + t
+            n = max(length_of(lengths, b, table.shape[1], size) - (queries - 1 - t), 0)
+            at, named = slots(table[b], n, size, num_pages)
+            at = at[named]
+            if at.size == 0:
+                continue
+            adds = 2 * f32 * (n / (32 if tiles else 4) + 64)
+            for h in range(heads):
+                kk, vv = k[at, h], np.abs(v[at, h])
+                s = scale * (q[row, h] @ kk.T)
+                p = np.exp(s - s.max(-1, keepdims=True))
+                p /= p.sum(-1, keepdims=True)
+                out = np.abs(p @ v[at, h])
+                ds = f32 * ((D + 8) * abs(scale) * (np.abs(q[row, h]) @ np.abs(kk).T) +
+                            4 * np.abs(s))
+                lim[row, h] = step * out + (parts + adds) * (p @ vv) + \
+                    2 * ((p * ds) @ vv + (p * ds).sum(-1, keepdims=True) * out)
+                if tiles and dtype == "f16":
+                    lim[row, h] += 2.0 ** -39 * vv.sum(0)
+    # (Outputs below the type's normal numbers round in absolute steps.)
+    tiny = {"f32": 2.0 ** -149, "bf16": 2.0 ** -133, "f16": 2.0 ** -24}[dtype]
+    return lim + tiny

@@ -882,3 +882,45 @@ def test_small_weights_of_a_long_sequence_add_up():
             exp = (first + rest) / (1 + rest)
             # A step of the output, and of each weight 2^-11.
             assert np.abs(out - exp).max() <= 2.0 ** -10 * abs(exp) + 2.0 ** -11 * rest
+
+
+def tight(lengths, size, heads, group, D, dtype, queries=1, seed=21):
+    """An attention against the formula, by each row's own weights."""
+    print(f"tight {dtype} D={D} heads={heads} group={group} queries={queries} "
+          f"lengths={lengths[:6]}", flush=True)
+    rng = np.random.default_rng(seed)
+    table, length, pages = relation(rng, lengths, size)
+    g = tg.Graph.paged(torch.tensor(table, device=DEV), torch.tensor(length, device=DEV),
+                       page_size=size, num_pages=pages, queries=queries)
+    mk = lambda *s: torch.tensor(rng.standard_normal(s), device=DEV).to(TYPES[dtype])
+    q = mk(len(lengths) * queries, heads, group, D)
+    k, v = mk(pages * size, heads, D), mk(pages * size, heads, D)
+    out = Attention()(graph=g, src={"key": k[:, :, None], "value": v[:, :, None]},
+                      dst={"query": q}, scale=D ** -0.5)
+    args = (table, length, size, pages, queries, f64(q), f64(k), f64(v), D ** -0.5)
+    tiles = dtype != "f32" and D in (32, 64, 128)
+    err = np.abs(f64(out) - want.attention(*args))
+    lim = want.attention_bound(*args, dtype, tiles)
+    assert (err <= lim).all(), f"{(err / lim).max():.2f} of the bound"
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("queries,group", [(4, 4), (5, 4), (12, 5), (17, 4), (40, 4)])
+def test_accuracy_does_not_depend_on_how_many_ask(queries, group, dtype):
+    for D in (64, 128):
+        tight([700, 90, 33], 16, 2, group, D, dtype, queries=queries)
+
+
+@pytest.mark.parametrize("queries", [1, 6, 12, 30])
+def test_infinite_values_of_small_weights(queries):
+    """An Inf of a key whose weight is below fp16's numbers is an Inf."""
+    g = tg.Graph.paged(torch.arange(13, dtype=torch.int32, device=DEV)[None],
+                       torch.tensor([200], dtype=torch.int32, device=DEV), page_size=16,
+                       num_pages=13, queries=queries)
+    q = torch.zeros(queries, 1, 4, 64, device=DEV, dtype=torch.float16)
+    k, v = torch.zeros(2, 208, 1, 1, 64, device=DEV, dtype=torch.float16)
+    q[..., 0], k[0, ..., 0] = 1.0, 40.0
+    v[100, ..., 5], v[101, ..., 7] = float("inf"), float("-inf")
+    out = f64(Attention()(graph=g, src={"key": k, "value": v}, dst={"query": q}, scale=1.0))
+    assert np.isposinf(out[..., 5]).all() and np.isneginf(out[..., 7]).all()
+    assert np.isfinite(np.delete(out, (5, 7), axis=-1)).all()

@@ -259,10 +259,13 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedArgs a) {
 // one query for each 16 keys, which is P^T as the B operand of O^T = V^T P^T
 // under the key order {4g .. 4g + 3, 16 + 4g ..}; V^T is read down the columns
 // of a V tile staged in LDS (ds_read_b64_tr_b16).  A weight is multiplied as
-// the sum of two 16-bit values where the matrix unit has time to spare (up to
-// 64 queries: at D = 128, 24 instructions of 16 cycles for the 16 KB of 32
-// keys, which take some 700 cycles of a CU's share of memory), so that only
-// the output's rounding is left.
+// the sum of two 16-bit values, so that only the output's rounding is left.
+// Up to 64 queries the matrix unit has the time to spare (at D = 128, 24
+// instructions of 16 cycles for the 16 KB of 32 keys, which take some 700
+// cycles of a CU's share of memory).  Above it is the bound, and the second
+// part is kept all the same, so that a row's accuracy does not depend on how
+// many ask: 512 new tokens of four sequences of 3000 to 4000, 8 x 4 heads of
+// 128, bf16, take 283 us (400 TFLOP/s), 231 us with one part.
 //
 // Two kernels.  Up to 16 queries of one (sequence, head): paged_tile_kernel,
 // whose four waves run through every fourth step of KEYS keys by themselves
@@ -385,10 +388,7 @@ __device__ __forceinline__ void weigh(f32x4 (&c)[KT], float scale, bool masked,
     }
 }
 
-// o += V^T P^T over the 16 KT staged rows at `v`, for QT tiles of 16 queries.  Two
-// tiles a wave (more than 64 queries of a key head) are bound by the matrix
-// unit: their weights are multiplied in 16 bits, half a step off each, as the
-// dense tiles multiply theirs.
+// o += V^T P^T over the 16 KT staged rows at `v`, for QT tiles of 16 queries.
 template <typename T, int D, int KT, int QT>
 __device__ __forceinline__ void add_values(const T* v, const f32x4 (&c)[QT][KT], int g, int lr,
                                            f32x4 (&o)[QT][D / 16]) {
@@ -402,7 +402,7 @@ __device__ __forceinline__ void add_values(const T* v, const f32x4 (&c)[QT][KT],
       for (int j = 0; j < 8; ++j) {
         const float w = c[qt][2 * k2 + j / 4][j % 4];
         ph[qt][j] = static_cast<T>(w);
-        if constexpr (QT == 1) pl[qt][j] = static_cast<T>(w - static_cast<float>(ph[qt][j]));
+        pl[qt][j] = static_cast<T>(w - static_cast<float>(ph[qt][j]));
       }
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) {
@@ -414,7 +414,7 @@ __device__ __forceinline__ void add_values(const T* v, const f32x4 (&c)[QT][KT],
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) {
         o[qt][dt] = mfma(vt, ph[qt], o[qt][dt]);
-        if constexpr (QT == 1) o[qt][dt] = mfma(vt, pl[qt], o[qt][dt]);
+        o[qt][dt] = mfma(vt, pl[qt], o[qt][dt]);
       }
     }
   }
@@ -694,12 +694,13 @@ __global__ __launch_bounds__(256, (D == 128 || QT == 2 ? 2 : 3)) void paged_bloc
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt)
     q[qt] = Query<T, D>(a, p, th, kh, wrow + 16 * qt + lr, rows, g);
-  // The fewest and most positions any of the wave's queries sees, and of the workgroup's.
+  // The fewest and most positions any of the wave's queries sees, and the most of the
+  // workgroup's.
   auto sees = [&](int row) {
     return p.length - (r.queries - 1 - min(row, rows - 1) / a.group);
   };
   const int low = sees(wrow), wave_high = sees(wrow + 16 * QT - 1);
-  const int group_low = sees(row0), high = min(sees(row0 + QUERIES - 1), p.tile1 * kTile);
+  const int high = min(sees(row0 + QUERIES - 1), p.tile1 * kTile);
   const T* kb = static_cast<const T*>(a.k) + th * a.ks_table + kh * a.ks_head;
   const T* vb = static_cast<const T*>(a.v) + th * a.vs_table + kh * a.vs_head;
   const int32_t* table = r.table + p.seq * r.seq_stride + th * r.head_stride;
@@ -749,14 +750,12 @@ __global__ __launch_bounds__(256, (D == 128 || QT == 2 ? 2 : 3)) void paged_bloc
     next_id = page_id(p.tile0 + 1);
   }
   for (int tile = p.tile0; tile < last; ++tile) {
-    // (Weights in one part need the look for NaN and Inf only where some are hidden.)
-    const bool look = QT == 1 || (r.queries > 1 && tile * kTile + kTile > group_low);
     __syncthreads();   // the tile before has been read
     Largest<T> largest;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int at = threadIdx.x + 256 * i;
-      if (look) largest.see(vr[i]);
+      largest.see(vr[i]);
       *reinterpret_cast<vec8<T>*>(ks + at / CPR * ROW + at % CPR * 8) = kr[i];
       *reinterpret_cast<vec8<T>*>(vs + at / CPR * ROW + at % CPR * 8) = vr[i];
     }
@@ -789,7 +788,7 @@ __global__ __launch_bounds__(256, (D == 128 || QT == 2 ? 2 : 3)) void paged_bloc
     for (int qt = 0; qt < QT; ++qt)
       weigh<T>(c[qt], a.scale_log2, gone || pos + 16 * KT > low, gone >> key0, pos, q[qt].limit, g,
             m[qt], l[qt], o[qt]);
-    if (!look || !sh_odd[tile & 1]) {
+    if (!sh_odd[tile & 1]) {
       add_values<T, D, KT, QT>(vs + key0 * ROW, c, g, lr, o);
     } else {
 #pragma unroll
