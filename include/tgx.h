@@ -829,7 +829,8 @@ int tgx_paged_attn_workspace(const tgx_paged* p, int heads, int group, int D, in
  *   out [rows, heads, group, D] contiguous
  *   strides, host array of nine, in elements, multiples of 16 bytes: q's row,
  *     head, group; k's slot, table head, head; v's slot, table head, head
- * Other shapes: TGX_UNSUPPORTED. */
+ * Other shapes, and more sequences, heads and queries than one launch has workgroups
+ * for: TGX_UNSUPPORTED. */
 int tgx_paged_attn(const tgx_paged* p, const void* q_dev, const void* k_dev, const void* v_dev,
                    const int64_t* strides, float scale, void* out_dev, int heads, int group,
                    int D, int dtype, void* workspace_dev, size_t workspace_bytes, void* stream);

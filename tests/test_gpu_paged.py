@@ -924,3 +924,20 @@ def test_infinite_values_of_small_weights(queries):
     out = f64(Attention()(graph=g, src={"key": k, "value": v}, dst={"query": q}, scale=1.0))
     assert np.isposinf(out[..., 5]).all() and np.isneginf(out[..., 7]).all()
     assert np.isfinite(np.delete(out, (5, 7), axis=-1)).all()
+
+
+def test_more_queries_than_a_launch_has_workgroups():
+    """17 * 2^20 queries of one key head: tiles of 128 of them."""
+    queries, group = 1 << 20, 17
+    g = tg.Graph.paged(torch.arange(13, dtype=torch.int32, device=DEV)[None],
+                       torch.tensor([40], dtype=torch.int32, device=DEV), page_size=16,
+                       num_pages=13, queries=queries)
+    q = torch.randn(1, 1, group, 32, device=DEV).half().expand(queries, -1, -1, -1)
+    k, v = torch.randn(2, 208, 1, 1, 32, device=DEV).half()
+    kernel = Attention()
+    out = kernel(graph=g, src={"key": k, "value": v}, dst={"query": q}, scale=0.2)
+    assert kernel.last_variant.pattern == "paged-attention"
+    assert not out[:-40].any()
+    few = tg.Graph.paged(g.page_table, g.lengths, page_size=16, num_pages=13, queries=40)
+    same = Attention()(graph=few, src={"key": k, "value": v}, dst={"query": q[:40]}, scale=0.2)
+    assert torch.equal(out[-40:], same)

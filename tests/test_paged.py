@@ -1,11 +1,14 @@
 """Graph.paged, its append and select_pages, and attention over it, on host
 tensors against the formulas in float64; and what they refuse."""
 
+import ctypes
+
 import numpy as np
 import pytest
 import torch
 
 import tiga as tg
+from tiga import _native
 
 import paged_reference as want
 
@@ -245,3 +248,24 @@ def test_forward_mode_over_host_tensors():
         assert got is not None
         # Central differences in 64 bits: h^2 times third derivatives of order 10.
         assert ((f(q + 1e-5 * dq) - f(q - 1e-5 * dq)) / 2e-5 - got).abs().max() <= 1e-8
+
+
+def paged_attention_workspace(n_seqs, heads, group, queries, D, dtype, pages=64, size=16):
+    """Status of the native launch's size check."""
+    p = _native.Paged(1, pages, 0, 1, n_seqs, 1, pages, size, pages, queries)
+    need = ctypes.c_size_t()
+    status = _native.lib().tgx_paged_attn_workspace(ctypes.byref(p), heads, group, D, dtype,
+                                                    ctypes.byref(need))
+    return status, need.value
+
+
+def test_launches_that_need_no_workgroup_per_query_take_prompts():
+    """16 sequences of 32768 new tokens on matrix tiles of 128 queries; what a
+    workgroup a query cannot be launched for is told as uncovered."""
+    assert paged_attention_workspace(16, 8, 4, 32768, 128, 0, pages=4096) == (0, 0)
+    # A join of more queries than a launch has workgroups is left out.
+    assert paged_attention_workspace(600, 8, 4, 1024, 128, 0, pages=4096) == (0, 0)
+    unsupported = 2
+    assert paged_attention_workspace(16, 8, 4, 32768, 128, 2, pages=4096)[0] == unsupported
+    assert paged_attention_workspace(16, 8, 4, 32768, 96, 0, pages=4096)[0] == unsupported
+    assert paged_attention_workspace(1 << 20, 64, 1, 1, 128, 0)[0] == unsupported

@@ -908,7 +908,8 @@ struct Cut {
 // 242 us).
 //
 // Nothing is split where it cannot be (a table of kMinTiles), where one
-// piece has as many workgroups as are wanted, and where short tables (up
+// piece has as many workgroups as are wanted, where the join, a workgroup a
+// query, would be more than one launch, and where short tables (up
 // to kWholeTiles) of many sequences give every CU a workgroup: the join's
 // launch costs more than the unevenness (32 sequences of 8 heads over 24
 // pages of 64: attention 44 us, 36 us).
@@ -921,7 +922,9 @@ Cut cut_of(const tgx_paged& p, int heads, int group, int D, int dtype) {
   const int64_t each = workgroups_per_piece(p, heads, group, D, dtype);
   const int64_t tiles = ceil_div(static_cast<int64_t>(p.pages_per_seq) * p.page_size, kTile);
   const int64_t wanted = cus * (held_queries(p, group, D, dtype) > 64 ? 2 : 4) / each;
-  if (tiles <= kMinTiles || wanted <= 1 || (tiles <= kWholeTiles && p.n_seqs * each >= cus))
+  const int64_t queries = static_cast<int64_t>(p.table_heads) * heads * p.queries * group;
+  if (tiles <= kMinTiles || wanted <= 1 || p.n_seqs > kMaxBlocks256 / queries ||
+      (tiles <= kWholeTiles && p.n_seqs * each >= cus))
     return Cut{1, p.n_seqs, false};
   return Cut{wanted, std::min(wanted + p.n_seqs, p.n_seqs * ceil_div(tiles, kMinTiles)), true};
 }
@@ -940,11 +943,11 @@ int check_attn(const tgx_paged* p, int heads, int group, int D, int dtype) {
                   p->n_seqs * std::max<int64_t>(tiles, 1) < (int64_t{1} << 31),
               "paged attention: sizes past 32 bits");
   const int64_t each = workgroups_per_piece(*p, heads, group, D, dtype);
-  const int64_t pairs = static_cast<int64_t>(p->table_heads) * heads;
-  TGX_REQUIRE(each <= kMaxBlocks256 && pairs * rows <= kMaxBlocks256 &&
-                  cut_of(*p, heads, group, D, dtype).launched <= kMaxBlocks256 / each - 8 &&
-                  p->n_seqs <= kMaxBlocks256 / (pairs * rows),
-              "paged attention: too many sequences, heads and queries for one launch");
+  if (each > kMaxBlocks256 ||
+      cut_of(*p, heads, group, D, dtype).launched > kMaxBlocks256 / each - 8) {
+    set_error("paged attention: too many sequences, heads and queries for one launch");
+    return TGX_UNSUPPORTED;
+  }
   return TGX_OK;
 }
 

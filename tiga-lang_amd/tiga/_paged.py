@@ -65,6 +65,21 @@ def csr_takes(D: int) -> bool:
     return D % 8 == 0 and 8 <= D <= 512 and (D // 8) & (D // 8 - 1) == 0
 
 
+def attention_workspace(graph, heads: int, group: int, D: int, code: int) -> int | None:
+    """Workspace bytes of an attention launch, None where no launch covers the
+    sizes; asked once a relation and shape."""
+    state = graph.paged_state
+    key = ("attention-workspace", heads, group, D, code)
+    need = state.checked.get(key)
+    if need is None:
+        bytes_ = ctypes.c_size_t()
+        with torch.cuda.device(graph.device):
+            takes = _native.covered("tgx_paged_attn_workspace", state.native(), heads, group, D,
+                                    code, ctypes.byref(bytes_))
+        need = state.checked[key] = bytes_.value if takes else -1
+    return None if need < 0 else need
+
+
 def bind_attention(graph, q, k, v, scale: float, heads: int, group: int):
     """The attention launch with its native arguments bound: a zero-argument
     callable that returns a new output."""
@@ -82,13 +97,10 @@ def bind_attention(graph, q, k, v, scale: float, heads: int, group: int):
         k.stride(0) * tables, k.stride(0) if tables > 1 else 0, by_head(k),
         v.stride(0) * tables, v.stride(0) if tables > 1 else 0, by_head(v))
     code = DTYPES[q.dtype]
-    need = state.checked.get(("attention-workspace", heads, group, D, code))
+    need = attention_workspace(graph, heads, group, D, code)
     if need is None:
-        bytes_ = ctypes.c_size_t()
-        with torch.cuda.device(q.device):
-            _native.call("tgx_paged_attn_workspace", state.native(), heads, group, D, code,
-                         ctypes.byref(bytes_))
-        need = state.checked["attention-workspace", heads, group, D, code] = bytes_.value
+        raise NotImplementedError("paged attention: too many sequences, heads and queries for one "
+                                  "launch")
     shape, dtype, device = q.shape, q.dtype, q.device
     tensors = (q.data_ptr(), k.data_ptr() if k.numel() else None,
                v.data_ptr() if v.numel() else None)

@@ -890,7 +890,8 @@ class MessagePassing(Kernel):
             return None
         if not (_paged.rows_on_16_bytes(k) and _paged.rows_on_16_bytes(v)):
             return None     # (a copy of the whole cache would be made each call)
-        _native.lib()
+        if _paged.attention_workspace(graph, heads, group, D, _paged.DTYPES[q.dtype]) is None:
+            return None
         scale = dot.scale
 
         def run(q, k, v):
