@@ -941,3 +941,13 @@ def test_more_queries_than_a_launch_has_workgroups():
     few = tg.Graph.paged(g.page_table, g.lengths, page_size=16, num_pages=13, queries=40)
     same = Attention()(graph=few, src={"key": k, "value": v}, dst={"query": q[:40]}, scale=0.2)
     assert torch.equal(out[-40:], same)
+
+
+def test_a_cache_of_one_slot_whose_stride_is_odd():
+    """The stride of a dimension of one element moves nothing."""
+    g = tg.Graph.paged(torch.zeros(1, 1, dtype=torch.int32, device=DEV),
+                       torch.ones(1, dtype=torch.int32, device=DEV), page_size=1, num_pages=1)
+    k = torch.randn(3, 129, device=DEV).half()[:, :128].view(3, 2, 64)[:1]
+    q = torch.randn(1, 2, 64, device=DEV).half()
+    out = Attention()(graph=g, src={"key": k, "value": k}, dst={"query": q}, scale=1.0)
+    assert torch.equal(out, k)

@@ -348,3 +348,17 @@ def test_forward_mode_is_refused_on_the_kernels():
                 call(*dual)
             call(*args)     # (a level alone changes nothing)
     call(*args)
+
+
+def test_one_token_whose_strides_are_odd():
+    """The stride of a dimension of one element moves nothing."""
+    q, k, w, pos, freqs, _ = make(1, 2, 2, 64, (32,), torch.bfloat16)
+    call = lambda q, k: tg.nn.norm_rotary(q, k, pos, freqs, query_weight=w[0], key_weight=w[1])
+    exp = call(q, k)
+    odd = lambda t: torch.zeros(3, 129, device=DEV, dtype=t.dtype)[:, :128].view(3, 2, 64)[:1] \
+        .copy_(t.detach())
+    assert odd(q).stride() == (129, 64, 1)
+    for a, b in zip(call(odd(q), odd(k)), exp):
+        assert torch.equal(a, b)
+    one = torch.zeros(1, 2, 65, device=DEV, dtype=q.dtype)[:, :1, :64].copy_(q.detach()[:, :1])
+    assert torch.equal(call(one, k)[0], exp[0][:, :1])

@@ -91,11 +91,13 @@ def bind_attention(graph, q, k, v, scale: float, heads: int, group: int):
     tables = state.table_heads
     D = q.shape[-1]
     by_head = lambda t: t.stride(1) if heads > 1 else 0
-    # A row of a relation with a table per head is (token, table head).
+    # A row of a relation with a table per head is (token, table head).  (The
+    # stride of a dimension of one element may be any.)
+    by_row = lambda t: t.stride(0) if t.shape[0] > 1 else 0
     strides = (ctypes.c_int64 * 9)(
-        q.stride(0) if q.shape[0] > 1 else 0, by_head(q), q.stride(-2) if group > 1 else 0,
-        k.stride(0) * tables, k.stride(0) if tables > 1 else 0, by_head(k),
-        v.stride(0) * tables, v.stride(0) if tables > 1 else 0, by_head(v))
+        by_row(q), by_head(q), q.stride(-2) if group > 1 else 0,
+        by_row(k) * tables, by_row(k) if tables > 1 else 0, by_head(k),
+        by_row(v) * tables, by_row(v) if tables > 1 else 0, by_head(v))
     code = DTYPES[q.dtype]
     need = attention_workspace(graph, heads, group, D, code)
     if need is None:

@@ -34,10 +34,18 @@ def covered(form: Form, query, key, weights) -> bool:
             (key is None or key.dtype == dtype) and given <= set(_DTYPES) and len(given) <= 1)
 
 
+def _steps(t: torch.Tensor) -> tuple[int, int]:
+    """Strides of tokens and heads; 0 where there is one, whose stride may be any."""
+    (n, heads, _), s = t.shape, t.stride()
+    return s[0] if n > 1 else 0, s[1] if heads > 1 else 0
+
+
 def _rows_ok(t: torch.Tensor) -> bool:
     """Rows are dense and start on two values, counted from the tensor's start."""
-    s = t.stride()
-    return t.numel() == 0 or (s[2] == 1 and s[0] % 2 == 0 and s[1] % 2 == 0)
+    if t.numel() == 0:
+        return True
+    token, head = _steps(t)
+    return t.stride(2) == 1 and token % 2 == 0 and head % 2 == 0
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -54,7 +62,7 @@ def _struct(form: Form, query, key, query_weight, key_weight, positions,
     p = _native.NormRotary()
     for i, x in enumerate((query, key)):
         if x is not None:
-            p.token_stride[i], p.head_stride[i] = x.stride()[:2]
+            p.token_stride[i], p.head_stride[i] = _steps(x)
             p.heads[i] = x.shape[1]
     p.w_dtype = next((_DTYPES[w.dtype] for w in (query_weight, key_weight) if w is not None), 2)
     p.positions_bits = _native.idx_bits(positions)
