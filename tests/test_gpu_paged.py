@@ -951,3 +951,44 @@ def test_a_cache_of_one_slot_whose_stride_is_odd():
     q = torch.randn(1, 2, 64, device=DEV).half()
     out = Attention()(graph=g, src={"key": k, "value": k}, dst={"query": q}, scale=1.0)
     assert torch.equal(out, k)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lengths,D", [([20000], 128), ([9000, 1, 0, 300, 4111], 64),
+                                       ([3000] * 12, 128), ([5000], 32), ([2000, 77], 80)])
+def test_long_lengths_to_the_last_rounding(lengths, D, dtype):
+    tight(lengths, 16, 2, 4, D, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lengths,heads,group,queries,D", [
+    ([20001], 1, 4, 1, 128), ([1, 0, 640, 9001], 2, 4, 3, 64), ([3000] * 40, 2, 1, 1, 32),
+    ([2100, 5], 1, 8, 4, 128), ([2100, 5], 1, 8, 7, 64), ([2100, 5, 130], 1, 8, 20, 128),
+    ([777, 3000], 2, 3, 1, 96)])
+def test_every_key_counts_once(lengths, heads, group, queries, D, dtype):
+    """All scores equal: a row is the mean of the values it sees.  Column d holds
+    a one for every D-th key of a window, so n times the row is the number of
+    those it sees: at most 64, off by at most 64 * 2^-8 = 1/4 and never by one."""
+    print(f"count {dtype} {lengths[:4]} queries={queries} D={D}", flush=True)
+    rng = np.random.default_rng(22)
+    table, length, pages = relation(rng, lengths, 16)
+    g = tg.Graph.paged(torch.tensor(table, device=DEV), torch.tensor(length, device=DEV),
+                       page_size=16, num_pages=pages, queries=queries)
+    q = torch.zeros(len(lengths) * queries, heads, group, D, device=DEV, dtype=TYPES[dtype])
+    k = torch.randn(pages * 16, heads, 1, D, device=DEV).to(TYPES[dtype])
+    kernel = Attention()
+    for start in range(0, max(lengths), 64 * D):
+        v = np.zeros((pages * 16, D))
+        exp = np.zeros((len(lengths), queries, D))
+        for b, n in enumerate(lengths):
+            at, _ = want.slots(table[b], n, 16, pages)
+            for j in range(start, min(n, start + 64 * D)):
+                v[at[j], j % D] = 1.0
+                exp[b, max(j - (n - queries), 0):, j % D] += 1.0
+        values = torch.tensor(v, device=DEV).to(TYPES[dtype])[:, None, None].expand(
+            -1, heads, 1, D).contiguous()
+        out = kernel(graph=g, src={"key": k, "value": values}, dst={"query": q}, scale=1.0)
+        seen = np.maximum(np.asarray(lengths)[:, None] - np.arange(queries - 1, -1, -1), 0)
+        got = f64(out).reshape(len(lengths), queries, heads * group, D)
+        got = got * seen[:, :, None, None]
+        assert np.array_equal(np.rint(got), np.broadcast_to(exp[:, :, None], got.shape))

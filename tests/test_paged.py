@@ -269,3 +269,27 @@ def test_launches_that_need_no_workgroup_per_query_take_prompts():
     assert paged_attention_workspace(16, 8, 4, 32768, 128, 2, pages=4096)[0] == unsupported
     assert paged_attention_workspace(16, 8, 4, 32768, 96, 0, pages=4096)[0] == unsupported
     assert paged_attention_workspace(1 << 20, 64, 1, 1, 128, 0)[0] == unsupported
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("n,lost", [(20000, 320), (3000, 256)])
+def test_the_bound_of_the_kernels_rejects_what_is_lost(n, lost, dtype):
+    """Zeros, and an output without one piece of the keys, lie outside of what
+    rounding may do; the rounded formula lies inside."""
+    rng = np.random.default_rng(30)
+    size, D = 16, 128
+    pages = -(-n // size)
+    table, mk = np.arange(pages)[None], rng.standard_normal
+    q, k, v = mk((1, 2, 4, D)), mk((pages * size, 2, D)), mk((pages * size, 2, D))
+    args = (table, [n], size, pages, 1, q, k)
+    exp = want.attention(*args, v, D ** -0.5)
+    lim = want.attention_bound(*args, v, D ** -0.5, dtype, dtype != "f32")
+    rounded = torch.tensor(exp).to({"bf16": torch.bfloat16, "f16": torch.float16,
+                                    "f32": torch.float32}[dtype]).double().numpy()
+    assert (np.abs(rounded - exp) <= lim).all()
+    assert (np.abs(exp) > lim).mean() > 0.9             # zeros
+    for first in (0, n // 2 // lost * lost, n - lost):
+        short = np.delete(np.arange(n), np.arange(first, first + lost))
+        kk, vv = (np.concatenate([x[short], x[:lost]]) for x in (k, v))
+        without = want.attention(table, [n - lost], size, pages, 1, q, kk, vv, D ** -0.5)
+        assert (np.abs(without - exp) > lim).mean() > 0.25
