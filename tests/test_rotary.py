@@ -122,3 +122,16 @@ def test_refusals():
         f(q, k, pos, freqs, eps=-1.0)
     with pytest.raises(NotImplementedError, match="gradient"):
         f(q, k, pos, freqs.clone().requires_grad_())
+
+
+def test_forms_go_by_value():
+    """A number that a program keeps in a tensor and changes is read at each call."""
+    q, _, _, _, positions, freqs = inputs(3, 2, 1, 8, (4,))
+    eps, norm = torch.tensor(1e-3), torch.tensor(True)
+    call = lambda eps, norm: tg.nn.norm_rotary(torch.tensor(q), None, torch.tensor(positions),
+                                               torch.tensor(freqs), eps=eps, norm=norm)
+    call(eps, norm)
+    eps.fill_(0.5)
+    assert torch.equal(call(eps, norm), call(0.5, True))
+    norm.fill_(False)
+    assert torch.equal(call(eps, norm), call(0.5, False))

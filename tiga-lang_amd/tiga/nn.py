@@ -427,7 +427,7 @@ def norm_rotary(query: torch.Tensor, key: torch.Tensor | None, positions: torch.
     tensors = (query, key, positions, frequencies, query_weight, key_weight)
     try:
         spec = (*[None if t is None else (t.dtype, t.shape, t.stride(), t.device)
-                  for t in tensors], eps, norm, sections, interleaved)
+                  for t in tensors], float(eps), bool(norm), sections, bool(interleaved))
         plan = _ROTARY_PLANS.get(spec)
     except (AttributeError, TypeError):
         plan = spec = None
