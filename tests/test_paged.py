@@ -293,3 +293,12 @@ def test_the_bound_of_the_kernels_rejects_what_is_lost(n, lost, dtype):
         kk, vv = (np.concatenate([x[short], x[:lost]]) for x in (k, v))
         without = want.attention(table, [n - lost], size, pages, 1, q, kk, vv, D ** -0.5)
         assert (np.abs(without - exp) > lim).mean() > 0.25
+
+
+def test_tables_are_advanced_in_place_not_replaced():
+    """The launches are sized by the tables a relation was made of."""
+    g = graph()
+    for name, value in (("page_table", TABLE[:, :1]), ("lengths", LENGTHS[:1]), ("page_size", 1),
+                        ("num_pages", 99), ("queries", 2)):
+        with pytest.raises(AttributeError):
+            setattr(g.paged_state, name, value)

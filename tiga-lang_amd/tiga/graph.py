@@ -50,10 +50,10 @@ class GraphSchema:
                 str(self.index_dtype), self.sorted_by_dst)
 
 
-@dataclass
+@dataclass(frozen=True, eq=False)
 class PagedState:
     """The tables of a paged relation (``Graph.paged``): tensors whose contents
-    every use reads as they stand."""
+    every use reads as they stand, and the sizes its launches are made for."""
 
     page_table: torch.Tensor   # [sequences, pages] or [sequences, heads, pages] int32
     lengths: torch.Tensor      # [sequences] int32
@@ -62,9 +62,14 @@ class PagedState:
     queries: int
 
     def __post_init__(self):
-        self._native = None
+        t = self.page_table
+        native = _native.Paged(
+            None, t.stride(0), t.stride(1) if t.ndim == 3 else 0, None, t.shape[0],
+            self.table_heads, t.shape[-1], self.page_size, self.num_pages, self.queries)
+        object.__setattr__(self, "_native", native)
+        object.__setattr__(self, "_native_ref", ctypes.byref(native))
         # Operand shapes and layouts that append and select_pages have checked.
-        self.checked: dict[tuple, object] = {}
+        object.__setattr__(self, "checked", {})
 
     @property
     def table_heads(self) -> int:
@@ -72,13 +77,7 @@ class PagedState:
 
     def native(self):
         """The relation as the native entry points take it."""
-        t = self.page_table
-        if self._native is None:
-            self._native = _native.Paged(
-                None, t.stride(0), t.stride(1) if t.ndim == 3 else 0, None, t.shape[0],
-                self.table_heads, t.shape[-1], self.page_size, self.num_pages, self.queries)
-            self._native_ref = ctypes.byref(self._native)
-        self._native.page_table_dev = t.data_ptr() or None
+        self._native.page_table_dev = self.page_table.data_ptr() or None
         self._native.lengths_dev = self.lengths.data_ptr() or None
         return self._native_ref
 
