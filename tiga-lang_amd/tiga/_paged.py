@@ -54,10 +54,10 @@ def heads_of(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor):
     return (1, q.shape[1]) if k.shape[1] == 1 else None
 
 
-def wants_derivative(*tensors) -> bool:
-    """Whether a result of these tensors has to carry gradients or a tangent."""
-    return carries_tangent(*tensors) or (
-        torch.is_grad_enabled() and any(t.requires_grad for t in tensors))
+def wants_derivative(q, k, v) -> bool:
+    """Whether attention of these has to carry gradients or a tangent."""
+    return ((q.requires_grad or k.requires_grad or v.requires_grad) and
+            torch.is_grad_enabled()) or carries_tangent(q, k, v)
 
 
 def csr_takes(D: int) -> bool:
