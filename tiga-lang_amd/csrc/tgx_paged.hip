@@ -9,8 +9,11 @@
 // page holds no key; a row that sees no key is zero.  A row's masked keys
 // and values never reach it, whatever they hold.
 //
-// Bound: every cached row is read once, 4 * D bytes a key and head at 16
-// bits, against 4 * group * D operations: memory, for any group a model has.
+// Bound: a cached row has to be read once, 4 * D bytes a key and head at 16
+// bits, against 4 * group * D operations a new token: memory, for any group a
+// model has and few new tokens.  The matrix tiles (16 bits, D = 32, 64, 128) read it
+// once for 128 queries of its key head; paged_rows_kernel, which takes every other
+// width and fp32, once for each query.
 //
 // Work split.  Lengths are only known on the device, so the launch is sized
 // from the host's bounds and every workgroup finds its piece itself: the keys
@@ -160,7 +163,10 @@ struct State8 {
 
 // One workgroup per (piece, head, query): LPK lanes hold a row of D values, 8
 // each, and a wave's 64 / LPK lane groups take a key each; the states of the
-// groups and the four waves are merged at the end.
+// groups and the four waves are merged at the end.  A key head's queries read
+// its rows one by one, from L2 where they meet there: 64 sequences of 100 to
+// 4000 tokens, fp32, 8 heads of 128: 225 us with one query a head (4.9 TB/s),
+// 663 us with four; bf16 with four, heads of 256 780 us, of 96 432 us.
 template <int DT, int LPK>
 __global__ __launch_bounds__(256) void paged_rows_kernel(PagedArgs a) {
   using V = Vals<DT, 8>;
@@ -899,13 +905,15 @@ struct Cut {
   bool split;
 };
 
-// Workgroups wanted in all: what the GPU holds at once (two a CU at D = 128, four
-// below), twice over at D = 128.  Four sequences of 100k to 131k tokens: 346 us
-// with two rounds that fit, 368-420 us with rounds that end half full; more
-// and smaller pieces pay for their first loads, fewer end unevenly.  A
-// workgroup of more than 64 queries writes and joins as much as it reads of a
-// few tiles of keys: half as many (512 new tokens of four sequences: 322 us,
-// 242 us).
+// Workgroups wanted in all: four a CU.  The tile kernel holds two at once at D =
+// 128, three at D = 64 and four at D = 32 (its launch bounds), so these are two
+// full rounds, one and a third, and one.  Four sequences of 100k to 131k tokens, D =
+// 128: 346 us with two rounds that fit, 368-420 us with rounds that end half full;
+// more and smaller pieces pay for their first loads, fewer end unevenly.  (Ragged
+// sequences do not fill the rounds: find_piece takes a piece a sequence off before
+// it sizes them, 95 of 128 for 64 sequences of 100 to 4000.)  A workgroup of more
+// than 64 queries writes and joins as much as it reads of a few tiles of keys:
+// half as many (512 new tokens of four sequences: 315 us with four a CU, 282 us).
 //
 // Nothing is split where it cannot be (a table of kMinTiles), where one
 // piece has as many workgroups as are wanted, where the join, a workgroup a

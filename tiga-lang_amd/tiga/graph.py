@@ -481,8 +481,15 @@ class Graph:
 
         Dot-product attention over the relation, with query heads grouped on
         key heads if the fields broadcast (query [rows, heads, group, D] on key
-        and value [slots, heads, 1, D]), runs on the paged kernels; any other
-        edge function, and attention that needs gradients, on `snapshot()`.
+        and value [slots, heads, 1, D]), runs on the paged kernels: bf16, fp16 and
+        fp32, widths that are multiples of 8 up to 512; scores, softmax and sums in
+        fp32, a weight as two 16-bit values in the matrix tiles.  Any other edge
+        function, and attention that needs gradients, runs on `snapshot()`.  That
+        writes the relation's edges (8 bytes a row and key), and gradients copy keys
+        and values of the whole cache for each of a key head's query heads: they
+        are for short caches, not for training.  Widths whose eighth is no power of
+        two have gradients on Torch operations only (``tiga.config.strict`` refuses
+        them), and forward mode is refused where a kernel would run.
 
         A page_table [sequences, heads, pages] is a table for each head
         (`select_pages` returns such a relation): the rows are then
@@ -560,7 +567,9 @@ class Graph:
         [slots, heads, D] its sources; all of one type, strided as they come.
         page_sums [num_pages, heads, D] fp32: the sum of the keys of every page
         written to is formed again from the page's slots up to the newest token
-        (what `select_pages` ranks pages by).  No gradients.
+        (what `select_pages` ranks pages by).  No gradients and no forward mode;
+        64-bit caches run on Torch operations (``tiga.config.strict`` refuses them
+        on the GPU).
 
         Each sequence's written pages must be its own and named once in its
         table (two writers of a slot leave either's row there), and key and
@@ -622,7 +631,9 @@ class Graph:
             score = sum_d (sum_g query[row, h, g, d]) * page_sums[page, h, d],
 
         formed in 64 bits; equal scores go to the earlier page, a NaN counts as
-        -inf, and a row of no more than `count` pages keeps them all.
+        -inf, and a row of no more than `count` pages keeps them all.  64-bit
+        queries run on Torch operations (``tiga.config.strict`` refuses them on
+        the GPU).
 
         query [rows, heads, group, D] or [rows, heads, D]; page_sums
         [num_pages, heads, D] fp32, as `append` keeps them.  The result has a

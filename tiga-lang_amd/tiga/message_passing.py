@@ -907,11 +907,15 @@ class MessagePassing(Kernel):
         kind = str(q.dtype).split(".")[-1]
         derivative = _paged.wants_derivative(q, k, v)
 
+        # (As csrc/tgx_paged.hip chooses its kernel.)
+        reads = ("once for 128 queries of a key head" if q.dtype != torch.float32 and
+                 D in (32, 64, 128) else "once for each query")
+
         def describe():
             if not derivative:
                 return self._variant(
                     graph, "paged-attention", ("tgx_paged_attn",),
-                    f"{kind} rows of the cache read once through the page tables, {group} query "
+                    f"{kind} rows of the cache read {reads} through the page tables, {group} query "
                     f"heads on each of {heads} key heads, fp32 online softmax; long sequences in "
                     "pieces, joined in order; gradients on the relation's snapshot")
             if not _paged.csr_takes(D):

@@ -418,7 +418,8 @@ def norm_rotary(query: torch.Tensor, key: torch.Tensor | None, positions: torch.
     number of frequencies of each axis in order; integers, of either sign and
     any size (angles are formed in 64 bits).  Arithmetic is in fp32, rounded
     once.  Returns the new query, or (query, key).  Gradients: query, key and
-    weights; the same inputs give the same bits.
+    weights; the same inputs give the same bits.  Forward mode is refused on the
+    kernels.
 
     On the GPU bf16, fp16 and fp32, D a multiple of 4 up to 256, an even number
     of frequencies, at most 4 axes and weights of one type run on the HIP
