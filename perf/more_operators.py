@@ -235,7 +235,8 @@ def _scale_of(amax, cache):
     """The power of two that a block of largest magnitude `amax` is stored by."""
     largest, shift = LARGEST[cache]
     part, exponent = torch.frexp(amax)
-    return _power((exponent - shift + (part > largest / 2 ** shift)).clamp(min=-126))
+    exponent = torch.where(amax == 0, -126, exponent - shift + (part > largest / 2 ** shift))
+    return _power(exponent.clamp(min=-126))
 
 
 def _round_to(x, cache):
