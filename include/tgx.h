@@ -835,6 +835,57 @@ int tgx_paged_attn(const tgx_paged* p, const void* q_dev, const void* k_dev, con
                    const int64_t* strides, float scale, void* out_dev, int heads, int group,
                    int D, int dtype, void* workspace_dev, size_t workspace_bytes, void* stream);
 
+/* What attention sees of a paged relation, and how its cache is held.
+ * window > 0: a token sees the last `window` of its positions and the first
+ * `sinks`; 0 (and no sinks): all of them.
+ * code 0: k and v of the queries' type.  TGX_CODE_E4M3, TGX_CODE_INT8: codes of one
+ * byte, times scales, fp32 [slots / block, table_heads, heads] contiguous, the pages
+ * whole blocks. */
+#define TGX_CODE_E4M3 1
+#define TGX_CODE_INT8 2
+typedef struct {
+  int32_t window;
+  int32_t sinks;
+  int32_t code;
+  int32_t block;
+  const float* k_scales_dev;
+  const float* v_scales_dev;
+} tgx_paged_view;
+
+/* tgx_paged_attn over a view.  The strides of k and v, in elements, are multiples of
+ * 8 for codes, whose start is a multiple of 8 bytes (of 16 for the tiles that
+ * read each row once); dtype is the queries' and the output's. */
+int tgx_paged_attn_view_workspace(const tgx_paged* p, const tgx_paged_view* view, int heads,
+                                  int group, int D, int dtype, size_t* bytes);
+int tgx_paged_attn_view(const tgx_paged* p, const tgx_paged_view* view, const void* q_dev,
+                        const void* k_dev, const void* v_dev, const int64_t* strides, float scale,
+                        void* out_dev, int heads, int group, int D, int dtype, void* workspace_dev,
+                        size_t workspace_bytes, void* stream);
+
+/* tgx_paged_append into a cache of codes (Graph.append, tiga.BlockScaled): for each
+ * touched block of `block` slots and head, with M = 448 (E4M3) or 127 (INT8),
+ *   s = the smallest power of two >= 2^-126 with max |new| <= M s, or the scale of
+ *       the block's older tokens, if there are any and it is more; NaN if a new
+ *       value is a NaN or an infinity, or that scale is NaN
+ *   code = new / s to nearest, ties to even; older codes times old scale / s likewise
+ * New rows of bf16, fp16 or fp32 (dtype); D a multiple of 8 up to 512; scales fp32
+ * [slots / block, heads] contiguous; page sums of the rows as they are held.
+ *   strides, host array of eight as tgx_paged_append's: the caches' multiples of 8,
+ *     the rows' of 16 bytes */
+int tgx_paged_append_scaled(const tgx_paged* p, void* key_codes_dev, float* key_scales_dev,
+                            const void* key_dev, void* value_codes_dev, float* value_scales_dev,
+                            const void* value_dev, const int64_t* strides, float* page_sums_dev,
+                            int heads, int D, int dtype, int code, int block, void* stream);
+
+/* The newest tokens' rows out of a cache of codes (Graph.read): key_dev and value_dev
+ * [n_seqs * queries, heads, D] contiguous, of dtype; a row whose position is
+ * negative or whose page id names no page is zero.
+ *   strides, host array of four: the key cache's slot and head, the value cache's */
+int tgx_paged_read(const tgx_paged* p, const void* key_codes_dev, const float* key_scales_dev,
+                   const void* value_codes_dev, const float* value_scales_dev,
+                   const int64_t* strides, void* key_dev, void* value_dev, int heads, int D,
+                   int dtype, int code, int block, void* stream);
+
 /* The newest tokens' keys and values into their slots (Graph.append): rows b *
  * queries + t of key and value, `heads` rows of D values each; tokens at
  * positions below zero do not exist.  Page sums, if given (fp32
@@ -862,6 +913,43 @@ int tgx_select_pages(const tgx_paged* p, const void* q_dev, const int64_t* strid
                      const float* page_sums_dev, int heads, int group, int D, int dtype,
                      int count, int32_t* table_dev, int32_t* lengths_dev, void* workspace_dev,
                      size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Attention of packed sequences over a window                               */
+/* ------------------------------------------------------------------------ */
+
+/* Causal attention of packed sequences (Graph.cu_seqlens, Graph.triangular with
+ * window and sinks): position i of a sequence sees the keys j <= i of it with
+ * i - j < window or j < sinks; `group` query heads (up to 128) on each of `heads`
+ * key heads; bf16 or fp16, D 32, 64 or 128.
+ *
+ * tgx_window_tasks: the host lists of a relation (cu_host [n_blocks + 1]), XCD by
+ * XCD.  kind 0: query tiles [n, 4]; 1: key tiles [n, 8], with *n_slots partial
+ * sums; 2: the key tiles joined from those [n, 8].  tasks_host NULL asks for the
+ * counts.  The lists go to the device unchanged. */
+int tgx_window_tasks(const int32_t* cu_host, int n_blocks, int heads, int group, int window,
+                     int sinks, int kind, int32_t* tasks_host, int64_t* n_tasks,
+                     int64_t* n_slots);
+
+/* out [n, heads, group, D] contiguous, lse [n, heads, group] fp32 (natural log).
+ * strides, host array of seven, in elements, multiples of 8: q's token, head, group;
+ * k's token, head; v's token, head. */
+int tgx_window_attn_fwd(const int32_t* cu_dev, const int32_t* tasks_dev, int64_t n_tasks,
+                        const void* q, const void* k, const void* v, const int64_t* strides,
+                        float scale, int window, int sinks, void* out, float* lse, int64_t n,
+                        int heads, int group, int D, int dtype, void* stream);
+
+/* dq [n, heads, group, D], dk and dv [n, heads, D] from the forward's out and lse and
+ * from dout (contiguous like out).  No atomics: the same inputs give the same bits. */
+int tgx_window_attn_bwd_workspace(int64_t n, int64_t n_slots, int heads, int group, int D,
+                                  size_t* bytes);
+int tgx_window_attn_bwd(const int32_t* cu_dev, const int32_t* q_tasks_dev, int64_t n_q_tasks,
+                        const int32_t* k_tasks_dev, int64_t n_k_tasks, const int32_t* joins_dev,
+                        int64_t n_joins, int64_t n_slots, const void* q, const void* k,
+                        const void* v, const int64_t* strides, const void* out, const float* lse,
+                        const void* dout, float scale, int window, int sinks, void* dq, void* dk,
+                        void* dv, int64_t n, int heads, int group, int D, int dtype,
+                        void* workspace_dev, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------ */
 /* Norm and rotation of queries and keys                                     */

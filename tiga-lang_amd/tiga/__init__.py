@@ -5,6 +5,7 @@ Public names follow the reference package (python/tiga/__init__.py:45-66):
 """
 
 from . import interop, nn, reducer
+from .blockscaled import BlockScaled
 from .graph import Graph, GraphSchema
 from .kernel import CompiledVariant, Kernel
 from .message_passing import MessagePassing, config
@@ -21,6 +22,7 @@ from .reducer import sum  # noqa: A004
 __version__ = "0.1.0"
 
 __all__ = [
+    "BlockScaled",
     "CompiledVariant",
     "Graph",
     "GraphSchema",

@@ -62,6 +62,13 @@ class Paged(ctypes.Structure):
                 ("num_pages", c_i64), ("queries", ctypes.c_int32)]
 
 
+class PagedView(ctypes.Structure):
+    """Mirror of ``tgx_paged_view``."""
+
+    _fields_ = [("window", ctypes.c_int32), ("sinks", ctypes.c_int32), ("code", ctypes.c_int32),
+                ("block", ctypes.c_int32), ("k_scales_dev", c_vp), ("v_scales_dev", c_vp)]
+
+
 class NormRotary(ctypes.Structure):
     """Mirror of ``tgx_norm_rotary``."""
 
@@ -171,6 +178,21 @@ _SIGNATURES: dict[str, list] = {
     "tgx_paged_attn_workspace": [P(Paged), c_int, c_int, c_int, c_int, P(c_size)],
     "tgx_paged_attn": [P(Paged), c_vp, c_vp, c_vp, P(c_i64), c_f32, c_vp, c_int, c_int, c_int,
                        c_int, c_vp, c_size, c_vp],
+    "tgx_paged_attn_view_workspace": [P(Paged), P(PagedView), c_int, c_int, c_int, c_int,
+                                      P(c_size)],
+    "tgx_paged_attn_view": [P(Paged), P(PagedView), c_vp, c_vp, c_vp, P(c_i64), c_f32, c_vp, c_int,
+                            c_int, c_int, c_int, c_vp, c_size, c_vp],
+    "tgx_paged_append_scaled": [P(Paged), c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, P(c_i64), c_vp,
+                                c_int, c_int, c_int, c_int, c_int, c_vp],
+    "tgx_paged_read": [P(Paged), c_vp, c_vp, c_vp, c_vp, P(c_i64), c_vp, c_vp, c_int, c_int, c_int,
+                       c_int, c_int, c_vp],
+    "tgx_window_tasks": [c_vp, c_int, c_int, c_int, c_int, c_int, c_int, c_vp, P(c_i64), P(c_i64)],
+    "tgx_window_attn_fwd": [c_vp, c_vp, c_i64, c_vp, c_vp, c_vp, P(c_i64), c_f32, c_int, c_int,
+                            c_vp, c_vp, c_i64, c_int, c_int, c_int, c_int, c_vp],
+    "tgx_window_attn_bwd_workspace": [c_i64, c_i64, c_int, c_int, c_int, P(c_size)],
+    "tgx_window_attn_bwd": [c_vp, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp,
+                            P(c_i64), c_vp, c_vp, c_vp, c_f32, c_int, c_int, c_vp, c_vp, c_vp,
+                            c_i64, c_int, c_int, c_int, c_int, c_vp, c_size, c_vp],
     "tgx_paged_append": [P(Paged), c_vp, c_vp, c_vp, c_vp, P(c_i64), c_vp, c_int, c_int, c_int,
                          c_vp],
     "tgx_select_pages_workspace": [P(Paged), c_int, c_int, P(c_size)],

@@ -12,8 +12,10 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native
+from ._dual import carries_tangent
 from .graph import Graph
 
 
@@ -413,6 +415,91 @@ class BlockAttentionFunction(torch.autograd.Function):
             _native.call("tgx_attn_bwd", *args, *tail)
         return dq, dk, dv, None, None, None
 
+
+# ---------------------------------------------------------------------------
+# Attention over a window (tgx_window.hip)
+
+# Query heads of a key head that the tiles take.
+WINDOW_MAX_GROUP = 128
+_WINDOW_MAX_TOKEN_STRIDE = 1 << 24
+
+
+def _window_rows(t: torch.Tensor) -> torch.Tensor:
+    """`t` with dense rows on 16 bytes and strides the tiles take."""
+    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(
+        n <= 1 or (s % 8 == 0 and 0 <= s < _WINDOW_MAX_TOKEN_STRIDE)
+        for n, s in zip(t.shape[:-1], t.stride()))
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def _window_strides(q, k, v):
+    step = lambda t, d: t.stride(d) if t.shape[d] > 1 else 0
+    return (ctypes.c_int64 * 7)(step(q, 0), step(q, 1), step(q, 2), step(k, 0), step(k, 1),
+                                step(v, 0), step(v, 1))
+
+
+class WindowAttentionFunction(torch.autograd.Function):
+    """Causal dot-product attention that looks back over the graph's window and
+    sinks: q [n, heads, group, D], k and v [n, heads, D], bf16 or fp16, D in {32,
+    64, 128}; out contiguous [n, heads, group, D]."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, scale: float, graph: Graph):
+        _on_graph_device(graph, q, k, v)
+        n, heads, group, D = q.shape
+        q, k, v = _window_rows(q), _window_rows(k), _window_rows(v)
+        out = torch.empty((n, heads, group, D), dtype=q.dtype, device=q.device)
+        lse = torch.empty((n, heads, group), dtype=torch.float32, device=q.device)
+        if n:
+            cu, tasks, count, _ = graph._window_tasks(0, heads, group)
+            _native.launch(q, "tgx_window_attn_fwd", cu.data_ptr(), tasks.data_ptr(), count,
+                           q.data_ptr(), k.data_ptr(), v.data_ptr(), _window_strides(q, k, v),
+                           float(scale), *graph._window, out.data_ptr(), lse.data_ptr(), n, heads,
+                           group, D, _ATTN_DTYPES[q.dtype])
+        ctx.graph, ctx.scale = graph, float(scale)
+        ctx.save_for_backward(q, k, v, out, lse)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse = ctx.saved_tensors
+        graph: Graph = ctx.graph
+        n, heads, group, D = q.shape
+        dout = dout.to(q.dtype).contiguous()
+        if dout.data_ptr() % 16:
+            dout = dout.clone()
+        dq = torch.empty_like(out)
+        dk = torch.empty((n, heads, D), dtype=q.dtype, device=q.device)
+        dv = torch.empty_like(dk)
+        if n:
+            cu, qtasks, nq, _ = graph._window_tasks(0, heads, group)
+            _, ktasks, nk, slots = graph._window_tasks(1, heads, group)
+            _, joins, nj, _ = graph._window_tasks(2, heads, group)
+            need = ctypes.c_size_t()
+            _native.call("tgx_window_attn_bwd_workspace", n, slots, heads, group, D,
+                         ctypes.byref(need))
+            work = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+            _native.launch(q, "tgx_window_attn_bwd", cu.data_ptr(), qtasks.data_ptr(), nq,
+                           ktasks.data_ptr(), nk, joins.data_ptr(), nj, slots, q.data_ptr(),
+                           k.data_ptr(), v.data_ptr(), _window_strides(q, k, v), out.data_ptr(),
+                           lse.data_ptr(), dout.data_ptr(), ctx.scale, *graph._window,
+                           dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), n, heads, group, D,
+                           _ATTN_DTYPES[q.dtype], work.data_ptr(), need.value)
+        return dq, dk, dv, None, None
+
+
+def window_attention(q, k, v, scale: float, heads: int, group: int, graph: Graph):
+    """Attention over a windowed relation of fields [n, heads, group, D] on
+    [n, heads, 1, D], [n, heads, D] on the same, or [n, group, D] on [n, 1, D]."""
+    if carries_tangent(q, k, v):
+        raise NotImplementedError("attention over a window has no forward-mode derivative on the "
+                                  "HIP kernels")
+    D = q.shape[-1]
+    if k.ndim == 4:
+        k, v = k[:, :, 0], v[:, :, 0]
+    rows = q if q.ndim == 4 else q[:, :, None] if group == 1 else q[:, None]
+    return WindowAttentionFunction.apply(rows, k, v, scale, graph).view(q.shape)
 
 
 # ---------------------------------------------------------------------------

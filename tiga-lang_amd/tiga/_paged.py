@@ -1,6 +1,7 @@
 """Launches over a paged cache relation (``Graph.paged``): attention, the
-upkeep of the cache and the choice of pages (csrc/tgx_paged.hip,
-csrc/tgx_pages.hip), and the same on Torch operations for host tensors.
+upkeep of the cache, reading it back and the choice of pages
+(csrc/tgx_paged.hip, csrc/tgx_paged_scaled.hip, csrc/tgx_pages.hip,
+csrc/tgx_pages_scaled.hip), and the same on Torch operations for host tensors.
 
 The page tables and lengths are read by the kernels at every launch, so none
 of these copies them to the host or synchronises; outputs and workspaces are
@@ -15,6 +16,7 @@ import torch
 
 from . import _native
 from ._dual import carries_tangent
+from .blockscaled import CODES, BlockScaled, encode, scale_of
 
 # Element types of the paged kernels (TGX_DTYPE_*).
 DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -57,7 +59,32 @@ def heads_of(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor):
 def wants_derivative(q, k, v) -> bool:
     """Whether attention of these has to carry gradients or a tangent."""
     return ((q.requires_grad or k.requires_grad or v.requires_grad) and
-            torch.is_grad_enabled()) or carries_tangent(q, k, v)
+            torch.is_grad_enabled()) or carries_tangent(q, _carrier(k), _carrier(v))
+
+
+def _carrier(t) -> torch.Tensor:
+    """The tensor of a field that could carry a tangent."""
+    return t.scales if isinstance(t, BlockScaled) else t
+
+
+def cache_kind(k, v):
+    """(code, block) of key and value fields, (0, 1) of tensors; None where
+    one is in 8 bits and the other is not, or in another form."""
+    if not isinstance(k, BlockScaled) and not isinstance(v, BlockScaled):
+        return 0, 1
+    if not isinstance(k, BlockScaled) or not isinstance(v, BlockScaled) or \
+            (k.dtype, k.block, k.tables) != (v.dtype, v.block, v.tables):
+        return None
+    return CODES[k.dtype], k.block
+
+
+def cache_rows_ok(k, v) -> bool:
+    """Whether a launch can read these key and value fields in place."""
+    if isinstance(k, BlockScaled):
+        # (Codes are read by eights, or sixteens where the rows allow it.)
+        return all(t.codes.data_ptr() % 8 == 0 and all(
+            n <= 1 or s % 8 == 0 for n, s in zip(t.shape[:-1], t.codes.stride())) for t in (k, v))
+    return rows_on_16_bytes(k) and rows_on_16_bytes(v)
 
 
 def csr_takes(D: int) -> bool:
@@ -65,17 +92,34 @@ def csr_takes(D: int) -> bool:
     return D % 8 == 0 and 8 <= D <= 512 and (D // 8) & (D // 8 - 1) == 0
 
 
-def attention_workspace(graph, heads: int, group: int, D: int, code: int) -> int | None:
+def _view(state, k=None, v=None):
+    """The native tgx_paged_view of a launch, None where tgx_paged_attn covers it."""
+    scaled = isinstance(k, BlockScaled)
+    if not scaled and state.window is None:
+        return None
+    return _native.PagedView(
+        state.window or 0, state.sinks, CODES[k.dtype] if scaled else 0,
+        k.block if scaled else 1, k.scales.data_ptr() or None if scaled else None,
+        v.scales.data_ptr() or None if scaled else None)
+
+
+def attention_workspace(graph, k, v, heads: int, group: int, D: int, code: int) -> int | None:
     """Workspace bytes of an attention launch, None where no launch covers the
     sizes; asked once a relation and shape."""
     state = graph.paged_state
-    key = ("attention-workspace", heads, group, D, code)
+    key = ("attention-workspace", heads, group, D, code, cache_kind(k, v))
     need = state.checked.get(key)
     if need is None:
         bytes_ = ctypes.c_size_t()
+        view = _view(state, k, v)
         with torch.cuda.device(graph.device):
-            takes = _native.covered("tgx_paged_attn_workspace", state.native(), heads, group, D,
-                                    code, ctypes.byref(bytes_))
+            if view is None:
+                takes = _native.covered("tgx_paged_attn_workspace", state.native(), heads, group,
+                                        D, code, ctypes.byref(bytes_))
+            else:
+                takes = _native.covered("tgx_paged_attn_view_workspace", state.native(),
+                                        ctypes.byref(view), heads, group, D, code,
+                                        ctypes.byref(bytes_))
         need = state.checked[key] = bytes_.value if takes else -1
     return None if need < 0 else need
 
@@ -87,7 +131,12 @@ def bind_attention(graph, q, k, v, scale: float, heads: int, group: int):
     for t in (q, k, v):
         if t.device != graph.device:
             raise ValueError(f"operand on {t.device} for a graph on {graph.device}")
-    q, k, v = (_on_16_bytes(t) for t in (q, k, v))
+    q, view = _on_16_bytes(q), _view(state, k, v)
+    fields = (k, v)
+    if isinstance(k, BlockScaled):
+        k, v = k.codes, v.codes
+    else:
+        k, v = fields = (_on_16_bytes(k), _on_16_bytes(v))
     tables = state.table_heads
     D = q.shape[-1]
     by_head = lambda t: t.stride(1) if heads > 1 else 0
@@ -99,20 +148,23 @@ def bind_attention(graph, q, k, v, scale: float, heads: int, group: int):
         by_row(k) * tables, by_row(k) if tables > 1 else 0, by_head(k),
         by_row(v) * tables, by_row(v) if tables > 1 else 0, by_head(v))
     code = DTYPES[q.dtype]
-    need = attention_workspace(graph, heads, group, D, code)
+    need = attention_workspace(graph, *fields, heads, group, D, code)
     if need is None:
         raise NotImplementedError("paged attention: too many sequences, heads and queries for one "
                                   "launch")
     shape, dtype, device = q.shape, q.dtype, q.device
     tensors = (q.data_ptr(), k.data_ptr() if k.numel() else None,
                v.data_ptr() if v.numel() else None)
+    name, relation = "tgx_paged_attn", ()
+    if view is not None:
+        name, relation = "tgx_paged_attn_view", (ctypes.byref(view),)
 
-    def launch(keep=(q, k, v)):
+    def launch(keep=(q, _carrier(fields[0]), _carrier(fields[1])), rows=(k, v)):
         if carries_tangent(*keep):
             raise NotImplementedError("paged attention has no forward-mode derivative")
         out = torch.empty(shape, dtype=dtype, device=device)
         work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-        _native.launch(out, "tgx_paged_attn", state.native(), *tensors, strides, scale,
+        _native.launch(out, name, state.native(), *relation, *tensors, strides, scale,
                        out.data_ptr(), heads, group, D, code,
                        work.data_ptr() if need else None, need)
         return out
@@ -142,6 +194,9 @@ def _on_torch_operations(name: str, t: torch.Tensor) -> bool:
 
 def append(graph, key_cache, key, value_cache, value, page_sums) -> None:
     state = graph.paged_state
+    if isinstance(key_cache, BlockScaled):
+        _append_scaled(state, key_cache, key, value_cache, value, page_sums)
+        return
     if _on_torch_operations("append", key_cache):
         _append_torch(state, key_cache, key, value_cache, value, page_sums)
         return
@@ -186,6 +241,143 @@ def _append_torch(state, key_cache, key, value_cache, value, page_sums) -> None:
     rows = key_cache.view(state.num_pages, size, *key_cache.shape[1:])[ids].float()
     inside = torch.arange(size, device=length.device) < held[:, None]
     page_sums[ids] = torch.where(inside[..., None, None], rows, 0.0).sum(1)
+
+
+# ---------------------------------------------------------------------------
+# Caches in 8 bits
+
+def _scaled_on_torch_operations(name: str, width: int, caches) -> bool:
+    """Whether caches of this width run on Torch operations, which strict
+    mode refuses on the GPU."""
+    if not caches[0].device.type == "cuda":
+        return True
+    if width % 8 == 0 and 0 < width <= 512 and cache_rows_ok(*caches):
+        return False
+    from .message_passing import config
+
+    if config.strict:
+        raise RuntimeError(f"{name}: no HIP kernel covers 8-bit rows of {width} values (multiples "
+                           "of 8 up to 512, on 8 bytes) and tiga.config.strict is set")
+    return True
+
+
+def _step(t: torch.Tensor, dim: int) -> int:
+    """A stride; 0 for a dimension of one element, whose stride may be any."""
+    return t.stride(dim) if t.shape[dim] > 1 else 0
+
+
+def _append_scaled(state, key_cache, key, value_cache, value, page_sums) -> None:
+    if carries_tangent(key, value, page_sums, key_cache.scales, value_cache.scales):
+        raise NotImplementedError("append has no forward-mode derivative: detach its operands")
+    rows, heads, D = key.shape
+    written = (key_cache.codes, key_cache.scales, value_cache.codes, value_cache.scales)
+    if _scaled_on_torch_operations("append", D, (key_cache, value_cache)):
+        for cache, new in ((key_cache, key), (value_cache, value)):
+            _append_scaled_torch(state, cache, new)
+        if page_sums is not None:
+            _sum_scaled_torch(state, key_cache, page_sums)
+        return
+    if rows * heads * D == 0 or key_cache.shape[0] == 0:
+        return
+    key, value = _on_16_bytes(key), _on_16_bytes(value)
+    k, v = key_cache.codes, value_cache.codes
+    strides = (ctypes.c_int64 * 8)(_step(k, 0), _step(k, 1), _step(key, 0), _step(key, 1),
+                                   _step(v, 0), _step(v, 1), _step(value, 0), _step(value, 1))
+    _native.launch(key, "tgx_paged_append_scaled", state.native(), k.data_ptr(),
+                   key_cache.scales.data_ptr(), key.data_ptr(), v.data_ptr(),
+                   value_cache.scales.data_ptr(), value.data_ptr(), strides,
+                   _native.ptr(page_sums), heads, D, DTYPES[key.dtype], CODES[k.dtype],
+                   key_cache.block)
+    torch.autograd.graph.increment_version(
+        written if page_sums is None else (*written, page_sums))
+
+
+def _positions(state, first, count: int, size: int):
+    """(slots, named) [sequences, count, size] of the positions of `count` runs of
+    `size` from run first[b] of each sequence on; named: cached, on a page that
+    exists."""
+    at = (first[:, None] + torch.arange(count, device=first.device)) * size
+    at = at[..., None] + torch.arange(size, device=first.device)
+    page = (at // state.page_size).clamp(max=state.page_table.shape[1] - 1)
+    ids = state.page_table.long().gather(1, page.flatten(1)).view(at.shape)
+    named = (at < state.clamped_lengths()[:, None, None]) & (ids >= 0) & (ids < state.num_pages)
+    return torch.where(named, ids * state.page_size + at % state.page_size, 0), named, at
+
+
+def _append_scaled_torch(state, cache, new) -> None:
+    if state.page_table.numel() == 0 or state.num_pages == 0 or new.numel() == 0:
+        return
+    queries, block, dtype = state.queries, cache.block, cache.dtype
+    length = state.clamped_lengths()
+    fresh = (length - queries).clamp(min=0)
+    slots, named, at = _positions(state, fresh // block, (queries - 1) // block + 2, block)
+    row = at - length[:, None, None] + queries + \
+        torch.arange(length.numel(), device=length.device)[:, None, None] * queries
+    is_new = named & (at >= fresh[:, None, None])
+    x = torch.where(is_new[..., None, None], new[torch.where(is_new, row, 0)].float(), 0.0)
+    # (amax of a NaN is a NaN.)
+    scale = scale_of(x.abs().amax((2, 4)), dtype)                  # [sequences, blocks, heads]
+    blocks = slots[:, :, 0] // block
+    held = cache.scales[blocks]
+    begun = (named[:, :, 0] & ~is_new[:, :, 0])[..., None]
+    scale = torch.where(begun, torch.maximum(scale, held), scale)
+    raw = cache.codes.view(torch.int8)
+    codes = raw[slots].view(dtype).float()
+    # (By a NaN: codes whose values are NaN in any case.)
+    ratio = torch.where(begun, torch.nan_to_num(held / scale, nan=1.0), 1.0)
+    got = torch.where(is_new[..., None, None], x / scale[:, :, None, :, None],
+                      codes * ratio[:, :, None, :, None])
+    raw[slots[named]] = encode(got, dtype).view(torch.int8)[named]
+    touched = is_new.any(-1)
+    cache.scales[blocks[touched]] = scale[touched]
+
+
+def _sum_scaled_torch(state, cache, page_sums) -> None:
+    if state.page_table.numel() == 0 or state.num_pages == 0:
+        return
+    size = state.page_size
+    fresh = (state.clamped_lengths() - state.queries).clamp(min=0)
+    slots, named, at = _positions(state, fresh // size, (state.queries - 1) // size + 2, size)
+    rows = cache.codes.view(torch.int8)[slots].view(cache.dtype).float() * \
+        cache.scales[slots // cache.block][..., None]
+    total = torch.where(named[..., None, None], rows, 0.0).sum(2)
+    touched = (named & (at >= fresh[:, None, None])).any(-1)
+    page_sums[(slots[:, :, 0] // size)[touched]] = total[touched]
+
+
+def read(graph, key_cache, value_cache, dtype) -> tuple[torch.Tensor, torch.Tensor]:
+    state = graph.paged_state
+    rows, (heads, D) = graph.schema.num_dst, key_cache.shape[1:]
+    if carries_tangent(key_cache.scales, value_cache.scales):
+        raise NotImplementedError("read has no forward-mode derivative: detach the scales")
+    if _scaled_on_torch_operations("read", D, (key_cache, value_cache)):
+        return tuple(_read_torch(state, c, dtype) for c in (key_cache, value_cache))
+    key = torch.empty(rows, heads, D, dtype=dtype, device=graph.device)
+    value = torch.empty_like(key)
+    if key.numel() == 0:
+        return key, value
+    k, v = key_cache.codes, value_cache.codes
+    strides = (ctypes.c_int64 * 4)(_step(k, 0), _step(k, 1), _step(v, 0), _step(v, 1))
+    _native.launch(key, "tgx_paged_read", state.native(), k.data_ptr() or None,
+                   key_cache.scales.data_ptr() or None, v.data_ptr() or None,
+                   value_cache.scales.data_ptr() or None, strides, key.data_ptr(),
+                   value.data_ptr(), heads, D, DTYPES[dtype], CODES[k.dtype], key_cache.block)
+    return key, value
+
+
+def _read_torch(state, cache, dtype) -> torch.Tensor:
+    heads, D = cache.shape[1:]
+    rows = state.page_table.shape[0] * state.queries
+    if state.page_table.numel() == 0 or state.num_pages == 0:
+        return torch.zeros(rows, heads, D, dtype=dtype, device=state.lengths.device)
+    length = state.clamped_lengths()
+    at = length[:, None] - state.queries + torch.arange(state.queries, device=length.device)
+    ids = state.page_table.long().gather(1, at.clamp(min=0) // state.page_size)
+    named = (at >= 0) & (ids >= 0) & (ids < state.num_pages)
+    slots = torch.where(named, ids * state.page_size + at % state.page_size, 0).flatten()
+    got = cache.codes.view(torch.int8)[slots].view(cache.dtype).float() * \
+        cache.scales[slots // cache.block][..., None]
+    return torch.where(named.flatten()[:, None, None], got, 0.0).to(dtype)
 
 
 # ---------------------------------------------------------------------------
@@ -262,7 +454,8 @@ def csr(state):
     ids = table[:, :, position // size]                           # [sequences, heads, positions]
     there = (ids >= 0) & (ids < state.num_pages)
     column = (ids * size + position % size) * heads + torch.arange(heads, device=device)[:, None]
-    edge = there[:, None] & (position < limit[:, :, None, None])  # [.., queries, heads, ..]
+    # [sequences, queries, heads, positions]
+    edge = there[:, None] & state.sees(position, limit[:, :, None, None])
     row_ptr = torch.zeros(limit.numel() * heads + 1, dtype=torch.int64, device=device)
     torch.cumsum(edge.sum(-1).reshape(-1), 0, out=row_ptr[1:])
     return row_ptr, column[:, None].expand(edge.shape)[edge]

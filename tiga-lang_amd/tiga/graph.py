@@ -21,6 +21,7 @@ from typing import Literal
 import torch
 
 from . import _native
+from .blockscaled import BlockScaled
 
 _INDEX_DTYPES = (torch.int32, torch.int64)
 
@@ -28,6 +29,9 @@ _INDEX_DTYPES = (torch.int32, torch.int64)
 # split into CHUNK_EDGES-edge chunks whose partial states are merged.
 WAVE_MAX = 512
 CHUNK_EDGES = 512
+
+# Types of the rows that a cache in 8 bits is written from and read to.
+_SCALED_FROM = (torch.bfloat16, torch.float16, torch.float32)
 
 
 @dataclass(frozen=True)
@@ -60,6 +64,8 @@ class PagedState:
     page_size: int
     num_pages: int
     queries: int
+    window: int | None = None  # newest positions a token sees; None: all
+    sinks: int = 0             # and first positions, beside a window
 
     def __post_init__(self):
         t = self.page_table
@@ -89,6 +95,13 @@ class PagedState:
         """Positions each query row sees, int64 [sequences, queries]."""
         back = torch.arange(self.queries - 1, -1, -1, device=self.lengths.device)
         return (self.clamped_lengths()[:, None] - back).clamp(min=0)
+
+    def sees(self, position: torch.Tensor, limit: torch.Tensor) -> torch.Tensor:
+        """Whether a query row of `limit` positions sees `position`."""
+        seen = position < limit
+        if self.window is None:
+            return seen
+        return seen & ((position >= limit - self.window) | (position < self.sinks))
 
 
 def _paged():
@@ -296,6 +309,8 @@ class Graph:
         self._causal = causal
         # Implicit dense relations: None (every pair) or "lower_inclusive".
         self._dense_boundary = None
+        # (window, sinks) of a causal relation that looks back so far only.
+        self._window: tuple[int, int] | None = None
         self.paged_state: PagedState | None = None
         self._device = torch.device(device) if device is not None else None
         self._destination_index_cache = None
@@ -407,16 +422,27 @@ class Graph:
         return cls.from_csr(row_ptr, col_idx, num_src=num_nodes)
 
     @classmethod
-    def cu_seqlens(cls, cu_seqlens: torch.Tensor, *, causal: bool = True) -> "Graph":
+    def cu_seqlens(cls, cu_seqlens: torch.Tensor, *, causal: bool = True,
+                   window: int | None = None, sinks: int = 0) -> "Graph":
         """Block-diagonal packed varlen relation; kept implicit until needed.
 
         Row i of sequence k relates to sources [s_k, i] (causal) or
         [s_k, s_{k+1}) — the reference materializes this CSR at construction;
         here it is materialized only if an edge function needs the CSR.
+
+        With `window` (causal relations) row i relates to the last `window` of
+        those sources, itself among them, and to the sequence's first `sinks`.
+        Dot-product attention over it runs in tiles that read only what is
+        seen, with gradients: bf16 and fp16, widths 32, 64 and 128, query heads
+        grouped on key heads if the fields broadcast (query [tokens, heads, group,
+        D] on key and value [tokens, heads, 1, D]).
         """
         cls._validate_index_tensor("cu_seqlens", cu_seqlens)
         if not isinstance(causal, bool):
             raise TypeError("causal must be bool")
+        limits = cls._validate_window(window, sinks)
+        if limits is not None and not causal:
+            raise ValueError("a window needs a causal relation")
         if cu_seqlens.numel() == 0 or int(cu_seqlens[0].item()) != 0:
             raise ValueError("cu_seqlens must start at zero")
         if bool(torch.any(cu_seqlens[1:] < cu_seqlens[:-1]).item()):
@@ -424,7 +450,24 @@ class Graph:
         total = int(cu_seqlens[-1].item())
         schema = GraphSchema(num_src=total, num_dst=total, origin="cu_seqlens",
                              realization="implicit_varlen", index_dtype=cu_seqlens.dtype)
-        return cls(schema, cu_seqlens=cu_seqlens, causal=causal, device=cu_seqlens.device)
+        graph = cls(schema, cu_seqlens=cu_seqlens, causal=causal, device=cu_seqlens.device)
+        graph._window = limits
+        return graph
+
+    @staticmethod
+    def _validate_window(window, sinks) -> tuple[int, int] | None:
+        for name, value, least in (("window", window, 1), ("sinks", sinks, 0)):
+            if name == "window" and value is None:
+                continue
+            if not isinstance(value, int) or isinstance(value, bool) or \
+                    not least <= value < 2**31:
+                raise ValueError(f"{name} must be an integer from {least} to 2**31 - 1")
+        if window is None:
+            if sinks:
+                raise ValueError("sinks are the tokens that stay visible beside a window: give "
+                                 "window as well")
+            return None
+        return window, sinks
 
     @classmethod
     def dense(cls, num_src: int, num_dst: int | None = None, *, device=None,
@@ -449,19 +492,23 @@ class Graph:
 
     @classmethod
     def triangular(cls, num_entities: int, *, device=None,
-                   index_dtype: torch.dtype = torch.int64) -> "Graph":
+                   index_dtype: torch.dtype = torch.int64, window: int | None = None,
+                   sinks: int = 0) -> "Graph":
         """Lower-inclusive dense relation: row i relates to sources 0..i
-        (reference graph.py:576-592)."""
+        (reference graph.py:576-592); with `window`, to the last `window` of them
+        and the first `sinks`, as in `cu_seqlens`."""
+        limits = cls._validate_window(window, sinks)
         graph = cls.dense(num_entities, num_entities, device=device, index_dtype=index_dtype)
         graph._schema = GraphSchema(num_src=num_entities, num_dst=num_entities,
                                     origin="lower_triangular", realization="implicit_dense",
                                     index_dtype=index_dtype)
         graph._dense_boundary = "lower_inclusive"
+        graph._window = limits
         return graph
 
     @classmethod
     def paged(cls, page_table: torch.Tensor, lengths: torch.Tensor, *, page_size: int,
-              num_pages: int, queries: int = 1,
+              num_pages: int, queries: int = 1, window: int | None = None, sinks: int = 0,
               validate: Literal["basic", "full"] = "basic") -> "Graph":
         """Relation of each sequence's newest tokens to the slots of a paged cache.
 
@@ -491,9 +538,20 @@ class Graph:
         two have gradients on Torch operations only (``tiga.config.strict`` refuses
         them), and forward mode is refused where a kernel would run.
 
+        With `window`, a token relates to the last `window` of its positions only,
+        its own among them, and to the first `sinks` of its sequence.  Pages that
+        lie between are not read, whatever their table entries hold; the kernels'
+        time goes by what is seen.  `append` and `read` are the same with a window
+        and without.
+
+        Key and value fields may be caches in 8 bits (``tiga.BlockScaled``, both of one
+        type and block): a code is exact in the tiles, its key's scale multiplies
+        the score and its value's the weight; the output has the query's type.
+
         A page_table [sequences, heads, pages] is a table for each head
         (`select_pages` returns such a relation): the rows are then
         ``(b * queries + t) * heads + h``, the sources ``slot * heads + h``."""
+        limits = cls._validate_window(window, sinks)
         for name, value in (("page_table", page_table), ("lengths", lengths)):
             if not isinstance(value, torch.Tensor):
                 raise TypeError(f"{name} must be a torch.Tensor")
@@ -519,7 +577,8 @@ class Graph:
         if max(num_pages * page_size, page_table.shape[-1] * page_size + 4096,
                page_table.shape[0] * queries, queries) >= 2**31:
             raise ValueError("a paged relation has fewer than 2**31 slots, positions and rows")
-        state = PagedState(page_table, lengths, page_size, num_pages, queries)
+        state = PagedState(page_table, lengths, page_size, num_pages, queries,
+                           *(limits or (None, 0)))
         if validate == "full":
             state_lengths = lengths.long()
             if bool(((state_lengths < 0) |
@@ -556,8 +615,9 @@ class Graph:
             raise ValueError(f"{method} needs one page table per sequence, not one per head")
         return self.paged_state
 
-    def append(self, key_cache: torch.Tensor, key: torch.Tensor, value_cache: torch.Tensor,
-               value: torch.Tensor, *, page_sums: torch.Tensor | None = None) -> None:
+    def append(self, key_cache: "torch.Tensor | BlockScaled", key: torch.Tensor,
+               value_cache: "torch.Tensor | BlockScaled", value: torch.Tensor, *,
+               page_sums: torch.Tensor | None = None) -> None:
         """Write the newest tokens' keys and values into their slots of the
         cache, in place.
 
@@ -571,14 +631,28 @@ class Graph:
         64-bit caches run on Torch operations (``tiga.config.strict`` refuses them
         on the GPU).
 
+        Caches in 8 bits (``tiga.BlockScaled``, both of one type and block, pages of
+        whole blocks) are written from bf16, fp16 or fp32 rows, for each block and
+        head by a power of two, with M = 448 (float8_e4m3fn) or 127 (int8):
+
+            s = the smallest power of two of at least 2^-126 with max |new| <= M s,
+                or the scale that the block's older tokens have, if that is more
+            code = new / s, rounded to nearest, ties to even
+
+        A block whose scale grows has its older tokens' codes rounded again by the new
+        one.  A NaN or an infinity among the new values makes the scale NaN until the
+        block is begun again, and every row of the block and head reads back as NaN.
+        Page sums are those of the rows as they are held.  Widths that are no
+        multiple of 8, or over 512, run on Torch operations.
+
         Each sequence's written pages must be its own and named once in its
         table (two writers of a slot leave either's row there), and key and
         value must not lie in the caches they are written to."""
         state = self.paged_state
         tensors = (key_cache, key, value_cache, value, page_sums)
         try:
-            spec = tuple([None if x is None else (x.dtype, x.shape, x.stride(), x.device)
-                          for x in tensors])
+            spec = tuple([None if x is None else x.spec if type(x) is BlockScaled else
+                          (x.dtype, x.shape, x.stride(), x.device) for x in tensors])
         except AttributeError:
             spec = None
         if state is None or spec is None or ("append", spec) not in state.checked:
@@ -593,6 +667,10 @@ class Graph:
         state = self._paged_only("append")
         rows, slots = self._schema.num_dst, self._schema.num_src
         tensors = {"key_cache": key_cache, "key": key, "value_cache": value_cache, "value": value}
+        scaled = isinstance(key_cache, BlockScaled) or isinstance(value_cache, BlockScaled)
+        if scaled:
+            self._check_scaled(key_cache, value_cache)
+            tensors["key_cache"], tensors["value_cache"] = key_cache.codes, value_cache.codes
         for name, t in tensors.items():
             if not isinstance(t, torch.Tensor):
                 raise TypeError(f"{name} must be a torch.Tensor")
@@ -601,7 +679,12 @@ class Graph:
             if t.ndim != 3 or tuple(t.shape) != (want, *key.shape[1:]):
                 raise ValueError(f"{name} must have shape [{want}, heads, D] like the others, "
                                  f"got {tuple(t.shape)}")
-            if t.dtype != key_cache.dtype or not t.is_floating_point():
+            if scaled and name.endswith("cache"):
+                pass
+            elif scaled and (t.dtype != key.dtype or t.dtype not in _SCALED_FROM):
+                raise TypeError("key and value must both be bfloat16, float16 or float32 for a "
+                                f"cache in 8 bits, {name} is {t.dtype}")
+            elif not scaled and (t.dtype != key_cache.dtype or not t.is_floating_point()):
                 raise TypeError("key_cache, key, value_cache and value must have one floating type")
             if t.device != self.device:
                 raise ValueError(f"{name} is on {t.device}, but graph is on {self.device}")
@@ -621,6 +704,55 @@ class Graph:
             if page_sums.device != self.device:
                 raise ValueError(f"page_sums is on {page_sums.device}, but graph is on "
                                  f"{self.device}")
+
+    def _check_scaled(self, key_cache, value_cache) -> None:
+        """Caches in 8 bits as append and read take them."""
+        for name, c in (("key_cache", key_cache), ("value_cache", value_cache)):
+            if not isinstance(c, BlockScaled):
+                raise TypeError(f"{name} must be a tiga.BlockScaled like the other cache")
+            if c.ndim != 3 or c.tables != 1:
+                raise ValueError(f"{name} must be [slots, heads, D]")
+        if key_cache.dtype != value_cache.dtype or key_cache.block != value_cache.block:
+            raise TypeError("key_cache and value_cache must have one code type and one block")
+        if self.paged_state.page_size % key_cache.block:
+            raise ValueError(f"pages of {self.paged_state.page_size} slots are no whole blocks of "
+                             f"{key_cache.block}")
+
+    def read(self, key_cache: BlockScaled, value_cache: BlockScaled, *,
+             dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
+        """The newest tokens' keys and values out of caches in 8 bits: two new
+        tensors [rows, heads, D] of this relation's destination rows (row
+        ``b * queries + t`` is position ``lengths[b] - queries + t``), each value the
+        code times its scale, rounded to `dtype` (bfloat16, float16 or float32).
+        A row whose position is negative, or whose page id names no page, is zero.
+        A relation with ``queries`` of the longest length reads whole sequences.
+        No gradients.  Widths that are no multiple of 8, or over 512, run on
+        Torch operations."""
+        state = self.paged_state
+        try:
+            spec = ("read", key_cache.spec, value_cache.spec, dtype)
+        except AttributeError:
+            spec = None
+        if state is None or spec is None or spec not in state.checked:
+            self._check_read(key_cache, value_cache, dtype)
+            state.checked[spec] = True
+        if torch.is_grad_enabled() and (key_cache.requires_grad or value_cache.requires_grad):
+            raise NotImplementedError("read has no gradient: detach the scales or run it under "
+                                      "torch.no_grad()")
+        return _paged().read(self, key_cache, value_cache, dtype)
+
+    def _check_read(self, key_cache, value_cache, dtype) -> None:
+        self._paged_only("read")
+        self._check_scaled(key_cache, value_cache)
+        if dtype not in _SCALED_FROM:
+            raise TypeError(f"dtype must be bfloat16, float16 or float32, got {dtype}")
+        slots = self._schema.num_src
+        for name, c in (("key_cache", key_cache), ("value_cache", value_cache)):
+            if tuple(c.shape) != (slots, *key_cache.shape[1:]):
+                raise ValueError(f"{name} must have shape [{slots}, heads, D] like the other, got "
+                                 f"{tuple(c.shape)}")
+            if c.device != self.device:
+                raise ValueError(f"{name} is on {c.device}, but graph is on {self.device}")
 
     def select_pages(self, query: torch.Tensor, page_sums: torch.Tensor, count: int, *,
                      out: "Graph | None" = None) -> "Graph":
@@ -672,6 +804,9 @@ class Graph:
 
     def _check_select(self, query, page_sums, count) -> None:
         state = self._paged_only("select_pages")
+        if state.window is not None:
+            raise ValueError("select_pages chooses among all pages of a sequence: it needs a "
+                             "relation without a window")
         if not isinstance(query, torch.Tensor) or not isinstance(page_sums, torch.Tensor):
             raise TypeError("query and page_sums must be torch.Tensor")
         if query.ndim not in (3, 4) or query.shape[0] != self._schema.num_dst or \
@@ -702,15 +837,18 @@ class Graph:
             raise ValueError("all blocks must share a device")
         # Causal (or all-pairs) square blocks stay implicit: their cat is one
         # cu_seqlens relation.
+        window, sinks = blocks[0]._window or (None, 0)
         for causal in (True, False):
-            if all(b._square_blocks(causal) is not None for b in blocks):
+            if all(b._square_blocks(causal) is not None and b._window == blocks[0]._window
+                   for b in blocks):
                 parts = [torch.zeros(1, dtype=torch.int64, device=device)]
                 offset = 0
                 for b in blocks:
                     cu = b._square_blocks(causal)
                     parts.append(cu[1:] + offset)
                     offset += int(cu[-1].item())
-                return cls.cu_seqlens(torch.cat(parts), causal=causal)
+                return cls.cu_seqlens(torch.cat(parts), causal=causal, window=window,
+                                      sinks=sinks)
         # Materialized blocks: every block's CSR shifted by the edges and
         # sources of the blocks before it; the block edge counts come back in
         # one host transfer.
@@ -775,8 +913,17 @@ class Graph:
             return torch.tensor([0, self._schema.num_dst], dtype=torch.int64, device=self.device)
         return None
 
+    def _window_lengths(self) -> torch.Tensor:
+        """Lengths (int64, on the host) of the sequences of an implicit relation
+        with a window, whose row i of a sequence has min(i + 1, window + sinks)
+        edges."""
+        cu = self._square_blocks(True).cpu()
+        return cu[1:] - cu[:-1]
+
     @property
     def num_edges(self) -> int:
+        if self._window is not None and self._row_ptr is None:
+            return self._degree_stats()[2]
         if self.is_dense and self._row_ptr is None:
             n = self._schema.num_dst
             if self._dense_boundary == "lower_inclusive":
@@ -795,6 +942,10 @@ class Graph:
         if self.is_paged:
             # As the tables stand now: never kept.
             return _paged().csr(self.paged_state)
+        if self._row_ptr is None and self._window is not None:
+            self._row_ptr, self._col_idx = _window_csr(self._square_blocks(True), *self._window,
+                                                       self._schema.index_dtype)
+            return self._row_ptr, self._col_idx
         if self._row_ptr is None and self.is_dense:
             # Only an edge function no tile covers gets here (eager path).
             dtype, dev = self._schema.index_dtype, self.device
@@ -878,7 +1029,12 @@ class Graph:
         if got is not None:
             return got
         n_dst, n_src = self._schema.num_dst, self._schema.num_src
-        if self.is_dense and self._row_ptr is None:
+        if self._window is not None and self._row_ptr is None:
+            most, lengths = sum(self._window), self._window_lengths()
+            short = lengths.clamp(max=most)
+            total = int((short * (short + 1) // 2 + (lengths - short) * most).sum())
+            got = (1, int(short.max()), total) if n_dst else (0, 0, 0)
+        elif self.is_dense and self._row_ptr is None:
             if self._dense_boundary == "lower_inclusive":
                 got = (1, n_dst, n_dst * (n_dst + 1) // 2) if n_dst else (0, 0, 0)
             else:
@@ -923,7 +1079,13 @@ class Graph:
         got = self._native_cache.get("histogram")
         if got is None:
             n_dst = self._schema.num_dst
-            if self.is_dense and self._row_ptr is None:
+            if self._window is not None and self._row_ptr is None:
+                counts = [0] * (maximum + 1)
+                for length in self._window_lengths().tolist():
+                    for d in range(1, min(length, maximum) + 1):
+                        counts[d] += 1
+                    counts[maximum] += max(0, length - maximum)
+            elif self.is_dense and self._row_ptr is None:
                 counts = [0] * (maximum + 1)
                 if self._dense_boundary == "lower_inclusive":
                     counts[1:] = [1] * maximum
@@ -986,11 +1148,13 @@ class Graph:
             # The sizes only: what the tables hold may change between calls.
             p = self.paged_state
             return (s.origin, s.realization, s.num_src, s.num_dst, str(s.index_dtype),
-                    str(self.device), tuple(p.page_table.shape), p.page_size, p.queries)
+                    str(self.device), tuple(p.page_table.shape), p.page_size, p.queries,
+                    *(() if p.window is None else (p.window, p.sinks)))
         locality = (self.source_index_span_ratio()
                     if self._row_ptr is not None else "implicit")
         return (s.origin, s.realization, s.num_src, s.num_dst, str(s.index_dtype),
-                str(self.device), self.degree_statistics(), locality, self._dense_boundary)
+                str(self.device), self.degree_statistics(), locality, self._dense_boundary,
+                *(self._window or ()))
 
     def _reference_plan_remarks(self, has_node_epilogue: bool = False) -> tuple[str, ...]:
         """The reference planner's decision for this CSR
@@ -1166,6 +1330,35 @@ class Graph:
                 self._native_cache[key] = None
         return self._native_cache[key]
 
+    def _window_tasks(self, kind: int, heads: int, group: int):
+        """(cu_seqlens on the device, tasks, count, partial sums) for attention over
+        this relation's window; kind 0 = query tiles, 1 = key tiles, 2 = the key tiles
+        joined from partial sums (tgx_window_tasks)."""
+        key = ("window", kind, heads, group)
+        got = self._native_cache.get(key)
+        if got is None:
+            import numpy as np
+
+            cu = self._native_cache.get("window-cu")
+            if cu is None:
+                host = (self._cu_seqlens.cpu().numpy() if self.is_varlen
+                        else np.array([0, self._schema.num_dst]))
+                if host[-1] >= 2**31:
+                    raise ValueError("the HIP attention tiles support fewer than 2**31 tokens")
+                host = np.ascontiguousarray(host, dtype=np.int32)
+                cu = host, torch.as_tensor(host, device=self.device)
+                self._native_cache["window-cu"] = cu
+            host, device_cu = cu
+            n, slots = ctypes.c_int64(), ctypes.c_int64()
+            args = (host.ctypes.data, host.size - 1, heads, group, *self._window, kind)
+            _native.call("tgx_window_tasks", *args, None, ctypes.byref(n), ctypes.byref(slots))
+            tasks = np.zeros((4 if kind == 0 else 8) * max(n.value, 1), dtype=np.int32)
+            _native.call("tgx_window_tasks", *args, tasks.ctypes.data, ctypes.byref(n),
+                         ctypes.byref(slots))
+            got = (device_cu, torch.as_tensor(tasks, device=self.device), n.value, slots.value)
+            self._native_cache[key] = got
+        return got
+
     def _row_plan(self, wave_max: int = WAVE_MAX, chunk_edges: int = CHUNK_EDGES) -> RowPlanHandle:
         key = ("plan", wave_max, chunk_edges)
         handle = self._native_cache.get(key)
@@ -1219,6 +1412,27 @@ def _varlen_csr(cu_seqlens: torch.Tensor, causal: bool):
         torch.cumsum(torch.cat(degrees), 0, out=row_ptr[1:])
     col_idx = torch.cat(columns) if columns else torch.zeros(0, device=device, dtype=dtype)
     return row_ptr, col_idx
+
+
+def _window_csr(cu_seqlens: torch.Tensor, window: int, sinks: int, dtype: torch.dtype):
+    """The causal relation of `cu_seqlens` whose row i of a sequence reads the
+    columns [0, min(sinks, i + 1 - window)) and [max(0, i + 1 - window), i] of it."""
+    device = cu_seqlens.device
+    total = int(cu_seqlens[-1].item())
+    start = torch.repeat_interleave(cu_seqlens[:-1], cu_seqlens[1:] - cu_seqlens[:-1],
+                                    output_size=total)
+    i = torch.arange(total, device=device) - start
+    degree = (i + 1).clamp(max=window + sinks)
+    row_ptr = torch.zeros(total + 1, dtype=torch.int64, device=device)
+    torch.cumsum(degree, 0, out=row_ptr[1:])
+    n_edges = int(row_ptr[-1].item())
+    row = torch.repeat_interleave(torch.arange(total, device=device), degree,
+                                  output_size=n_edges)
+    at = torch.arange(n_edges, device=device) - row_ptr[row]
+    behind = (i + 1 - window).clamp(min=0)[row]
+    first = behind.clamp(max=sinks)
+    col = start[row] + torch.where(at < first, at, at - first + behind)
+    return row_ptr.to(dtype), col.to(dtype)
 
 
 __all__ = ["Graph", "GraphSchema", "PagedState", "build_coo_csr", "build_row_plan", "build_transpose",

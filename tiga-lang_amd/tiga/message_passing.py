@@ -48,6 +48,7 @@ import torch
 
 from . import _eager, _native
 from . import capture as cap
+from .blockscaled import BlockScaled
 from .graph import Graph
 from .kernel import CompiledVariant, Kernel
 from .reducer import OnlineSoftmaxReducer, SumReducer
@@ -94,8 +95,20 @@ def _resolve_node_fields(graph, src, dst, ndata):
     return src, dst
 
 
-def _spec(t: torch.Tensor) -> tuple:
+def _spec(t: "torch.Tensor | BlockScaled") -> tuple:
+    if type(t) is BlockScaled:
+        return t.spec
     return (t.dtype, t.shape, t.stride(), t.device)
+
+
+def _dequantized(src, dst) -> dict:
+    """Source fields with caches in 8 bits as their values, in fp32 or the
+    widest type of the destination fields if that is wider."""
+    wide = torch.float32
+    for t in dst.values():
+        if t.is_floating_point():
+            wide = torch.promote_types(wide, t.dtype)
+    return {n: v.dequantize(wide) if isinstance(v, BlockScaled) else v for n, v in src.items()}
 
 
 def _param_signature(params: Mapping[str, Any]) -> tuple:
@@ -242,7 +255,7 @@ class _Guarded:
         except (KeyError, TypeError):
             return _MISS
         for t, spec in zip(operands, self.specs):
-            if not isinstance(t, torch.Tensor) or _spec(t) != spec:
+            if not isinstance(t, (torch.Tensor, BlockScaled)) or _spec(t) != spec:
                 return _MISS
         if launch.aliases:
             groups = {"src": src, "dst": dst, "edge": edge, "param": params}
@@ -276,11 +289,15 @@ class MessagePassing(Kernel):
 
     # ------------------------------------------------------------------
     @staticmethod
-    def _validate_fields(role: str, fields, entity_count: int, device) -> None:
+    def _validate_fields(role: str, fields, entity_count: int, device, scaled=False) -> None:
         if not isinstance(fields, Mapping):
             raise TypeError(f"{role} fields must be a mapping")
         for name, value in fields.items():
-            if not isinstance(value, torch.Tensor):
+            if isinstance(value, BlockScaled):
+                if not scaled:
+                    raise TypeError(f"{role}.{name}: a cache in 8 bits (tiga.BlockScaled) is a "
+                                    "source field of a paged relation (Graph.paged)")
+            elif not isinstance(value, torch.Tensor):
                 raise TypeError(f"{role}.{name} must be a torch.Tensor")
             if value.ndim == 0 or value.shape[0] != entity_count:
                 raise ValueError(
@@ -317,7 +334,7 @@ class MessagePassing(Kernel):
     def _dispatch(self, graph, src, dst, edge, params):
         """The cold path: validate, capture, recognize, run."""
         device = graph.device
-        self._validate_fields("src", src, graph.schema.num_src, device)
+        self._validate_fields("src", src, graph.schema.num_src, device, graph.is_paged)
         self._validate_fields("dst", dst, graph.schema.num_dst, device)
         if edge:
             # Before any launch: a kernel would dereference a host pointer
@@ -338,7 +355,12 @@ class MessagePassing(Kernel):
             if launch is None:
                 # The relation as its tables stand, for everything the paged
                 # attention does not cover.
-                return self._dispatch(graph.snapshot(), src, dst, edge, params)
+                if not any(isinstance(t, BlockScaled) for t in src.values()):
+                    return self._dispatch(graph.snapshot(), src, dst, edge, params)
+                out = self._dispatch(graph.snapshot(), _dequantized(src, dst), dst, edge, params)
+                dot = cap.recognize_dot(captured)
+                # (Attention has the query's type, as the kernels' has.)
+                return out if dot is None else out.to(dst[dot.q_field].dtype)
         elif device.type == "cuda" and captured is not None:
             launch = self._plan_native(captured, graph, src, dst, edge, params)
         elif captured is not None:
@@ -481,10 +503,11 @@ class MessagePassing(Kernel):
         src, dst = _resolve_node_fields(graph, src, dst, ndata)
         edge = {} if edge is None else edge
         device = graph.device
-        self._validate_fields("src", src, graph.schema.num_src, device)
+        self._validate_fields("src", src, graph.schema.num_src, device, graph.is_paged)
         self._validate_fields("dst", dst, graph.schema.num_dst, device)
         if edge:
             self._validate_fields("edge", edge, graph.num_edges, device)
+        src = _dequantized(src, dst)
         aggregate = _eager.evaluate(self, graph, src, dst, edge, params)
         return self._epilogue(dst, aggregate, params)
 
@@ -825,6 +848,8 @@ class MessagePassing(Kernel):
         q, k, v = dst.get(dot.q_field), src.get(dot.k_field), src.get(dot.v_field)
         if q is None or k is None or v is None:
             return None
+        if graph._window is not None:
+            return self._plan_window(dot, graph, q, k, v)
         if q.ndim != 3 or k.shape[1:] != q.shape[1:] or v.shape[1:] != q.shape[1:]:
             return None
         if graph.is_varlen or graph.is_dense:
@@ -881,16 +906,22 @@ class MessagePassing(Kernel):
         q, k, v = dst.get(dot.q_field), src.get(dot.k_field), src.get(dot.v_field)
         if q is None or k is None or v is None:
             return None
-        got = _paged.heads_of(q, k, v)
-        if got is None or not (q.dtype == k.dtype == v.dtype) or q.dtype not in _paged.DTYPES:
+        got, kind = _paged.heads_of(q, k, v), _paged.cache_kind(k, v)
+        if got is None or kind is None or q.dtype not in _paged.DTYPES:
+            return None
+        scaled = kind[0] != 0
+        if scaled and (k.tables != graph.paged_state.table_heads):
+            return None
+        if not scaled and not (q.dtype == k.dtype == v.dtype):
             return None
         heads, group = got
         D = q.shape[-1]
         if D % 8 or not 8 <= D <= 512 or not heads or not group:
             return None
-        if not (_paged.rows_on_16_bytes(k) and _paged.rows_on_16_bytes(v)):
+        if not _paged.cache_rows_ok(k, v):
             return None     # (a copy of the whole cache would be made each call)
-        if _paged.attention_workspace(graph, heads, group, D, _paged.DTYPES[q.dtype]) is None:
+        if _paged.attention_workspace(graph, k, v, heads, group, D,
+                                      _paged.DTYPES[q.dtype]) is None:
             return None
         scale = dot.scale
 
@@ -900,11 +931,17 @@ class MessagePassing(Kernel):
             return _paged.bind_attention(graph, q, k, v, scale, heads, group)()
 
         def bind(q, k, v):
-            if any(t.data_ptr() % 16 for t in (q, k, v)) or not _paged.rows_on_16_bytes(q):
+            if any(t.data_ptr() % 16 for t in ((q,) if scaled else (q, k, v))) or \
+                    not _paged.rows_on_16_bytes(q):
                 return None     # the launch reads a copy, which would not stay live
             return _paged.bind_attention(graph, q, k, v, scale, heads, group)
 
         kind = str(q.dtype).split(".")[-1]
+        window, sinks = graph.paged_state.window, graph.paged_state.sinks
+        over = (f", {str(k.dtype).split('.')[-1]} codes by a scale for {k.block} slots and head"
+                if scaled else "") + \
+            (f", the last {window} and first {sinks} positions" if window is not None else "")
+        entry = "tgx_paged_attn" if window is None and not scaled else "tgx_paged_attn_view"
         derivative = _paged.wants_derivative(q, k, v)
 
         # (As csrc/tgx_paged.hip chooses its kernel.)
@@ -914,10 +951,10 @@ class MessagePassing(Kernel):
         def describe():
             if not derivative:
                 return self._variant(
-                    graph, "paged-attention", ("tgx_paged_attn",),
+                    graph, "paged-attention", (entry,),
                     f"{kind} rows of the cache read {reads} through the page tables, {group} query "
-                    f"heads on each of {heads} key heads, fp32 online softmax; long sequences in "
-                    "pieces, joined in order; gradients on the relation's snapshot")
+                    f"heads on each of {heads} key heads, fp32 online softmax{over}; long "
+                    "sequences in pieces, joined in order; gradients on the relation's snapshot")
             if not _paged.csr_takes(D):
                 return self._eager_variant(graph)
             return self._variant(
@@ -937,6 +974,11 @@ class MessagePassing(Kernel):
         width, else on Torch operations in fp32."""
         from . import _ops, _paged
 
+        if isinstance(k, BlockScaled):
+            # (The codes' values in fp32, whose gradient goes to the scales.)
+            out = self._paged_with_gradients(dot, graph, q.float(), k.dequantize(),
+                                             v.dequantize(), params)
+            return out.to(q.dtype)
         snapshot = graph.snapshot()
         D = q.shape[-1]
         if _paged.csr_takes(D) and snapshot.num_edges:
@@ -949,6 +991,36 @@ class MessagePassing(Kernel):
         fields = {dot.k_field: k.float(), dot.v_field: v.float()}
         out = _eager.evaluate(self, snapshot, fields, {dot.q_field: q.float()}, {}, params)
         return out.to(q.dtype)
+
+    def _plan_window(self, dot, graph, q, k, v) -> _Launch | None:
+        """Dot-product attention over Graph.cu_seqlens / triangular with a
+        window: bf16 and fp16 fields of one type, widths 32, 64 and 128, query
+        heads grouped on key heads."""
+        from . import _ops, _paged
+
+        if dot.bias_field is not None or self.reducer.block_prune_threshold is not None:
+            return None
+        got = _paged.heads_of(q, k, v)
+        if got is None or not (q.dtype == k.dtype == v.dtype) or q.dtype not in _ops._ATTN_DTYPES:
+            return None
+        heads, group = got
+        if not heads or not 0 < group <= _ops.WINDOW_MAX_GROUP or q.shape[-1] not in (32, 64, 128):
+            return None
+        _native.lib()
+        scale = dot.scale
+
+        def run(q, k, v):
+            return _ops.window_attention(q, k, v, scale, heads, group, graph)
+
+        window, sinks = graph._window
+        describe = lambda: self._variant(
+            graph, "window-attention", ("tgx_window_attn_fwd", "tgx_window_attn_bwd"),
+            f"MFMA 16x16x32 {str(q.dtype).split('.')[-1]} tiles over the last {window} and first "
+            f"{sinks} positions of each sequence, {group} query heads on each of {heads} key "
+            "heads as rows of one tile; only key tiles that are seen are read; dK/dV of the "
+            "first positions in chunks of rows, joined in order; no atomics")
+        operands = (("dst", dot.q_field), ("src", dot.k_field), ("src", dot.v_field))
+        return _Launch(graph, operands, run, describe)
 
     def _plan_block_attention(self, dot, graph, q, k, v) -> _Launch | None:
         """Dot-product attention over Graph.cu_seqlens / dense / triangular
