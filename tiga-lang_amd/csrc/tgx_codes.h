@@ -77,26 +77,60 @@ __device__ __forceinline__ float block_scale(uint32_t amax) {
   return __uint_as_float(static_cast<uint32_t>((a == 0.f ? -126 : max(e, -126)) + 127) << 23);
 }
 
-// Eight values of at most M as codes, to the nearest, ties to even.
+// Eight values times `by`, products of at most M, as codes, to the nearest, ties to
+// even.  (The fused add of 1.5 * 2^23 leaves a product's nearest integer in the low
+// bits, rounded once.)
 template <int CODE>
-__device__ __forceinline__ u32x2 encode8(const float (&f)[8]) {
+__device__ __forceinline__ u32x2 encode8(const float (&f)[8], float by) {
   u32x2 w;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     if constexpr (CODE == TGX_CODE_E4M3) {
-      int v = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * k], f[4 * k + 1], 0, false);
-      v = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * k + 2], f[4 * k + 3], v, true);
+      int v = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * k] * by, f[4 * k + 1] * by, 0, false);
+      v = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * k + 2] * by, f[4 * k + 3] * by, v, true);
       w[k] = static_cast<uint32_t>(v);
     } else {
-      uint32_t v = 0;
+      uint32_t n[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        v |= (static_cast<uint32_t>(static_cast<int>(rintf(f[4 * k + i]))) & 0xFFu) << (8 * i);
-      w[k] = v;
+        n[i] = __float_as_uint(__builtin_fmaf(f[4 * k + i], by, 12582912.f));
+      w[k] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(n[3], n[2], 0x0C0C0400u),
+                                   __builtin_amdgcn_perm(n[1], n[0], 0x0C0C0400u), 0x05040100u);
     }
   }
   return w;
 }
+
+// The largest magnitude among values seen, as the bits of an fp32 number (a NaN's and
+// an infinity's are above all others).
+template <int DT>
+struct Magnitude {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  u16x2 top = {0, 0};
+  __device__ __forceinline__ void see(u32x4 raw) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, raw[i] & 0x7FFF7FFFu));
+  }
+  __device__ __forceinline__ uint32_t bits() const {
+    const uint32_t m = max(static_cast<uint32_t>(top[0]), static_cast<uint32_t>(top[1]));
+    if (DT == TGX_DTYPE_BF16) return m << 16;
+    return __float_as_uint(
+        static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(m))));
+  }
+};
+template <>
+struct Magnitude<TGX_DTYPE_F32> {
+  uint32_t top = 0;
+  __device__ __forceinline__ void see(const Vals<TGX_DTYPE_F32, 8>::Raw& raw) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      top = max(top, __float_as_uint(raw.lo[i]) & 0x7FFFFFFFu);
+      top = max(top, __float_as_uint(raw.hi[i]) & 0x7FFFFFFFu);
+    }
+  }
+  __device__ __forceinline__ uint32_t bits() const { return top; }
+};
 
 // How a cache's rows are held: as the queries' type (code 0), or as codes.
 template <int DT, int CODE>

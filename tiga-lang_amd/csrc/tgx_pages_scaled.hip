@@ -46,21 +46,29 @@ struct ScaledAppendArgs {
   int touched;           // pages a sequence's new tokens lie on at most
 };
 
-// One workgroup per (sequence, touched page, head), a wave per block of the page in
-// turn: LPR lanes hold a row, 8 values each, and 64 / LPR rows are taken at a time.
-// A block's new rows are read twice, the second time from the caches.
+// One workgroup per (sequence, touched page, head), two waves for the keys and two for
+// the values, which take the page's blocks in turn; of pages of one block, a
+// workgroup per two heads.  LPR lanes hold a row, 8 values each, and a wave takes 64 /
+// LPR rows at a time, kHold times of them in flight and kept until the scale is known
+// (of longer blocks the rest is read again, from the caches).
 // Bound: memory for prompts (16-bit rows read, codes written), latency for a single
 // token.
+constexpr int kHold = 4;
+
 template <int DT, int LPR, int CODE>
 __global__ __launch_bounds__(256) void append_scaled_kernel(ScaledAppendArgs a) {
   using V = Vals<DT, 8>;
   using T = typename V::T;
   constexpr int RPI = 64 / LPR;
-  __shared__ float part[4 * RPI][LPR * 8];
+  __shared__ float part[2][RPI][LPR * 8];
   const PagedRel& r = a.rel;
-  const int h = blockIdx.x % a.heads;
-  const int item = blockIdx.x / a.heads;
+  const bool pair = r.page_size == a.block;      // two heads a workgroup
+  const int groups = pair ? (a.heads + 1) / 2 : a.heads;
+  // A page's heads are workgroups 8 apart, on one XCD's L2: they write parts of its lines.
+  const int of8 = blockIdx.x / 8, group = of8 % groups;
+  const int item = of8 / groups * 8 + blockIdx.x % 8;
   const int b = item / a.touched;
+  if (b >= r.n_seqs) return;
   const int length = paged_length(r, b);
   const int fresh = min(length, r.queries);        // new tokens that exist
   const int page = (length - fresh) / r.page_size + item % a.touched;
@@ -74,81 +82,118 @@ __global__ __launch_bounds__(256) void append_scaled_kernel(ScaledAppendArgs a) 
   const int64_t slot0 = static_cast<int64_t>(id) * r.page_size;
   const int64_t row0 = static_cast<int64_t>(b) * r.queries + base - (length - r.queries);
   const int wave = uniform(threadIdx.x >> 6), lane = lane_id();
+  const int half = wave >> 1;
+  const bool keys = (wave & 1) == 0, sums = keys && a.sums;
+  const int h = pair ? group * 2 + half : group;
   const int sub = lane / LPR, d = lane % LPR * 8;
   const bool has = d < a.D;
   float sum[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) sum[i] = 0.f;
 
-  auto cache = [&](uint8_t* codes, int64_t c_slot, int64_t c_head, float* scales, const void* rows,
-                   int64_t x_row, int64_t x_head, bool keys) {
-    uint8_t* cb = codes + slot0 * c_slot + h * c_head + d;
-    const T* xb = static_cast<const T*>(rows) + row0 * x_row + h * x_head + d;
-    const int64_t scale0 = slot0 / a.block * a.heads + h;
-    const int first = keys && a.sums ? 0 : old / a.block;
-    for (int j = first + wave; j * a.block < held; j += 4) {
+  if (h < a.heads) {
+    const int64_t c_slot = keys ? a.kc_slot : a.vc_slot, x_row = keys ? a.k_row : a.v_row;
+    uint8_t* cb = (keys ? a.kc : a.vc) + slot0 * c_slot + h * (keys ? a.kc_head : a.vc_head) + d;
+    const T* xb = static_cast<const T*>(keys ? a.k : a.v) + row0 * x_row +
+                  h * (keys ? a.k_head : a.v_head) + d;
+    float* scales = (keys ? a.ks : a.vs) + slot0 / a.block * a.heads + h;
+    const int first = sums ? 0 : old / a.block, step = pair ? 1 : 2;
+    for (int j = pair ? first : first + ((first ^ half) & 1); j * a.block < held; j += step) {
       const int s0 = j * a.block, s1 = min(s0 + a.block, held);
       const int from = min(max(old, s0), s1);        // the block's first new slot
-      float* at = scales + scale0 + static_cast<int64_t>(j) * a.heads;
+      float* at = scales + static_cast<int64_t>(j) * a.heads;
       float scale = from > s0 ? *at : 0.f;
       const float before = scale;
+      // The lane's first new slot: slot s0 + sub + k RPI is always its own, so that
+      // sums are in one order however the rows came in.
+      const int begin = s0 + sub + (max(from - s0 - sub, 0) + RPI - 1) / RPI * RPI;
+      typename V::Raw x[kHold];
       if (from < s1) {
-        uint32_t top = 0;
-        for (int s = from + sub; s < s1; s += RPI) {
-          float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-          if (has) V::unpack(V::load(xb + s * x_row), f);
+        Magnitude<DT> top;
+        for (int s = begin + kHold * RPI; has && s < s1; s += RPI) top.see(V::load(xb + s * x_row));
 #pragma unroll
-          for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(f[i]) & 0x7FFFFFFFu);
-        }
-        const float need = block_scale<CODE>(wave_largest(top));
+        for (int u = 0; u < kHold; ++u)
+          x[u] = has && begin + u * RPI < s1 ? V::load(xb + (begin + u * RPI) * x_row)
+                                             : typename V::Raw{};
+#pragma unroll
+        for (int u = 0; u < kHold; ++u) top.see(x[u]);
+        const float need = block_scale<CODE>(wave_largest(top.bits()));
         // (Either one's NaN stays.)
         scale = from == s0 || !(need <= scale) ? (scale != scale ? scale : need) : scale;
         if (lane == 0) *at = scale;
       }
       const bool lost = scale != scale;
+      auto add = [&](u32x2 w) {
+        float f[8];
+        widen8<CODE>(w, f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum[i] += f[i] * scale;
+      };
+      // The older tokens, by the new scale.
       const bool again = from > s0 && from < s1 && scale != before && !lost;
-      const float ratio = again ? before / scale : 1.f;
-      for (int s = (keys && a.sums) || again ? s0 + sub : from + sub; s < s1; s += RPI) {
-        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        u32x2 w = {0u, 0u};
-        if (has) {
-          if (s < from) {
-            w = *reinterpret_cast<const u32x2*>(cb + s * c_slot);
-            if (again) {
-              widen8<CODE>(w, f);
-#pragma unroll
-              for (int i = 0; i < 8; ++i) f[i] *= ratio;
-              w = encode8<CODE>(f);
-            }
-          } else if (!lost) {
-            V::unpack(V::load(xb + s * x_row), f);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = f[i] / scale;
-            w = encode8<CODE>(f);
+      if ((sums || again) && has) {
+        const float ratio = again ? before / scale : 1.f;
+        for (int s = s0 + sub; s < from; s += RPI) {
+          u32x2 w = *reinterpret_cast<const u32x2*>(cb + s * c_slot);
+          if (again) {
+            float f[8];
+            widen8<CODE>(w, f);
+            w = encode8<CODE>(f, ratio);
+            *reinterpret_cast<u32x2*>(cb + s * c_slot) = w;
           }
-          if (s >= from || again) *reinterpret_cast<u32x2*>(cb + s * c_slot) = w;
-        }
-        if (keys && a.sums) {
-          widen8<CODE>(w, f);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) sum[i] += f[i] * scale;
+          if (sums) add(w);
         }
       }
-    }
-  };
-  cache(a.kc, a.kc_slot, a.kc_head, a.ks, a.k, a.k_row, a.k_head, true);
-  cache(a.vc, a.vc_slot, a.vc_head, a.vs, a.v, a.v_row, a.v_head, false);
-  if (!a.sums) return;
+      // By a power of two the quotient is a product; by a scale that the block had from
+      // elsewhere it is divided.
+      const bool power = (__float_as_uint(scale) & 0x7FFFFFu) == 0;
+      const float by = power ? 1.f / scale : 1.f;
+      auto put = [&](int s, const typename V::Raw& raw) {
+        u32x2 w = {0u, 0u};
+        if (!lost) {
+          float f[8];
+          V::unpack(raw, f);
+          if (!power) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) part[wave * RPI + sub][d + i] = sum[i];
+            for (int i = 0; i < 8; ++i) f[i] = f[i] / scale;
+          }
+          w = encode8<CODE>(f, by);
+        }
+        *reinterpret_cast<u32x2*>(cb + s * c_slot) = w;
+        if (sums) add(w);
+      };
+      if (from < s1 && has) {
+#pragma unroll
+        for (int u = 0; u < kHold; ++u)
+          if (begin + u * RPI < s1) put(begin + u * RPI, x[u]);
+        for (int s = begin + kHold * RPI; s < s1; s += RPI) put(s, V::load(xb + s * x_row));
+      }
+    }
+  }
+  if (!a.sums) return;
+  if (keys) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) part[half][sub][d + i] = sum[i];
+  }
   __syncthreads();
-  for (int c = threadIdx.x; c < a.D; c += 256) {
+  const int page_heads = pair ? 2 : 1;
+  for (int c = threadIdx.x; c < page_heads * a.D; c += 256) {
+    const int which = c / a.D, e = c % a.D;
+    const int head = pair ? group * 2 + which : h;
+    if (head >= a.heads) continue;
     float total = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4 * RPI; ++w) total += part[w][c];
-    a.sums[(static_cast<int64_t>(id) * a.heads + h) * a.D + c] = total;
+    for (int w = 0; w < RPI; ++w) total += part[which][w][e];
+    if (!pair) {
+#pragma unroll
+      for (int w = 0; w < RPI; ++w) total += part[1][w][e];
+    }
+    a.sums[(static_cast<int64_t>(id) * a.heads + head) * a.D + e] = total;
   }
 }
+
+constexpr unsigned kFewReads = 512;
+constexpr int64_t kPastCaches = int64_t{32} << 20;
 
 struct ScaledReadArgs {
   PagedRel rel;
@@ -161,32 +206,66 @@ struct ScaledReadArgs {
   int64_t rows;
 };
 
-// A thread per 8 values of a row; a row's chunks are consecutive threads.
+// A thread per 8 values of a row and kRead rows' parts at once, keys and values alike;
+// consecutive threads hold a row's consecutive parts.
 // Bound: memory (codes read, twice as many bytes written).
-template <int DT, int CODE>
+template <int DT, int CODE, int kRead, bool PAST>
 __global__ __launch_bounds__(256) void read_kernel(ScaledReadArgs a) {
   using V = Vals<DT, 8>;
   using T = typename V::T;
   const PagedRel& r = a.rel;
-  const unsigned chunks = a.heads * static_cast<unsigned>(a.D / 8);
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const int b = static_cast<int>(row / r.queries);
-    const int pos = paged_length(r, b) - r.queries + static_cast<int>(row % r.queries);
-    const int slot = pos < 0 ? -1 : paged_slot(r, r.table + b * r.seq_stride, pos);
-    for (unsigned c = threadIdx.x; c < chunks; c += 256) {
-      const int h = c / (a.D / 8), d = c % (a.D / 8) * 8;
+  const unsigned per_head = static_cast<unsigned>(a.D / 8), parts = a.heads * per_head;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * (256 * kRead) + threadIdx.x;
+  int64_t row[kRead];
+  unsigned part[kRead];
+  int slot[kRead];
 #pragma unroll
-      for (int which = 0; which < 2; ++which) {
-        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (slot >= 0) {
-          const u32x2 w = *reinterpret_cast<const u32x2*>(
-              a.codes[which] + slot * a.slot[which] + h * a.head[which] + d);
-          const float s = a.scales[which][static_cast<int64_t>(slot / a.block) * a.heads + h];
-          widen8<CODE>(w, f);
+  for (int u = 0; u < kRead; ++u) {
+    const int64_t i = first + 256 * u;
+    slot[u] = -1;
+    row[u] = a.rows;
+    if (i >= a.rows * parts) continue;
+    row[u] = i / parts;
+    part[u] = static_cast<unsigned>(i - row[u] * parts);
+    // (Rows are fewer than 2^31.)
+    const int b = static_cast<unsigned>(row[u]) / static_cast<unsigned>(r.queries);
+    const int pos = paged_length(r, b) - r.queries + (static_cast<int>(row[u]) - b * r.queries);
+    if (pos >= 0) slot[u] = paged_slot(r, r.table + b * r.seq_stride, pos);
+  }
+  u32x2 w[kRead][2];
+  float s[kRead][2];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] *= s;
-        }
-        V::store(static_cast<T*>(a.out[which]) + (row * a.heads + h) * a.D + d, f);
+  for (int u = 0; u < kRead; ++u) {
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      w[u][which] = u32x2{0u, 0u};
+      s[u][which] = 0.f;
+      if (slot[u] < 0) continue;
+      const int h = part[u] / per_head, d = part[u] % per_head * 8;
+      w[u][which] = *reinterpret_cast<const u32x2*>(a.codes[which] + slot[u] * a.slot[which] +
+                                                    h * a.head[which] + d);
+      s[u][which] = a.scales[which][static_cast<int64_t>(slot[u] / a.block) * a.heads + h];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kRead; ++u) {
+    if (row[u] >= a.rows) continue;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      float f[8];
+      widen8<CODE>(w[u][which], f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] *= s[u][which];
+      T* to = static_cast<T*>(a.out[which]) + (row[u] * parts + part[u]) * 8;
+      if constexpr (PAST && DT != TGX_DTYPE_F32) {
+        u32x4 x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          x[i] = DT == TGX_DTYPE_BF16 ? pack_bf16x2(f[2 * i], f[2 * i + 1])
+                                      : pack_f16x2(f[2 * i], f[2 * i + 1]);
+        __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(to));
+      } else {
+        V::store(to, f);
       }
     }
   }
@@ -245,7 +324,8 @@ extern "C" int tgx_paged_append_scaled(const tgx_paged* p, void* key_codes_dev,
   const int touched = static_cast<int>(
       std::min<int64_t>(p->pages_per_seq, (int64_t{p->queries} - 1) / p->page_size + 2));
   const int64_t blocks = p->n_seqs * touched;
-  if (blocks > kMaxBlocks256 / heads) {
+  const int groups = p->page_size == block ? (heads + 1) / 2 : heads;
+  if (blocks > kMaxBlocks256 / groups - 8) {
     set_error("append: too many sequences, pages and heads for one launch");
     return TGX_UNSUPPORTED;
   }
@@ -273,7 +353,7 @@ extern "C" int tgx_paged_append_scaled(const tgx_paged* p, void* key_codes_dev,
   TGX_PROFILE("append_scaled", s);
   with_types(dtype, code, [&](auto dt, auto cd) {
     constexpr int DT = decltype(dt)::value, CODE = decltype(cd)::value;
-    const dim3 grid(static_cast<uint32_t>(blocks * heads));
+    const dim3 grid(static_cast<uint32_t>(ceil_div(blocks, 8) * 8 * groups));
     if (D <= 64) append_scaled_kernel<DT, 8, CODE><<<grid, dim3(256), 0, s>>>(a);
     else if (D <= 128) append_scaled_kernel<DT, 16, CODE><<<grid, dim3(256), 0, s>>>(a);
     else append_scaled_kernel<DT, 64, CODE><<<grid, dim3(256), 0, s>>>(a);
@@ -313,12 +393,21 @@ extern "C" int tgx_paged_read(const tgx_paged* p, const void* key_codes_dev,
                    p->n_seqs * p->queries};
   // Without pages there is no slot to read, whatever the lengths say.
   if (p->num_pages == 0) a.rel.pages_per_seq = 0;
+  const int64_t parts = a.rows * heads * (D / 8);
+  if (ceil_div(parts, 1024) > kMaxBlocks256) {
+    set_error("read: too many rows for one launch");
+    return TGX_UNSUPPORTED;
+  }
   hipStream_t s = as_stream(stream);
   TGX_PROFILE("paged_read", s);
   with_types(dtype, code, [&](auto dt, auto cd) {
-    const int64_t grid = std::min<int64_t>(a.rows, 1 << 20);
-    read_kernel<decltype(dt)::value, decltype(cd)::value>
-        <<<dim3(static_cast<uint32_t>(grid)), dim3(256), 0, s>>>(a);
+    constexpr int DT = decltype(dt)::value, CODE = decltype(cd)::value;
+    const dim3 one(static_cast<uint32_t>(std::min(ceil_div(parts, 256), kMaxBlocks256)));
+    const dim3 four(static_cast<uint32_t>(ceil_div(parts, 1024)));
+    const bool past = 16 * parts * dtype_bytes(dtype) > kPastCaches;
+    if (four.x < kFewReads) read_kernel<DT, CODE, 1, false><<<one, dim3(256), 0, s>>>(a);
+    else if (past) read_kernel<DT, CODE, 4, true><<<four, dim3(256), 0, s>>>(a);
+    else read_kernel<DT, CODE, 4, false><<<four, dim3(256), 0, s>>>(a);
     return 0;
   });
   TGX_LAUNCHED("paged_read");

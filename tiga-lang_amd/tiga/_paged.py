@@ -82,8 +82,7 @@ def cache_rows_ok(k, v) -> bool:
     """Whether a launch can read these key and value fields in place."""
     if isinstance(k, BlockScaled):
         # (Codes are read by eights, or sixteens where the rows allow it.)
-        return all(t.codes.data_ptr() % 8 == 0 and all(
-            n <= 1 or s % 8 == 0 for n, s in zip(t.shape[:-1], t.codes.stride())) for t in (k, v))
+        return k.eights and v.eights and (k.codes.data_ptr() | v.codes.data_ptr()) % 8 == 0
     return rows_on_16_bytes(k) and rows_on_16_bytes(v)
 
 
@@ -192,10 +191,22 @@ def _on_torch_operations(name: str, t: torch.Tensor) -> bool:
     return True
 
 
-def append(graph, key_cache, key, value_cache, value, page_sums) -> None:
+def plan_append(key_cache, key, value_cache, value, page_sums):
+    """What append keeps for operands of some types, shapes and strides: for caches
+    in 8 bits the native arguments but for addresses, else True."""
+    if not isinstance(key_cache, BlockScaled):
+        return True
+    k, v, (_, heads, D) = key_cache.codes, value_cache.codes, key.shape
+    strides = (ctypes.c_int64 * 8)(_step(k, 0), _step(k, 1), _step(key, 0), _step(key, 1),
+                                   _step(v, 0), _step(v, 1), _step(value, 0), _step(value, 1))
+    return strides, rows_on_16_bytes(key) and rows_on_16_bytes(value), heads, D, \
+        DTYPES[key.dtype], CODES[k.dtype], key_cache.block
+
+
+def append(graph, key_cache, key, value_cache, value, page_sums, plan) -> None:
     state = graph.paged_state
-    if isinstance(key_cache, BlockScaled):
-        _append_scaled(state, key_cache, key, value_cache, value, page_sums)
+    if plan is not True:
+        _append_scaled(state, key_cache, key, value_cache, value, page_sums, plan)
         return
     if _on_torch_operations("append", key_cache):
         _append_torch(state, key_cache, key, value_cache, value, page_sums)
@@ -249,7 +260,7 @@ def _append_torch(state, key_cache, key, value_cache, value, page_sums) -> None:
 def _scaled_on_torch_operations(name: str, width: int, caches) -> bool:
     """Whether caches of this width run on Torch operations, which strict
     mode refuses on the GPU."""
-    if not caches[0].device.type == "cuda":
+    if not caches[0].codes.is_cuda:
         return True
     if width % 8 == 0 and 0 < width <= 512 and cache_rows_ok(*caches):
         return False
@@ -266,28 +277,30 @@ def _step(t: torch.Tensor, dim: int) -> int:
     return t.stride(dim) if t.shape[dim] > 1 else 0
 
 
-def _append_scaled(state, key_cache, key, value_cache, value, page_sums) -> None:
+def _append_scaled(state, key_cache, key, value_cache, value, page_sums, plan) -> None:
     if carries_tangent(key, value, page_sums, key_cache.scales, value_cache.scales):
         raise NotImplementedError("append has no forward-mode derivative: detach its operands")
-    rows, heads, D = key.shape
-    written = (key_cache.codes, key_cache.scales, value_cache.codes, value_cache.scales)
+    strides, dense, heads, D, dtype, code, block = plan
     if _scaled_on_torch_operations("append", D, (key_cache, value_cache)):
         for cache, new in ((key_cache, key), (value_cache, value)):
             _append_scaled_torch(state, cache, new)
         if page_sums is not None:
             _sum_scaled_torch(state, key_cache, page_sums)
         return
-    if rows * heads * D == 0 or key_cache.shape[0] == 0:
-        return
-    key, value = _on_16_bytes(key), _on_16_bytes(value)
     k, v = key_cache.codes, value_cache.codes
-    strides = (ctypes.c_int64 * 8)(_step(k, 0), _step(k, 1), _step(key, 0), _step(key, 1),
-                                   _step(v, 0), _step(v, 1), _step(value, 0), _step(value, 1))
+    if key.numel() == 0 or k.numel() == 0:
+        return
+    at = key.data_ptr(), value.data_ptr()
+    if not dense or (at[0] | at[1]) % 16:
+        key, value = _on_16_bytes(key), _on_16_bytes(value)
+        strides = plan_append(key_cache, key, value_cache, value, page_sums)[0]
+        at = key.data_ptr(), value.data_ptr()
     _native.launch(key, "tgx_paged_append_scaled", state.native(), k.data_ptr(),
-                   key_cache.scales.data_ptr(), key.data_ptr(), v.data_ptr(),
-                   value_cache.scales.data_ptr(), value.data_ptr(), strides,
-                   _native.ptr(page_sums), heads, D, DTYPES[key.dtype], CODES[k.dtype],
-                   key_cache.block)
+                   key_cache.scales.data_ptr(), at[0], v.data_ptr(),
+                   value_cache.scales.data_ptr(), at[1], strides,
+                   None if page_sums is None else page_sums.data_ptr(), heads, D, dtype, code,
+                   block)
+    written = (k, key_cache.scales, v, value_cache.scales)
     torch.autograd.graph.increment_version(
         written if page_sums is None else (*written, page_sums))
 
@@ -345,23 +358,29 @@ def _sum_scaled_torch(state, cache, page_sums) -> None:
     page_sums[(slots[:, :, 0] // size)[touched]] = total[touched]
 
 
-def read(graph, key_cache, value_cache, dtype) -> tuple[torch.Tensor, torch.Tensor]:
+def plan_read(graph, key_cache, value_cache, dtype):
+    """The native arguments of a read but for addresses."""
+    k, v, (heads, D) = key_cache.codes, value_cache.codes, key_cache.shape[1:]
+    strides = (ctypes.c_int64 * 4)(_step(k, 0), _step(k, 1), _step(v, 0), _step(v, 1))
+    return strides, (graph.schema.num_dst, heads, D), heads, D, DTYPES[dtype], CODES[k.dtype], \
+        key_cache.block
+
+
+def read(graph, key_cache, value_cache, dtype, plan) -> tuple[torch.Tensor, torch.Tensor]:
     state = graph.paged_state
-    rows, (heads, D) = graph.schema.num_dst, key_cache.shape[1:]
     if carries_tangent(key_cache.scales, value_cache.scales):
         raise NotImplementedError("read has no forward-mode derivative: detach the scales")
+    strides, shape, heads, D, out_type, code, block = plan
     if _scaled_on_torch_operations("read", D, (key_cache, value_cache)):
         return tuple(_read_torch(state, c, dtype) for c in (key_cache, value_cache))
-    key = torch.empty(rows, heads, D, dtype=dtype, device=graph.device)
-    value = torch.empty_like(key)
-    if key.numel() == 0:
-        return key, value
     k, v = key_cache.codes, value_cache.codes
-    strides = (ctypes.c_int64 * 4)(_step(k, 0), _step(k, 1), _step(v, 0), _step(v, 1))
-    _native.launch(key, "tgx_paged_read", state.native(), k.data_ptr() or None,
-                   key_cache.scales.data_ptr() or None, v.data_ptr() or None,
-                   value_cache.scales.data_ptr() or None, strides, key.data_ptr(),
-                   value.data_ptr(), heads, D, DTYPES[dtype], CODES[k.dtype], key_cache.block)
+    key = torch.empty(shape, dtype=dtype, device=k.device)
+    value = torch.empty(shape, dtype=dtype, device=k.device)
+    if key.numel():
+        _native.launch(key, "tgx_paged_read", state.native(), k.data_ptr() or None,
+                       key_cache.scales.data_ptr() or None, v.data_ptr() or None,
+                       value_cache.scales.data_ptr() or None, strides, key.data_ptr(),
+                       value.data_ptr(), heads, D, out_type, code, block)
     return key, value
 
 

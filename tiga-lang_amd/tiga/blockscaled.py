@@ -56,6 +56,8 @@ class BlockScaled:
         if codes.shape[-1] > 1 and codes.stride(-1) != 1:
             raise ValueError("the rows of codes must be dense")
         self.codes, self.scales, self.block, self.tables = codes, scales, block, tables
+        # Whether rows start a multiple of 8 bytes from the first.
+        self.eights = all(n <= 1 or s % 8 == 0 for n, s in zip(codes.shape[:-1], codes.stride()))
         # What a launch depends on beside the contents and addresses.
         self.spec = (codes.dtype, codes.shape, codes.stride(), codes.device, scales.shape, block,
                      tables)

@@ -655,13 +655,14 @@ class Graph:
                           (x.dtype, x.shape, x.stride(), x.device) for x in tensors])
         except AttributeError:
             spec = None
-        if state is None or spec is None or ("append", spec) not in state.checked:
+        plan = None if state is None or spec is None else state.checked.get(("append", spec))
+        if plan is None:
             self._check_append(*tensors)
-            state.checked["append", spec] = True
+            plan = state.checked["append", spec] = _paged().plan_append(*tensors)
         if torch.is_grad_enabled() and any([x is not None and x.requires_grad for x in tensors]):
             raise NotImplementedError("append has no gradient: detach its operands or run it "
                                       "under torch.no_grad()")
-        _paged().append(self, key_cache, key, value_cache, value, page_sums)
+        _paged().append(self, key_cache, key, value_cache, value, page_sums, plan)
 
     def _check_append(self, key_cache, key, value_cache, value, page_sums) -> None:
         state = self._paged_only("append")
@@ -733,13 +734,14 @@ class Graph:
             spec = ("read", key_cache.spec, value_cache.spec, dtype)
         except AttributeError:
             spec = None
-        if state is None or spec is None or spec not in state.checked:
+        plan = None if state is None or spec is None else state.checked.get(spec)
+        if plan is None:
             self._check_read(key_cache, value_cache, dtype)
-            state.checked[spec] = True
+            plan = state.checked[spec] = _paged().plan_read(self, key_cache, value_cache, dtype)
         if torch.is_grad_enabled() and (key_cache.requires_grad or value_cache.requires_grad):
             raise NotImplementedError("read has no gradient: detach the scales or run it under "
                                       "torch.no_grad()")
-        return _paged().read(self, key_cache, value_cache, dtype)
+        return _paged().read(self, key_cache, value_cache, dtype, plan)
 
     def _check_read(self, key_cache, value_cache, dtype) -> None:
         self._paged_only("read")
