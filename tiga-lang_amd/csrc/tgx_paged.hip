@@ -55,14 +55,24 @@ Cut cut_of(const tgx_paged& p, const tgx_paged_view& w, int heads, int group, in
   int dev = 0, cus = 256;
   if (hipGetDevice(&dev) == hipSuccess)
     (void)hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
+  const int held = held_queries(p, group, D, dtype);
   const int64_t each = workgroups_per_piece(p, heads, group, D, dtype);
   const int64_t tiles = most_tiles(p, w);
-  const int64_t wanted = cus * (held_queries(p, group, D, dtype) > 64 ? 2 : 4) / each;
+  const bool by_heads = held == 16 && (w.code != 0 || w.window > 0);
+  const int per_cu = held > 64 ? 2 : !by_heads ? 4 : D == 128 ? 2 : D == 64 ? 3 : 4;
+  const int64_t wanted = cus * per_cu / each;
   const int64_t queries = static_cast<int64_t>(p.table_heads) * heads * p.queries * group;
   if (tiles <= kMinTiles || wanted <= 1 || p.n_seqs > kMaxBlocks256 / queries ||
       (tiles <= kWholeTiles && p.n_seqs * each >= cus))
     return Cut{1, p.n_seqs, false};
-  return Cut{wanted, std::min(wanted + p.n_seqs, p.n_seqs * ceil_div(tiles, kMinTiles)), true};
+  Cut cut{wanted, 0, true};
+  // Workgroups of several heads: pieces of as many tiles a wave, and as many
+  // workgroups, as of one.
+  if (by_heads) cut.heads_held = heads % 4 == 0 ? 4 : heads % 2 == 0 ? 2 : 1;
+  cut.wanted *= cut.heads_held;
+  cut.min_tiles = kMinTiles / cut.heads_held;
+  cut.launched = std::min(cut.wanted + p.n_seqs, p.n_seqs * ceil_div(tiles, cut.min_tiles));
+  return cut;
 }
 
 int check_attn(const tgx_paged* p, const tgx_paged_view& w, int heads, int group, int D,
@@ -139,7 +149,9 @@ int launch_tiles(const PagedArgs& a, const Cut& cut, int held, hipStream_t strea
   const int64_t pieces = cut.launched * a.rel.heads * a.heads;
   TGX_PROFILE("paged_tiles", stream);
   if (held == 16) {
-    paged_tile_kernel<T, D, WIN><<<dim3(static_cast<uint32_t>(pieces)), dim3(256), 0, stream>>>(a);
+    const int64_t blocks =
+        WIN ? ceil_div(cut.launched, 8) * 8 * a.rel.heads * a.heads / a.held : pieces;
+    paged_tile_kernel<T, D, WIN><<<dim3(static_cast<uint32_t>(blocks)), dim3(256), 0, stream>>>(a);
   } else {
     const dim3 grid(static_cast<uint32_t>(ceil_div(pieces, 8) * 8 * ceil_div(rows, held)));
     if (held == 32) paged_block_kernel<T, D, 2, 1, 0, WIN><<<grid, dim3(256), 0, stream>>>(a);
@@ -237,6 +249,8 @@ static int attn(const tgx_paged* p, const tgx_paged_view& w, const void* q_dev, 
   a.group = group;
   a.D = D;
   a.pieces = static_cast<int>(cut.wanted);
+  a.min_tiles = cut.min_tiles;
+  a.held = cut.heads_held;
   if (cut.split) {
     a.meta = static_cast<int2*>(workspace_dev);
     a.partial = reinterpret_cast<float*>(static_cast<char*>(workspace_dev) + meta_bytes(*p));

@@ -66,6 +66,8 @@ struct PagedArgs {
   int group;              // query heads per key head
   int D;
   int pieces;             // W
+  int min_tiles;          // tiles a piece has at least
+  int held;               // key heads a workgroup of the tile kernels holds (Wave)
   int2* meta;             // [n_seqs] first piece and pieces of a sequence; null: one piece each
   float* partial;         // [piece, head, query] (D + 2) floats: output, maximum (log2), sum
   int window, sinks;      // WIN: at most the positions a table holds
@@ -79,6 +81,8 @@ struct PagedArgs {
 struct Cut {
   int64_t wanted, launched;
   bool split;
+  int heads_held = 1;   // adjacent key heads of a workgroup (PagedArgs::held)
+  int min_tiles = 4;    // tiles a piece has at least, where the sequence has them
 };
 
 // The launches over caches in 8 bits (tgx_paged_scaled.hip), without the join.
@@ -89,7 +93,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTile = 64;       // keys a tile
-constexpr int kMinTiles = 4;    // tiles a piece has at least, where the sequence has them
+constexpr int kMinTiles = 4;    // tiles that four waves of one head share at least
 
 
 // 2^x on the hardware unit: exact 0 for -inf.
@@ -170,7 +174,7 @@ __device__ __forceinline__ Piece find_piece(const PagedArgs& a, int x) {
     p.length = paged_length(r, 0);
     const int n = seen_tiles<WIN>(a, p.length);
     if (WIN) p.gap = skipped_tiles(a, p.length);
-    const int c = max(kMinTiles, (n + pieces - 1) / pieces);
+    const int c = max(a.min_tiles, (n + pieces - 1) / pieces);
     p.count = max(1, (n + c - 1) / c);
     if (x >= p.count) return p;
     p.seq = 0;
@@ -185,7 +189,7 @@ __device__ __forceinline__ Piece find_piece(const PagedArgs& a, int x) {
   const int total = read_lane(wave_prefix(tiles), 63);
   // Rounding up adds a piece a sequence at most, which are taken off first.
   const int room = max(pieces - r.n_seqs, (pieces + 1) / 2);
-  const int c = max(kMinTiles, (total + room - 1) / room);
+  const int c = max(a.min_tiles, (total + room - 1) / room);
   int mine = 0;
   if (per == 1)
     mine = b0 < b1 ? max(1, (tiles + c - 1) / c) : 0;
@@ -625,6 +629,82 @@ __device__ __forceinline__ void join_waves(const PagedArgs& a, const Piece& p, i
     }
   }
 }
+// What a wave of a tile kernel does: workgroups of one piece hold a.held adjacent key
+// heads each, of one table, with 4 / a.held waves a head that take its steps in turn.
+struct Wave {
+  int x, head, th, kh;       // piece; head over all tables; table head and key head
+  int group, part, parts;    // head of the workgroup; turn, of how many
+  __device__ __forceinline__ Wave(const PagedArgs& a, int wave) {
+    const unsigned heads = a.rel.heads * a.heads / static_cast<unsigned>(a.held);
+    // A piece's heads are workgroups 8 apart, on one XCD.
+    const unsigned of8 = blockIdx.x / 8u;
+    x = static_cast<int>(of8 / heads * 8u + blockIdx.x % 8u);
+    parts = 4 / a.held;
+    group = wave / parts;
+    part = wave % parts;
+    head = static_cast<int>(of8 % heads) * a.held + group;
+    th = head / a.heads;
+    kh = head % a.heads;
+  }
+};
+
+// join_waves for 16 queries of each of the workgroup's heads.
+template <typename T, int D>
+__device__ __forceinline__ void join_heads(const PagedArgs& a, const Piece& p, const Wave& wv,
+                                           int rows, char* smem, float m, float l,
+                                           const f32x4 (&o)[D / 16]) {
+  float* jo = reinterpret_cast<float*>(smem);
+  float* jm = jo + 4 * 16 * (D + 4);
+  const int wave = threadIdx.x >> 6, lane = lane_id(), g = lane >> 4, lr = lane & 15;
+  __syncthreads();
+  const float sum_l = group4_sum(l);
+#pragma unroll
+  for (int dt = 0; dt < D / 16; ++dt)
+    *reinterpret_cast<f32x4*>(jo + (wave * 16 + lr) * (D + 4) + 16 * dt + 4 * g) = o[dt];
+  if (g == 0) {
+    jm[2 * (wave * 16 + lr)] = m;
+    jm[2 * (wave * 16 + lr) + 1] = sum_l;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.held * 16 * (D / 4); i += 256) {
+    const int group = i / (16 * (D / 4)), row = i / (D / 4) % 16, d = i % (D / 4) * 4;
+    if (row >= rows) continue;
+    const int at0 = group * wv.parts * 16 + row;
+    float mx = kNegInf;
+    for (int w = 0; w < wv.parts; ++w) mx = fmaxf(mx, jm[2 * (at0 + 16 * w)]);
+    float sum = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int w = 0; w < wv.parts; ++w) {
+      // (A wave without a maximum has no weight, or a NaN of its own.)
+      const float mw = jm[2 * (at0 + 16 * w)];
+      const float f = mw == kNegInf ? 1.f : exp2_hw(mw - mx);
+      sum += f * jm[2 * (at0 + 16 * w) + 1];
+      acc += f * *reinterpret_cast<const f32x4*>(jo + (at0 + 16 * w) * (D + 4) + d);
+    }
+    const int head = wv.head - wv.group + group, kh = wv.kh - wv.group + group;
+    if (p.count == 1) {
+      const int t = row / a.group, gq = row % a.group;
+      const int64_t q_row =
+          (static_cast<int64_t>(p.seq) * a.rel.queries + t) * a.rel.heads + wv.th;
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      vec4<T> w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = static_cast<T>(acc[e] * inv);
+      *reinterpret_cast<vec4<T>*>(static_cast<T*>(a.out) +
+                                  ((q_row * a.heads + kh) * a.group + gq) * D + d) = w;
+    } else {
+      float* dst = a.partial +
+                   ((static_cast<int64_t>(wv.x) * a.rel.heads * a.heads + head) * rows + row) *
+                       (D + 2);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dst[d + e] = acc[e];
+      if (d == 0) {
+        dst[D] = mx;
+        dst[D + 1] = sum;
+      }
+    }
+  }
+}
 template <int D>
 constexpr size_t kJoinBytes = sizeof(float) * 4 * 16 * (D + 4 + 2);
 
@@ -651,15 +731,20 @@ __global__ __launch_bounds__(256, (D == 128 ? 2 : D == 64 ? 3 : 4)) void paged_t
   const PagedRel& r = a.rel;
   const unsigned all_heads = r.heads * a.heads;
   const int rows = r.queries * a.group;
-  const int head = static_cast<int>(blockIdx.x % all_heads);
-  const int x = static_cast<int>(blockIdx.x / all_heads);
-  const Piece p = find_piece<WIN>(a, x);
-  if (p.seq < 0) return;
-  const int th = head / a.heads, kh = head % a.heads;
-  if (a.meta && p.index == 0 && head == 0 && threadIdx.x == 0)
-    a.meta[p.seq] = make_int2(x, p.count);
-
   const int wave = uniform(threadIdx.x >> 6), lane = lane_id();
+  Wave wv(a, wave);
+  if (!WIN) {   // one head a workgroup, in order
+    wv.head = static_cast<int>(blockIdx.x % all_heads);
+    wv.x = static_cast<int>(blockIdx.x / all_heads);
+    wv.th = wv.head / a.heads, wv.kh = wv.head % a.heads;
+    wv.group = 0, wv.part = wave, wv.parts = 4;
+  }
+  const Piece p = find_piece<WIN>(a, wv.x);
+  if (p.seq < 0) return;
+  const int th = wv.th, kh = wv.kh, parts = wv.parts;
+  if (a.meta && p.index == 0 && wv.head == 0 && threadIdx.x == 0)
+    a.meta[p.seq] = make_int2(wv.x, p.count);
+
   const int g = lane >> 4, lr = lane & 15;
   const Query<T, D, WIN> q(a, p, th, kh, lr, rows, g);
   // What the oldest and the newest of the queries see, and the piece's end.
@@ -672,9 +757,9 @@ __global__ __launch_bounds__(256, (D == 128 ? 2 : D == 64 ? 3 : 4)) void paged_t
   T* stage = reinterpret_cast<T*>(smem) + wave * KEYS * ROW;
   float* weights = reinterpret_cast<float*>(smem + kStage) + wave * KEYS * 16;
 
-  // Steps of this wave: first + 4 i < last.  Lane l keeps the page id of key
+  // Steps of this wave: first + parts i < last.  Lane l keeps the page id of key
   // l (mod KEYS) of a step.
-  const int first = p.tile0 * (kTile / KEYS) + wave;
+  const int first = p.tile0 * (kTile / KEYS) + wv.part;
   constexpr int PER = kTile / KEYS;
   const int last = WIN ? min(p.tile1 * PER, (high + KEYS - 1) / KEYS - p.gap.skip * PER)
                        : (high + KEYS - 1) / KEYS;
@@ -712,10 +797,10 @@ __global__ __launch_bounds__(256, (D == 128 ? 2 : D == 64 ? 3 : 4)) void paged_t
     int slot = slot_of(first, page_id(first));
     load(kf, kb, a.ks_slot, slot);
     load(vf, vb, a.vs_slot, slot);
-    int next_id = page_id(first + 4);
-    for (int step = first; step < last; step += 4) {
-      const int next = slot_of(step + 4, next_id);
-      next_id = page_id(step + 8);
+    int next_id = page_id(first + parts);
+    for (int step = first; step < last; step += parts) {
+      const int next = slot_of(step + parts, next_id);
+      next_id = page_id(step + 2 * parts);
       const unsigned long long gone = __ballot(slot < 0);   // bit k: key k is not there
       f32x4 c[1][KT];
 #pragma unroll
@@ -761,7 +846,10 @@ __global__ __launch_bounds__(256, (D == 128 ? 2 : D == 64 ? 3 : 4)) void paged_t
       slot = next;
     }
   }
-  join_waves<T, D, 4>(a, p, x, head, th, kh, 0, 16, rows, smem, m, l, o[0]);
+  if constexpr (WIN)
+    join_heads<T, D>(a, p, wv, rows, smem, m, l, o[0]);
+  else
+    join_waves<T, D, 4>(a, p, wv.x, wv.head, th, kh, 0, 16, rows, smem, m, l, o[0]);
 }
 
 // More than 16 queries.  The four waves stage 64 keys together, the next tile's

@@ -14,29 +14,29 @@ namespace {
 // V's become bf16 on their way to the wave's LDS rows.  bf16 holds any code, and a
 // weight times a value's scale for any scale, which fp16 would not: so weights
 // and values are multiplied in bf16 (two parts a weight) for fp16 queries too.
-constexpr int K8 = 32;
+template <int D>
+constexpr int kKeys8 = D == 128 ? 64 : 32;
 template <typename T, int D, int CODE, bool WIN>
 __global__ __launch_bounds__(256, (D == 128 ? 2 : D == 64 ? 3 : 4)) void paged_tile8_kernel(
     PagedArgs a) {
   using VT = __bf16;
-  constexpr int KT = K8 / 16, ROW = kRow<D>, BYTES = D == 32 ? 8 : 16, NR = D == 128 ? 2 : 1;
+  constexpr int K8 = kKeys8<D>, KT = K8 / 16, PART = 32, PT = PART / 16, ROW = kRow<D>, BYTES = D == 32 ? 8 : 16, NR = D == 128 ? 2 : 1;
   using Raw = std::conditional_t<D == 32, u32x2, u32x4>;
-  constexpr size_t kStage = sizeof(VT) * 4 * K8 * ROW;
-  constexpr size_t kWeights = sizeof(float) * 4 * K8 * 16;
+  constexpr size_t kStage = sizeof(VT) * 4 * PART * ROW;
+  constexpr size_t kWeights = sizeof(float) * 4 * PART * 16;
   constexpr size_t kBytes = kStage + kWeights + sizeof(float) * 4 * 2 * K8;
   __shared__ __align__(16) char smem[kBytes > kJoinBytes<D> ? kBytes : kJoinBytes<D>];
   const PagedRel& r = a.rel;
   const unsigned all_heads = r.heads * a.heads;
   const int rows = r.queries * a.group;
-  const int head = static_cast<int>(blockIdx.x % all_heads);
-  const int x = static_cast<int>(blockIdx.x / all_heads);
-  const Piece p = find_piece<WIN>(a, x);
-  if (p.seq < 0) return;
-  const int th = head / a.heads, kh = head % a.heads;
-  if (a.meta && p.index == 0 && head == 0 && threadIdx.x == 0)
-    a.meta[p.seq] = make_int2(x, p.count);
-
   const int wave = uniform(threadIdx.x >> 6), lane = lane_id();
+  const Wave wv(a, wave);
+  const Piece p = find_piece<WIN>(a, wv.x);
+  if (p.seq < 0) return;
+  const int th = wv.th, kh = wv.kh, head = wv.head, parts = wv.parts;
+  if (a.meta && p.index == 0 && head == 0 && threadIdx.x == 0)
+    a.meta[p.seq] = make_int2(wv.x, p.count);
+
   const int g = lane >> 4, lr = lane & 15;
   const Query<T, D, WIN, D != 32> q(a, p, th, kh, lr, rows, g);
   // What the oldest and the newest of the queries see, and the piece's end.
@@ -49,11 +49,11 @@ __global__ __launch_bounds__(256, (D == 128 ? 2 : D == 64 ? 3 : 4)) void paged_t
   const int32_t* table = r.table + p.seq * r.seq_stride + th * r.head_stride;
   // The wave's staged V, its weights where they are taken key by key, and its
   // keys' scales.
-  VT* stage = reinterpret_cast<VT*>(smem) + wave * K8 * ROW;
-  float* weights = reinterpret_cast<float*>(smem + kStage) + wave * K8 * 16;
+  VT* stage = reinterpret_cast<VT*>(smem) + wave * PART * ROW;
+  float* weights = reinterpret_cast<float*>(smem + kStage) + wave * PART * 16;
   float* scales = reinterpret_cast<float*>(smem + kStage + kWeights) + wave * 2 * K8;
 
-  const int first = p.tile0 * (kTile / K8) + wave;
+  const int first = p.tile0 * (kTile / K8) + wv.part;
   constexpr int PER = kTile / K8;
   const int last = WIN ? min(p.tile1 * PER, (high + K8 - 1) / K8 - p.gap.skip * PER)
                        : (high + K8 - 1) / K8;
@@ -96,10 +96,10 @@ __global__ __launch_bounds__(256, (D == 128 ? 2 : D == 64 ? 3 : 4)) void paged_t
     load(kf, kb, a.ks_slot, slot);
     load(vf, vb, a.vs_slot, slot);
     float ks = scale_of(a.k_scales, slot), vs = scale_of(a.v_scales, slot);
-    int next_id = page_id(first + 4);
-    for (int step = first; step < last; step += 4) {
-      const int next = slot_of(step + 4, next_id);
-      next_id = page_id(step + 8);
+    int next_id = page_id(first + parts);
+    for (int step = first; step < last; step += parts) {
+      const int next = slot_of(step + parts, next_id);
+      next_id = page_id(step + 2 * parts);
       const unsigned long long gone = __ballot(slot < 0);   // bit k: key k is not there
       const float vs_here = slot < 0 ? 0.f : vs;
       if (lane < K8) {
@@ -140,7 +140,8 @@ __global__ __launch_bounds__(256, (D == 128 ? 2 : D == 64 ? 3 : 4)) void paged_t
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) c[0][kt] *= by[kt];
 
-      // Stage V; a key that is not there counts as a row of zeros.
+      // V by 32 keys through the wave's rows; a key that is not there counts as a
+      // row of zeros.
       if (gone) {
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt)
@@ -149,36 +150,46 @@ __global__ __launch_bounds__(256, (D == 128 ? 2 : D == 64 ? 3 : 4)) void paged_t
             for (int i = 0; i < NR; ++i) vf[kt][i] = Raw{};
           }
       }
-      // A NaN among the values matters where some query does not see all keys.
-      Largest<VT> largest;
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt)
+      for (int half = 0; half < K8 / PART; ++half) {
+        // A NaN among the values matters where some query does not see all keys.
+        Largest<VT> largest;
+        if (half) __builtin_amdgcn_wave_barrier();   // the rows before have been read
 #pragma unroll
-        for (int i = 0; i < NR; ++i) {
-          VT* to = stage + (16 * kt + lr) * ROW + 64 * i + BYTES * g;
-          const vec8<VT> lo = __builtin_bit_cast(
-              vec8<VT>, code_octet<VT, CODE>(u32x2{vf[kt][i][0], vf[kt][i][1]}));
-          if (CODE != TGX_CODE_INT8 && part) largest.see(lo);
-          *reinterpret_cast<vec8<VT>*>(to) = lo;
-          if constexpr (D != 32) {
-            const vec8<VT> hi = __builtin_bit_cast(
-                vec8<VT>, code_octet<VT, CODE>(u32x2{vf[kt][i][2], vf[kt][i][3]}));
-            if (CODE != TGX_CODE_INT8 && part) largest.see(hi);
-            *reinterpret_cast<vec8<VT>*>(to + 8) = hi;
+        for (int k = 0; k < PT; ++k)
+#pragma unroll
+          for (int i = 0; i < NR; ++i) {
+            const Raw raw = vf[half * PT + k][i];
+            VT* to = stage + (16 * k + lr) * ROW + 64 * i + BYTES * g;
+            const vec8<VT> lo =
+                __builtin_bit_cast(vec8<VT>, code_octet<VT, CODE>(u32x2{raw[0], raw[1]}));
+            if (CODE != TGX_CODE_INT8 && part) largest.see(lo);
+            *reinterpret_cast<vec8<VT>*>(to) = lo;
+            if constexpr (D != 32) {
+              const vec8<VT> hi =
+                  __builtin_bit_cast(vec8<VT>, code_octet<VT, CODE>(u32x2{raw[2], raw[3]}));
+              if (CODE != TGX_CODE_INT8 && part) largest.see(hi);
+              *reinterpret_cast<vec8<VT>*>(to + 8) = hi;
+            }
           }
+        const bool odd = part && __any(largest.odd() || !(fabsf(vs_here) < __builtin_huge_valf()));
+        if (half == K8 / PART - 1) {
+          load(vf, vb, a.vs_slot, next);
+          vs = scale_of(a.v_scales, next);
         }
-      const bool odd = part && __any(largest.odd() || !(fabsf(vs_here) < __builtin_huge_valf()));
-      load(vf, vb, a.vs_slot, next);
-      vs = scale_of(a.v_scales, next);
-      __builtin_amdgcn_wave_barrier();
-      if (!odd)
-        add_values<VT, D, KT, 1>(stage, c, g, lr, o);
-      else
-        add_seen_values<VT, D, WIN>(stage, c[0], g, lr, pos, q.sees, weights, o[0]);
+        __builtin_amdgcn_wave_barrier();
+        f32x4 w[1][PT];
+#pragma unroll
+        for (int k = 0; k < PT; ++k) w[0][k] = c[0][half * PT + k];
+        if (!odd)
+          add_values<VT, D, PT, 1>(stage, w, g, lr, o);
+        else
+          add_seen_values<VT, D, WIN>(stage, w[0], g, lr, pos + PART * half, q.sees, weights, o[0]);
+      }
       slot = next;
     }
   }
-  join_waves<T, D, 4>(a, p, x, head, th, kh, 0, 16, rows, smem, m, l, o[0]);
+  join_heads<T, D>(a, p, wv, rows, smem, m, l, o[0]);
 }
 
 template <typename T, int D, int CODE, bool WIN>
@@ -188,7 +199,8 @@ int launch_tiles(const PagedArgs& a, const Cut& cut, int held, hipStream_t strea
   TGX_PROFILE("paged_scaled_tiles", stream);
   if (held == 16) {
     paged_tile8_kernel<T, D, CODE, WIN>
-        <<<dim3(static_cast<uint32_t>(pieces)), dim3(256), 0, stream>>>(a);
+        <<<dim3(static_cast<uint32_t>(ceil_div(cut.launched, 8) * 8 * a.rel.heads * a.heads / a.held)),
+           dim3(256), 0, stream>>>(a);
   } else {
     const dim3 grid(static_cast<uint32_t>(ceil_div(pieces, 8) * 8 * ceil_div(rows, held)));
     // (Chunks of rows are the work here: the bounds of a window cost nothing beside it.)
