@@ -77,6 +77,7 @@ __device__ __forceinline__ void split_row(const Form& f, int q0, int rem, int r,
   g = static_cast<int>(n - up * static_cast<uint32_t>(f.group));
 }
 
+// (No key is seen from position -1.)
 __device__ __forceinline__ bool sees(const Form& f, int q, int key) {
   return key <= q && (q - key < f.window || key < f.sinks);
 }
@@ -112,60 +113,98 @@ __device__ __forceinline__ bool any_odd(const vec8<T>& x) {
   return odd;
 }
 
-// Thread t's chunks of a staged tile of 64 rows: row and byte offset of chunk i.
+// A staged tile: 64 rows of D values, filled straight from memory (a wave's load
+// writes 1 KB in lane order, so rows are not padded) with a row's 16-byte chunk c at
+// place c ^ turn(row).  turn() is even steps first, so that both what 16 rows read of
+// one chunk (fragments) and what four rows read of two chunks (transposed fragments)
+// fall on distinct banks.
+typedef __attribute__((address_space(3))) void lds_void;
+typedef const __attribute__((address_space(1))) void global_void;
 template <typename T, int D>
-struct Chunks {
-  static constexpr int CPR = D / 8, N = 64 * CPR / 256;
-  static __device__ __forceinline__ int row(int i) { return (threadIdx.x + 256 * i) / CPR; }
-  static __device__ __forceinline__ int col(int i) { return (threadIdx.x + 256 * i) % CPR * 8; }
-};
-
-template <typename T, int D>
-struct Staged {
-  vec8<T> at[Chunks<T, D>::N];
-};
-
-// Rows base .. base + 63 of one head, from `x` (its row 0) on; zeros from row `end`.
-template <typename T, int D>
-__device__ __forceinline__ void load_keys(Staged<T, D>& st, const T* x, int64_t token,
-                                          int base, int end) {
-  using C = Chunks<T, D>;
-  const T* from = x + base * token;
-#pragma unroll
-  for (int i = 0; i < C::N; ++i) {
-    const int r = C::row(i);
-    st.at[i] = base + r < end
-                   ? ld8(from + static_cast<uint32_t>(r * static_cast<int>(token)) + C::col(i))
-                   : vec8<T>{};
+struct Tile {
+  static constexpr int kRowBytes = 2 * D, kBytes = 64 * kRowBytes;
+  static constexpr int kChunks = D / 8, kRowsPerLoad = 64 / kChunks;
+  static constexpr int kLoads = 64 / kRowsPerLoad / 4;   // of each of the four waves
+  static __device__ __forceinline__ int turn(int row) {
+    const int h = row / (128 / D);   // rows that begin on the same bank
+    constexpr int kHalf = kChunks / 2;
+    return (h % kHalf) * 2 + h / kHalf % 2;
   }
-}
-template <typename T, int D, int PAD>
-__device__ __forceinline__ void store_rows(const Staged<T, D>& st, T (*to)[PAD]) {
-  using C = Chunks<T, D>;
+  // The row of this lane's part of load i, and the first of the eight values it brings.
+  static __device__ __forceinline__ int row(int wave, int i) {
+    return (wave * kLoads + i) * kRowsPerLoad + lane_id() / kChunks;
+  }
+  static __device__ __forceinline__ int col(int r) {
+    return (lane_id() % kChunks ^ turn(r)) * 8;
+  }
+  static __device__ __forceinline__ void load(const T* from, char* tile, int wave, int i) {
+    __builtin_amdgcn_global_load_lds((global_void*)from,
+                                     (lds_void*)(tile + (wave * kLoads + i) * 1024), 16, 0, 0);
+  }
+  // Where the lane's fragments begin: eight values of row lr (mod 16) from 8 g on, and
+  // what tr_frag reads down the columns.  Row r0 of either is a multiple of 16.
+  int at, down;
+  __device__ __forceinline__ Tile(int g, int lr) {
+    at = lr * kRowBytes + ((g % kChunks) ^ turn(lr)) * 16;
+    const int r = 4 * g + (lr >> 2);
+    down = r * kRowBytes + (((lr & 3) >> 1) ^ turn(r)) * 16 + (lr & 1) * 8;
+  }
+  // Values 32 kc + 8 g .. of row r0 + lr.
+  __device__ __forceinline__ vec8<T> frag(const char* tile, int r0, int kc) const {
+    return *reinterpret_cast<const vec8<T>*>(tile + r0 * kRowBytes + (at ^ (kc * 64)));
+  }
+  // Rows r0 + 4 g .. + 3 and r0 + 16 + 4 g .. + 3 of column 16 dt + lr.
+  __device__ __forceinline__ vec8<T> column(const char* tile, int r0, int dt) const {
+    const char* p = tile + r0 * kRowBytes + (down ^ (dt * 32));
+    const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(p));
+    const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(p + 16 * kRowBytes));
+    const u32x2 aw = __builtin_bit_cast(u32x2, a);
+    const u32x2 bw = __builtin_bit_cast(u32x2, b);
+    return __builtin_bit_cast(vec8<T>, (u32x4{aw[0], aw[1], bw[0], bw[1]}));
+  }
+  // Four values of a row from column d (a multiple of 4) on.
+  static __device__ __forceinline__ vec4<T> four(const char* tile, int r, int d) {
+    return *reinterpret_cast<const vec4<T>*>(tile + r * kRowBytes +
+                                             ((d / 8 ^ turn(r % 16)) * 16) + d % 8 * 2);
+  }
+  // Whether this thread's part of the tile has a NaN or Inf.
+  static __device__ __forceinline__ bool odd(const char* tile) {
+    bool found = false;
 #pragma unroll
-  for (int i = 0; i < C::N; ++i)
-    *reinterpret_cast<vec8<T>*>(&to[C::row(i)][C::col(i)]) = st.at[i];
-}
-template <typename T, int D>
-__device__ __forceinline__ bool rows_odd(const Staged<T, D>& st) {
-  bool odd = false;
-#pragma unroll
-  for (int i = 0; i < Chunks<T, D>::N; ++i) odd |= any_odd<T>(st.at[i]);
-  return odd;
+    for (int i = 0; i < kBytes / 4096; ++i)
+      found |= any_odd<T>(
+          *reinterpret_cast<const vec8<T>*>(tile + (threadIdx.x + 256 * i) * 16));
+    return found;
+  }
+};
+
+// Waits for this wave's loads into LDS and joins the workgroup.
+__device__ __forceinline__ void loads_done() {
+  __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0)
+  __syncthreads();
 }
 
-// acc[dt][e] += sum_r w[r][column lr] x[r][16 dt + 4 g + e] over the 16 rows x that the
+// Whether any thread of the workgroup has `mine` (a barrier; `room`: four words of
+// LDS that are written once between two barriers of the caller's).
+__device__ __forceinline__ bool any_thread(bool mine, int* room) {
+  const bool found = __any(mine);
+  if (lane_id() == 0) room[threadIdx.x >> 6] = found;
+  __syncthreads();
+  return room[0] | room[1] | room[2] | room[3];
+}
+
+// acc[dt][e] += sum_r w[r][column lr] x[r0 + r][16 dt + 4 g + e] over the 16 rows that the
 // column sees (`seen(r)`); w: the wave's 16 x 16 floats of LDS.
-template <typename T, int DT, int PAD, typename Seen>
-__device__ __forceinline__ void add_seen(const T (*x)[PAD], const float* w, int g, int lr,
+template <typename T, int D, typename Seen>
+__device__ __forceinline__ void add_seen(const char* x, int r0, const float* w, int g, int lr,
                                          Seen&& seen, f32x4v* acc, int stride) {
 #pragma unroll 1
   for (int r = 0; r < 16; ++r) {
     if (!seen(r)) continue;
     const float by = w[r * 16 + lr];
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      const vec4<T> v = *reinterpret_cast<const vec4<T>*>(&x[r][16 * dt + 4 * g]);
+    for (int dt = 0; dt < D / 16; ++dt) {
+      const vec4<T> v = Tile<T, D>::four(x, r0 + r, 16 * dt + 4 * g);
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[dt * stride][e] += by * static_cast<float>(v[e]);
     }
@@ -180,9 +219,10 @@ __device__ __forceinline__ void add_seen(const T (*x)[PAD], const float* w, int 
 template <typename T, int D>
 __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs<T> a) {
   constexpr int KC = D / 32, DT = D / 16;
-  __shared__ T ks[2][kKeys][FPAD<D>];
-  __shared__ T vs[2][kKeys][FPAD<D>];
-  __shared__ int sh_odd[3];   // tile t's V has a NaN or Inf: sh_odd[t % 3]
+  using TL = Tile<T, D>;
+  __shared__ __align__(1024) char ks[2][TL::kBytes];
+  __shared__ __align__(1024) char vs[2][TL::kBytes];
+  __shared__ int sh_odd[4];
   const Form& f = a.f;
   const int32_t* task = a.tasks + 4 * static_cast<int64_t>(blockIdx.x);
   const int blk = task[0];
@@ -240,30 +280,26 @@ __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs<T
 #pragma unroll
   for (int j = 0; j < 8; ++j) ones[j] = static_cast<T>(1.f);
 
-  if (threadIdx.x < 3) sh_odd[threadIdx.x] = 0;
-  __syncthreads();
-  Staged<T, D> kst, vst;
+  const TL tl(g, lr);
+  // Rows past the sequence are its last one's again: no row sees them.
   auto load = [&](int v) {
     const int base = tiles.tile(v) * kKeys;
-    load_keys<T, D>(kst, kh, a.k_token, base, len);
-    load_keys<T, D>(vst, vh, a.v_token, base, len);
-  };
-  auto store = [&](int v) {
-    store_rows(kst, ks[v & 1]);
-    store_rows(vst, vs[v & 1]);
-    // Where some row sees only a part of the tile.
-    if (!sees_all(f, q0, q1, tiles.tile(v) * kKeys) && rows_odd<T, D>(vst)) sh_odd[v % 3] = 1;
+#pragma unroll
+    for (int i = 0; i < TL::kLoads; ++i) {
+      const int r = TL::row(wave, i), key = min(base + r, len - 1), c = TL::col(r);
+      TL::load(kh + key * a.k_token + c, ks[v & 1], wave, i);
+      TL::load(vh + key * a.v_token + c, vs[v & 1], wave, i);
+    }
   };
   load(0);
-  store(0);
   for (int v = 0; v < tiles.count; ++v) {
-    __syncthreads();
+    loads_done();
     const int buf = v & 1;
     const int kbase = tiles.tile(v) * kKeys;
-    const bool odd = sh_odd[v % 3];
-    if (threadIdx.x == 0) sh_odd[(v + 2) % 3] = 0;   // (tile v - 1's, which all have read)
-    const bool more = v + 1 < tiles.count;
-    if (more) load(v + 1);
+    if (v + 1 < tiles.count) load(v + 1);
+    // (Where some row of the workgroup sees only a part of the tile.)
+    bool odd = false;
+    if (!sees_all(f, q0, q1, kbase)) odd = any_thread(TL::odd(vs[buf]), sh_odd);
 
     const bool active = !sees_none(f, w0, w1, kbase);
     f32x4v c[4][2];
@@ -277,7 +313,7 @@ __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs<T
       for (int kc = 0; kc < KC; ++kc) {
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt) {
-          const vec8<T> kf = ld8(&ks[buf][16 * kt + lr][32 * kc + 8 * g]);
+          const vec8<T> kf = tl.frag(ks[buf], 16 * kt, kc);
 #pragma unroll
           for (int qt = 0; qt < 2; ++qt) c[kt][qt] = mfma(kf, qf[qt][kc], c[kt][qt]);
         }
@@ -340,7 +376,7 @@ __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs<T
         for (int k2 = 0; k2 < 2; ++k2) {
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt) {
-            const vec8<T> vf = tr_frag(vs[buf], 32 * k2, 16 * dt, lr, g);
+            const vec8<T> vf = tl.column(vs[buf], 32 * k2, dt);
 #pragma unroll
             for (int qt = 0; qt < 2; ++qt) o[dt][qt] = mfma(vf, pf[qt][k2], o[dt][qt]);
           }
@@ -355,7 +391,7 @@ __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs<T
       // rows hold each wave's weights of 16 keys and 16 rows at a time.
       __syncthreads();
       if (active) {
-        float* w = reinterpret_cast<float*>(&ks[buf][0][0]) + wave * 256;
+        float* w = reinterpret_cast<float*>(ks[buf]) + wave * 256;
 #pragma unroll
         for (int qt = 0; qt < 2; ++qt)
 #pragma unroll
@@ -365,8 +401,8 @@ __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs<T
             for (int r = 0; r < 4; ++r) w[(4 * g + r) * 16 + lr] = c[kt][qt][r];
             __builtin_amdgcn_wave_barrier();
             const int key0 = kbase + 16 * kt;
-            add_seen<T, DT, FPAD<D>>(
-                &vs[buf][16 * kt], w, g, lr, [&](int r) { return sees(f, qpos[qt], key0 + r); },
+            add_seen<T, D>(
+                vs[buf], 16 * kt, w, g, lr, [&](int r) { return sees(f, qpos[qt], key0 + r); },
                 &o[0][qt], 2);
             float sum = 0.f;
 #pragma unroll 1
@@ -375,7 +411,6 @@ __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs<T
           }
       }
     }
-    if (more) store(v + 1);
   }
 
 #pragma unroll
@@ -436,13 +471,13 @@ struct WinBwdArgs {
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void window_dkdv_kernel(WinBwdArgs<T> b) {
   constexpr int KC = D / 32, DT = D / 16;
-  using C = Chunks<T, D>;
-  __shared__ T qs[kKeys][TPAD];
-  __shared__ T dos[kKeys][TPAD];
-  __shared__ float lse_s[kKeys], del_s[kKeys];
-  __shared__ int pos_s[kKeys];
+  using TL = Tile<T, D>;
+  __shared__ __align__(1024) char qs[2][TL::kBytes];
+  __shared__ __align__(1024) char dos[2][TL::kBytes];
+  __shared__ __align__(16) float lse_s[2][kKeys], del_s[2][kKeys];
+  __shared__ __align__(16) int pos_s[2][kKeys];
   __shared__ float sh_w[4][2][256];   // P and dS of 16 rows and 16 keys, a wave's
-  __shared__ int sh_odd[2];
+  __shared__ int sh_odd[4];
   const WinArgs<T>& a = b.a;
   const Form& f = a.f;
   const int32_t* task = a.tasks + 8 * static_cast<int64_t>(blockIdx.x);
@@ -464,6 +499,7 @@ __global__ __launch_bounds__(256, 2) void window_dkdv_kernel(WinBwdArgs<T> b) {
       vf[kc] = key < len ? ld8(vrow + 32 * kc) : vec8<T>{};
     }
   }
+  const float score_log2 = a.scale_log2 * a.sign;
   f32x4v dkt[DT], dvt[DT];   // dK^T and dV^T [d = 16 dt + 4 g + e][key]
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) {
@@ -471,52 +507,50 @@ __global__ __launch_bounds__(256, 2) void window_dkdv_kernel(WinBwdArgs<T> b) {
     dvt[dt] = f32x4v{0.f, 0.f, 0.f, 0.f};
   }
 
-  Staged<T, D> qst, dst;
+  const TL tl(g, lr);
   float lse_n = 0.f, del_n = 0.f;
   int pos_n = 0;
-  // Rows 64 block .. +63 (zeros, of no weight, past the sequence).
-  auto load = [&](int block) {
+  // Rows 64 block .. +63; past the sequence its last one's again, at no position.
+  auto load = [&](int block, int buf) {
     const int q0 = block * kKeys / f.group, rem = block * kKeys % f.group;
-#pragma unroll
-    for (int i = 0; i < C::N; ++i) {
-      int pos, head;
-      split_row(f, q0, rem, C::row(i), pos, head);
-      const bool ok = pos < len;
-      const int64_t token = s0 + pos;
-      qst.at[i] = ok ? ld8(a.q + token * a.q_token + h * a.q_head + head * a.q_group + C::col(i))
-                     : vec8<T>{};
-      dst.at[i] = ok ? ld8(a.out + ((token * f.heads + h) * f.group + head) * D + C::col(i))
-                     : vec8<T>{};
-    }
     if (threadIdx.x < kKeys) {
       int pos, head;
       split_row(f, q0, rem, threadIdx.x, pos, head);
       const int64_t at = (static_cast<int64_t>(s0 + min(pos, len - 1)) * f.heads + h) * f.group + head;
       lse_n = a.lse[at];
       del_n = b.delta[at];
-      pos_n = pos;
+      pos_n = pos < len ? pos : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < TL::kLoads; ++i) {
+      const int r = TL::row(wave, i), c = TL::col(r);
+      int pos, head;
+      split_row(f, q0, rem, r, pos, head);
+      const int64_t token = s0 + min(pos, len - 1);
+      TL::load(a.q + token * a.q_token + h * a.q_head + head * a.q_group + c, qs[buf], wave, i);
+      TL::load(a.out + ((token * f.heads + h) * f.group + head) * D + c, dos[buf], wave, i);
     }
   };
-  if (threadIdx.x < 2) sh_odd[threadIdx.x] = 0;
-  if (blocks > 0) load(block0);
-  for (int step = 0; step < blocks; ++step) {
-    const int row0 = (block0 + step) * kKeys;
-    const int p0 = row0 / f.group, p1 = min((row0 + kKeys - 1) / f.group, len - 1);
-    const bool part = !sees_all(f, p0, p1, k0);   // some row sees only a part of the tile
-    __syncthreads();   // the block before has been read
-    store_rows(qst, qs);
-    store_rows(dst, dos);
+  auto note = [&](int buf) {
     if (threadIdx.x < kKeys) {
-      const bool ok = pos_n < len;
-      lse_s[threadIdx.x] = ok ? lse_n * kLog2e : __builtin_huge_valf();
-      del_s[threadIdx.x] = ok ? del_n : 0.f;
-      pos_s[threadIdx.x] = pos_n;
+      lse_s[buf][threadIdx.x] = lse_n * kLog2e;
+      del_s[buf][threadIdx.x] = del_n;
+      pos_s[buf][threadIdx.x] = pos_n;
     }
-    if (part && (rows_odd<T, D>(qst) || rows_odd<T, D>(dst))) sh_odd[step & 1] = 1;
-    if (threadIdx.x == 0) sh_odd[(step + 1) & 1] = 0;
-    __syncthreads();
-    const bool odd = sh_odd[step & 1];
-    if (step + 1 < blocks) load(block0 + step + 1);
+  };
+  if (blocks > 0) {
+    load(block0, 0);
+    note(0);
+  }
+  for (int step = 0; step < blocks; ++step) {
+    const int row0 = (block0 + step) * kKeys, buf = step & 1;
+    const int p0 = row0 / f.group, p1 = (row0 + kKeys - 1) / f.group;
+    // Some row sees only a part of the tile, or is none.
+    const bool part = p1 >= len || !sees_all(f, p0, p1, k0);
+    loads_done();
+    if (step + 1 < blocks) load(block0 + step + 1, buf ^ 1);
+    bool odd = false;
+    if (part) odd = any_thread(TL::odd(qs[buf]) || TL::odd(dos[buf]), sh_odd);
 
     f32x4v sc[4], dp[4];
 #pragma unroll
@@ -529,8 +563,8 @@ __global__ __launch_bounds__(256, 2) void window_dkdv_kernel(WinBwdArgs<T> b) {
     for (int kc = 0; kc < KC; ++kc) {
 #pragma unroll
       for (int qt = 0; qt < 4; ++qt) {
-        const vec8<T> qa = ld8(&qs[16 * qt + lr][32 * kc + 8 * g]);
-        const vec8<T> da = ld8(&dos[16 * qt + lr][32 * kc + 8 * g]);
+        const vec8<T> qa = tl.frag(qs[buf], 16 * qt, kc);
+        const vec8<T> da = tl.frag(dos[buf], 16 * qt, kc);
         sc[qt] = mfma(qa, kf[kc], sc[qt]);
         dp[qt] = mfma(da, vf[kc], dp[qt]);
       }
@@ -540,12 +574,14 @@ __global__ __launch_bounds__(256, 2) void window_dkdv_kernel(WinBwdArgs<T> b) {
     auto weights = [&](auto masked) {
 #pragma unroll
       for (int qt = 0; qt < 4; ++qt) {
+        const f32x4v lse = *reinterpret_cast<const f32x4v*>(&lse_s[buf][16 * qt + 4 * g]);
+        const f32x4v del = *reinterpret_cast<const f32x4v*>(&del_s[buf][16 * qt + 4 * g]);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int qi = 16 * qt + 4 * g + r;
-          float p = exp2_hw(sc[qt][r] * a.scale_log2 * a.sign - lse_s[qi]);
-          float ds = p * (dp[qt][r] - del_s[qi]);
-          if (decltype(masked)::value && !sees(f, pos_s[qi], key)) p = ds = 0.f;
+          float p = exp2_hw(sc[qt][r] * score_log2 - lse[r]);
+          float ds = p * (dp[qt][r] - del[r]);
+          if (decltype(masked)::value && !sees(f, pos_s[buf][16 * qt + 4 * g + r], key))
+            p = ds = 0.f;
           pb[qt >> 1][4 * (qt & 1) + r] = static_cast<T>(p);
           sb[qt >> 1][4 * (qt & 1) + r] = static_cast<T>(ds);
         }
@@ -561,8 +597,8 @@ __global__ __launch_bounds__(256, 2) void window_dkdv_kernel(WinBwdArgs<T> b) {
       for (int k2 = 0; k2 < 2; ++k2) {
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-          const vec8<T> ot = tr_frag(dos, 32 * k2, 16 * dt, lr, g);
-          const vec8<T> qtv = tr_frag(qs, 32 * k2, 16 * dt, lr, g);
+          const vec8<T> ot = tl.column(dos[buf], 32 * k2, dt);
+          const vec8<T> qtv = tl.column(qs[buf], 32 * k2, dt);
           dvt[dt] = mfma(ot, pb[k2], dvt[dt]);
           dkt[dt] = mfma(qtv, sb[k2], dkt[dt]);
         }
@@ -579,11 +615,12 @@ __global__ __launch_bounds__(256, 2) void window_dkdv_kernel(WinBwdArgs<T> b) {
           w[1][(4 * g + r) * 16 + lr] = static_cast<float>(sb[qt >> 1][4 * (qt & 1) + r]);
         }
         __builtin_amdgcn_wave_barrier();
-        auto seen = [&](int r) { return sees(f, pos_s[16 * qt + r], key); };
-        add_seen<T, DT, TPAD>(&dos[16 * qt], w[0], g, lr, seen, dvt, 1);
-        add_seen<T, DT, TPAD>(&qs[16 * qt], w[1], g, lr, seen, dkt, 1);
+        auto seen = [&](int r) { return sees(f, pos_s[buf][16 * qt + r], key); };
+        add_seen<T, D>(dos[buf], 16 * qt, w[0], g, lr, seen, dvt, 1);
+        add_seen<T, D>(qs[buf], 16 * qt, w[1], g, lr, seen, dkt, 1);
       }
     }
+    if (step + 1 < blocks) note(buf ^ 1);
   }
   if (slot >= 0) {
     float* part = b.partial + static_cast<int64_t>(slot) * 2 * kKeys * D + (16 * wave + lr) * D;
@@ -640,10 +677,11 @@ __global__ __launch_bounds__(256) void window_merge_kernel(WinBwdArgs<T> b,
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void window_dq_kernel(WinBwdArgs<T> b) {
   constexpr int KC = D / 32, DT = D / 16;
-  __shared__ T ks[kKeys][TPAD];
-  __shared__ T vs[kKeys][TPAD];
+  using TL = Tile<T, D>;
+  __shared__ __align__(1024) char ks[2][TL::kBytes];
+  __shared__ __align__(1024) char vs[2][TL::kBytes];
   __shared__ float sh_w[4][256];
-  __shared__ int sh_odd[2];
+  __shared__ int sh_odd[4];
   const WinArgs<T>& a = b.a;
   const Form& f = a.f;
   const int32_t* task = a.tasks + 4 * static_cast<int64_t>(blockIdx.x);
@@ -690,24 +728,24 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(WinBwdArgs<T> b) {
   const KeyTiles tiles(f, q0, q1);
   const T* kh = a.k + s0 * a.k_token + h * a.k_head;
   const T* vh = a.v + s0 * a.v_token + h * a.v_head;
-  Staged<T, D> kst, vst;
-  auto load = [&](int v) {
+  const TL tl(g, lr);
+  const float score_log2 = a.scale_log2 * a.sign;
+  auto load = [&](int v) {   // (as the forward's)
     const int base = tiles.tile(v) * kKeys;
-    load_keys<T, D>(kst, kh, a.k_token, base, len);
-    load_keys<T, D>(vst, vh, a.v_token, base, len);
+#pragma unroll
+    for (int i = 0; i < TL::kLoads; ++i) {
+      const int r = TL::row(wave, i), key = min(base + r, len - 1), c = TL::col(r);
+      TL::load(kh + key * a.k_token + c, ks[v & 1], wave, i);
+      TL::load(vh + key * a.v_token + c, vs[v & 1], wave, i);
+    }
   };
-  if (threadIdx.x < 2) sh_odd[threadIdx.x] = 0;
   load(0);
   for (int v = 0; v < tiles.count; ++v) {
-    const int kbase = tiles.tile(v) * kKeys;
-    __syncthreads();
-    store_rows(kst, ks);
-    store_rows(vst, vs);
-    if (!sees_all(f, q0, q1, kbase) && rows_odd<T, D>(kst)) sh_odd[v & 1] = 1;
-    if (threadIdx.x == 0) sh_odd[(v + 1) & 1] = 0;
-    __syncthreads();
-    const bool odd = sh_odd[v & 1];
+    const int kbase = tiles.tile(v) * kKeys, buf = v & 1;
+    loads_done();
     if (v + 1 < tiles.count) load(v + 1);
+    bool odd = false;
+    if (!sees_all(f, q0, q1, kbase)) odd = any_thread(TL::odd(ks[buf]), sh_odd);
     if (sees_none(f, w0, w1, kbase)) continue;
     const bool part = !sees_all(f, w0, w1, kbase);
     vec8<T> sb[2][2];
@@ -722,8 +760,8 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(WinBwdArgs<T> b) {
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int kc = 0; kc < KC; ++kc) {
-        const vec8<T> ka = ld8(&ks[16 * kt + lr][32 * kc + 8 * g]);
-        const vec8<T> va = ld8(&vs[16 * kt + lr][32 * kc + 8 * g]);
+        const vec8<T> ka = tl.frag(ks[buf], 16 * kt, kc);
+        const vec8<T> va = tl.frag(vs[buf], 16 * kt, kc);
 #pragma unroll
         for (int qt = 0; qt < 2; ++qt) {
           sc[qt] = mfma(ka, qf[qt][kc], sc[qt]);
@@ -736,7 +774,7 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(WinBwdArgs<T> b) {
         for (int qt = 0; qt < 2; ++qt) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float p = exp2_hw(sc[qt][r] * a.scale_log2 * a.sign - lse2[qt]);
+            const float p = exp2_hw(sc[qt][r] * score_log2 - lse2[qt]);
             float ds = p * (dp[qt][r] - del[qt]);
             if (decltype(masked)::value && !sees(f, qpos[qt], kbase + 16 * kt + 4 * g + r))
               ds = 0.f;
@@ -755,7 +793,7 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(WinBwdArgs<T> b) {
       for (int k2 = 0; k2 < 2; ++k2) {
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-          const vec8<T> kta = tr_frag(ks, 32 * k2, 16 * dt, lr, g);
+          const vec8<T> kta = tl.column(ks[buf], 32 * k2, dt);
 #pragma unroll
           for (int qt = 0; qt < 2; ++qt) dqt[dt][qt] = mfma(kta, sb[qt][k2], dqt[dt][qt]);
         }
@@ -773,8 +811,8 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(WinBwdArgs<T> b) {
                 static_cast<float>(sb[qt][kt >> 1][4 * (kt & 1) + r]);
           __builtin_amdgcn_wave_barrier();
           const int key0 = kbase + 16 * kt;
-          add_seen<T, DT, TPAD>(
-              &ks[16 * kt], sh_w[wave], g, lr,
+          add_seen<T, D>(
+              ks[buf], 16 * kt, sh_w[wave], g, lr,
               [&](int r) { return sees(f, qpos[qt], key0 + r); }, &dqt[0][qt], 2);
         }
     }
