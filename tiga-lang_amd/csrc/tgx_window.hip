@@ -149,13 +149,19 @@ struct Tile {
     const int r = 4 * g + (lr >> 2);
     down = r * kRowBytes + (((lr & 3) >> 1) ^ turn(r)) * 16 + (lr & 1) * 8;
   }
-  // Values 32 kc + 8 g .. of row r0 + lr.
-  __device__ __forceinline__ vec8<T> frag(const char* tile, int r0, int kc) const {
-    return *reinterpret_cast<const vec8<T>*>(tile + r0 * kRowBytes + (at ^ (kc * 64)));
+  // The same in the other of two buffers.
+  __device__ __forceinline__ void flip() {
+    at ^= kBytes;
+    down ^= kBytes;
+  }
+  // Values 32 kc + 8 g .. of row r0 + lr of the current buffer of `tiles`.  (What is
+  // the same in every step is an instruction's own offset, not a register.)
+  __device__ __forceinline__ vec8<T> frag(const char* tiles, int r0, int kc) const {
+    return *reinterpret_cast<const vec8<T>*>(tiles + r0 * kRowBytes + (at ^ (kc * 64)));
   }
   // Rows r0 + 4 g .. + 3 and r0 + 16 + 4 g .. + 3 of column 16 dt + lr.
-  __device__ __forceinline__ vec8<T> column(const char* tile, int r0, int dt) const {
-    const char* p = tile + r0 * kRowBytes + (down ^ (dt * 32));
+  __device__ __forceinline__ vec8<T> column(const char* tiles, int r0, int dt) const {
+    const char* p = tiles + r0 * kRowBytes + (down ^ (dt * 32));
     const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(p));
     const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(p + 16 * kRowBytes));
     const u32x2 aw = __builtin_bit_cast(u32x2, a);
@@ -177,6 +183,20 @@ struct Tile {
     return found;
   }
 };
+
+// Zeros in the place of this thread's NaN and Inf of the tile.
+template <typename T, int D>
+__device__ __forceinline__ void clear_odd(char* tile) {
+  constexpr uint32_t kExponent = std::is_same_v<T, __bf16> ? 0x7F80u : 0x7C00u;
+#pragma unroll 1
+  for (int i = threadIdx.x * 4; i < Tile<T, D>::kBytes; i += 1024) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(tile + i);
+    uint32_t x = *w;
+    if ((x & kExponent) == kExponent) x &= 0xFFFF0000u;
+    if ((x >> 16 & kExponent) == kExponent) x &= 0xFFFFu;
+    *w = x;
+  }
+}
 
 // Waits for this wave's loads into LDS and joins the workgroup.
 __device__ __forceinline__ void loads_done() {
@@ -220,8 +240,9 @@ template <typename T, int D>
 __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs<T> a) {
   constexpr int KC = D / 32, DT = D / 16;
   using TL = Tile<T, D>;
-  __shared__ __align__(1024) char ks[2][TL::kBytes];
-  __shared__ __align__(1024) char vs[2][TL::kBytes];
+  __shared__ __align__(1024) char tiles_s[2][2][TL::kBytes];
+  auto& ks = tiles_s[0];
+  auto& vs = tiles_s[1];
   __shared__ int sh_odd[4];
   const Form& f = a.f;
   const int32_t* task = a.tasks + 4 * static_cast<int64_t>(blockIdx.x);
@@ -280,7 +301,7 @@ __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs<T
 #pragma unroll
   for (int j = 0; j < 8; ++j) ones[j] = static_cast<T>(1.f);
 
-  const TL tl(g, lr);
+  TL tl(g, lr);
   // Rows past the sequence are its last one's again: no row sees them.
   auto load = [&](int v) {
     const int base = tiles.tile(v) * kKeys;
@@ -313,7 +334,7 @@ __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs<T
       for (int kc = 0; kc < KC; ++kc) {
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt) {
-          const vec8<T> kf = tl.frag(ks[buf], 16 * kt, kc);
+          const vec8<T> kf = tl.frag(ks[0], 16 * kt, kc);
 #pragma unroll
           for (int qt = 0; qt < 2; ++qt) c[kt][qt] = mfma(kf, qf[qt][kc], c[kt][qt]);
         }
@@ -376,7 +397,7 @@ __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs<T
         for (int k2 = 0; k2 < 2; ++k2) {
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt) {
-            const vec8<T> vf = tl.column(vs[buf], 32 * k2, dt);
+            const vec8<T> vf = tl.column(vs[0], 32 * k2, dt);
 #pragma unroll
             for (int qt = 0; qt < 2; ++qt) o[dt][qt] = mfma(vf, pf[qt][k2], o[dt][qt]);
           }
@@ -411,6 +432,7 @@ __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs<T
           }
       }
     }
+    tl.flip();
   }
 
 #pragma unroll
@@ -472,8 +494,9 @@ template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void window_dkdv_kernel(WinBwdArgs<T> b) {
   constexpr int KC = D / 32, DT = D / 16;
   using TL = Tile<T, D>;
-  __shared__ __align__(1024) char qs[2][TL::kBytes];
-  __shared__ __align__(1024) char dos[2][TL::kBytes];
+  __shared__ __align__(1024) char tiles_s[2][2][TL::kBytes];
+  auto& qs = tiles_s[0];
+  auto& dos = tiles_s[1];
   __shared__ __align__(16) float lse_s[2][kKeys], del_s[2][kKeys];
   __shared__ __align__(16) int pos_s[2][kKeys];
   __shared__ float sh_w[4][2][256];   // P and dS of 16 rows and 16 keys, a wave's
@@ -507,7 +530,7 @@ __global__ __launch_bounds__(256, 2) void window_dkdv_kernel(WinBwdArgs<T> b) {
     dvt[dt] = f32x4v{0.f, 0.f, 0.f, 0.f};
   }
 
-  const TL tl(g, lr);
+  TL tl(g, lr);
   float lse_n = 0.f, del_n = 0.f;
   int pos_n = 0;
   // Rows 64 block .. +63; past the sequence its last one's again, at no position.
@@ -563,8 +586,8 @@ __global__ __launch_bounds__(256, 2) void window_dkdv_kernel(WinBwdArgs<T> b) {
     for (int kc = 0; kc < KC; ++kc) {
 #pragma unroll
       for (int qt = 0; qt < 4; ++qt) {
-        const vec8<T> qa = tl.frag(qs[buf], 16 * qt, kc);
-        const vec8<T> da = tl.frag(dos[buf], 16 * qt, kc);
+        const vec8<T> qa = tl.frag(qs[0], 16 * qt, kc);
+        const vec8<T> da = tl.frag(dos[0], 16 * qt, kc);
         sc[qt] = mfma(qa, kf[kc], sc[qt]);
         dp[qt] = mfma(da, vf[kc], dp[qt]);
       }
@@ -597,8 +620,8 @@ __global__ __launch_bounds__(256, 2) void window_dkdv_kernel(WinBwdArgs<T> b) {
       for (int k2 = 0; k2 < 2; ++k2) {
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-          const vec8<T> ot = tl.column(dos[buf], 32 * k2, dt);
-          const vec8<T> qtv = tl.column(qs[buf], 32 * k2, dt);
+          const vec8<T> ot = tl.column(dos[0], 32 * k2, dt);
+          const vec8<T> qtv = tl.column(qs[0], 32 * k2, dt);
           dvt[dt] = mfma(ot, pb[k2], dvt[dt]);
           dkt[dt] = mfma(qtv, sb[k2], dkt[dt]);
         }
@@ -621,6 +644,7 @@ __global__ __launch_bounds__(256, 2) void window_dkdv_kernel(WinBwdArgs<T> b) {
       }
     }
     if (step + 1 < blocks) note(buf ^ 1);
+    tl.flip();
   }
   if (slot >= 0) {
     float* part = b.partial + static_cast<int64_t>(slot) * 2 * kKeys * D + (16 * wave + lr) * D;
@@ -673,14 +697,18 @@ __global__ __launch_bounds__(256) void window_merge_kernel(WinBwdArgs<T> b,
                               (static_cast<int64_t>(s0 + k0 + key) * f.heads + h) * D + d) = w;
 }
 
-// dQ: S^T = K Q^T and dP^T = V dO^T give dS^T, the B operand of dQ^T = K^T dS^T.
+// dQ: S^T = K Q^T and dP^T = V dO^T give dS^T, the B operand of dQ^T = K^T dS^T.  In a
+// masked tile with a NaN or Inf among K, those count as zeros in the last product: a
+// row that sees such a key has a NaN in dS already, or (a score of -inf) no weight for
+// it.  (Multiplying row by row, as the other kernels do, needs registers that spill
+// here: a spilled fragment's reload waits for the tile in flight.)
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void window_dq_kernel(WinBwdArgs<T> b) {
   constexpr int KC = D / 32, DT = D / 16;
   using TL = Tile<T, D>;
-  __shared__ __align__(1024) char ks[2][TL::kBytes];
-  __shared__ __align__(1024) char vs[2][TL::kBytes];
-  __shared__ float sh_w[4][256];
+  __shared__ __align__(1024) char tiles_s[2][2][TL::kBytes];
+  auto& ks = tiles_s[0];
+  auto& vs = tiles_s[1];
   __shared__ int sh_odd[4];
   const WinArgs<T>& a = b.a;
   const Form& f = a.f;
@@ -702,22 +730,21 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(WinBwdArgs<T> b) {
   vec8<T> qf[2][KC], df[2][KC];
   float lse2[2], del[2];
   int qpos[2];
-  int64_t at[2];
 #pragma unroll
   for (int qt = 0; qt < 2; ++qt) {
     int head;
     split_row(f, q0, rem, 32 * wave + 16 * qt + lr, qpos[qt], head);
     const bool ok = qpos[qt] < len;
     const int64_t token = s0 + qpos[qt];
-    at[qt] = ok ? (token * f.heads + h) * f.group + head : -1;
+    const int64_t at = (token * f.heads + h) * f.group + head;
     const T* row = a.q + token * a.q_token + h * a.q_head + head * a.q_group;
 #pragma unroll
     for (int kc = 0; kc < KC; ++kc) {
       qf[qt][kc] = ok ? ld8(row + 32 * kc + 8 * g) : vec8<T>{};
-      df[qt][kc] = ok ? ld8(a.out + at[qt] * D + 32 * kc + 8 * g) : vec8<T>{};
+      df[qt][kc] = ok ? ld8(a.out + at * D + 32 * kc + 8 * g) : vec8<T>{};
     }
-    lse2[qt] = ok ? a.lse[at[qt]] * kLog2e : __builtin_huge_valf();
-    del[qt] = ok ? b.delta[at[qt]] : 0.f;
+    lse2[qt] = ok ? a.lse[at] * kLog2e : __builtin_huge_valf();
+    del[qt] = ok ? b.delta[at] : 0.f;
     qpos[qt] = min(qpos[qt], len - 1);
   }
   f32x4v dqt[DT][2];   // dQ^T [d = 16 dt + 4 g + r][row]
@@ -728,7 +755,7 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(WinBwdArgs<T> b) {
   const KeyTiles tiles(f, q0, q1);
   const T* kh = a.k + s0 * a.k_token + h * a.k_head;
   const T* vh = a.v + s0 * a.v_token + h * a.v_head;
-  const TL tl(g, lr);
+  TL tl(g, lr);
   const float score_log2 = a.scale_log2 * a.sign;
   auto load = [&](int v) {   // (as the forward's)
     const int base = tiles.tile(v) * kKeys;
@@ -746,81 +773,80 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(WinBwdArgs<T> b) {
     if (v + 1 < tiles.count) load(v + 1);
     bool odd = false;
     if (!sees_all(f, q0, q1, kbase)) odd = any_thread(TL::odd(ks[buf]), sh_odd);
-    if (sees_none(f, w0, w1, kbase)) continue;
+    const bool active = !sees_none(f, w0, w1, kbase);
     const bool part = !sees_all(f, w0, w1, kbase);
     vec8<T> sb[2][2];
+    if (active) {
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
-      f32x4v sc[2], dp[2];
-#pragma unroll
-      for (int qt = 0; qt < 2; ++qt) {
-        sc[qt] = f32x4v{0.f, 0.f, 0.f, 0.f};
-        dp[qt] = f32x4v{0.f, 0.f, 0.f, 0.f};
-      }
-      __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-      for (int kc = 0; kc < KC; ++kc) {
-        const vec8<T> ka = tl.frag(ks[buf], 16 * kt, kc);
-        const vec8<T> va = tl.frag(vs[buf], 16 * kt, kc);
+      for (int kt = 0; kt < 4; ++kt) {
+        f32x4v sc[2], dp[2];
 #pragma unroll
         for (int qt = 0; qt < 2; ++qt) {
-          sc[qt] = mfma(ka, qf[qt][kc], sc[qt]);
-          dp[qt] = mfma(va, df[qt][kc], dp[qt]);
+          sc[qt] = f32x4v{0.f, 0.f, 0.f, 0.f};
+          dp[qt] = f32x4v{0.f, 0.f, 0.f, 0.f};
         }
-      }
-      __builtin_amdgcn_s_setprio(0);
-      auto weights = [&](auto masked) {
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int qt = 0; qt < 2; ++qt) {
+        for (int kc = 0; kc < KC; ++kc) {
+          const vec8<T> ka = tl.frag(ks[0], 16 * kt, kc);
+          const vec8<T> va = tl.frag(vs[0], 16 * kt, kc);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float p = exp2_hw(sc[qt][r] * score_log2 - lse2[qt]);
-            float ds = p * (dp[qt][r] - del[qt]);
-            if (decltype(masked)::value && !sees(f, qpos[qt], kbase + 16 * kt + 4 * g + r))
-              ds = 0.f;
-            sb[qt][kt >> 1][4 * (kt & 1) + r] = static_cast<T>(ds);
+          for (int qt = 0; qt < 2; ++qt) {
+            sc[qt] = mfma(ka, qf[qt][kc], sc[qt]);
+            dp[qt] = mfma(va, df[qt][kc], dp[qt]);
           }
         }
-      };
-      if (part)
-        weights(std::true_type{});
-      else
-        weights(std::false_type{});
+        __builtin_amdgcn_s_setprio(0);
+        auto weights = [&](auto masked) {
+#pragma unroll
+          for (int qt = 0; qt < 2; ++qt) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float p = exp2_hw(sc[qt][r] * score_log2 - lse2[qt]);
+              float ds = p * (dp[qt][r] - del[qt]);
+              if (decltype(masked)::value && !sees(f, qpos[qt], kbase + 16 * kt + 4 * g + r))
+                ds = 0.f;
+              sb[qt][kt >> 1][4 * (kt & 1) + r] = static_cast<T>(ds);
+            }
+          }
+        };
+        if (part)
+          weights(std::true_type{});
+        else
+          weights(std::false_type{});
+        // (Fragments read ahead past this would not fit the registers at D = 128.)
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
-    if (!odd) {
+    if (odd) {   // (of the whole workgroup)
+      __syncthreads();
+      clear_odd<T, D>(ks[buf]);
+      __syncthreads();
+    }
+    if (active) {
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int k2 = 0; k2 < 2; ++k2) {
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-          const vec8<T> kta = tl.column(ks[buf], 32 * k2, dt);
+          const vec8<T> kta = tl.column(ks[0], 32 * k2, dt);
 #pragma unroll
           for (int qt = 0; qt < 2; ++qt) dqt[dt][qt] = mfma(kta, sb[qt][k2], dqt[dt][qt]);
         }
       }
       __builtin_amdgcn_s_setprio(0);
-    } else {
-#pragma unroll
-      for (int qt = 0; qt < 2; ++qt)
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt) {
-          __builtin_amdgcn_wave_barrier();
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            sh_w[wave][(4 * g + r) * 16 + lr] =
-                static_cast<float>(sb[qt][kt >> 1][4 * (kt & 1) + r]);
-          __builtin_amdgcn_wave_barrier();
-          const int key0 = kbase + 16 * kt;
-          add_seen<T, D>(
-              ks[buf], 16 * kt, sh_w[wave], g, lr,
-              [&](int r) { return sees(f, qpos[qt], key0 + r); }, &dqt[0][qt], 2);
-        }
     }
+    tl.flip();
   }
+  // (Where a row goes is found again, not kept in registers over the loop.)
+  int again = q0;
+  asm volatile("" : "+s"(again));
 #pragma unroll
   for (int qt = 0; qt < 2; ++qt) {
-    if (at[qt] < 0) continue;
-    T* row = b.dq + at[qt] * D;
+    int pos, head;
+    split_row(f, again, rem, 32 * wave + 16 * qt + lr, pos, head);
+    if (pos >= len) continue;
+    T* row = b.dq + ((static_cast<int64_t>(s0 + pos) * f.heads + h) * f.group + head) * D;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       vec4<T> w;
