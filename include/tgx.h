@@ -931,7 +931,8 @@ int tgx_window_tasks(const int32_t* cu_host, int n_blocks, int heads, int group,
                      int sinks, int kind, int32_t* tasks_host, int64_t* n_tasks,
                      int64_t* n_slots);
 
-/* out [n, heads, group, D] contiguous, lse [n, heads, group] fp32 (natural log).
+/* out [n, heads, group, D] contiguous; lse [n, heads, group] fp32, for the backward: the
+ * logarithm to base 2 of each row's sum of exponentials.
  * strides, host array of seven, in elements, multiples of 8: q's token, head, group;
  * k's token, head; v's token, head. */
 int tgx_window_attn_fwd(const int32_t* cu_dev, const int32_t* tasks_dev, int64_t n_tasks,

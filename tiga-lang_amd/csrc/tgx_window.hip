@@ -64,7 +64,7 @@ struct WinArgs {
   float scale_log2;    // |scale| log2(e); 1 for a scale of 0
   float sign;          // what the queries are multiplied by first: 1, -1 or 0
   T* out;              // [n, heads, group, D]; backward: dO
-  float* lse;          // [n, heads, group], natural log
+  float* lse;          // [n, heads, group]: log2 of the sum of 2^(scores * scale_log2)
 };
 
 // Position and head in the group of the row that lies `r` (< 128) rows behind row
@@ -119,7 +119,26 @@ __device__ __forceinline__ bool any_odd(const vec8<T>& x) {
 // one chunk (fragments) and what four rows read of two chunks (transposed fragments)
 // fall on distinct banks.
 typedef __attribute__((address_space(3))) void lds_void;
-typedef const __attribute__((address_space(1))) void global_void;
+
+// BYTES bytes a lane from memory to `to` + BYTES * lane in LDS.  The load has no result
+// in registers, and what it writes is read after loads_done() only.  (Of the compiler's
+// builtin every read of LDS that follows waits for it at once, also one of the other
+// buffer: dQ of 17k tokens 215 us by it.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"   // (m0 is nobody else's: it is named all the same)
+template <int BYTES>
+__device__ __forceinline__ void load_lds(const void* from, void* to) {
+  static_assert(BYTES == 16 || BYTES == 4, "a lane brings 16 bytes or 4");
+  const uint32_t at = uniform(static_cast<int>(reinterpret_cast<uintptr_t>((lds_void*)to)));
+  if constexpr (BYTES == 16)
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %0, off"
+                 ::"v"(from), "s"(at) : "m0", "memory");
+  else
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 1\n\tglobal_load_lds_dword %0, off"
+                 ::"v"(from), "s"(at) : "m0", "memory");
+}
+#pragma clang diagnostic pop
+
 template <typename T, int D>
 struct Tile {
   static constexpr int kRowBytes = 2 * D, kBytes = 64 * kRowBytes;
@@ -138,8 +157,7 @@ struct Tile {
     return (lane_id() % kChunks ^ turn(r)) * 8;
   }
   static __device__ __forceinline__ void load(const T* from, char* tile, int wave, int i) {
-    __builtin_amdgcn_global_load_lds((global_void*)from,
-                                     (lds_void*)(tile + (wave * kLoads + i) * 1024), 16, 0, 0);
+    load_lds<16>(from, tile + (wave * kLoads + i) * 1024);
   }
   // Where the lane's fragments begin: eight values of row lr (mod 16) from 8 g on, and
   // what tr_frag reads down the columns.  Row r0 of either is a multiple of 16.
@@ -200,7 +218,7 @@ __device__ __forceinline__ void clear_odd(char* tile) {
 
 // Waits for this wave's loads into LDS and joins the workgroup.
 __device__ __forceinline__ void loads_done() {
-  __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0)
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
 }
 
@@ -448,7 +466,7 @@ __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs<T
       for (int r = 0; r < 4; ++r) w[r] = static_cast<T>(o[dt][qt][r] * inv);
       *reinterpret_cast<vec4<T>*>(row + 16 * dt + 4 * g) = w;
     }
-    if (g == 0) a.lse[at[qt]] = (m[qt] + __log2f(l)) * kLn2;
+    if (g == 0) a.lse[at[qt]] = m[qt] + __log2f(l);
   }
 }
 
@@ -531,18 +549,19 @@ __global__ __launch_bounds__(256, 2) void window_dkdv_kernel(WinBwdArgs<T> b) {
   }
 
   TL tl(g, lr);
-  float lse_n = 0.f, del_n = 0.f;
-  int pos_n = 0;
   // Rows 64 block .. +63; past the sequence its last one's again, at no position.
   auto load = [&](int block, int buf) {
     const int q0 = block * kKeys / f.group, rem = block * kKeys % f.group;
-    if (threadIdx.x < kKeys) {
+    if (wave < 2) {
       int pos, head;
-      split_row(f, q0, rem, threadIdx.x, pos, head);
+      split_row(f, q0, rem, lane, pos, head);
       const int64_t at = (static_cast<int64_t>(s0 + min(pos, len - 1)) * f.heads + h) * f.group + head;
-      lse_n = a.lse[at];
-      del_n = b.delta[at];
-      pos_n = pos < len ? pos : -1;
+      if (wave == 0) {
+        load_lds<4>(a.lse + at, lse_s[buf]);
+        pos_s[buf][lane] = pos < len ? pos : -1;
+      } else {
+        load_lds<4>(b.delta + at, del_s[buf]);
+      }
     }
 #pragma unroll
     for (int i = 0; i < TL::kLoads; ++i) {
@@ -554,17 +573,7 @@ __global__ __launch_bounds__(256, 2) void window_dkdv_kernel(WinBwdArgs<T> b) {
       TL::load(a.out + ((token * f.heads + h) * f.group + head) * D + c, dos[buf], wave, i);
     }
   };
-  auto note = [&](int buf) {
-    if (threadIdx.x < kKeys) {
-      lse_s[buf][threadIdx.x] = lse_n * kLog2e;
-      del_s[buf][threadIdx.x] = del_n;
-      pos_s[buf][threadIdx.x] = pos_n;
-    }
-  };
-  if (blocks > 0) {
-    load(block0, 0);
-    note(0);
-  }
+  if (blocks > 0) load(block0, 0);
   for (int step = 0; step < blocks; ++step) {
     const int row0 = (block0 + step) * kKeys, buf = step & 1;
     const int p0 = row0 / f.group, p1 = (row0 + kKeys - 1) / f.group;
@@ -643,7 +652,6 @@ __global__ __launch_bounds__(256, 2) void window_dkdv_kernel(WinBwdArgs<T> b) {
         add_seen<T, D>(qs[buf], 16 * qt, w[1], g, lr, seen, dkt, 1);
       }
     }
-    if (step + 1 < blocks) note(buf ^ 1);
     tl.flip();
   }
   if (slot >= 0) {
@@ -743,7 +751,7 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(WinBwdArgs<T> b) {
       qf[qt][kc] = ok ? ld8(row + 32 * kc + 8 * g) : vec8<T>{};
       df[qt][kc] = ok ? ld8(a.out + at * D + 32 * kc + 8 * g) : vec8<T>{};
     }
-    lse2[qt] = ok ? a.lse[at] * kLog2e : __builtin_huge_valf();
+    lse2[qt] = ok ? a.lse[at] : __builtin_huge_valf();
     del[qt] = ok ? b.delta[at] : 0.f;
     qpos[qt] = min(qpos[qt], len - 1);
   }
