@@ -115,9 +115,11 @@ __device__ __forceinline__ bool any_odd(const vec8<T>& x) {
 
 // A staged tile: 64 rows of D values, filled straight from memory (a wave's load
 // writes 1 KB in lane order, so rows are not padded) with a row's 16-byte chunk c at
-// place c ^ turn(row).  turn() is even steps first, so that both what 16 rows read of
-// one chunk (fragments) and what four rows read of two chunks (transposed fragments)
-// fall on distinct banks.
+// place c ^ turn(row).  turn() goes in steps of two: what four rows read of two chunks
+// (transposed fragments) falls on distinct banks, and so does what sixteen lanes read
+// together of fragments (lanes 0-3, 12-15, 20-27 and so on: four rows each of chunk g
+// and of g + 1).  With steps that fill the odd places for rows 8-15 a third of dK/dV's
+// LDS cycles were conflicts.
 typedef __attribute__((address_space(3))) void lds_void;
 
 // BYTES bytes a lane from memory to `to` + BYTES * lane in LDS.  The load has no result
@@ -145,9 +147,7 @@ struct Tile {
   static constexpr int kChunks = D / 8, kRowsPerLoad = 64 / kChunks;
   static constexpr int kLoads = 64 / kRowsPerLoad / 4;   // of each of the four waves
   static __device__ __forceinline__ int turn(int row) {
-    const int h = row / (128 / D);   // rows that begin on the same bank
-    constexpr int kHalf = kChunks / 2;
-    return (h % kHalf) * 2 + h / kHalf % 2;
+    return row / (128 / D) % (kChunks / 2) * 2;   // (128 / D rows fill all banks)
   }
   // The row of this lane's part of load i, and the first of the eight values it brings.
   static __device__ __forceinline__ int row(int wave, int i) {
