@@ -139,6 +139,12 @@ __device__ __forceinline__ void load_lds(const void* from, void* to) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 1\n\tglobal_load_lds_dword %0, off"
                  ::"v"(from), "s"(at) : "m0", "memory");
 }
+// 16 bytes a lane from `offset` bytes behind `base`, which is the same for all.
+__device__ __forceinline__ void load_lds(const void* base, uint32_t offset, void* to) {
+  const uint32_t at = uniform(static_cast<int>(reinterpret_cast<uintptr_t>((lds_void*)to)));
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %0, %1"
+               ::"v"(offset), "s"(base), "s"(at) : "m0", "memory");
+}
 #pragma clang diagnostic pop
 
 template <typename T, int D>
@@ -158,6 +164,10 @@ struct Tile {
   }
   static __device__ __forceinline__ void load(const T* from, char* tile, int wave, int i) {
     load_lds<16>(from, tile + (wave * kLoads + i) * 1024);
+  }
+  static __device__ __forceinline__ void load(const T* base, uint32_t offset, char* tile,
+                                              int wave, int i) {
+    load_lds(base, offset, tile + (wave * kLoads + i) * 1024);
   }
   // Where the lane's fragments begin: eight values of row lr (mod 16) from 8 g on, and
   // what tr_frag reads down the columns.  Row r0 of either is a multiple of 16.
@@ -215,6 +225,48 @@ __device__ __forceinline__ void clear_odd(char* tile) {
     *w = x;
   }
 }
+
+// Key tiles of a head: rows base .. base + 63 of K and V from `k` and `v` (its rows 0) into
+// the tiles `ks` and `vs`.  The parts' offsets are the same for every whole tile; rows
+// past the sequence are its last one's again, which no row sees.
+template <typename T, int D>
+struct KeyLoads {
+  using TL = Tile<T, D>;
+  const T* k;
+  const T* v;
+  int64_t k_token, v_token;
+  int len;
+  uint32_t k_off[TL::kLoads], v_off[TL::kLoads];
+  __device__ __forceinline__ KeyLoads(const WinArgs<T>& a, int s0, int h, int length, int wave)
+      : k(a.k + s0 * a.k_token + h * a.k_head),
+        v(a.v + s0 * a.v_token + h * a.v_head),
+        k_token(a.k_token),
+        v_token(a.v_token),
+        len(length) {
+#pragma unroll
+    for (int i = 0; i < TL::kLoads; ++i) {
+      const int r = TL::row(wave, i), c = TL::col(r);
+      k_off[i] = static_cast<uint32_t>(r * static_cast<int>(k_token) + c) * sizeof(T);
+      v_off[i] = static_cast<uint32_t>(r * static_cast<int>(v_token) + c) * sizeof(T);
+    }
+  }
+  __device__ __forceinline__ void operator()(int base, char* ks, char* vs, int wave) const {
+    if (base + kKeys <= len) {
+#pragma unroll
+      for (int i = 0; i < TL::kLoads; ++i) {
+        TL::load(k + base * k_token, k_off[i], ks, wave, i);
+        TL::load(v + base * v_token, v_off[i], vs, wave, i);
+      }
+      return;
+    }
+#pragma unroll 1
+    for (int i = 0; i < TL::kLoads; ++i) {
+      const int r = TL::row(wave, i), key = min(base + r, len - 1), c = TL::col(r);
+      TL::load(k + key * k_token + c, ks, wave, i);
+      TL::load(v + key * v_token + c, vs, wave, i);
+    }
+  }
+};
 
 // Waits for this wave's loads into LDS and joins the workgroup.
 __device__ __forceinline__ void loads_done() {
@@ -304,8 +356,6 @@ __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs<T
   }
 
   const KeyTiles tiles(f, q0, q1);
-  const T* kh = a.k + s0 * a.k_token + h * a.k_head;
-  const T* vh = a.v + s0 * a.v_token + h * a.v_head;
   const float sl2 = a.scale_log2;
   float m[2] = {kNegInf, kNegInf};
   f32x4v o[DT][2];
@@ -320,16 +370,8 @@ __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs<T
   for (int j = 0; j < 8; ++j) ones[j] = static_cast<T>(1.f);
 
   TL tl(g, lr);
-  // Rows past the sequence are its last one's again: no row sees them.
-  auto load = [&](int v) {
-    const int base = tiles.tile(v) * kKeys;
-#pragma unroll
-    for (int i = 0; i < TL::kLoads; ++i) {
-      const int r = TL::row(wave, i), key = min(base + r, len - 1), c = TL::col(r);
-      TL::load(kh + key * a.k_token + c, ks[v & 1], wave, i);
-      TL::load(vh + key * a.v_token + c, vs[v & 1], wave, i);
-    }
-  };
+  const KeyLoads<T, D> keys(a, s0, h, len, wave);
+  auto load = [&](int v) { keys(tiles.tile(v) * kKeys, ks[v & 1], vs[v & 1], wave); };
   load(0);
   for (int v = 0; v < tiles.count; ++v) {
     loads_done();
@@ -549,6 +591,19 @@ __global__ __launch_bounds__(256, 2) void window_dkdv_kernel(WinBwdArgs<T> b) {
   }
 
   TL tl(g, lr);
+  // Where the group divides 64 the parts' offsets are the same for every whole block.
+  const bool even = kKeys % f.group == 0 && a.q_token < kMaxTokenStride &&
+                    a.q_group < kMaxTokenStride && f.heads * f.group * D < kMaxTokenStride;
+  uint32_t q_off[TL::kLoads], d_off[TL::kLoads];
+#pragma unroll
+  for (int i = 0; i < TL::kLoads; ++i) {
+    const int r = TL::row(wave, i), c = TL::col(r);
+    int pos, head;
+    split_row(f, 0, 0, r, pos, head);
+    q_off[i] = static_cast<uint32_t>(pos * static_cast<int>(a.q_token) +
+                                     head * static_cast<int>(a.q_group) + c) * sizeof(T);
+    d_off[i] = static_cast<uint32_t>((pos * f.heads * f.group + head) * D + c) * sizeof(T);
+  }
   // Rows 64 block .. +63; past the sequence its last one's again, at no position.
   auto load = [&](int block, int buf) {
     const int q0 = block * kKeys / f.group, rem = block * kKeys % f.group;
@@ -563,7 +618,17 @@ __global__ __launch_bounds__(256, 2) void window_dkdv_kernel(WinBwdArgs<T> b) {
         load_lds<4>(b.delta + at, del_s[buf]);
       }
     }
+    if (even && q0 + kKeys / f.group <= len) {
+      const T* qb = a.q + (s0 + q0) * a.q_token + h * a.q_head;
+      const T* db = a.out + (static_cast<int64_t>(s0 + q0) * f.heads + h) * f.group * D;
 #pragma unroll
+      for (int i = 0; i < TL::kLoads; ++i) {
+        TL::load(qb, q_off[i], qs[buf], wave, i);
+        TL::load(db, d_off[i], dos[buf], wave, i);
+      }
+      return;
+    }
+#pragma unroll 1
     for (int i = 0; i < TL::kLoads; ++i) {
       const int r = TL::row(wave, i), c = TL::col(r);
       int pos, head;
@@ -761,19 +826,10 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(WinBwdArgs<T> b) {
 #pragma unroll
     for (int qt = 0; qt < 2; ++qt) dqt[dt][qt] = f32x4v{0.f, 0.f, 0.f, 0.f};
   const KeyTiles tiles(f, q0, q1);
-  const T* kh = a.k + s0 * a.k_token + h * a.k_head;
-  const T* vh = a.v + s0 * a.v_token + h * a.v_head;
   TL tl(g, lr);
   const float score_log2 = a.scale_log2 * a.sign;
-  auto load = [&](int v) {   // (as the forward's)
-    const int base = tiles.tile(v) * kKeys;
-#pragma unroll
-    for (int i = 0; i < TL::kLoads; ++i) {
-      const int r = TL::row(wave, i), key = min(base + r, len - 1), c = TL::col(r);
-      TL::load(kh + key * a.k_token + c, ks[v & 1], wave, i);
-      TL::load(vh + key * a.v_token + c, vs[v & 1], wave, i);
-    }
-  };
+  const KeyLoads<T, D> keys(a, s0, h, len, wave);
+  auto load = [&](int v) { keys(tiles.tile(v) * kKeys, ks[v & 1], vs[v & 1], wave); };
   load(0);
   for (int v = 0; v < tiles.count; ++v) {
     const int kbase = tiles.tile(v) * kKeys, buf = v & 1;
