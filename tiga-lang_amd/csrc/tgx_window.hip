@@ -1081,8 +1081,13 @@ extern "C" int tgx_window_tasks(const int32_t* cu_host, int n_blocks, int heads,
     queue[std::min<int64_t>(kXcds - 1, done * kXcds / std::max<int64_t>(total, 1))].push_back(i);
     done += tasks[i].work;
   }
+  // The largest first: the rounds of workgroups then end evenly.
   size_t longest = 0;
-  for (const auto& x : queue) longest = std::max(longest, x.size());
+  for (auto& x : queue) {
+    std::stable_sort(x.begin(), x.end(),
+                     [&](size_t i, size_t j) { return tasks[i].work > tasks[j].work; });
+    longest = std::max(longest, x.size());
+  }
   const int64_t n = static_cast<int64_t>(longest) * kXcds;
   TGX_REQUIRE(n < kMaxBlocks256, "too many tasks");
   *n_tasks = n;
