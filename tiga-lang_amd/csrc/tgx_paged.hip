@@ -66,9 +66,12 @@ Cut cut_of(const tgx_paged& p, const tgx_paged_view& w, int heads, int group, in
       (tiles <= kWholeTiles && p.n_seqs * each >= cus))
     return Cut{1, p.n_seqs, false};
   Cut cut{wanted, 0, true};
-  // Workgroups of several heads: pieces of as many tiles a wave, and as many
-  // workgroups, as of one.
-  if (by_heads) cut.heads_held = heads % 4 == 0 ? 4 : heads % 2 == 0 ? 2 : 1;
+  // Workgroups of several heads, pieces of as many tiles a wave, and as many
+  // workgroups, as of one; not where the smallest pieces of all sequences are
+  // resident at once: the time is one of latency there, and more pieces to join
+  // (8 sequences that see 1088 keys, 8 heads: 14.8 us with one head, 17.8 with four).
+  const bool few = p.n_seqs * ceil_div(tiles, kMinTiles) * each <= int64_t{cus} * per_cu;
+  if (by_heads && !few) cut.heads_held = heads % 4 == 0 ? 4 : heads % 2 == 0 ? 2 : 1;
   cut.wanted *= cut.heads_held;
   cut.min_tiles = kMinTiles / cut.heads_held;
   cut.launched = std::min(cut.wanted + p.n_seqs, p.n_seqs * ceil_div(tiles, cut.min_tiles));

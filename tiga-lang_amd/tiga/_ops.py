@@ -438,6 +438,33 @@ def _window_strides(q, k, v):
                                 step(v, 0), step(v, 1))
 
 
+class WindowPlan:
+    """What attention over a windowed relation keeps for a head layout: its task
+    lists, the backward's workspace size and the strides of contiguous fields."""
+
+    def __init__(self, graph: Graph, n: int, heads: int, group: int, D: int):
+        self.cu, self.q_tasks, self.n_q, _ = graph._window_tasks(0, heads, group)
+        _, self.k_tasks, self.n_k, slots = graph._window_tasks(1, heads, group)
+        _, self.joins, self.n_joins, _ = graph._window_tasks(2, heads, group)
+        need = ctypes.c_size_t()
+        _native.call("tgx_window_attn_bwd_workspace", n, slots, heads, group, D,
+                     ctypes.byref(need))
+        self.work_bytes = need.value
+        self.strides = (ctypes.c_int64 * 7)(heads * group * D, group * D, D, heads * D, D,
+                                            heads * D, D)
+        self.forward = (self.cu.data_ptr(), self.q_tasks.data_ptr(), self.n_q)
+        self.backward = (*self.forward, self.k_tasks.data_ptr(), self.n_k, self.joins.data_ptr(),
+                         self.n_joins, slots)
+
+
+def _window_plan(graph: Graph, n: int, heads: int, group: int, D: int) -> WindowPlan:
+    key = ("window-plan", heads, group, D)
+    plan = graph._native_cache.get(key)
+    if plan is None:
+        plan = graph._native_cache[key] = WindowPlan(graph, n, heads, group, D)
+    return plan
+
+
 class WindowAttentionFunction(torch.autograd.Function):
     """Causal dot-product attention that looks back over the graph's window and
     sinks: q [n, heads, group, D], k and v [n, heads, D], bf16 or fp16, D in {32,
@@ -447,16 +474,21 @@ class WindowAttentionFunction(torch.autograd.Function):
     def forward(ctx, q, k, v, scale: float, graph: Graph):
         _on_graph_device(graph, q, k, v)
         n, heads, group, D = q.shape
-        q, k, v = _window_rows(q), _window_rows(k), _window_rows(v)
         out = torch.empty((n, heads, group, D), dtype=q.dtype, device=q.device)
         lse = torch.empty((n, heads, group), dtype=torch.float32, device=q.device)
+        plan = strides = None
         if n:
-            cu, tasks, count, _ = graph._window_tasks(0, heads, group)
-            _native.launch(q, "tgx_window_attn_fwd", cu.data_ptr(), tasks.data_ptr(), count,
-                           q.data_ptr(), k.data_ptr(), v.data_ptr(), _window_strides(q, k, v),
-                           float(scale), *graph._window, out.data_ptr(), lse.data_ptr(), n, heads,
-                           group, D, _ATTN_DTYPES[q.dtype])
-        ctx.graph, ctx.scale = graph, float(scale)
+            plan = _window_plan(graph, n, heads, group, D)
+            if q.is_contiguous() and k.is_contiguous() and v.is_contiguous() and \
+                    not (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
+                strides = plan.strides
+            else:
+                q, k, v = _window_rows(q), _window_rows(k), _window_rows(v)
+                strides = _window_strides(q, k, v)
+            _native.launch(q, "tgx_window_attn_fwd", *plan.forward, q.data_ptr(), k.data_ptr(),
+                           v.data_ptr(), strides, scale, *graph._window, out.data_ptr(),
+                           lse.data_ptr(), n, heads, group, D, _ATTN_DTYPES[q.dtype])
+        ctx.graph, ctx.scale, ctx.plan, ctx.strides = graph, scale, plan, strides
         ctx.save_for_backward(q, k, v, out, lse)
         return out
 
@@ -464,28 +496,23 @@ class WindowAttentionFunction(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse = ctx.saved_tensors
-        graph: Graph = ctx.graph
-        n, heads, group, D = q.shape
-        dout = dout.to(q.dtype).contiguous()
-        if dout.data_ptr() % 16:
-            dout = dout.clone()
+        graph, plan = ctx.graph, ctx.plan
+        n, heads, group, D = out.shape
         dq = torch.empty_like(out)
-        dk = torch.empty((n, heads, D), dtype=q.dtype, device=q.device)
+        dk = torch.empty((n, heads, D), dtype=out.dtype, device=out.device)
         dv = torch.empty_like(dk)
         if n:
-            cu, qtasks, nq, _ = graph._window_tasks(0, heads, group)
-            _, ktasks, nk, slots = graph._window_tasks(1, heads, group)
-            _, joins, nj, _ = graph._window_tasks(2, heads, group)
-            need = ctypes.c_size_t()
-            _native.call("tgx_window_attn_bwd_workspace", n, slots, heads, group, D,
-                         ctypes.byref(need))
-            work = torch.empty(need.value, dtype=torch.uint8, device=q.device)
-            _native.launch(q, "tgx_window_attn_bwd", cu.data_ptr(), qtasks.data_ptr(), nq,
-                           ktasks.data_ptr(), nk, joins.data_ptr(), nj, slots, q.data_ptr(),
-                           k.data_ptr(), v.data_ptr(), _window_strides(q, k, v), out.data_ptr(),
-                           lse.data_ptr(), dout.data_ptr(), ctx.scale, *graph._window,
-                           dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), n, heads, group, D,
-                           _ATTN_DTYPES[q.dtype], work.data_ptr(), need.value)
+            if dout.dtype != out.dtype:
+                dout = dout.to(out.dtype)
+            dout = dout.contiguous()
+            if dout.data_ptr() % 16:
+                dout = dout.clone()
+            work = torch.empty(plan.work_bytes, dtype=torch.uint8, device=out.device)
+            _native.launch(out, "tgx_window_attn_bwd", *plan.backward, q.data_ptr(), k.data_ptr(),
+                           v.data_ptr(), ctx.strides, out.data_ptr(), lse.data_ptr(),
+                           dout.data_ptr(), ctx.scale, *graph._window, dq.data_ptr(),
+                           dk.data_ptr(), dv.data_ptr(), n, heads, group, D,
+                           _ATTN_DTYPES[out.dtype], work.data_ptr(), plan.work_bytes)
         return dq, dk, dv, None, None
 
 
@@ -499,7 +526,7 @@ def window_attention(q, k, v, scale: float, heads: int, group: int, graph: Graph
     if k.ndim == 4:
         k, v = k[:, :, 0], v[:, :, 0]
     rows = q if q.ndim == 4 else q[:, :, None] if group == 1 else q[:, None]
-    return WindowAttentionFunction.apply(rows, k, v, scale, graph).view(q.shape)
+    return WindowAttentionFunction.apply(rows, k, v, float(scale), graph).view(q.shape)
 
 
 # ---------------------------------------------------------------------------
