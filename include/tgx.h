@@ -931,24 +931,25 @@ int tgx_window_tasks(const int32_t* cu_host, int n_blocks, int heads, int group,
                      int sinks, int kind, int32_t* tasks_host, int64_t* n_tasks,
                      int64_t* n_slots);
 
-/* out [n, heads, group, D] contiguous; lse [n, heads, group] fp32, for the backward: the
- * logarithm to base 2 of each row's sum of exponentials.
+/* out [n, heads, group, D] contiguous.  For the backward: rest, like out, what rounding
+ * took from it (NULL without a backward), and lse [n, heads, group] fp32, the logarithm
+ * to base 2 of each row's sum of exponentials.
  * strides, host array of seven, in elements, multiples of 8: q's token, head, group;
  * k's token, head; v's token, head. */
 int tgx_window_attn_fwd(const int32_t* cu_dev, const int32_t* tasks_dev, int64_t n_tasks,
                         const void* q, const void* k, const void* v, const int64_t* strides,
-                        float scale, int window, int sinks, void* out, float* lse, int64_t n,
-                        int heads, int group, int D, int dtype, void* stream);
+                        float scale, int window, int sinks, void* out, void* rest, float* lse,
+                        int64_t n, int heads, int group, int D, int dtype, void* stream);
 
-/* dq [n, heads, group, D], dk and dv [n, heads, D] from the forward's out and lse and
- * from dout (contiguous like out).  No atomics: the same inputs give the same bits. */
+/* dq [n, heads, group, D], dk and dv [n, heads, D] from the forward's out, rest and lse
+ * and from dout (contiguous like out).  No atomics: the same inputs give the same bits. */
 int tgx_window_attn_bwd_workspace(int64_t n, int64_t n_slots, int heads, int group, int D,
                                   size_t* bytes);
 int tgx_window_attn_bwd(const int32_t* cu_dev, const int32_t* q_tasks_dev, int64_t n_q_tasks,
                         const int32_t* k_tasks_dev, int64_t n_k_tasks, const int32_t* joins_dev,
                         int64_t n_joins, int64_t n_slots, const void* q, const void* k,
-                        const void* v, const int64_t* strides, const void* out, const float* lse,
-                        const void* dout, float scale, int window, int sinks, void* dq, void* dk,
+                        const void* v, const int64_t* strides, const void* out,
+                        const void* rest, const float* lse, const void* dout, float scale, int window, int sinks, void* dq, void* dk,
                         void* dv, int64_t n, int heads, int group, int D, int dtype,
                         void* workspace_dev, size_t workspace_bytes, void* stream);
 

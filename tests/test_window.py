@@ -213,8 +213,8 @@ def test_native_entries_refuse_what_they_do_not_take():
             task(**kw)
     one, seven = 0x1000, (ctypes.c_int64 * 7)(*[64] * 7)
     fwd = lambda q=one, s=seven, window=1, D=64, dtype=0, group=1, n=4: _native.call(
-        "tgx_window_attn_fwd", one, one, 8, q, one, one, s, 1.0, window, 0, one, one, n, 1, group, D,
-        dtype, None)
+        "tgx_window_attn_fwd", one, one, 8, q, one, one, s, 1.0, window, 0, one, one, one, n, 1, group,
+        D, dtype, None)
     for kw in (dict(q=None), dict(q=one + 8), dict(s=None), dict(s=(ctypes.c_int64 * 7)(*[4] * 7)),
                dict(window=0), dict(group=0), dict(group=129), dict(n=-1), dict(n=2**31)):
         with pytest.raises(RuntimeError):
@@ -226,7 +226,7 @@ def test_native_entries_refuse_what_they_do_not_take():
     _native.call("tgx_window_attn_bwd_workspace", 4, 3, 1, 1, 64, ctypes.byref(need))
     bwd = lambda work=one, size=need.value, dq=one: _native.call(
         "tgx_window_attn_bwd", one, one, 8, one, 8, one, 1, 3, one, one, one, seven, one, one, one,
-        1.0, 1, 0, dq, one, one, 4, 1, 1, 64, 0, work, size, None)
+        one, 1.0, 1, 0, dq, one, one, 4, 1, 1, 64, 0, work, size, None)
     for kw in (dict(work=None), dict(size=need.value - 1), dict(dq=None), dict(dq=one + 8)):
         with pytest.raises(RuntimeError):
             bwd(**kw)

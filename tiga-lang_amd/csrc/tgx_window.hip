@@ -21,8 +21,12 @@
 // against some 4 D / window bytes a pair).
 //
 // Rounding.  Scores, softmax statistics, delta and all sums are fp32; P and dS are
-// rounded to the inputs' type to be multiplied (half a step of each, whose
-// errors do not add up in one direction; the sum of the weights is of the rounded ones).
+// rounded to the inputs' type to be multiplied (half a step of each, whose errors do
+// not add up in one direction; the sum of the weights is of the rounded ones: of the
+// others it would take 5% longer for a tenth of the error).  With a backward to come the
+// forward also stores what rounding took from the output (`rest`), for delta: without
+// it dQ and dK were 1.5 times (window of 2: 2.4 times) as far off as results rounded
+// once are, with it 1.45 times, for 3% of a training step.
 //
 // Keys and rows that a row does not see never reach it, whatever they hold: a masked
 // tile that has a NaN or Inf among what it contracts over is multiplied row by row.
@@ -64,12 +68,13 @@ struct WinArgs {
   float scale_log2;    // |scale| log2(e); 1 for a scale of 0
   float sign;          // what the queries are multiplied by first: 1, -1 or 0
   T* out;              // [n, heads, group, D]; backward: dO
+  T* rest;             // forward: out before rounding less out, or null
   float* lse;          // [n, heads, group]: log2 of the sum of 2^(scores * scale_log2)
 };
 
 // Position and head in the group of the row that lies `r` (< 128) rows behind row
-// q0 * group + rem.  Exact: n = rem + r < 256, group <= 128, so n times the excess of
-// by_group over 2^16 / group is below 2^16.
+// q0 * group + rem.  Exact: n = rem + r < 256 times the excess (< 1) of by_group over
+// 2^16 / group is below 2^16 / group (>= 512), what parts two quotients.
 __device__ __forceinline__ void split_row(const Form& f, int q0, int rem, int r, int& pos, int& g) {
   const uint32_t n = static_cast<uint32_t>(rem + r);
   const uint32_t up = (n * f.by_group) >> 16;
@@ -503,10 +508,15 @@ __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs<T
     T* row = a.out + at[qt] * D;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
-      vec4<T> w;
+      vec4<T> w, rest;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) w[r] = static_cast<T>(o[dt][qt][r] * inv);
+      for (int r = 0; r < 4; ++r) {
+        const float x = o[dt][qt][r] * inv;
+        w[r] = static_cast<T>(x);
+        rest[r] = static_cast<T>(x - static_cast<float>(w[r]));
+      }
       *reinterpret_cast<vec4<T>*>(row + 16 * dt + 4 * g) = w;
+      if (a.rest) *reinterpret_cast<vec4<T>*>(a.rest + at[qt] * D + 16 * dt + 4 * g) = rest;
     }
     if (g == 0) a.lse[at[qt]] = m[qt] + __log2f(l);
   }
@@ -519,6 +529,7 @@ __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs<T
 template <typename T, int D>
 __global__ __launch_bounds__(256) void window_delta_kernel(const T* __restrict__ dout,
                                                            const T* __restrict__ out,
+                                                           const T* __restrict__ rest,
                                                            float* __restrict__ delta,
                                                            int64_t rows) {
   constexpr int LPR = D / 8;
@@ -526,9 +537,10 @@ __global__ __launch_bounds__(256) void window_delta_kernel(const T* __restrict__
   float s = 0.f;
   if (row < rows) {
     const int64_t off = row * D + threadIdx.x % LPR * 8;
-    const vec8<T> x = ld8(dout + off), y = ld8(out + off);
+    const vec8<T> x = ld8(dout + off), y = ld8(out + off), z = ld8(rest + off);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s += static_cast<float>(x[j]) * static_cast<float>(y[j]);
+    for (int j = 0; j < 8; ++j)
+      s += static_cast<float>(x[j]) * (static_cast<float>(y[j]) + static_cast<float>(z[j]));
   }
   s = group_sum<LPR>(s);
   if (row < rows && threadIdx.x % LPR == 0) delta[row] = s;
@@ -1108,20 +1120,22 @@ extern "C" int tgx_window_tasks(const int32_t* cu_host, int n_blocks, int heads,
 extern "C" int tgx_window_attn_fwd(const int32_t* cu_dev, const int32_t* tasks_dev,
                                    int64_t n_tasks, const void* q, const void* k, const void* v,
                                    const int64_t* strides, float scale, int window, int sinks,
-                                   void* out, float* lse, int64_t n, int heads, int group, int D,
-                                   int dtype, void* stream) {
+                                   void* out, void* rest, float* lse, int64_t n, int heads,
+                                   int group, int D, int dtype, void* stream) {
   const WinShape s{n, heads, group, D, dtype};
   if (int st = check_shape(s, strides, window, sinks)) return st;
   TGX_REQUIRE(n_tasks >= 0 && n_tasks < kMaxBlocks256, "bad task count");
   if (n == 0 || n_tasks == 0) return TGX_OK;
   TGX_REQUIRE(cu_dev && tasks_dev && q && k && v && out && lse, "null pointer");
-  TGX_REQUIRE(on16(q) && on16(k) && on16(v) && on16(out), "operands must start on 16 bytes");
+  TGX_REQUIRE(on16(q) && on16(k) && on16(v) && on16(out) && on16(rest),
+              "operands must start on 16 bytes");
   hipStream_t hs = as_stream(stream);
   return with_tile(s, [&](auto t, auto d) -> int {
     typedef decltype(t) T;
     WinArgs<T> a = make_args<T>(s, cu_dev, q, k, v, strides, scale, window, sinks);
     a.tasks = tasks_dev;
     a.out = static_cast<T*>(out);
+    a.rest = static_cast<T*>(rest);
     a.lse = lse;
     TGX_PROFILE("window_fwd", hs);
     window_fwd_kernel<T, decltype(d)::value>
@@ -1142,8 +1156,8 @@ extern "C" int tgx_window_attn_bwd(const int32_t* cu_dev, const int32_t* q_tasks
                                    int64_t n_q_tasks, const int32_t* k_tasks_dev,
                                    int64_t n_k_tasks, const int32_t* joins_dev, int64_t n_joins,
                                    int64_t n_slots, const void* q, const void* k, const void* v,
-                                   const int64_t* strides, const void* out, const float* lse,
-                                   const void* dout, float scale, int window, int sinks, void* dq,
+                                   const int64_t* strides, const void* out, const void* rest,
+                                   const float* lse, const void* dout, float scale, int window, int sinks, void* dq,
                                    void* dk, void* dv, int64_t n, int heads, int group, int D,
                                    int dtype, void* workspace_dev, size_t workspace_bytes,
                                    void* stream) {
@@ -1154,11 +1168,11 @@ extern "C" int tgx_window_attn_bwd(const int32_t* cu_dev, const int32_t* q_tasks
                   n_slots >= 0,
               "bad task counts");
   if (n == 0 || n_q_tasks == 0) return TGX_OK;
-  TGX_REQUIRE(cu_dev && q_tasks_dev && k_tasks_dev && q && k && v && out && lse && dout && dq &&
-                  dk && dv && (n_joins == 0 || joins_dev),
+  TGX_REQUIRE(cu_dev && q_tasks_dev && k_tasks_dev && q && k && v && out && rest && lse && dout &&
+                  dq && dk && dv && (n_joins == 0 || joins_dev),
               "null pointer");
-  TGX_REQUIRE(on16(q) && on16(k) && on16(v) && on16(out) && on16(dout) && on16(dq) && on16(dk) &&
-                  on16(dv),
+  TGX_REQUIRE(on16(q) && on16(k) && on16(v) && on16(out) && on16(rest) && on16(dout) && on16(dq) &&
+                  on16(dk) && on16(dv),
               "operands must start on 16 bytes");
   size_t need = 0;
   if (int st = tgx_window_attn_bwd_workspace(n, n_slots, heads, group, D, &need)) return st;
@@ -1185,7 +1199,7 @@ extern "C" int tgx_window_attn_bwd(const int32_t* cu_dev, const int32_t* q_tasks
       TGX_REQUIRE(blocks <= kMaxBlocks256, "too many rows for one launch");
       TGX_PROFILE("window_delta", hs);
       window_delta_kernel<T, DD><<<dim3(static_cast<uint32_t>(blocks)), dim3(256), 0, hs>>>(
-          b.a.out, static_cast<const T*>(out), delta, rows);
+          b.a.out, static_cast<const T*>(out), static_cast<const T*>(rest), delta, rows);
       TGX_LAUNCHED("window_delta");
     }
     {

@@ -188,11 +188,11 @@ _SIGNATURES: dict[str, list] = {
                        c_int, c_int, c_vp],
     "tgx_window_tasks": [c_vp, c_int, c_int, c_int, c_int, c_int, c_int, c_vp, P(c_i64), P(c_i64)],
     "tgx_window_attn_fwd": [c_vp, c_vp, c_i64, c_vp, c_vp, c_vp, P(c_i64), c_f32, c_int, c_int,
-                            c_vp, c_vp, c_i64, c_int, c_int, c_int, c_int, c_vp],
+                            c_vp, c_vp, c_vp, c_i64, c_int, c_int, c_int, c_int, c_vp],
     "tgx_window_attn_bwd_workspace": [c_i64, c_i64, c_int, c_int, c_int, P(c_size)],
     "tgx_window_attn_bwd": [c_vp, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp,
-                            P(c_i64), c_vp, c_vp, c_vp, c_f32, c_int, c_int, c_vp, c_vp, c_vp,
-                            c_i64, c_int, c_int, c_int, c_int, c_vp, c_size, c_vp],
+                            P(c_i64), c_vp, c_vp, c_vp, c_vp, c_f32, c_int, c_int, c_vp, c_vp,
+                            c_vp, c_i64, c_int, c_int, c_int, c_int, c_vp, c_size, c_vp],
     "tgx_paged_append": [P(Paged), c_vp, c_vp, c_vp, c_vp, P(c_i64), c_vp, c_int, c_int, c_int,
                          c_vp],
     "tgx_select_pages_workspace": [P(Paged), c_int, c_int, P(c_size)],

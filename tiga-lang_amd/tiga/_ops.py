@@ -476,6 +476,8 @@ class WindowAttentionFunction(torch.autograd.Function):
         n, heads, group, D = q.shape
         out = torch.empty((n, heads, group, D), dtype=q.dtype, device=q.device)
         lse = torch.empty((n, heads, group), dtype=torch.float32, device=q.device)
+        # What rounding takes from the output, for the backward's row sums.
+        rest = torch.empty_like(out) if any(ctx.needs_input_grad) else None
         plan = strides = None
         if n:
             plan = _window_plan(graph, n, heads, group, D)
@@ -486,16 +488,16 @@ class WindowAttentionFunction(torch.autograd.Function):
                 q, k, v = _window_rows(q), _window_rows(k), _window_rows(v)
                 strides = _window_strides(q, k, v)
             _native.launch(q, "tgx_window_attn_fwd", *plan.forward, q.data_ptr(), k.data_ptr(),
-                           v.data_ptr(), strides, scale, *graph._window, out.data_ptr(),
+                           v.data_ptr(), strides, scale, *graph._window, out.data_ptr(), _p(rest),
                            lse.data_ptr(), n, heads, group, D, _ATTN_DTYPES[q.dtype])
         ctx.graph, ctx.scale, ctx.plan, ctx.strides = graph, scale, plan, strides
-        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.save_for_backward(q, k, v, out, rest, lse)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse = ctx.saved_tensors
+        q, k, v, out, rest, lse = ctx.saved_tensors
         graph, plan = ctx.graph, ctx.plan
         n, heads, group, D = out.shape
         dq = torch.empty_like(out)
@@ -509,8 +511,8 @@ class WindowAttentionFunction(torch.autograd.Function):
                 dout = dout.clone()
             work = torch.empty(plan.work_bytes, dtype=torch.uint8, device=out.device)
             _native.launch(out, "tgx_window_attn_bwd", *plan.backward, q.data_ptr(), k.data_ptr(),
-                           v.data_ptr(), ctx.strides, out.data_ptr(), lse.data_ptr(),
-                           dout.data_ptr(), ctx.scale, *graph._window, dq.data_ptr(),
+                           v.data_ptr(), ctx.strides, out.data_ptr(), rest.data_ptr(),
+                           lse.data_ptr(), dout.data_ptr(), ctx.scale, *graph._window, dq.data_ptr(),
                            dk.data_ptr(), dv.data_ptr(), n, heads, group, D,
                            _ATTN_DTYPES[out.dtype], work.data_ptr(), plan.work_bytes)
         return dq, dk, dv, None, None
