@@ -253,6 +253,17 @@ def test_what_is_refused():
         Sum()(graph=g, src={"x": tg.BlockScaled.zeros(8, 2, 8, block=4)}, dst={})
 
 
+def test_append_refuses_one_cache_for_keys_and_values():
+    """(Each would form the other's older codes again.)"""
+    g, x = graph(), torch.ones(4, 2, 8)
+    kc, vc = (tg.BlockScaled.zeros(PAGES * SIZE, 2, 8, block=BLOCK) for _ in range(2))
+    for other in (kc, tg.BlockScaled(kc.codes, vc.scales, block=BLOCK),
+                  tg.BlockScaled(vc.codes, kc.scales, block=BLOCK)):
+        with pytest.raises(ValueError, match="share"):
+            g.append(kc, x, other, x)
+    g.append(kc, x, vc, x)
+
+
 def test_native_entries_refuse_what_they_do_not_take():
     """Bad arguments come back as a status before anything is launched."""
     p = _native.Paged(None, 0, 0, 0x1000, 2, 1, 3, 8, 12, 1)

@@ -14,13 +14,23 @@ namespace {
 // V's become bf16 on their way to the wave's LDS rows.  bf16 holds any code, and a
 // weight times a value's scale for any scale, which fp16 would not: so weights
 // and values are multiplied in bf16 (two parts a weight) for fp16 queries too.
+//
+// A workgroup holds four adjacent key heads (two, or one, where they do not divide
+// so), a wave each, so that it reads whole stretches of a cache's slots: 4 sequences of
+// 100k-131k tokens, 8 x 4 heads of 128 in int8, took 222 us with one head a
+// workgroup, 197 with two, 184 with four; 64 sequences of 100-4000 95, 85 and 70 us.
+// What is left is the order of the reads: the loads alone, with nothing computed, take
+// 177 us.  64 keys a step keep as many bytes in flight at D = 128 as 32 of a 16-bit
+// cache (and measured as 32 do); narrower heads would not fit three and four
+// workgroups a CU with them.
 template <int D>
 constexpr int kKeys8 = D == 128 ? 64 : 32;
 template <typename T, int D, int CODE, bool WIN>
 __global__ __launch_bounds__(256, (D == 128 ? 2 : D == 64 ? 3 : 4)) void paged_tile8_kernel(
     PagedArgs a) {
   using VT = __bf16;
-  constexpr int K8 = kKeys8<D>, KT = K8 / 16, PART = 32, PT = PART / 16, ROW = kRow<D>, BYTES = D == 32 ? 8 : 16, NR = D == 128 ? 2 : 1;
+  constexpr int K8 = kKeys8<D>, KT = K8 / 16, PART = 32, PT = PART / 16, ROW = kRow<D>;
+  constexpr int BYTES = D == 32 ? 8 : 16, NR = D == 128 ? 2 : 1;   // a lane's part, parts
   using Raw = std::conditional_t<D == 32, u32x2, u32x4>;
   constexpr size_t kStage = sizeof(VT) * 4 * PART * ROW;
   constexpr size_t kWeights = sizeof(float) * 4 * PART * 16;
@@ -198,15 +208,16 @@ int launch_tiles(const PagedArgs& a, const Cut& cut, int held, hipStream_t strea
   const int64_t pieces = cut.launched * a.rel.heads * a.heads;
   TGX_PROFILE("paged_scaled_tiles", stream);
   if (held == 16) {
+    const int64_t blocks = ceil_div(cut.launched, 8) * 8 * a.rel.heads * a.heads / a.held;
     paged_tile8_kernel<T, D, CODE, WIN>
-        <<<dim3(static_cast<uint32_t>(ceil_div(cut.launched, 8) * 8 * a.rel.heads * a.heads / a.held)),
-           dim3(256), 0, stream>>>(a);
+        <<<dim3(static_cast<uint32_t>(blocks)), dim3(256), 0, stream>>>(a);
   } else {
     const dim3 grid(static_cast<uint32_t>(ceil_div(pieces, 8) * 8 * ceil_div(rows, held)));
     // (Chunks of rows are the work here: the bounds of a window cost nothing beside it.)
-    if (held == 32) paged_block_kernel<T, D, 2, 1, CODE, true><<<grid, dim3(256), 0, stream>>>(a);
-    else if (held == 64) paged_block_kernel<T, D, 1, 1, CODE, true><<<grid, dim3(256), 0, stream>>>(a);
-    else paged_block_kernel<T, D, 1, 2, CODE, true><<<grid, dim3(256), 0, stream>>>(a);
+    const dim3 all(256);
+    if (held == 32) paged_block_kernel<T, D, 2, 1, CODE, true><<<grid, all, 0, stream>>>(a);
+    else if (held == 64) paged_block_kernel<T, D, 1, 1, CODE, true><<<grid, all, 0, stream>>>(a);
+    else paged_block_kernel<T, D, 1, 2, CODE, true><<<grid, all, 0, stream>>>(a);
   }
   TGX_LAUNCHED("paged_scaled_tiles");
   return TGX_OK;

@@ -18,12 +18,16 @@
 // Tiles.  Keys in tiles of 64 of the sequence; a query tile runs through those that
 // a row of it sees (the sinks', then the window's), masked where it does not see all
 // of one.  Bound: the matrix units (4 D operations a pair forward and 10 D backward,
-// against some 4 D / window bytes a pair).
+// against some 4 D / window bytes a pair); at two waves a SIMD the latency between
+// LDS, products and softmax stays.  17k tokens, 4 x 4 heads of 128, bf16, a window of
+// 1024: forward 185 us with a backward to come (490 TFLOP/s of what is seen), dK/dV 385
+// us (470), dQ 200 us (680 with the scores and dP that it forms again; keeping dS for it
+// would move 1.3 GB); a prompt of 32768, 8 x 4 heads: 700 us (785).
 //
 // Rounding.  Scores, softmax statistics, delta and all sums are fp32; P and dS are
 // rounded to the inputs' type to be multiplied (half a step of each, whose errors do
 // not add up in one direction; the sum of the weights is of the rounded ones: of the
-// others it would take 5% longer for a tenth of the error).  With a backward to come the
+// others it would take 3% longer for a tenth of the error).  With a backward to come the
 // forward also stores what rounding took from the output (`rest`), for delta: without
 // it dQ and dK were 1.5 times (window of 2: 2.4 times) as far off as results rounded
 // once are, with it 1.45 times, for 3% of a training step.
@@ -307,8 +311,10 @@ __device__ __forceinline__ void add_seen(const char* x, int r0, const float* w, 
 }
 
 // ---------------------------------------------------------------------------
-// Forward: a workgroup per tile of 128 rows, a wave per 32 of them, as the dense
-// tiles do it: S^T = K Q^T, so that a lane's results are four keys of one row for
+// Forward: a workgroup per tile of 128 rows, a wave per 32 of them, tiles of keys two
+// deep in LDS with one barrier each (the prompt of 32768: 782 us with tiles staged
+// through registers, 726 so, 700 with parts' offsets formed once), as the dense tiles
+// do it: S^T = K Q^T, so that a lane's results are four keys of one row for
 // each 16 keys, which is P^T as the B operand of O^T = V^T P^T.
 
 template <typename T, int D>
@@ -345,7 +351,7 @@ __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs<T
     int head;
     split_row(f, q0, rem, 32 * wave + 16 * qt + lr, qpos[qt], head);
     const bool ok = qpos[qt] < len;
-    const int64_t token = s0 + qpos[qt];
+    const int64_t token = int64_t{s0} + qpos[qt];
     at[qt] = ok ? (token * f.heads + h) * f.group + head : -1;
     const T* row = a.q + token * a.q_token + h * a.q_head + head * a.q_group;
 #pragma unroll
@@ -605,7 +611,8 @@ __global__ __launch_bounds__(256, 2) void window_dkdv_kernel(WinBwdArgs<T> b) {
   TL tl(g, lr);
   // Where the group divides 64 the parts' offsets are the same for every whole block.
   const bool even = kKeys % f.group == 0 && a.q_token < kMaxTokenStride &&
-                    a.q_group < kMaxTokenStride && f.heads * f.group * D < kMaxTokenStride;
+                    a.q_group < kMaxTokenStride &&
+                    int64_t{f.heads} * f.group * D < kMaxTokenStride;
   uint32_t q_off[TL::kLoads], d_off[TL::kLoads];
 #pragma unroll
   for (int i = 0; i < TL::kLoads; ++i) {
@@ -622,7 +629,8 @@ __global__ __launch_bounds__(256, 2) void window_dkdv_kernel(WinBwdArgs<T> b) {
     if (wave < 2) {
       int pos, head;
       split_row(f, q0, rem, lane, pos, head);
-      const int64_t at = (static_cast<int64_t>(s0 + min(pos, len - 1)) * f.heads + h) * f.group + head;
+      const int64_t token = s0 + min(pos, len - 1);
+      const int64_t at = (token * f.heads + h) * f.group + head;
       if (wave == 0) {
         load_lds<4>(a.lse + at, lse_s[buf]);
         pos_s[buf][lane] = pos < len ? pos : -1;
@@ -1157,10 +1165,10 @@ extern "C" int tgx_window_attn_bwd(const int32_t* cu_dev, const int32_t* q_tasks
                                    int64_t n_k_tasks, const int32_t* joins_dev, int64_t n_joins,
                                    int64_t n_slots, const void* q, const void* k, const void* v,
                                    const int64_t* strides, const void* out, const void* rest,
-                                   const float* lse, const void* dout, float scale, int window, int sinks, void* dq,
-                                   void* dk, void* dv, int64_t n, int heads, int group, int D,
-                                   int dtype, void* workspace_dev, size_t workspace_bytes,
-                                   void* stream) {
+                                   const float* lse, const void* dout, float scale, int window,
+                                   int sinks, void* dq, void* dk, void* dv, int64_t n, int heads,
+                                   int group, int D, int dtype, void* workspace_dev,
+                                   size_t workspace_bytes, void* stream) {
   const WinShape s{n, heads, group, D, dtype};
   if (int st = check_shape(s, strides, window, sinks)) return st;
   TGX_REQUIRE(n_q_tasks >= 0 && n_q_tasks < kMaxBlocks256 && n_k_tasks >= 0 &&

@@ -281,13 +281,17 @@ def _append_scaled(state, key_cache, key, value_cache, value, page_sums, plan) -
     if carries_tangent(key, value, page_sums, key_cache.scales, value_cache.scales):
         raise NotImplementedError("append has no forward-mode derivative: detach its operands")
     strides, dense, heads, D, dtype, code, block = plan
+    k, v = key_cache.codes, value_cache.codes
+    if k.numel() and (k.data_ptr() == v.data_ptr() or
+                      key_cache.scales.data_ptr() == value_cache.scales.data_ptr()):
+        raise ValueError("key_cache and value_cache must not share their codes or scales: each "
+                         "is written by its own rows")
     if _scaled_on_torch_operations("append", D, (key_cache, value_cache)):
         for cache, new in ((key_cache, key), (value_cache, value)):
             _append_scaled_torch(state, cache, new)
         if page_sums is not None:
             _sum_scaled_torch(state, key_cache, page_sums)
         return
-    k, v = key_cache.codes, value_cache.codes
     if key.numel() == 0 or k.numel() == 0:
         return
     at = key.data_ptr(), value.data_ptr()

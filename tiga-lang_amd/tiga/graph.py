@@ -434,8 +434,10 @@ class Graph:
         those sources, itself among them, and to the sequence's first `sinks`.
         Dot-product attention over it runs in tiles that read only what is
         seen, with gradients: bf16 and fp16, widths 32, 64 and 128, query heads
-        grouped on key heads if the fields broadcast (query [tokens, heads, group,
-        D] on key and value [tokens, heads, 1, D]).
+        grouped on key heads, up to 128 on one, if the fields broadcast (query
+        [tokens, heads, group, D] on key and value [tokens, heads, 1, D]).  Until its
+        backward a call keeps the output in two 16-bit parts.  Other types and widths
+        run on the materialized CSR.
         """
         cls._validate_index_tensor("cu_seqlens", cu_seqlens)
         if not isinstance(causal, bool):
@@ -647,7 +649,8 @@ class Graph:
 
         Each sequence's written pages must be its own and named once in its
         table (two writers of a slot leave either's row there), and key and
-        value must not lie in the caches they are written to."""
+        value must not lie in the caches they are written to.  Caches in 8 bits must
+        not share codes or scales with each other."""
         state = self.paged_state
         tensors = (key_cache, key, value_cache, value, page_sums)
         try:
