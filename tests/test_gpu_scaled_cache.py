@@ -644,6 +644,28 @@ def test_another_stream():
     assert torch.equal(a, b) and torch.equal(rk, g.read(kc, vc)[0])
 
 
+def test_codes_of_one_layout_at_other_addresses():
+    """A kept call takes codes that do not start on 8 bytes, too."""
+    rng = np.random.default_rng(5)
+    table, length, pages = relation(rng, [100, 33], 16)
+    g = tg.Graph.paged(dev(table, torch.int32), dev(length, torch.int32), page_size=16,
+                       num_pages=pages)
+    c, _ = cache(rng, pages * 16, 2, 64, "int8", 16)
+    n = c.codes.numel()
+    room = torch.zeros(n + 8, dtype=torch.int8, device=DEV)
+    q = dev(rng.standard_normal((2, 2, 64)), torch.bfloat16)
+    kernel, got = Attention(), []
+    for at in (0, 8, 4, 3, 0):
+        codes = room[at:at + n].view(c.codes.shape)
+        codes.copy_(c.codes)
+        held = tg.BlockScaled(codes, c.scales, block=16)
+        got.append(kernel(graph=g, src={"key": held, "value": held}, dst={"query": q}, scale=0.125))
+    # (By eights or sixteens: each within half a step of the same value, and sums of
+    # values below 4 in two parts of a weight and another order within 4 2^-15.)
+    assert all(torch.allclose(x.float(), got[0].float(), rtol=2 * HALF["bf16"], atol=2.0 ** -13)
+               for x in got)
+
+
 def test_empty_calls():
     table = torch.zeros(0, 3, dtype=torch.int32, device=DEV)
     lengths = torch.zeros(0, dtype=torch.int32, device=DEV)

@@ -512,8 +512,8 @@ class WindowAttentionFunction(torch.autograd.Function):
             work = torch.empty(plan.work_bytes, dtype=torch.uint8, device=out.device)
             _native.launch(out, "tgx_window_attn_bwd", *plan.backward, q.data_ptr(), k.data_ptr(),
                            v.data_ptr(), ctx.strides, out.data_ptr(), rest.data_ptr(),
-                           lse.data_ptr(), dout.data_ptr(), ctx.scale, *graph._window, dq.data_ptr(),
-                           dk.data_ptr(), dv.data_ptr(), n, heads, group, D,
+                           lse.data_ptr(), dout.data_ptr(), ctx.scale, *graph._window,
+                           dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), n, heads, group, D,
                            _ATTN_DTYPES[out.dtype], work.data_ptr(), plan.work_bytes)
         return dq, dk, dv, None, None
 

@@ -133,7 +133,8 @@ def bind_attention(graph, q, k, v, scale: float, heads: int, group: int):
     q, view = _on_16_bytes(q), _view(state, k, v)
     fields = (k, v)
     if isinstance(k, BlockScaled):
-        k, v = k.codes, v.codes
+        # (Another call's of the same layout may lie elsewhere.)
+        k, v = (c.codes if c.codes.data_ptr() % 8 == 0 else c.codes.clone() for c in (k, v))
     else:
         k, v = fields = (_on_16_bytes(k), _on_16_bytes(v))
     tables = state.table_heads
@@ -281,12 +282,14 @@ def _append_scaled(state, key_cache, key, value_cache, value, page_sums, plan) -
     if carries_tangent(key, value, page_sums, key_cache.scales, value_cache.scales):
         raise NotImplementedError("append has no forward-mode derivative: detach its operands")
     strides, dense, heads, D, dtype, code, block = plan
+    on_torch = _scaled_on_torch_operations("append", D, (key_cache, value_cache))
     k, v = key_cache.codes, value_cache.codes
-    if k.numel() and (k.data_ptr() == v.data_ptr() or
-                      key_cache.scales.data_ptr() == value_cache.scales.data_ptr()):
+    if key.numel() and k.numel() and (
+            k.data_ptr() == v.data_ptr() or
+            key_cache.scales.data_ptr() == value_cache.scales.data_ptr()):
         raise ValueError("key_cache and value_cache must not share their codes or scales: each "
                          "is written by its own rows")
-    if _scaled_on_torch_operations("append", D, (key_cache, value_cache)):
+    if on_torch:
         for cache, new in ((key_cache, key), (value_cache, value)):
             _append_scaled_torch(state, cache, new)
         if page_sums is not None:

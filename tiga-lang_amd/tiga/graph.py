@@ -437,7 +437,8 @@ class Graph:
         grouped on key heads, up to 128 on one, if the fields broadcast (query
         [tokens, heads, group, D] on key and value [tokens, heads, 1, D]).  Until its
         backward a call keeps the output in two 16-bit parts.  Other types and widths
-        run on the materialized CSR.
+        run on Torch operations over the materialized CSR (``tiga.config.strict`` refuses
+        them).
         """
         cls._validate_index_tensor("cu_seqlens", cu_seqlens)
         if not isinstance(causal, bool):

@@ -932,7 +932,7 @@ class MessagePassing(Kernel):
 
         def bind(q, k, v):
             if any(t.data_ptr() % 16 for t in ((q,) if scaled else (q, k, v))) or \
-                    not _paged.rows_on_16_bytes(q):
+                    not _paged.rows_on_16_bytes(q) or not _paged.cache_rows_ok(k, v):
                 return None     # the launch reads a copy, which would not stay live
             return _paged.bind_attention(graph, q, k, v, scale, heads, group)
 
