@@ -865,8 +865,8 @@ int tgx_paged_attn_view(const tgx_paged* p, const tgx_paged_view* view, const vo
 /* tgx_paged_append into a cache of codes (Graph.append, tiga.BlockScaled): for each
  * touched block of `block` slots and head, with M = 448 (E4M3) or 127 (INT8),
  *   s = the smallest power of two >= 2^-126 with max |new| <= M s, or the scale of
- *       the block's older tokens, if there are any and it is more; NaN if a new
- *       value is a NaN or an infinity, or that scale is NaN
+ *       the block's older tokens, if there are any and its magnitude is as large (it
+ *       may be negative); NaN if a new value is a NaN or an infinity, or that scale is NaN
  *   code = new / s to nearest, ties to even; older codes times old scale / s likewise
  * New rows of bf16, fp16 or fp32 (dtype); D a multiple of 8 up to 512; scales fp32
  * [slots / block, heads] contiguous; page sums of the rows as they are held.

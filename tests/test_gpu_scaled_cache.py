@@ -687,3 +687,45 @@ def test_empty_calls():
     out = Attention()(graph=none, src={"key": c.grouped(), "value": c.grouped()},
                       dst={"query": x[:, :, None]}, scale=1.0)
     assert not out.any()
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("queries", [1, 5, 40])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_scales_of_either_sign(code, queries, dtype):
+    """Caches stored elsewhere, with negative scales that are no powers of two: a code by -s
+    is the opposite code by s, so what append leaves follows from positive scales."""
+    print(f"{code} {dtype} queries={queries}", flush=True)
+    rng = np.random.default_rng(40 + queries)
+    size, block, heads, D = 16, 8, 3, 64
+    table, length, pages = relation(rng, [3, 15, 22, 60], size)
+    g = tg.Graph.paged(torch.tensor(table, device=DEV), torch.tensor(length, device=DEV),
+                       page_size=size, num_pages=pages, queries=queries)
+    args = (table, length, size, pages)
+    caches, new, exp = [], [], []
+    for _ in range(2):
+        # (Of few bits, as the new values: a code times a scale is exact in 32 bits, and a
+        # quotient lies on a tie or away from it by far more than its rounding.)
+        scales = rng.integers(8, 16, (pages * size // block, heads)) * \
+            4.0 ** rng.integers(-8, 2, (pages * size // block, heads))
+        sign = rng.choice([-1, 1], size=scales.shape)
+        codes = want.rounded(rng.uniform(-want.LARGEST[code], want.LARGEST[code],
+                                         (pages * size, heads, D)), code)
+        held = dev(codes * np.repeat(sign, block, 0)[:, :, None]).to(CODES[code])
+        caches.append(tg.BlockScaled(held, dev(scales * sign), block=block))
+        big = 4.0 ** rng.integers(-3, 6, (len(length) * queries, heads, 1))
+        new.append(dev(rng.standard_normal((len(length) * queries, heads, D)) * big,
+                       torch.bfloat16).to(TYPES[dtype]))
+        exp.append(want.append(*args, queries, codes, scales, f64(new[-1]), code, block))
+    sums = torch.zeros(pages, heads, D, device=DEV)
+    g.append(caches[0], new[0], caches[1], new[1], page_sums=sums)
+    every = table.shape[1] * size
+    for c, (codes, scales) in zip(caches, exp):
+        assert np.array_equal(np.abs(f64(c.scales)), scales)
+        got = want.values(f64(c.codes.float()), f64(c.scales), block)
+        assert np.array_equal(want.read(*args, every, got),
+                              want.read(*args, every, want.values(codes, scales, block)))
+    total, most = (want.page_sums(*args, queries, x, np.zeros((pages, heads, D)))
+                   for x in (want.values(*exp[0], block), np.abs(want.values(*exp[0], block))))
+    # A page's sum: at most 16 values, each addition off by half a step of the sum so far.
+    assert (np.abs(f64(sums) - total) <= (size + 1) * 2.0 ** -24 * most).all()

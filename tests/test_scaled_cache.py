@@ -310,3 +310,55 @@ def test_native_entries_refuse_what_they_do_not_take():
             read(**kw)
     with pytest.raises(NotImplementedError):
         read(D=12)
+
+
+def signed(rng, code, heads=2, D=8, slots=PAGES * SIZE, block=BLOCK):
+    """A cache stored elsewhere, whose scales are of either sign and no powers of two, and
+    the same rows by positive scales: (cache, codes, scales)."""
+    scales = rng.integers(8, 16, (slots // block, heads)) * \
+        4.0 ** rng.integers(-11, 2, (slots // block, heads))
+    sign = rng.choice([-1, 1], size=scales.shape)
+    codes = want.rounded(rng.uniform(-want.LARGEST[code], want.LARGEST[code], (slots, heads, D)),
+                         code)
+    held = codes * np.repeat(sign, block, 0)[:, :, None]
+    return tg.BlockScaled(torch.tensor(held, dtype=torch.float32).to(CODES[code]),
+                          torch.tensor(scales * sign, dtype=torch.float32), block=block), codes, scales
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("queries", [1, 3, 11])
+def test_scales_of_either_sign(code, queries):
+    """A code by -s is the opposite code by s: append leaves the rows that it leaves of the
+    same cache by positive scales."""
+    rng = np.random.default_rng(20 + queries)
+    lengths = torch.tensor([3, 15, 22, 40], dtype=torch.int32)
+    g = graph(queries, lengths)
+    (kc, kn, ks), (vc, vn, vs) = signed(rng, code), signed(rng, code)
+    big = np.exp(rng.standard_normal((4 * queries, 2, 1)) * 3)
+    k, v = (torch.tensor(rng.standard_normal((4 * queries, 2, 8)) * big).to(torch.float32)
+            for _ in range(2))
+    g.append(kc, k, vc, v)
+    args = (TABLE.numpy(), lengths.numpy(), SIZE, PAGES, queries)
+    for c, n, s, x in ((kc, kn, ks, k), (vc, vn, vs, v)):
+        codes, scales = want.append(*args, n, s, f64(x), code, BLOCK)
+        assert np.array_equal(np.abs(f64(c.scales)), scales)
+        rows = [want.read(*args[:4], 24, want.values(a, b, BLOCK)) for a, b in (
+            (f64(c.codes.float()), f64(c.scales)), (codes, scales))]
+        assert np.array_equal(*rows)                     # (of all positions that are cached)
+
+
+@pytest.mark.parametrize("code,scale,held", [("int8", -4.0, 100.0), ("int8", -8.0, 100.0),
+                                             ("e4m3", -1.0, 416.0), ("e4m3", -8.0, 104.0)])
+def test_small_tokens_behind_a_negative_scale(code, scale, held):
+    g = tg.Graph.paged(torch.tensor([[0]], dtype=torch.int32), torch.tensor([2], dtype=torch.int32),
+                       page_size=4, num_pages=1)
+    kc, vc = (tg.BlockScaled.zeros(4, 1, 8, block=4, dtype=CODES[code]) for _ in range(2))
+    kc.scales.fill_(scale)
+    kc.codes.view(torch.int8)[0] = torch.full((1, 8), held).to(CODES[code]).view(torch.int8)
+    before = kc.dequantize()[0].clone()
+    one = torch.ones(1, 1, 8)
+    g.append(kc, one, vc, one)
+    assert float(kc.scales) == scale
+    assert torch.equal(kc.dequantize()[0], before)
+    # What is new by that scale: to the nearest code, -1 / 4 and so on.
+    assert np.array_equal(f64(kc.codes.float())[1], want.rounded(np.full((1, 8), 1 / scale), code))

@@ -5,7 +5,8 @@
 // M the largest code:
 //
 //   s' = the smallest power of two >= 2^-126 with max |x| <= M s'
-//   s  = max(s', the scale of the block's older tokens), s' where there are none
+//   s  = the scale s_old of the block's older tokens where s' <= |s_old|, else s'
+//        (s' where there are none)
 //   code = rne(x / s);  an older token's code = rne(code * s_old / s)
 //
 // x / s is exact for a power of two, so a code is the definition's whatever the
@@ -120,8 +121,8 @@ __global__ __launch_bounds__(256) void append_scaled_kernel(ScaledAppendArgs a) 
 #pragma unroll
         for (int u = 0; u < kHold; ++u) top.see(x[u]);
         const float need = block_scale<CODE>(wave_largest(top.bits()));
-        // (Either one's NaN stays.)
-        scale = from == s0 || !(need <= scale) ? (scale != scale ? scale : need) : scale;
+        // By magnitude: a scale from elsewhere may be negative.  (Either one's NaN stays.)
+        scale = from == s0 || !(need <= fabsf(scale)) ? (scale != scale ? scale : need) : scale;
         if (lane == 0) *at = scale;
       }
       const bool lost = scale != scale;

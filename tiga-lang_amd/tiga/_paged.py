@@ -340,7 +340,9 @@ def _append_scaled_torch(state, cache, new) -> None:
     blocks = slots[:, :, 0] // block
     held = cache.scales[blocks]
     begun = (named[:, :, 0] & ~is_new[:, :, 0])[..., None]
-    scale = torch.where(begun, torch.maximum(scale, held), scale)
+    # (By magnitude: a scale from elsewhere may be negative.  Either one's NaN stays.)
+    stays = begun & ((scale <= held.abs()) | held.isnan())
+    scale = torch.where(stays, held, scale)
     raw = cache.codes.view(torch.int8)
     codes = raw[slots].view(dtype).float()
     # (By a NaN: codes whose values are NaN in any case.)

@@ -638,8 +638,8 @@ class Graph:
         whole blocks) are written from bf16, fp16 or fp32 rows, for each block and
         head by a power of two, with M = 448 (float8_e4m3fn) or 127 (int8):
 
-            s = the smallest power of two of at least 2^-126 with max |new| <= M s,
-                or the scale that the block's older tokens have, if that is more
+            s = the smallest power of two of at least 2^-126 with max |new| <= M s, or
+                the scale that the block's older tokens have, if its magnitude is as large
             code = new / s, rounded to nearest, ties to even
 
         A block whose scale grows has its older tokens' codes rounded again by the new
