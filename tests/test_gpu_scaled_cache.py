@@ -729,3 +729,24 @@ def test_scales_of_either_sign(code, queries, dtype):
                    for x in (want.values(*exp[0], block), np.abs(want.values(*exp[0], block))))
     # A page's sum: at most 16 values, each addition off by half a step of the sum so far.
     assert (np.abs(f64(sums) - total) <= (size + 1) * 2.0 ** -24 * most).all()
+
+
+@pytest.mark.parametrize("new", [1.0, 4096.0])
+def test_older_codes_that_are_nan_stay_nan(new):
+    """As on host tensors: an older e4m3 NaN reads back as one, whether the scale stays or
+    grows, and the other codes are those of the host's append."""
+    make = lambda where: tg.Graph.paged(
+        torch.tensor([[0]], dtype=torch.int32, device=where),
+        torch.tensor([3], dtype=torch.int32, device=where), page_size=4, num_pages=1)
+    raw = torch.zeros(4, 1, 8, dtype=torch.int8)
+    raw[:2] = torch.tensor([0x7F, -1, 0, -128, 1, 0x38, -0x48, 0x7E], dtype=torch.int8)
+    got = []
+    for where in ("cpu", DEV):
+        kc, vc = (tg.BlockScaled(raw.to(where, copy=True).view(CODES["e4m3"]),
+                                 torch.ones(1, 1, device=where), block=4) for _ in range(2))
+        x = torch.full((1, 1, 8), new, device=where)
+        make(where).append(kc, x, vc, x)
+        got.append((kc.dequantize().cpu(), kc.scales.cpu(), vc.dequantize().cpu()))
+    assert got[1][0][:2, 0, :2].isnan().all() and not got[1][0][:2, 0, 2:].isnan().any()
+    for a, b in zip(*got):
+        assert torch.equal(a.nan_to_num(9999), b.nan_to_num(9999))

@@ -362,3 +362,38 @@ def test_small_tokens_behind_a_negative_scale(code, scale, held):
     assert torch.equal(kc.dequantize()[0], before)
     # What is new by that scale: to the nearest code, -1 / 4 and so on.
     assert np.array_equal(f64(kc.codes.float())[1], want.rounded(np.full((1, 8), 1 / scale), code))
+
+
+@pytest.mark.parametrize("new,kept", [(1.0, True), (4096.0, False)])
+def test_older_codes_that_are_nan_stay_nan(new, kept):
+    """An older e4m3 NaN reads back as one where the scale stays and where it grows, and
+    what stays is what was there to the bit."""
+    g = tg.Graph.paged(torch.tensor([[0]], dtype=torch.int32), torch.tensor([3], dtype=torch.int32),
+                       page_size=4, num_pages=1)
+    kc, vc = (tg.BlockScaled.zeros(4, 1, 8, block=4) for _ in range(2))
+    kc.scales.fill_(1.0)
+    raw = kc.codes.view(torch.int8)
+    raw[:2] = torch.tensor([0x7F, -1, 0, -128, 1, 0x38, -0x48, 0x7E], dtype=torch.int8)
+    before = raw.clone()
+    x = torch.full((1, 1, 8), new)
+    g.append(kc, x, vc, x)
+    rows = kc.dequantize()
+    assert rows[:2, 0, :2].isnan().all() and not rows[:2, 0, 2:].isnan().any()
+    assert (float(kc.scales) == 1.0) is kept and torch.equal(rows[2], x[0])
+    if kept:
+        assert torch.equal(raw[:2], before[:2])
+
+
+def test_unlike_blocks_of_one_call_keep_their_codes():
+    """Of two heads one's scale grows: the other's older codes are not written."""
+    g = tg.Graph.paged(torch.tensor([[0]], dtype=torch.int32), torch.tensor([3], dtype=torch.int32),
+                       page_size=4, num_pages=1)
+    kc, vc = (tg.BlockScaled.zeros(4, 2, 8, block=4, dtype=torch.int8) for _ in range(2))
+    kc.scales.fill_(0.5)
+    kc.codes[:2] = torch.tensor([-128, 127, 3, -1, 0, 5, 64, -64], dtype=torch.int8)
+    x = torch.tensor([1.0, 100.0])[None, :, None].expand(1, 2, 8)
+    g.append(kc, x, vc, x)
+    assert kc.scales.tolist() == [[0.5, 1.0]]
+    assert kc.codes[0, 0].tolist() == [-128, 127, 3, -1, 0, 5, 64, -64]
+    # Halves, ties to even.
+    assert kc.codes[0, 1].tolist() == [-64, 64, 2, 0, 0, 2, 32, -32]

@@ -344,12 +344,15 @@ def _append_scaled_torch(state, cache, new) -> None:
     stays = begun & ((scale <= held.abs()) | held.isnan())
     scale = torch.where(stays, held, scale)
     raw = cache.codes.view(torch.int8)
-    codes = raw[slots].view(dtype).float()
-    # (By a NaN: codes whose values are NaN in any case.)
-    ratio = torch.where(begun, torch.nan_to_num(held / scale, nan=1.0), 1.0)
-    got = torch.where(is_new[..., None, None], x / scale[:, :, None, :, None],
-                      codes * ratio[:, :, None, :, None])
-    raw[slots[named]] = encode(got, dtype).view(torch.int8)[named]
+    older = raw[slots]
+    got = encode(x / scale[:, :, None, :, None], dtype).view(torch.int8)
+    # Older codes of a scale that stays, or by a NaN, stay as they are; others are rounded
+    # again (and a NaN among them stays one).
+    moved = older.view(dtype).float() * (held / scale)[:, :, None, :, None]
+    moved = torch.where(moved.isnan(), older, encode(moved, dtype).view(torch.int8))
+    again = (begun & (held != scale) & ~scale.isnan())[:, :, None, :, None]
+    got = torch.where(is_new[..., None, None], got, torch.where(again, moved, older))
+    raw[slots[named]] = got[named]
     touched = is_new.any(-1)
     cache.scales[blocks[touched]] = scale[touched]
 
