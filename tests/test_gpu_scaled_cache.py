@@ -750,3 +750,26 @@ def test_older_codes_that_are_nan_stay_nan(new):
     assert got[1][0][:2, 0, :2].isnan().all() and not got[1][0][:2, 0, 2:].isnan().any()
     for a, b in zip(*got):
         assert torch.equal(a.nan_to_num(9999), b.nan_to_num(9999))
+
+
+def test_a_prepared_call_differentiates_scales():
+    rng = np.random.default_rng(9)
+    table, length, pages = relation(rng, [40, 3], 16)
+    g = tg.Graph.paged(dev(table, torch.int32), dev(length, torch.int32), page_size=16,
+                       num_pages=pages)
+    (kc, _), (vc, _) = (cache(rng, pages * 16, 2, 64, "int8", 16) for _ in range(2))
+    q = dev(rng.standard_normal((2, 2, 3, 64)))
+    call = dict(graph=g, src={"key": kc.grouped(), "value": vc.grouped()}, dst={"query": q},
+                scale=0.125)
+    before = Attention().prepare(**call)
+    fast = before()
+    assert not fast.requires_grad
+    vc.scales.requires_grad_(True)
+    exp = torch.autograd.grad(Attention()(**call).square().sum(), vc.scales)[0]
+    for run in (before, Attention().prepare(**call)):
+        out = run()
+        # fp32 sums of at most 40 products, by two kernels.
+        assert torch.allclose(out, fast, rtol=1e-5, atol=1e-5 * float(fast.abs().max()))
+        assert torch.equal(torch.autograd.grad(out.square().sum(), vc.scales)[0], exp)
+    with torch.no_grad():
+        assert not before().requires_grad

@@ -397,3 +397,31 @@ def test_unlike_blocks_of_one_call_keep_their_codes():
     assert kc.codes[0, 0].tolist() == [-128, 127, 3, -1, 0, 5, 64, -64]
     # Halves, ties to even.
     assert kc.codes[0, 1].tolist() == [-64, 64, 2, 0, 0, 2, 32, -32]
+
+
+def test_a_prepared_call_differentiates_scales(monkeypatch):
+    """prepare()'s bound launch has no gradients: a field that wants them, a cache's scales
+    among them, takes the ordinary path.  (A stand-in for the launch, on the host.)"""
+    from tiga import message_passing as mp
+
+    rng = np.random.default_rng(8)
+    (kc, _, _), (vc, _, _) = cache(rng, "int8"), cache(rng, "int8")
+    g, kernel = graph(), Attention()
+    src, dst = {"key": kc.grouped(), "value": vc.grouped()}, {"query": torch.randn(4, 2, 3, 8)}
+    plain = lambda *_: Attention()(graph=g, src=src, dst=dst, scale=0.1)
+    bound = torch.zeros(4, 2, 3, 8)
+
+    def dispatch(self, *_):
+        self._launch = mp._Launch(
+            g, (("dst", "query"), ("src", "key"), ("src", "value")), plain, lambda: None,
+            variant=mp.CompiledVariant(key=(), backend="hip", provider="", pattern="", lowering=""),
+            bind=lambda *_: lambda: bound)
+        return plain()
+
+    monkeypatch.setattr(kernel, "_dispatch", dispatch.__get__(kernel))
+    run = kernel.prepare(graph=g, src=src, dst=dst, scale=0.1)
+    assert run() is bound
+    kc.scales.requires_grad_(True)
+    out = run()
+    assert torch.equal(out, plain()) and out.requires_grad
+    assert torch.autograd.grad(out.sum(), kc.scales)[0].abs().max() > 0

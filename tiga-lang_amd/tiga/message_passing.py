@@ -475,10 +475,10 @@ class MessagePassing(Kernel):
         runner, epilogue = launch.runner, self._epilogue
         frozen_dst, frozen_params = dict(dst), dict(params)
         bound = launch.bind(*operands) if launch.bind is not None else None
-        tensors = tuple(t for t in operands if isinstance(t, torch.Tensor))
+        fields = tuple(t for t in operands if isinstance(t, (torch.Tensor, BlockScaled)))
 
         def run():
-            if bound is not None and not any(t.requires_grad for t in tensors):
+            if bound is not None and not any(t.requires_grad for t in fields):
                 return epilogue(frozen_dst, bound(), frozen_params)
             return epilogue(frozen_dst, runner(*operands), frozen_params)
 
