@@ -925,7 +925,7 @@ int tgx_select_pages(const tgx_paged* p, const void* q_dev, const int64_t* strid
  *
  * tgx_window_tasks: the host lists of a relation (cu_host [n_blocks + 1]), XCD by
  * XCD.  kind 0: query tiles [n, 4]; 1: key tiles [n, 8], with *n_slots partial
- * sums; 2: the key tiles joined from those [n, 8].  tasks_host NULL asks for the
+ * sums (at most 3072, each 512 D bytes of the backward's workspace); 2: the key tiles joined from those [n, 8].  tasks_host NULL asks for the
  * counts.  The lists go to the device unchanged. */
 int tgx_window_tasks(const int32_t* cu_host, int n_blocks, int heads, int group, int window,
                      int sinks, int kind, int32_t* tasks_host, int64_t* n_tasks,

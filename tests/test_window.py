@@ -230,3 +230,22 @@ def test_native_entries_refuse_what_they_do_not_take():
     for kw in (dict(work=None), dict(size=need.value - 1), dict(dq=None), dict(dq=one + 8)):
         with pytest.raises(RuntimeError):
             bwd(**kw)
+
+
+@pytest.mark.parametrize("lengths,heads,group,window,sinks", [
+    ([131072], 8, 4, 128, 1024), ([32768], 8, 4, 256, 4096), ([131072], 8, 8, 1024, 8192),
+    ([20000] * 6, 4, 16, 64, 20000), ([300] * 500, 32, 1, 1, 64), ([1000000], 1, 1, 64, 64)])
+def test_partial_sums_are_bounded(lengths, heads, group, window, sinks):
+    """The backward's workspace does not grow with sinks times tokens: of all the work a
+    piece has at least 1 / 2048, and a tile that is cut more than two pieces' work."""
+    keys, slots, _ = tasks_of(lengths, heads, group, window, sinks, 1)
+    joins, same, _ = tasks_of(lengths, heads, group, window, sinks, 2)
+    assert same == slots == joins[:, 4].sum() and slots <= 3072
+    need = ctypes.c_size_t()
+    n = sum(lengths)
+    _native.call("tgx_window_attn_bwd_workspace", n, slots, heads, group, 128, ctypes.byref(need))
+    assert need.value <= 4 * n * heads * group + 256 + 3072 * 2 * 64 * 128 * 4
+    # Nothing is longer than the longest tile without sinks, or two pieces.
+    total = int(keys[:, 4].sum())
+    piece = max(-(-(window + 63) * group // 64), 16, -(-total // 2048))
+    assert keys[:, 4].max() <= max(2 * piece, -(-(window + 63) * group // 64) + 1)

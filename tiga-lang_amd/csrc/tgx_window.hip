@@ -1024,6 +1024,26 @@ RowRange rows_seeing(int64_t len, int64_t k0, int group, int64_t window, int64_t
   return {first, ceil_div(end * group, kKeys) - first};
 }
 
+// Row blocks of a piece of a key tile that holds sinks, which every later row of its
+// sequence sees: a window's rows, so that pieces are as long as other tiles' tasks, and
+// at least what leaves kMaxPieces of all the work, four for each workgroup that is
+// resident at once.  A tile is cut where it has more than two pieces' blocks, so there
+// are at most 1.5 kMaxPieces slots (192 MB at D = 128), however many sinks and
+// tokens.  131072 tokens, 8 x 4 heads, a window of 128 and 1024 sinks, a training step:
+// pieces of a window's rows alone took 4.3 GB of slots and 18.1 ms, so 0.12 GB and 14.5 ms.
+constexpr int64_t kMaxPieces = 4 * 2 * 256;
+int64_t blocks_of_a_piece(const int32_t* cu, int n_blocks, int heads, int group, int64_t window,
+                          int64_t sinks) {
+  int64_t total = 0;
+  for (int b = 0; b < n_blocks; ++b) {
+    const int64_t len = int64_t{cu[b + 1]} - cu[b];
+    for (int64_t k0 = 0; k0 < len; k0 += kKeys)
+      total += rows_seeing(len, k0, group, window, sinks).blocks;
+  }
+  return std::max({ceil_div((window + kKeys - 1) * group, kKeys), int64_t{16},
+                   ceil_div(total * heads, kMaxPieces)});
+}
+
 }  // namespace
 }  // namespace tgx
 
@@ -1043,6 +1063,8 @@ extern "C" int tgx_window_tasks(const int32_t* cu_host, int n_blocks, int heads,
   };
   std::vector<Task> tasks, joins;
   int64_t slots = 0;
+  const int64_t piece =
+      kind == 0 ? 0 : blocks_of_a_piece(cu_host, n_blocks, heads, group, window, sinks);
   for (int b = 0; b < n_blocks; ++b) {
     const int64_t len = int64_t{cu_host[b + 1]} - cu_host[b];
     TGX_REQUIRE(len >= 0 && cu_host[b] >= 0, "cu_seqlens must be non-decreasing from 0");
@@ -1057,10 +1079,6 @@ extern "C" int tgx_window_tasks(const int32_t* cu_host, int n_blocks, int heads,
         }
         continue;
       }
-      // A tile with sinks has its rows cut into pieces of a window's rows, where they
-      // are more than twice that.
-      const int64_t piece =
-          std::max<int64_t>(ceil_div((int64_t{window} + kKeys - 1) * group, kKeys), 16);
       for (int64_t k0 = 0; k0 < len; k0 += kKeys) {
         const RowRange rows = rows_seeing(len, k0, group, window, sinks);
         const int32_t key = static_cast<int32_t>(k0);
