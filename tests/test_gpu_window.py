@@ -305,3 +305,27 @@ def test_prompt_then_steps():
     for queries in (1, 7, n):
         step = call(make(queries), q[-queries:], kc[:, :, None], vc[:, :, None])
         assert (np.abs(f64(step) - f64(full[-queries:])) <= 2 * lim[-queries:]).all()
+
+
+def test_leaves_without_gradients_pay_for_no_backward():
+    """Under no_grad the output is the same and nothing else of its size is kept, also for
+    inputs that require gradients; a step with gradients on the same relation follows."""
+    rng = np.random.default_rng(10)
+    lengths = [4000]
+    q, k, v, d = inputs(rng, lengths, 4, 4, 128, "bf16")
+    leaf = q.clone().requires_grad_(True)
+    g = tg.Graph.cu_seqlens(packed(lengths), window=30, sinks=2)
+    call = lambda: Attention()(graph=g, src={"key": k, "value": v}, dst={"query": leaf}, scale=0.1)
+    with torch.no_grad():
+        call()
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        out = call()
+        grown = torch.cuda.max_memory_allocated() - before
+    size = out.numel() * out.element_size()
+    assert not out.requires_grad and size <= grown < 1.5 * size
+    got = run(g, q, k, v, d, 0.1)
+    assert torch.equal(got[0], out)
+    assert all(torch.equal(a, b) for a, b in zip(got, run(
+        tg.Graph.cu_seqlens(packed(lengths), window=30, sinks=2), q, k, v, d, 0.1)))

@@ -249,3 +249,36 @@ def test_partial_sums_are_bounded(lengths, heads, group, window, sinks):
     total = int(keys[:, 4].sum())
     piece = max(-(-(window + 63) * group // 64), 16, -(-total // 2048))
     assert keys[:, 4].max() <= max(2 * piece, -(-(window + 63) * group // 64) + 1)
+
+
+def test_a_forward_alone_prepares_no_backward(monkeypatch):
+    """Without gradients, also of inputs that want them elsewhere, a call forms no lists of
+    key tiles and has no second part of the output written.  (Launches are recorded only.)"""
+    from tiga import _ops
+
+    calls = []
+    monkeypatch.setattr(_native, "launch", lambda t, name, *args: calls.append((name, args)))
+    rng = np.random.default_rng(4)
+    mk = lambda *s: torch.tensor(rng.standard_normal(s)).to(torch.bfloat16).requires_grad_(True)
+    q, k, v = mk(70, 2, 3, 32), mk(70, 2, 1, 32), mk(70, 2, 1, 32)
+    g = tg.Graph.cu_seqlens(packed([40, 30]), window=5, sinks=1)
+    run = lambda q: _ops.window_attention(q, k, v, 0.2, 2, 3, g)
+    plan = lambda: g._native_cache["window-plan", 2, 3, 32]
+    rest = lambda: calls[-1][1][11]
+    with torch.no_grad():
+        assert not run(q).requires_grad
+    assert calls[-1][0] == "tgx_window_attn_fwd" and rest() is None
+    assert plan().backward is None and ("window", 1, 2, 3) not in g._native_cache
+    out = run(q.detach())                        # (the keys and values want gradients)
+    assert rest() and plan().backward is not None
+    grads = torch.autograd.grad(out, (k, v), torch.ones_like(out))
+    assert [c[0] for c in calls[-2:]] == ["tgx_window_attn_fwd", "tgx_window_attn_bwd"]
+    assert calls[-1][1][13] == calls[-2][1][11]
+    assert [x.shape for x in grads] == [k.shape, v.shape]
+    with torch.no_grad():
+        run(q)
+    assert rest() is None
+    with torch.inference_mode():
+        run(q)
+    assert rest() is None
+

@@ -442,26 +442,34 @@ class WindowPlan:
     """What attention over a windowed relation keeps for a head layout: its task
     lists, the backward's workspace size and the strides of contiguous fields."""
 
-    def __init__(self, graph: Graph, n: int, heads: int, group: int, D: int):
+    def __init__(self, graph: Graph, heads: int, group: int, D: int):
         self.cu, self.q_tasks, self.n_q, _ = graph._window_tasks(0, heads, group)
+        self.strides = (ctypes.c_int64 * 7)(heads * group * D, group * D, D, heads * D, D,
+                                            heads * D, D)
+        self.forward = (self.cu.data_ptr(), self.q_tasks.data_ptr(), self.n_q)
+        self.backward = None
+
+    def add_backward(self, graph: Graph, n: int, heads: int, group: int, D: int) -> None:
+        """The backward's lists and workspace: by the first forward that has one to come
+        (a capture of the backward alone copies nothing from the host)."""
         _, self.k_tasks, self.n_k, slots = graph._window_tasks(1, heads, group)
         _, self.joins, self.n_joins, _ = graph._window_tasks(2, heads, group)
         need = ctypes.c_size_t()
         _native.call("tgx_window_attn_bwd_workspace", n, slots, heads, group, D,
                      ctypes.byref(need))
         self.work_bytes = need.value
-        self.strides = (ctypes.c_int64 * 7)(heads * group * D, group * D, D, heads * D, D,
-                                            heads * D, D)
-        self.forward = (self.cu.data_ptr(), self.q_tasks.data_ptr(), self.n_q)
         self.backward = (*self.forward, self.k_tasks.data_ptr(), self.n_k, self.joins.data_ptr(),
                          self.n_joins, slots)
 
 
-def _window_plan(graph: Graph, n: int, heads: int, group: int, D: int) -> WindowPlan:
+def _window_plan(graph: Graph, n: int, heads: int, group: int, D: int,
+                 backward: bool) -> WindowPlan:
     key = ("window-plan", heads, group, D)
     plan = graph._native_cache.get(key)
     if plan is None:
-        plan = graph._native_cache[key] = WindowPlan(graph, n, heads, group, D)
+        plan = graph._native_cache[key] = WindowPlan(graph, heads, group, D)
+    if backward and plan.backward is None:
+        plan.add_backward(graph, n, heads, group, D)
     return plan
 
 
@@ -471,16 +479,16 @@ class WindowAttentionFunction(torch.autograd.Function):
     64, 128}; out contiguous [n, heads, group, D]."""
 
     @staticmethod
-    def forward(ctx, q, k, v, scale: float, graph: Graph):
+    def forward(ctx, q, k, v, scale: float, graph: Graph, backward: bool):
         _on_graph_device(graph, q, k, v)
         n, heads, group, D = q.shape
         out = torch.empty((n, heads, group, D), dtype=q.dtype, device=q.device)
         lse = torch.empty((n, heads, group), dtype=torch.float32, device=q.device)
         # What rounding takes from the output, for the backward's row sums.
-        rest = torch.empty_like(out) if any(ctx.needs_input_grad) else None
+        rest = torch.empty_like(out) if backward else None
         plan = strides = None
         if n:
-            plan = _window_plan(graph, n, heads, group, D)
+            plan = _window_plan(graph, n, heads, group, D, backward)
             if q.is_contiguous() and k.is_contiguous() and v.is_contiguous() and \
                     not (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
                 strides = plan.strides
@@ -515,7 +523,7 @@ class WindowAttentionFunction(torch.autograd.Function):
                            lse.data_ptr(), dout.data_ptr(), ctx.scale, *graph._window,
                            dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), n, heads, group, D,
                            _ATTN_DTYPES[out.dtype], work.data_ptr(), plan.work_bytes)
-        return dq, dk, dv, None, None
+        return dq, dk, dv, None, None, None
 
 
 def window_attention(q, k, v, scale: float, heads: int, group: int, graph: Graph):
@@ -528,7 +536,10 @@ def window_attention(q, k, v, scale: float, heads: int, group: int, graph: Graph
     if k.ndim == 4:
         k, v = k[:, :, 0], v[:, :, 0]
     rows = q if q.ndim == 4 else q[:, :, None] if group == 1 else q[:, None]
-    return WindowAttentionFunction.apply(rows, k, v, float(scale), graph).view(q.shape)
+    # (Asked here: a Function's forward runs without gradients, and needs_input_grad is
+    # set under torch.no_grad() too.)
+    backward = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+    return WindowAttentionFunction.apply(rows, k, v, float(scale), graph, backward).view(q.shape)
 
 
 # ---------------------------------------------------------------------------
