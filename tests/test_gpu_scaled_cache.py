@@ -773,3 +773,20 @@ def test_a_prepared_call_differentiates_scales():
         assert torch.equal(torch.autograd.grad(out.square().sum(), vc.scales)[0], exp)
     with torch.no_grad():
         assert not before().requires_grad
+
+
+def test_a_variant_tells_how_rows_are_read():
+    rng = np.random.default_rng(1)
+    table, length, pages = relation(rng, [100], 16)
+    g = tg.Graph.paged(dev(table, torch.int32), dev(length, torch.int32), page_size=16,
+                       num_pages=pages)
+    c, _ = cache(rng, pages * 16, 1, 64, "int8", 16)
+    room = torch.zeros(pages * 16, 1, 72, dtype=torch.int8, device=DEV)
+    room[..., 8:] = c.codes
+    odd = tg.BlockScaled(room[..., 8:], c.scales, block=16)
+    q = dev(rng.standard_normal((1, 1, 4, 64)), torch.bfloat16)
+    for held, text in ((c, "once for 128 queries"), (odd, "once for each query")):
+        kernel = Attention()
+        kernel(graph=g, src={"key": held.grouped(), "value": held.grouped()}, dst={"query": q},
+               scale=0.125)
+        assert text in kernel.last_variant.lowering

@@ -425,3 +425,27 @@ def test_a_prepared_call_differentiates_scales(monkeypatch):
     out = run()
     assert torch.equal(out, plain()) and out.requires_grad
     assert torch.autograd.grad(out.sum(), kc.scales)[0].abs().max() > 0
+
+
+def test_what_the_tiles_take():
+    """Widths 32, 64 and 128 of 16-bit queries, over codes that lie on 16 bytes."""
+    from tiga import _paged
+
+    def fields(D, heads=2, gap=0, first=0):
+        slot = D + gap
+        room = torch.zeros(32 * heads * slot + 16, dtype=torch.int8)
+        first += -room.data_ptr() % 16
+        codes = room[first:first + 32 * heads * slot].view(32, heads, slot)[..., :D]
+        return tg.BlockScaled(codes, torch.zeros(4, heads), block=8).grouped()
+
+    q = lambda D, dtype=torch.bfloat16: torch.zeros(1, 2, 4, D, dtype=dtype)
+    good = fields(64)
+    assert _paged.tiles_take(q(64), good, good) and _paged.tiles_take(
+        q(64, torch.float16), good, fields(64, gap=16))
+    assert not _paged.tiles_take(q(64, torch.float32), good, good)
+    assert not _paged.tiles_take(q(40), fields(40), fields(40))
+    for other in (fields(64, gap=8), fields(64, first=8)):
+        assert not _paged.tiles_take(q(64), good, other)
+        assert not _paged.tiles_take(q(64), other, good)
+    cache16 = torch.zeros(32, 2, 1, 64, dtype=torch.bfloat16)
+    assert _paged.tiles_take(q(64), cache16, cache16)

@@ -86,6 +86,16 @@ def cache_rows_ok(k, v) -> bool:
     return rows_on_16_bytes(k) and rows_on_16_bytes(v)
 
 
+def tiles_take(q, k, v) -> bool:
+    """Whether the matrix tiles take a launch, as csrc/tgx_paged.hip chooses them; the
+    rows kernel takes every other."""
+    if q.dtype == torch.float32 or q.shape[-1] not in (32, 64, 128):
+        return False
+    # (Codes by sixteens; those that lie on 8 bytes only go to the rows kernel.)
+    return not isinstance(k, BlockScaled) or all(
+        rows_on_16_bytes(c.codes) and c.codes.data_ptr() % 16 == 0 for c in (k, v))
+
+
 def csr_takes(D: int) -> bool:
     """Whether the CSR attention kernels take heads of this width."""
     return D % 8 == 0 and 8 <= D <= 512 and (D // 8) & (D // 8 - 1) == 0

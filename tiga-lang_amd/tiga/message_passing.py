@@ -944,9 +944,8 @@ class MessagePassing(Kernel):
         entry = "tgx_paged_attn" if window is None and not scaled else "tgx_paged_attn_view"
         derivative = _paged.wants_derivative(q, k, v)
 
-        # (As csrc/tgx_paged.hip chooses its kernel.)
-        reads = ("once for 128 queries of a key head" if q.dtype != torch.float32 and
-                 D in (32, 64, 128) else "once for each query")
+        reads = ("once for 128 queries of a key head" if _paged.tiles_take(q, k, v)
+                 else "once for each query")
 
         def describe():
             if not derivative:
