@@ -351,3 +351,22 @@ def test_row_sums_take_the_output_to_twice_16_bits(dtype, D):
         once = torch.tensor(exp[i]).to(TYPES[dtype]).double().numpy()
         rms = lambda x: np.sqrt(np.square(x - exp[i]).mean())
         assert rms(f64(got[i]).reshape(exp[i].shape)) < 1.8 * rms(once)
+
+
+@pytest.mark.parametrize("heads,group", [(1, 128), (128, 1)])
+def test_offsets_past_32_bits(heads, group):
+    """Queries, or keys and values too, of more than 2^31 elements: the first and the last
+    sequence have the bits that they have alone."""
+    D, lengths, window = 128, [300, 131000, 500], 16
+    n = sum(lengths)
+    assert n * heads * group * D > 2 ** 31
+    gen = torch.Generator(device=DEV).manual_seed(12)
+    mk = lambda *s: torch.randn(s, device=DEV, dtype=torch.bfloat16, generator=gen)
+    q, d = mk(n, heads, group, D), mk(n, heads, group, D)
+    k, v = mk(n, heads, 1, D), mk(n, heads, 1, D)
+    got = run(tg.Graph.cu_seqlens(packed(lengths), window=window), q, k, v, d, 0.1)
+    for first, length in ((0, 300), (131300, 500)):
+        rows = slice(first, first + length)
+        alone = run(tg.Graph.cu_seqlens(packed([length]), window=window), q[rows], k[rows], v[rows],
+                    d[rows], 0.1)
+        assert all(torch.equal(a[rows], b) for a, b in zip(got, alone))
