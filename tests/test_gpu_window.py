@@ -370,3 +370,23 @@ def test_offsets_past_32_bits(heads, group):
         alone = run(tg.Graph.cu_seqlens(packed([length]), window=window), q[rows], k[rows], v[rows],
                     d[rows], 0.1)
         assert all(torch.equal(a[rows], b) for a, b in zip(got, alone))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D,group", [(32, 2), (64, 1), (128, 3)])
+def test_a_key_of_minus_infinity(dtype, D, group):
+    """A seen key with -Inf in a column where all queries are positive has a score of -Inf
+    and no weight: all is as with a key far down, but for 0 * -Inf in that column of dQ, in
+    tiles that are masked and in those that are not."""
+    rng = np.random.default_rng(13)
+    lengths, window, sinks, heads, at, column = [400, 90], 170, 2, 2, 140, 5
+    g = tg.Graph.cu_seqlens(packed(lengths), window=window, sinks=sinks)
+    q, k, v, d = inputs(rng, lengths, heads, group, D, dtype)
+    q[..., column] = q[..., column].abs() + 1
+    low = k.clone()
+    k[at, ..., column], low[at, ..., column] = -np.inf, -3e4     # (3e4 D^-1/2 > 2000)
+    got, exp = run(g, q, k, v, d, D ** -0.5), run(g, q, low, v, d, D ** -0.5)
+    sees = slice(at, at + window)
+    assert got[1][sees, ..., column].isnan().all()
+    got[1][sees, ..., column] = exp[1][sees, ..., column]
+    assert all(torch.equal(a, b) and torch.isfinite(a).all() for a, b in zip(got, exp))

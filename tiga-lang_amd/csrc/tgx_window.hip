@@ -210,6 +210,21 @@ struct Tile {
     return *reinterpret_cast<const vec4<T>*>(tile + r * kRowBytes +
                                              ((d / 8 ^ turn(r % 16)) * 16) + d % 8 * 2);
   }
+  // Bit 4 dt + e: whether value 16 dt + 4 g + e of row r is a NaN or Inf.
+  static __device__ __forceinline__ uint32_t odd_columns(const char* tile, int r, int g) {
+    uint32_t found = 0;
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) {
+      const vec4<T> v = four(tile, r, 16 * dt + 4 * g);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = static_cast<float>(v[e]);
+        found |= static_cast<uint32_t>(!(__builtin_fabsf(x) < __builtin_huge_valf()))
+                 << (4 * dt + e);
+      }
+    }
+    return found;
+  }
   // Whether this thread's part of the tile has a NaN or Inf.
   static __device__ __forceinline__ bool odd(const char* tile) {
     bool found = false;
@@ -791,10 +806,11 @@ __global__ __launch_bounds__(256) void window_merge_kernel(WinBwdArgs<T> b,
 }
 
 // dQ: S^T = K Q^T and dP^T = V dO^T give dS^T, the B operand of dQ^T = K^T dS^T.  In a
-// masked tile with a NaN or Inf among K, those count as zeros in the last product: a
-// row that sees such a key has a NaN in dS already, or (a score of -inf) no weight for
-// it.  (Multiplying row by row, as the other kernels do, needs registers that spill
-// here: a spilled fragment's reload waits for the tile in flight.)
+// masked tile with a NaN or Inf among K, those count as zeros in the last product, and
+// the columns where a row sees one are NaN in the end: such a row has a NaN in dS
+// already, or (a score of -inf) a weight of 0, which times Inf is one.  (Multiplying row
+// by row, as the other kernels do, needs registers that spill here: a spilled
+// fragment's reload waits for the tile in flight.)
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void window_dq_kernel(WinBwdArgs<T> b) {
   constexpr int KC = D / 32, DT = D / 16;
@@ -803,6 +819,9 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(WinBwdArgs<T> b) {
   auto& ks = tiles_s[0];
   auto& vs = tiles_s[1];
   __shared__ int sh_odd[4];
+  // A thread's: bit 4 dt + r, dqt[dt][.][r] is no number.  (In registers held over the
+  // loop they took 1% of a training step.)
+  __shared__ uint32_t bad_s[2][256];
   const WinArgs<T>& a = b.a;
   const Form& f = a.f;
   const int32_t* task = a.tasks + 4 * static_cast<int64_t>(blockIdx.x);
@@ -845,6 +864,7 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(WinBwdArgs<T> b) {
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int qt = 0; qt < 2; ++qt) dqt[dt][qt] = f32x4v{0.f, 0.f, 0.f, 0.f};
+  bad_s[0][threadIdx.x] = bad_s[1][threadIdx.x] = 0u;
   const KeyTiles tiles(f, q0, q1);
   TL tl(g, lr);
   const float score_log2 = a.scale_log2 * a.sign;
@@ -903,6 +923,15 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(WinBwdArgs<T> b) {
       }
     }
     if (odd) {   // (of the whole workgroup)
+      if (active) {
+#pragma unroll 1
+        for (int r = 0; r < kKeys; ++r) {
+          const uint32_t found = Tile<T, D>::odd_columns(ks[buf], r, g);
+#pragma unroll
+          for (int qt = 0; qt < 2; ++qt)
+            if (sees(f, qpos[qt], kbase + r)) bad_s[qt][threadIdx.x] |= found;
+        }
+      }
       __syncthreads();
       clear_odd<T, D>(ks[buf]);
       __syncthreads();
@@ -931,11 +960,14 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(WinBwdArgs<T> b) {
     split_row(f, again, rem, 32 * wave + 16 * qt + lr, pos, head);
     if (pos >= len) continue;
     T* row = b.dq + ((static_cast<int64_t>(s0 + pos) * f.heads + h) * f.group + head) * D;
+    const uint32_t bad = bad_s[qt][threadIdx.x];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       vec4<T> w;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) w[r] = static_cast<T>(dqt[dt][qt][r] * b.scale);
+      for (int r = 0; r < 4; ++r)
+        w[r] = static_cast<T>(bad >> (4 * dt + r) & 1 ? __builtin_nanf("")
+                                                      : dqt[dt][qt][r] * b.scale);
       *reinterpret_cast<vec4<T>*>(row + 16 * dt + 4 * g) = w;
     }
   }
