@@ -925,7 +925,8 @@ int tgx_select_pages(const tgx_paged* p, const void* q_dev, const int64_t* strid
  *
  * tgx_window_tasks: the host lists of a relation (cu_host [n_blocks + 1]), XCD by
  * XCD.  kind 0: query tiles [n, 4]; 1: key tiles [n, 8], with *n_slots partial
- * sums (at most 3072, each 512 D bytes of the backward's workspace); 2: the key tiles joined from those [n, 8].  tasks_host NULL asks for the
+ * sums (each 512 D bytes of the backward's workspace, 192 MB in all at most at D =
+ * 128); 2: the key tiles joined from those [n, 8].  tasks_host NULL asks for the
  * counts.  The lists go to the device unchanged. */
 int tgx_window_tasks(const int32_t* cu_host, int n_blocks, int heads, int group, int window,
                      int sinks, int kind, int32_t* tasks_host, int64_t* n_tasks,
@@ -949,9 +950,10 @@ int tgx_window_attn_bwd(const int32_t* cu_dev, const int32_t* q_tasks_dev, int64
                         const int32_t* k_tasks_dev, int64_t n_k_tasks, const int32_t* joins_dev,
                         int64_t n_joins, int64_t n_slots, const void* q, const void* k,
                         const void* v, const int64_t* strides, const void* out,
-                        const void* rest, const float* lse, const void* dout, float scale, int window, int sinks, void* dq, void* dk,
-                        void* dv, int64_t n, int heads, int group, int D, int dtype,
-                        void* workspace_dev, size_t workspace_bytes, void* stream);
+                        const void* rest, const float* lse, const void* dout, float scale,
+                        int window, int sinks, void* dq, void* dk, void* dv, int64_t n, int heads,
+                        int group, int D, int dtype, void* workspace_dev, size_t workspace_bytes,
+                        void* stream);
 
 /* ------------------------------------------------------------------------ */
 /* Norm and rotation of queries and keys                                     */
