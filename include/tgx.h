@@ -934,7 +934,7 @@ int tgx_window_tasks(const int32_t* cu_host, int n_blocks, int heads, int group,
 
 /* out [n, heads, group, D] contiguous.  For the backward: rest, like out, what rounding
  * took from it (NULL without a backward), and lse [n, heads, group] fp32, the logarithm
- * to base 2 of each row's sum of exponentials.
+ * to base 2 of each row's sum of exponentials, for fp16 less 14.
  * strides, host array of seven, in elements, multiples of 8: q's token, head, group;
  * k's token, head; v's token, head. */
 int tgx_window_attn_fwd(const int32_t* cu_dev, const int32_t* tasks_dev, int64_t n_tasks,

@@ -390,3 +390,27 @@ def test_a_key_of_minus_infinity(dtype, D, group):
     assert got[1][sees, ..., column].isnan().all()
     got[1][sees, ..., column] = exp[1][sees, ..., column]
     assert all(torch.equal(a, b) and torch.isfinite(a).all() for a, b in zip(got, exp))
+
+
+def test_small_fp16_weights_are_not_lost():
+    """Keys of weight e^-18.4, 2^-26.6 of the first one's and below fp16's smallest
+    number: what the rows have of their values, and they of the rows' gradients."""
+    rng = np.random.default_rng(14)
+    n, D = 30000, 32
+    part = lambda *s: rng.uniform(0.5, 1.5, s)
+    q, k = np.zeros((n, 1, 1, D)), np.zeros((n, 1, 1, D))
+    v, d = part(n, 1, 1, D), part(n, 1, 1, D)
+    q[..., 0], k[1:, ..., 0], v[0] = 1, -18.40625, 0
+    t = [torch.tensor(x, device=DEV).to(torch.float16) for x in (q, k, v, d)]
+    got = run(tg.Graph.triangular(n, device="cuda", window=n), *t, 1.0)
+    weight = np.exp(-18.40625)
+    total = 1 + weight * np.arange(n)
+    values, grads = f64(t[2])[:, 0, 0], f64(t[3])[:, 0, 0]
+    out = weight * np.cumsum(values, 0) / total[:, None]
+    dv = weight * np.cumsum((grads / total[:, None])[::-1], 0)[::-1]
+    # Half a step of a weight and of the result (or of the smallest number), fp32 sums 32
+    # keys at a time, and scores of 27 in 32 bits.
+    rel = 2 * HALF["f16"] + 2 * 2.0 ** -24 * (n / 32 + 64) + 2.0 ** -18
+    assert (np.abs(f64(got[0])[:, 0, 0] - out) <= rel * out + 2.0 ** -25).all()
+    assert (np.abs(f64(got[3])[1:, 0, 0] - dv[1:]) <= rel * dv[1:] + 2.0 ** -25).all()
+    assert out[-1].min() > 100 * 2.0 ** -25 and dv[1].min() > 100 * 2.0 ** -25

@@ -54,6 +54,22 @@ constexpr int kMaxGroup = 128;
 // Strides of a token stay below this, so that an offset in a tile fits 32 bits.
 constexpr int64_t kMaxTokenStride = int64_t{1} << 24;
 
+// The running maximum m moves when a tile's exceeds it by kRescale (log2 units), and a
+// weight is 2^(s - m + kLift): fp16 has no numbers below 2^-24, so its weights fill the
+// range up to 2^15, as over pages; and in the backward those are P 2^kLift.  (Unlifted,
+// keys of weights below 2^-25 = e^-17.3 of the largest are lost from out and dV.  The
+// moves take 1% of a step of 17k tokens.)  dS is as large as the output's gradient
+// makes it: below 2^-14 it rounds in steps of 2^-24, so it takes the scaled loss that fp16
+// training has.
+template <typename T>
+struct Weights {
+  static constexpr float kRescale = kRescaleLog2, kLift = 0.f, kUnlift = 1.f;
+};
+template <>
+struct Weights<_Float16> {
+  static constexpr float kRescale = 1.f, kLift = 14.f, kUnlift = 0x1p-14f;
+};
+
 struct Form {
   const int32_t* cu;   // [n_blocks + 1] first tokens of the sequences
   int heads, group;
@@ -73,7 +89,7 @@ struct WinArgs {
   float sign;          // what the queries are multiplied by first: 1, -1 or 0
   T* out;              // [n, heads, group, D]; backward: dO
   T* rest;             // forward: out before rounding less out, or null
-  float* lse;          // [n, heads, group]: log2 of the sum of 2^(scores * scale_log2)
+  float* lse;          // [n, heads, group]: log2 of the sum of 2^(scores * scale_log2), - kLift
 };
 
 // Position and head in the group of the row that lies `r` (< 128) rows behind row
@@ -446,7 +462,7 @@ __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs<T
           for (int r = 0; r < 4; ++r) x = fmaxf(x, c[kt][qt][r]);
         mt[qt] = group4_max(x) * sl2;
         // (The difference: a sum may round away from where m is large.)
-        grow |= mt[qt] - m[qt] > kRescaleLog2;
+        grow |= mt[qt] - m[qt] > Weights<T>::kRescale;
       }
       if (__any(grow)) {
 #pragma unroll
@@ -461,7 +477,7 @@ __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs<T
       }
 #pragma unroll
       for (int qt = 0; qt < 2; ++qt) {
-        const float mo = m[qt] == kNegInf ? 0.f : m[qt];
+        const float mo = m[qt] == kNegInf ? 0.f : m[qt] - Weights<T>::kLift;
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
@@ -539,7 +555,8 @@ __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs<T
       *reinterpret_cast<vec4<T>*>(row + 16 * dt + 4 * g) = w;
       if (a.rest) *reinterpret_cast<vec4<T>*>(a.rest + at[qt] * D + 16 * dt + 4 * g) = rest;
     }
-    if (g == 0) a.lse[at[qt]] = m[qt] + __log2f(l);
+    // (l is lifted itself.)
+    if (g == 0) a.lse[at[qt]] = m[qt] + __log2f(l) - 2.f * Weights<T>::kLift;
   }
 }
 
@@ -564,18 +581,18 @@ __global__ __launch_bounds__(256) void window_delta_kernel(const T* __restrict__
       s += static_cast<float>(x[j]) * (static_cast<float>(y[j]) + static_cast<float>(z[j]));
   }
   s = group_sum<LPR>(s);
-  if (row < rows && threadIdx.x % LPR == 0) delta[row] = s;
+  if (row < rows && threadIdx.x % LPR == 0) delta[row] = s * Weights<T>::kUnlift;
 }
 
 template <typename T>
 struct WinBwdArgs {
   WinArgs<T> a;        // out: dO
-  const float* delta;
+  const float* delta;  // times kUnlift
   float scale;
   T* dq;               // [n, heads, group, D]
   T* dk;               // [n, heads, D]
   T* dv;
-  float* partial;      // [slot, dK and dV, 64 keys, D]
+  float* partial;      // [slot, dK and dV (by 1 / kUnlift), 64 keys, D]
 };
 
 // dK/dV.  Task: (sequence, first key, head, first block of 64 rows, blocks, slot).  A
@@ -711,7 +728,7 @@ __global__ __launch_bounds__(256, 2) void window_dkdv_kernel(WinBwdArgs<T> b) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           float p = exp2_hw(sc[qt][r] * score_log2 - lse[r]);
-          float ds = p * (dp[qt][r] - del[r]);
+          float ds = p * (dp[qt][r] * Weights<T>::kUnlift - del[r]);
           if (decltype(masked)::value && !sees(f, pos_s[buf][16 * qt + 4 * g + r], key))
             p = ds = 0.f;
           pb[qt >> 1][4 * (qt & 1) + r] = static_cast<T>(p);
@@ -771,7 +788,7 @@ __global__ __launch_bounds__(256, 2) void window_dkdv_kernel(WinBwdArgs<T> b) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       wk[r] = static_cast<T>(dkt[dt][r] * b.scale);
-      wv[r] = static_cast<T>(dvt[dt][r]);
+      wv[r] = static_cast<T>(dvt[dt][r] * Weights<T>::kUnlift);
     }
     *reinterpret_cast<vec4<T>*>(b.dk + at + 16 * dt + 4 * g) = wk;
     *reinterpret_cast<vec4<T>*>(b.dv + at + 16 * dt + 4 * g) = wv;
@@ -797,7 +814,7 @@ __global__ __launch_bounds__(256) void window_merge_kernel(WinBwdArgs<T> b,
   f32x4v sum = {0.f, 0.f, 0.f, 0.f};
   for (int c = 0; c < count; ++c)
     sum += *reinterpret_cast<const f32x4v*>(src + static_cast<int64_t>(c) * 2 * kKeys * D);
-  if (which == 0) sum *= b.scale;
+  sum *= which == 0 ? b.scale : Weights<T>::kUnlift;
   vec4<T> w;
 #pragma unroll
   for (int r = 0; r < 4; ++r) w[r] = static_cast<T>(sum[r]);
@@ -907,7 +924,7 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(WinBwdArgs<T> b) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               const float p = exp2_hw(sc[qt][r] * score_log2 - lse2[qt]);
-              float ds = p * (dp[qt][r] - del[qt]);
+              float ds = p * (dp[qt][r] * Weights<T>::kUnlift - del[qt]);
               if (decltype(masked)::value && !sees(f, qpos[qt], kbase + 16 * kt + 4 * g + r))
                 ds = 0.f;
               sb[qt][kt >> 1][4 * (kt & 1) + r] = static_cast<T>(ds);
