@@ -1,5 +1,5 @@
 // What the dense attention tiles share (tgx_varlen.hip, tgx_window.hip): vector
-// types, MFMA and lane primitives, transposed fragments and LDS row strides.
+// types, MFMA and lane primitives, registers of the forward.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -36,25 +36,10 @@ using vec8 = typename Vec<T>::v8;
 template <typename T>
 using vec4 = typename Vec<T>::v4;
 
-// LDS row stride (elements) of a staged tile: 288 B rows keep both the 16 B
-// row-fragment reads and the transposing 8 B reads free of bank conflicts
-// (measured: SQ_LDS_BANK_CONFLICT = 0).  The backward's narrower heads use the
-// first part of each row.
-constexpr int TPAD = 144;
-// The forward's, by head dim, and the workgroups per CU its registers are held
-// to: 160 B rows are as free of conflicts (eight rows fall on distinct banks), 96
-// B ones nearly (2.7M conflict cycles a launch of the 96 us below, some 4 us of
-// it), and with 288 B ones the double-buffered K and V tiles left room for
-// two workgroups per CU at every D.  24 causal sequences of 500 to 2000
-// tokens: D = 64, 12 heads 125 -> 110 us, D = 32, 16 heads 118 -> 96 us.  (The
-// backward's tiles are single-buffered and not bound by LDS capacity: the same
-// rows there measured 273 -> 282 us.)
-template <int D>
-constexpr int FPAD = D == 128 ? 144 : D == 64 ? 80 : 48;
+// Workgroups per CU that a forward's registers are held to, by head dim.
 template <int D>
 constexpr int kFwdWaves = D == 128 ? 2 : D == 64 ? 3 : 4;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 // gfx950 (MI355X) has 8 XCDs, each with its own L2; workgroup i of a launch
 // runs on XCD i % 8.
 constexpr int kXcds = 8;
@@ -71,8 +56,8 @@ __device__ __forceinline__ vec8<T> ld8(const T* p) {
   return *reinterpret_cast<const vec8<T>*>(p);
 }
 
-// Max / sum of a value over the four 16-lane groups (lanes l, l^16, l^32,
-// l^48) with gfx950's row-swap permutes: with both operands equal, each swap
+// Max of a value over the four 16-lane groups (lanes l, l^16, l^32, l^48)
+// with gfx950's row-swap permutes: with both operands equal, each swap
 // hands every lane its partner's value in one of the two results.
 __device__ __forceinline__ float group4_max(float x) {
   const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x),
@@ -81,14 +66,6 @@ __device__ __forceinline__ float group4_max(float x) {
   const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x),
                                                   false, false);
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ __forceinline__ float group4_sum(float x) {
-  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x),
-                                                  false, false);
-  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x),
-                                                  false, false);
-  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
 // 2^x on the hardware unit (v_exp_f32): exact 0 for -inf; results below the
@@ -99,22 +76,6 @@ __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2
 // this many (log2 units): weights then stay below 2^8, exact in the final
 // normalisation, and the O rescale is skipped for nearly every tile.
 constexpr float kRescaleLog2 = 8.f;
-
-// A fragment of X^T (rows of X are the contraction index) from a row-major
-// LDS tile X[row][col] with row stride PAD: lane (lr, g) receives
-// X[r0 + 4g + j][c0 + lr] for j < 4 and X[r0 + 16 + 4g + j - 4][c0 + lr] for
-// j >= 4, i.e. 8 rows of one column in the permuted order of the B operand.
-template <typename T, int PAD>
-__device__ __forceinline__ vec8<T> tr_frag(T (*x)[PAD], int r0, int c0, int lr, int g) {
-  const T* p = &x[r0 + 4 * g + (lr >> 2)][c0 + 4 * (lr & 3)];
-  const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(p));
-  const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(p + 16 * PAD));
-  // Assemble at dword granularity (elements 0-3 from a, 4-7 from b).
-  const u32x2 aw = __builtin_bit_cast(u32x2, a);
-  const u32x2 bw = __builtin_bit_cast(u32x2, b);
-  const u32x4 w = {aw[0], aw[1], bw[0], bw[1]};
-  return __builtin_bit_cast(vec8<T>, w);
-}
 
 }  // namespace
 }  // namespace tgx

@@ -53,7 +53,7 @@ struct ScaledAppendArgs {
 // LPR rows at a time, kHold times of them in flight and kept until the scale is known
 // (of longer blocks the rest is read again, from the caches).
 // Bound: memory for prompts (16-bit rows read, codes written: 8 of 1500 tokens, 16
-// heads of 64, 21 us), latency for a single token (64 sequences: 8 us).  One pass over the
+// heads of 64, 15 us), latency for a single token (64 sequences: 5.2 us).  One pass over the
 // rows instead of two, codes by one product and one fused add, and keys and values on
 // waves of their own took those prompts, written and read back, from 58 to 32 us.
 constexpr int kHold = 4;
@@ -196,8 +196,14 @@ __global__ __launch_bounds__(256) void append_scaled_kernel(ScaledAppendArgs a) 
 }
 
 // Below this many workgroups of four parts a thread one part each fills more of the
-// GPU; and what is written is stored past the caches from this size on (64000 rows of 8
-// heads of 128: 113 us with one part a thread and through the caches, 58 us with both).
+// GPU; and what is written is stored past the caches from this size on.  8 heads of 128,
+// e4m3 to bf16, calls of a graph one after another: rows (workgroups of four parts, bytes
+// written) and us with one part a thread, with four, and with four past the caches:
+//   256 (32, 1 MB)        3.6    7.4    7.4       16384 (2048, 64 MB)   19.9   22.2   20.3
+//   4096 (512, 16 MB)     7.7   10.0    8.7       64000 (8000, 250 MB)  95     90     62
+//   8192 (1024, 32 MB)   12.4   14.7   12.5       200000 (25000, 0.8 GB) 290   261    250
+// (4 heads of 64 are the same by workgroups and bytes.)  One part would still be the
+// faster from 512 to 1024 workgroups, by 2.3 us at most.
 constexpr unsigned kFewReads = 512;
 constexpr int64_t kPastCaches = int64_t{32} << 20;
 

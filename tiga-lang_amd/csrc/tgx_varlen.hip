@@ -49,6 +49,39 @@ namespace {
 
 constexpr int VBM = 128;   // queries per workgroup (4 waves x 32)
 constexpr int VBN = 64;    // keys per iteration
+constexpr float kLn2 = 0.6931471805599453f;
+// LDS row stride (elements) of a staged tile: 288 B rows keep both the 16 B
+// row-fragment reads and the transposing 8 B reads free of bank conflicts
+// (measured: SQ_LDS_BANK_CONFLICT = 0).  The backward's narrower heads use the
+// first part of each row.
+constexpr int TPAD = 144;
+// The forward's, by head dim, and the workgroups per CU its registers are held
+// to: 160 B rows are as free of conflicts (eight rows fall on distinct banks), 96
+// B ones nearly (2.7M conflict cycles a launch of the 96 us below, some 4 us of
+// it), and with 288 B ones the double-buffered K and V tiles left room for
+// two workgroups per CU at every D.  24 causal sequences of 500 to 2000
+// tokens: D = 64, 12 heads 125 -> 110 us, D = 32, 16 heads 118 -> 96 us.  (The
+// backward's tiles are single-buffered and not bound by LDS capacity: the same
+// rows there measured 273 -> 282 us.)
+template <int D>
+constexpr int FPAD = D == 128 ? 144 : D == 64 ? 80 : 48;
+
+// A fragment of X^T (rows of X are the contraction index) from a row-major
+// LDS tile X[row][col] with row stride PAD: lane (lr, g) receives
+// X[r0 + 4g + j][c0 + lr] for j < 4 and X[r0 + 16 + 4g + j - 4][c0 + lr] for
+// j >= 4, i.e. 8 rows of one column in the permuted order of the B operand.
+template <typename T, int PAD>
+__device__ __forceinline__ vec8<T> tr_frag(T (*x)[PAD], int r0, int c0, int lr, int g) {
+  const T* p = &x[r0 + 4 * g + (lr >> 2)][c0 + 4 * (lr & 3)];
+  const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(p));
+  const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(p + 16 * PAD));
+  // Assemble at dword granularity (elements 0-3 from a, 4-7 from b).
+  const u32x2 aw = __builtin_bit_cast(u32x2, a);
+  const u32x2 bw = __builtin_bit_cast(u32x2, b);
+  const u32x4 w = {aw[0], aw[1], bw[0], bw[1]};
+  return __builtin_bit_cast(vec8<T>, w);
+}
+
 // Stored dS (the dK/dV kernel writes it, the dQ kernel reads it back instead
 // of recomputing S and dP): 64 x 64 tiles per (block, head), query blocks qi
 // and key blocks kj of 64 rows from the block's start; a causal (square)

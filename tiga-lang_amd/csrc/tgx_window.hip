@@ -195,7 +195,7 @@ struct Tile {
     load_lds(base, offset, tile + (wave * kLoads + i) * 1024);
   }
   // Where the lane's fragments begin: eight values of row lr (mod 16) from 8 g on, and
-  // what tr_frag reads down the columns.  Row r0 of either is a multiple of 16.
+  // what the transposing reads take down the columns.  Row r0 of either is a multiple of 16.
   int at, down;
   __device__ __forceinline__ Tile(int g, int lr) {
     at = lr * kRowBytes + ((g % kChunks) ^ turn(lr)) * 16;
