@@ -449,3 +449,17 @@ def test_what_the_tiles_take():
         assert not _paged.tiles_take(q(64), other, good)
     cache16 = torch.zeros(32, 2, 1, 64, dtype=torch.bfloat16)
     assert _paged.tiles_take(q(64), cache16, cache16)
+
+
+def test_what_a_cache_consists_of_is_fixed():
+    """Launches go by the sizes that were checked once: other scales would be read past
+    their end."""
+    c = tg.BlockScaled.zeros(16, 2, 8, block=4)
+    for name, value in (("scales", torch.zeros(1, 2)), ("codes", c.codes[:4]), ("block", 1),
+                        ("tables", 2), ("spec", ()), ("other", 1)):
+        with pytest.raises(AttributeError, match="fixed"):
+            setattr(c, name, value)
+    with pytest.raises(AttributeError, match="fixed"):
+        del c.scales
+    c.scales.fill_(2.0)
+    assert float(c.scales[3, 1]) == 2.0 and c.grouped().scales is c.scales

@@ -26,7 +26,8 @@ class BlockScaled:
     ``Graph.append`` writes such caches, ``Graph.read`` reads them back, and
     attention over ``Graph.paged`` takes them as its key and value fields; every
     other edge function over a paged relation sees them as `dequantize` gives
-    them.  The tensors are the caller's: their contents are read as they stand.
+    them.  The tensors are the caller's: their contents are read as they stand,
+    which tensors they are is fixed.
 
     A scale may be any finite number; `append` stores by powers of two, and a
     block that holds a NaN or an infinity by the scale NaN, with which all of
@@ -55,12 +56,21 @@ class BlockScaled:
             raise ValueError(f"scales are on {scales.device}, codes on {codes.device}")
         if codes.shape[-1] > 1 and codes.stride(-1) != 1:
             raise ValueError("the rows of codes must be dense")
-        self.codes, self.scales, self.block, self.tables = codes, scales, block, tables
-        # Whether rows start a multiple of 8 bytes from the first.
-        self.eights = all(n <= 1 or s % 8 == 0 for n, s in zip(codes.shape[:-1], codes.stride()))
-        # What a launch depends on beside the contents and addresses.
-        self.spec = (codes.dtype, codes.shape, codes.stride(), codes.device, scales.shape, block,
-                     tables)
+        vars(self).update(
+            codes=codes, scales=scales, block=block, tables=tables,
+            # Whether rows start a multiple of 8 bytes from the first.
+            eights=all(n <= 1 or s % 8 == 0 for n, s in zip(codes.shape[:-1], codes.stride())),
+            # What a launch depends on beside the contents and addresses.
+            spec=(codes.dtype, codes.shape, codes.stride(), codes.device, scales.shape, block,
+                  tables))
+
+    def __setattr__(self, name, value):
+        # (Launches go by what was checked here.)
+        raise AttributeError(f"a BlockScaled's {name} is fixed: write into its tensors, or make "
+                             "another of others")
+
+    def __delattr__(self, name):
+        self.__setattr__(name, None)
 
     @classmethod
     def zeros(cls, slots: int, heads: int, width: int, *, block: int,
