@@ -281,3 +281,15 @@ def test_a_forward_alone_prepares_no_backward(monkeypatch):
     with torch.inference_mode():
         run(q)
     assert rest() is None
+
+
+@pytest.mark.parametrize("kind", [0, 1, 2])
+def test_lists_too_long_for_a_launch_are_refused_before_they_are_formed(kind):
+    cu = np.array([0, 2 ** 20, 2 ** 30], dtype=np.int32)
+    n, slots = ctypes.c_int64(), ctypes.c_int64()
+    for blocks, heads in ((1, 2 ** 30), (1, 2 ** 11), (2, 1)):
+        if blocks == 2 and kind == 0:
+            continue
+        with pytest.raises(RuntimeError, match="too many tasks"):
+            _native.call("tgx_window_tasks", cu.ctypes.data, blocks, heads, 1, 64, 1, kind, None,
+                         ctypes.byref(n), ctypes.byref(slots))

@@ -37,6 +37,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <new>
 #include <type_traits>
 #include <vector>
 
@@ -1093,18 +1094,23 @@ int64_t blocks_of_a_piece(const int32_t* cu, int n_blocks, int heads, int group,
                    ceil_div(total * heads, kMaxPieces)});
 }
 
-}  // namespace
-}  // namespace tgx
-
-using namespace tgx;
-
-extern "C" int tgx_window_tasks(const int32_t* cu_host, int n_blocks, int heads, int group,
-                                int window, int sinks, int kind, int32_t* tasks_host,
-                                int64_t* n_tasks, int64_t* n_slots) {
+// (tgx_window_tasks; may throw.)
+int window_tasks(const int32_t* cu_host, int n_blocks, int heads, int group, int window, int sinks,
+                 int kind, int32_t* tasks_host, int64_t* n_tasks, int64_t* n_slots) {
   TGX_REQUIRE(cu_host && n_tasks && n_slots && n_blocks >= 0 && heads > 0 && group > 0 &&
                   group <= kMaxGroup && window > 0 && sinks >= 0,
               "bad arguments");
   TGX_REQUIRE(kind >= 0 && kind <= 2, "kind must be 0 (query tiles), 1 (key tiles) or 2 (joins)");
+  int64_t tiles = 0;   // (beside them there are 1.5 kMaxPieces tasks at most)
+  for (int b = 0; b < n_blocks; ++b) {
+    const int64_t len = int64_t{cu_host[b + 1]} - cu_host[b];
+    TGX_REQUIRE(len >= 0 && cu_host[b] >= 0, "cu_seqlens must be non-decreasing from 0");
+    TGX_REQUIRE(len * group < (int64_t{1} << 31) - 4 * kRows,
+                "rows of a key head must be fewer than 2^31");
+    tiles += kind == 0 ? ceil_div(len * group, kRows) : ceil_div(len, kKeys);
+  }
+  // (Before any of them is formed.)
+  TGX_REQUIRE(tiles * heads < kMaxBlocks256, "too many tasks");
   const int width = kind == 0 ? 4 : 8;
   struct Task {
     int64_t work;
@@ -1116,9 +1122,6 @@ extern "C" int tgx_window_tasks(const int32_t* cu_host, int n_blocks, int heads,
       kind == 0 ? 0 : blocks_of_a_piece(cu_host, n_blocks, heads, group, window, sinks);
   for (int b = 0; b < n_blocks; ++b) {
     const int64_t len = int64_t{cu_host[b + 1]} - cu_host[b];
-    TGX_REQUIRE(len >= 0 && cu_host[b] >= 0, "cu_seqlens must be non-decreasing from 0");
-    TGX_REQUIRE(len * group < (int64_t{1} << 31) - 4 * kRows,
-                "rows of a key head must be fewer than 2^31");
     for (int h = 0; h < heads; ++h) {
       if (kind == 0) {
         for (int64_t r = 0; r < len * group; r += kRows) {
@@ -1190,6 +1193,23 @@ extern "C" int tgx_window_tasks(const int32_t* cu_host, int n_blocks, int heads,
         }
       }
   return TGX_OK;
+}
+
+}  // namespace
+}  // namespace tgx
+
+using namespace tgx;
+
+extern "C" int tgx_window_tasks(const int32_t* cu_host, int n_blocks, int heads, int group,
+                                int window, int sinks, int kind, int32_t* tasks_host,
+                                int64_t* n_tasks, int64_t* n_slots) {
+  try {
+    return window_tasks(cu_host, n_blocks, heads, group, window, sinks, kind, tasks_host, n_tasks,
+                        n_slots);
+  } catch (const std::bad_alloc&) {
+    set_error("host allocation failed");
+    return TGX_OUT_OF_MEMORY;
+  }
 }
 
 extern "C" int tgx_window_attn_fwd(const int32_t* cu_dev, const int32_t* tasks_dev,
