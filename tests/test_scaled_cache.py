@@ -463,3 +463,17 @@ def test_what_a_cache_consists_of_is_fixed():
         del c.scales
     c.scales.fill_(2.0)
     assert float(c.scales[3, 1]) == 2.0 and c.grouped().scales is c.scales
+
+
+def test_older_codes_next_to_a_tie():
+    """60 by 0.3 (in fp32 a little more) is 4.5 by 4 and a little more: 5."""
+    g = tg.Graph.paged(torch.tensor([[0]], dtype=torch.int32), torch.tensor([2], dtype=torch.int32),
+                       page_size=4, num_pages=1)
+    kc, vc = (tg.BlockScaled.zeros(4, 1, 8, block=4, dtype=torch.int8) for _ in range(2))
+    kc.scales.fill_(0.3)
+    kc.codes[0] = torch.tensor([60, -60, 100, -100, 20, -20, 127, 0], dtype=torch.int8)
+    x = torch.full((1, 1, 8), 400.0)
+    g.append(kc, x, vc, x)
+    assert float(kc.scales) == 4.0 and (kc.codes[1] == 100).all()
+    exact = np.array([60, -60, 100, -100, 20, -20, 127, 0]) * (float(np.float32(0.3)) / 4)
+    assert kc.codes[0, 0].tolist() == np.rint(exact).tolist()

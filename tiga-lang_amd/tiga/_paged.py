@@ -358,7 +358,10 @@ def _append_scaled_torch(state, cache, new) -> None:
     got = encode(x / scale[:, :, None, :, None], dtype).view(torch.int8)
     # Older codes of a scale that stays, or by a NaN, stay as they are; others are rounded
     # again (and a NaN among them stays one).
-    moved = older.view(dtype).float() * (held / scale)[:, :, None, :, None]
+    # As on the kernels: int8 products rounded once, e4m3's to fp32 first (both exact where
+    # the older scale is a power of two).
+    wide = torch.float64 if dtype == torch.int8 else torch.float32
+    moved = older.view(dtype).to(wide) * (held / scale).to(wide)[:, :, None, :, None]
     moved = torch.where(moved.isnan(), older, encode(moved, dtype).view(torch.int8))
     again = (begun & (held != scale) & ~scale.isnan())[:, :, None, :, None]
     got = torch.where(is_new[..., None, None], got, torch.where(again, moved, older))

@@ -645,8 +645,10 @@ class Graph:
         A block whose scale grows has its older tokens' codes rounded again by the new
         one.  A NaN or an infinity among the new values makes the scale NaN until the
         block is begun again, and every row of the block and head reads back as NaN.
-        Page sums are those of the rows as they are held.  Widths that are no
-        multiple of 8, or over 512, run on Torch operations.
+        Page sums are those of the rows as they are held.  (By a scale from elsewhere that
+        is no power of two, quotients, and for float8_e4m3fn the older codes' products, are
+        rounded to fp32 first.)  Widths that are no multiple of 8, or over 512, run on
+        Torch operations.
 
         Each sequence's written pages must be its own and named once in its
         table (two writers of a slot leave either's row there), and key and
