@@ -414,3 +414,23 @@ def test_small_fp16_weights_are_not_lost():
     assert (np.abs(f64(got[0])[:, 0, 0] - out) <= rel * out + 2.0 ** -25).all()
     assert (np.abs(f64(got[3])[1:, 0, 0] - dv[1:]) <= rel * dv[1:] + 2.0 ** -25).all()
     assert out[-1].min() > 100 * 2.0 ** -25 and dv[1].min() > 100 * 2.0 ** -25
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_sinks_past_everything_are_causal_attention(dtype):
+    """All tokens as sinks: every key tile is cut into pieces, whose size goes by all the
+    work; over a window of all tokens none is.  The products are the same."""
+    rng = np.random.default_rng(15)
+    n, heads, group, D = 6000, 4, 4, 64
+    q, k, v, d = inputs(rng, [n], heads, group, D, dtype)
+    cut, whole = (tg.Graph.cu_seqlens(packed([n]), window=w, sinks=s) for w, s in ((1, n), (n, 0)))
+    got, exp = (run(g, q, k, v, d, 0.125) for g in (cut, whole))
+    assert 1000 < cut._window_tasks(1, heads, group)[3] <= 1.5 * 2048
+    assert whole._window_tasks(1, heads, group)[3] == 0
+    assert torch.equal(got[0], exp[0]) and torch.equal(got[1], exp[1])
+    for a, b in zip(got[2:], exp[2:]):
+        a, b = a.float(), b.float()
+        # fp32 sums of up to 24000 products in another order, each of them less than the
+        # largest sum: then a rounding of each.
+        lim = 2 * HALF[dtype] * b.abs() + 2 * 2.0 ** -24 * n * group * b.abs().max()
+        assert ((a - b).abs() <= lim).all()
